@@ -186,7 +186,15 @@ static dt_scratch * dt_scratch_of(cudaStream_t st, size_t bytes) {
     std::lock_guard<std::mutex> lock(mu);
     dt_scratch & s = all[std::make_pair(dev, st)];
     if (!s.err) {
-        if (cudaMalloc(&s.err, 4) != cudaSuccess || cudaMemset(s.err, 0, 4) != cudaSuccess || cudaMallocHost(&s.err_host, 4) != cudaSuccess) { cudaGetLastError(); s.err = nullptr; return nullptr; }
+        // a stream may be capturing when it asks for the first time: the allocation and the clearing, on a stream of its own, are no part of its graph
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaStream_t own = nullptr;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        const bool ok = cudaMalloc(&s.err, 4) == cudaSuccess && cudaMallocHost(&s.err_host, 4) == cudaSuccess && cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess &&
+                        cudaMemsetAsync(s.err, 0, 4, own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+        if (own) cudaStreamDestroy(own);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!ok) { cudaGetLastError(); s.err = nullptr; return nullptr; }
         *s.err_host = 0;
     }
     if (bytes > s.cap) {

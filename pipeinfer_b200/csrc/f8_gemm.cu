@@ -1,0 +1,273 @@
+// f8_gemm.cu -- 8-bit floating point weights with block scales times any number of tokens on tcgen05 (kind::f8f6f4), fp32 accumulation.
+//
+//   y[t][n] = sum over kb of (s[n/128][kb] d[kb][t]) P_kb[n][t],  P_kb = the product of the block's 128 columns
+//
+// The scales change from block to block, so a block's product is one accumulator in tensor memory (four MMAs of K 32) that is read back, scaled and added up in fp32 registers, while the
+// tensor core works on the next blocks' accumulators (512 / NB of them take turns).
+//   warp 0       streams a block of both operands by TMA (a row's 128 bytes are a line of the 128-byte swizzle) through a ring, and the block's activation scales through a ring of their own
+//   warp 1       issues the MMAs; a commit hands the operands back, another says that the accumulator is there
+//   warps 2..9   two groups of four, half of the columns each: a thread owns a weight row (lane) and adds acc[c] += P[c] (s d[c])
+// The CTAs walk the tiles (128 rows x NB tokens).  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks each and add their sums up through
+// distributed shared memory, in share order.
+// Every wait is bounded (tc_common.cuh).
+#include "f8_block.cuh"
+#include "tc_common.cuh"
+
+#include <dlfcn.h>
+
+#include <algorithm>
+
+#define FT_THREADS 320
+#define FT_BM      128
+#define FT_A_TILE  (FT_BM * 128)
+#define FT_RING    (192 * 1024)
+#define FT_STAGES  10                       // at most
+#define FT_DRING   8                        // scale rows under way
+#define FT_BARS    (2 * FT_STAGES + 2 * FT_DRING + 2 * 16)
+#define FT_SMEM    ((size_t) FT_RING + FT_DRING * 1024 + FT_BARS * 8 + 32 + 1024)
+
+__device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+    // a block: four MMAs of K 32, 32 bytes further along both operands each; the first one starts the accumulator
+    asm volatile("{\n\t.reg .pred q;\n\t.reg .b64 a, b;\n\telect.sync _|q, 0xffffffff;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%4, %4, %4, %4}, 0;\n\t"
+                 "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, {%4, %4, %4, %4}, 1;\n\t"
+                 "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, {%4, %4, %4, %4}, 1;\n\t"
+                 "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, {%4, %4, %4, %4}, 1;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void ft_tma_2d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void ft_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t ft_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t ft_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
+__device__ __forceinline__ void ft_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// M x N outputs of e4m3 x e4m3, fp32 accumulators, both operands K-major
+__host__ __device__ constexpr uint32_t ft_idesc(int M, int N) { return (1u << 4) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
+
+struct ft_args {
+    int b, KB, bp, tiles_m, tiles, shares;
+    int64_t N;
+    const float * ws, * ad;
+    float * y;
+    int * err;
+};
+
+template <int NB>
+__global__ void __launch_bounds__(FT_THREADS, 1)
+f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ ft_args A) {
+    constexpr int STAGE = FT_A_TILE + NB * 128, STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / NB < 8 ? 512 / NB : 8, HALF = NB / 2;
+    extern __shared__ __align__(1024) uint8_t ft_dsm[];
+    uint8_t *  sm  = ft_dsm + ((1024u - (dt_smem(ft_dsm) & 1023u)) & 1023u);
+    float *    dsc = reinterpret_cast<float *>(sm + FT_RING);                            // scale rows, 256 floats a place
+    uint64_t * bar = reinterpret_cast<uint64_t *>(sm + FT_RING + FT_DRING * 1024);       // operands there / read, scales there / read, accumulator there / read
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + FT_BARS);
+    volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FT_STAGES * 8, bar_d = bar_e + FT_STAGES * 8, bar_g = bar_d + FT_DRING * 8, bar_t = bar_g + FT_DRING * 8, bar_r = bar_t + 16 * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = A.shares, share = S > 1 ? (int) ft_rank() : 0;
+    const int unit = blockIdx.x / S, units = gridDim.x / S;
+    const int k0 = (int) ((int64_t) A.KB * share / S), nk = (int) ((int64_t) A.KB * (share + 1) / S) - k0;
+    const uint32_t sm0 = dt_smem(sm);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { dt_mbar_init(bar_f + s * 8, 1); dt_mbar_init(bar_e + s * 8, 1); }
+        for (int s = 0; s < FT_DRING; s++) { dt_mbar_init(bar_d + s * 8, 1); dt_mbar_init(bar_g + s * 8, 8); }
+        for (int a = 0; a < ACCS; a++) { dt_mbar_init(bar_t + a * 8, 1); dt_mbar_init(bar_r + a * 8, 8); }
+        *abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dt_smem(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    dt_fence_before();
+    __syncthreads();
+    dt_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pib_pdl_wait();
+    pib_pdl_trigger();
+    bool ok = true;
+
+    if (warp == 0) {
+        int s = 0, ds = 0;
+        uint32_t ph = 1, dph = 1;                                // the first round finds its places free
+        for (int tile = unit; tile < A.tiles && ok; tile += units) {
+            const int n0 = tile / A.tiles_m * FT_BM, m0 = tile % A.tiles_m * NB;
+            const uint32_t dbytes = (uint32_t) min(NB, A.bp - m0) * 4;
+            for (int kt = 0; kt < nk; kt++) {
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_e + s * 8, ph, abort_s) && dt_mbar_wait(bar_g + ds * 8, dph, abort_s));
+                if (!ok) break;
+                if (lane == 0) {
+                    dt_mbar_expect_tx(bar_f + s * 8, STAGE);
+                    ft_tma_2d(sm0 + s * STAGE, &wmap, bar_f + s * 8, (k0 + kt) * 128, n0);
+                    ft_tma_2d(sm0 + s * STAGE + FT_A_TILE, &xmap, bar_f + s * 8, (k0 + kt) * 128, m0);
+                    dt_mbar_expect_tx(bar_d + ds * 8, dbytes);
+                    ft_bulk(dt_smem(dsc + ds * 256), A.ad + (int64_t) (k0 + kt) * A.bp + m0, dbytes, bar_d + ds * 8);
+                }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++ds == FT_DRING) { ds = 0; dph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint64_t d0 = dt_desc(sm0);
+        int s = 0, a = 0;
+        uint32_t ph = 0, aph = 1;
+        for (int tile = unit; tile < A.tiles && ok; tile += units)
+            for (int kt = 0; kt < nk; kt++) {
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && dt_mbar_wait(bar_f + s * 8, ph, abort_s));
+                if (!ok) break;
+                dt_fence_after();
+                const uint64_t ad = d0 + (uint64_t) (s * STAGE >> 4);
+                ft_mma(tmem + a * NB, ad, ad + (FT_A_TILE >> 4), ft_idesc(FT_BM, NB));
+                dt_commit(bar_e + s * 8);
+                dt_commit(bar_t + a * 8);
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (++a == ACCS) { a = 0; aph ^= 1; }
+            }
+    } else {
+        const int q4 = warp & 3, hf = (warp - 2) >> 2;
+        const uint32_t lanes = (uint32_t) (q4 * 32) << 16;
+        float acc[HALF];
+        int a = 0, ds = 0;
+        uint32_t aph = 0, dph = 0;
+        for (int tile = unit; tile < A.tiles && ok; tile += units) {
+            const int64_t n = (int64_t) (tile / A.tiles_m) * FT_BM + q4 * 32 + lane;
+            const int m0 = tile % A.tiles_m * NB + hf * HALF;
+            const float * ws = A.ws + (int64_t) (tile / A.tiles_m) * A.KB + k0;
+#pragma unroll
+            for (int c = 0; c < HALF; c++) acc[c] = 0.f;
+            for (int kt = 0; kt < nk; kt++) {
+                const float w = __ldg(ws + kt);
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_d + ds * 8, dph, abort_s) && dt_mbar_wait(bar_t + a * 8, aph, abort_s));
+                if (!ok) break;
+                dt_fence_after();
+                const float4 * dv = reinterpret_cast<const float4 *>(dsc + ds * 256 + hf * HALF);
+                constexpr int STEP = HALF < 32 ? HALF : 32;
+#pragma unroll
+                for (int c0 = 0; c0 < HALF; c0 += STEP) {
+                    uint32_t v[32];
+                    if (STEP == 32) dt_ld32(tmem + lanes + a * NB + hf * HALF + c0, v);
+                    else {
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                                       "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(tmem + lanes + a * NB + hf * HALF + c0) : "memory");
+                    }
+                    dt_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < STEP; c += 4) {
+                        const float4 d = dv[(c0 + c) / 4];
+                        acc[c0 + c]     = fmaf(__uint_as_float(v[c]), w * d.x, acc[c0 + c]);
+                        acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), w * d.y, acc[c0 + c + 1]);
+                        acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), w * d.z, acc[c0 + c + 2]);
+                        acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), w * d.w, acc[c0 + c + 3]);
+                    }
+                }
+                dt_fence_before();
+                __syncwarp();
+                if (lane == 0) { dt_arrive(bar_r + a * 8); dt_arrive(bar_g + ds * 8); }
+                if (++a == ACCS) { a = 0; aph ^= 1; }
+                if (++ds == FT_DRING) { ds = 0; dph ^= 1; }
+            }
+            if (!ok) break;
+            if (S == 1) {
+                if (n < A.N)
+#pragma unroll
+                    for (int c = 0; c < HALF; c++) if (m0 + c < A.b) A.y[(int64_t) (m0 + c) * A.N + n] = acc[c];
+            } else {
+                // a share's sums, [token][row]: its MMAs have completed, the ring is free (one tile per cluster)
+                float * part = reinterpret_cast<float *>(sm);
+#pragma unroll
+                for (int c = 0; c < HALF; c++) part[(hf * HALF + c) * FT_BM + q4 * 32 + lane] = acc[c];
+            }
+        }
+    }
+    __syncwarp();
+    if (S > 1) {
+        ft_cluster_sync();
+        if (warp >= 2 && !*abort_s) {
+            const int q4 = warp & 3, hf = (warp - 2) >> 2;
+            const int64_t n = (int64_t) (unit / A.tiles_m) * FT_BM + q4 * 32 + lane;
+            const int m0 = unit % A.tiles_m * NB;
+            for (int c = share * 2 + hf; c < NB && m0 + c < A.b; c += S * 2) {
+                float v = 0.f;
+                for (int sh = 0; sh < S; sh++) {
+                    float o;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(ft_mapa(sm0 + (uint32_t) (c * FT_BM + q4 * 32 + lane) * 4, (uint32_t) sh)) : "memory");
+                    v += o;
+                }
+                if (n < A.N) A.y[(int64_t) (m0 + c) * A.N + n] = v;
+            }
+        }
+    }
+    dt_fence_before();
+    __syncthreads();
+    if (*abort_s) {
+        // a wait ran out: say so, give copies and MMAs still in flight time to land (bounded), then free the tensor memory
+        if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (S > 1) ft_cluster_sync();                                // the shares' sums have been read
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------
+typedef CUresult (*ft_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static ft_encode_fn ft_encode() {
+    static ft_encode_fn fn = [] {
+        void * p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); p = nullptr; }
+        return (ft_encode_fn) p;
+    }();
+    return fn;
+}
+// rows of Kp bytes, boxes of 128 bytes x `box` rows, 128-byte swizzle
+static int ft_map(CUtensorMap * map, const void * base, int64_t Kp, int64_t rows, int box) {
+    ft_encode_fn enc = ft_encode();
+    if (!enc) { pib_set_error("tensor map: cuTensorMapEncodeTiled not available"); return PIB_ERR_UNSUPP; }
+    const cuuint64_t gdim[2] = { (cuuint64_t) Kp, (cuuint64_t) rows }, gstr[1] = { (cuuint64_t) Kp };
+    const cuuint32_t bx[2] = { 128, (cuuint32_t) box }, es[2] = { 1, 1 };
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { pib_set_error("tensor map: cuTensorMapEncodeTiled failed (%d)", (int) r); return PIB_ERR_UNSUPP; }
+    return PIB_OK;
+}
+
+template <int NB> static int ft_launch(const CUtensorMap & wmap, const CUtensorMap & xmap, ft_args A, cudaStream_t st) {
+    static pib_per_device attrs;
+    PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(f8_gemm_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) FT_SMEM); }));
+    const int units = A.shares > 1 ? A.tiles : std::min(A.tiles, pib_num_sms());
+    PIB_CHECK(pib_launch_cluster(f8_gemm_kernel<NB>, dim3((unsigned) (units * A.shares)), dim3(FT_THREADS), dim3((unsigned) A.shares, 1, 1), FT_SMEM, st, wmap, xmap, A));
+    return PIB_OK;
+}
+
+int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st) {
+    int rc = pib_f8_rows_ok("pib_gemm", w, act, y, b, PIB_F8_MAX_ROWS);
+    if (rc != PIB_OK) return rc;
+    if ((uintptr_t) act & 15) { pib_set_error("pib_gemm: act_dev needs 16-byte alignment"); return PIB_ERR_ARG; }
+    const pib_f8_act L = pib_f8_act_of(w->K, b);
+    const int NB = b <= 32 ? 32 : b <= 64 ? 64 : b <= 128 ? 128 : 256;
+    ft_args A;
+    A.b = b; A.KB = L.KB; A.bp = L.bp; A.N = w->N; A.y = y;
+    A.ws = (const float *) w->d; A.ad = (const float *) ((const uint8_t *) act + L.d_off);
+    A.tiles_m = (b + NB - 1) / NB;
+    const int64_t tiles = pib_f8_blocks(w->N) * A.tiles_m;
+    if (tiles > 0x3fffffff) { pib_set_error("pib_gemm: %lld x %d outputs are too many", (long long) w->N, b); return PIB_ERR_ARG; }
+    A.tiles = (int) tiles;
+    A.shares = 1;
+    while (A.shares < 8 && A.tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
+    if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
+    CUtensorMap wmap, xmap;
+    if ((rc = ft_map(&wmap, w->qs, L.Kp, pib_f8_blocks(w->N) * PIB_F8_BLOCK, FT_BM)) != PIB_OK || (rc = ft_map(&xmap, act, L.Kp, b, NB)) != PIB_OK) return rc;
+    switch (NB) {
+        case 32:  return ft_launch<32>(wmap, xmap, A, st);
+        case 64:  return ft_launch<64>(wmap, xmap, A, st);
+        case 128: return ft_launch<128>(wmap, xmap, A, st);
+        default:  return ft_launch<256>(wmap, xmap, A, st);
+    }
+}

@@ -29,6 +29,7 @@
 #include <atomic>
 
 #include "q8k_quant.cuh"
+#include "f8_block.cuh"
 #include "tc_common.cuh"
 
 #define TG_BM      128                 // output rows per accumulator (UMMA M)
@@ -510,6 +511,7 @@ int pib_gemm_q4k_tc(const pib_weight * w, const void * act_dev, int b, float * y
 
 extern "C" size_t pib_gemm_scratch_bytes(int64_t K, int b) { return pib_gemm_xhat_bytes(K, b); }
 extern "C" int pib_gemm(const pib_weight * w, const void * act_dev, int b, float * y_dev, void * scratch_dev, pib_stream s) {
+    if (w && w->type == PIB_TYPE_F8) return pib_f8_gemm(w, act_dev, b, y_dev, (cudaStream_t) s);
     if (!act_dev || !y_dev || !scratch_dev || b > 256) { pib_set_error("pib_gemm: bad arguments"); return PIB_ERR_ARG; }
     return pib_gemm_q4k_tc(w, act_dev, b, y_dev, scratch_dev, (cudaStream_t) s);
 }
@@ -521,6 +523,7 @@ int pib_quantize_act_c(int wtype, const float * x_dev, int b, int64_t K, void * 
 
 // host-buffer convenience for the parity tests (like pib_mul_mat_host): x_host [b][K] fp32 -> y_host [b][N]
 extern "C" int pib_gemm_host(const pib_weight * w, const float * x_host, int b, float * y_host) {
+    if (w && w->type == PIB_TYPE_F8) return pib_f8_gemm_host(w, x_host, b, y_host);
     if (!w || b < 1 || b > 256) { pib_set_error("pib_gemm_host: bad arguments"); return PIB_ERR_ARG; }
     const size_t xb = (size_t) b * w->K * 4, yb = (size_t) b * w->N * 4, ab = pib_act_bytes(PIB_TYPE_Q4_K, w->K, b), hb = pib_gemm_xhat_bytes(w->K, b);
     uint8_t * buf = nullptr;
@@ -544,6 +547,7 @@ extern "C" int pib_gemm_host(const pib_weight * w, const float * x_host, int b, 
 }
 
 extern "C" int pib_quantize_act_rows(int wtype, const float * x_dev, int b, int64_t K, void * act_dev, pib_stream s) {
+    if (wtype == PIB_TYPE_F8) return pib_f8_quantize(x_dev, nullptr, 0.f, b, K, act_dev, nullptr, (cudaStream_t) s);
     if (b < 1 || b > 256) { pib_set_error("pib_quantize_act_rows: 1 <= b <= 256"); return PIB_ERR_ARG; }
     return pib_quantize_act_c(wtype, x_dev, b, K, act_dev, nullptr, (cudaStream_t) s);
 }

@@ -1,6 +1,6 @@
 // lib.cu -- library state (device, look-up tables, error string), small C-ABI helpers, GEMV dispatch, embedding rows.
 #include <algorithm>
-#include "pib_common.cuh"
+#include "f8_block.cuh"
 
 #include <math.h>
 #include <stdarg.h>
@@ -156,6 +156,7 @@ extern "C" int pib_gemv(const pib_weight * w, const void * act_dev, int b, float
         pib_set_error("pib_gemv: bad arguments (b = %d, limit %d)", b, PIB_MAX_BATCH);
         return PIB_ERR_ARG;
     }
+    if (w->type == PIB_TYPE_F8) return pib_f8_gemv(w, act_dev, b, y_dev, (cudaStream_t) s);
     if ((w->type == PIB_TYPE_Q6_K || w->type == PIB_TYPE_Q5_K || w->type == PIB_TYPE_Q3_K) && variant != 4 && variant != 7) variant = 0;   // one fast kernel for these types
     if (((variant == 3 || variant == 6) && !pib_gemv_mma_supported(w, b)) || (variant == 2 && !pib_gemv_mma_supported(w, b) && !pib_gemv_blk32_supported(w, b))) {
         pib_set_error("pib_gemv: variant 2 needs tiles (Q4_K, Q4_0, Q8_0), variants 3 and 6 Q4_K");
@@ -172,6 +173,7 @@ extern "C" int pib_gemv_fused(const pib_weight * w, int prologue, const float * 
         pib_set_error("pib_gemv_fused: bad arguments");
         return PIB_ERR_ARG;
     }
+    if (w->type == PIB_TYPE_F8) return pib_f8_gemv_fused(w, prologue, x_dev, x2_dev, addend_dev, sum_out_dev, xstride, eps, b, y_dev, (cudaStream_t) s);
     return pib_gemv_pro(w, prologue, x_dev, x2_dev, addend_dev, sum_out_dev, xstride, eps, b, y_dev, nullptr, (cudaStream_t) s);
 }
 
@@ -239,6 +241,7 @@ __global__ void get_rows_kernel(int type, const uint8_t * __restrict__ qs, const
 
 extern "C" int pib_get_rows(const pib_weight * w, const int32_t * ids_dev, int n, float * out_dev, pib_stream s) {
     if (!w || !ids_dev || !out_dev || n < 1) { pib_set_error("pib_get_rows: bad arguments"); return PIB_ERR_ARG; }
+    if (w->type == PIB_TYPE_F8) return pib_f8_get_rows(w, ids_dev, n, out_dev, (cudaStream_t) s);
     if (!w->qs) { pib_set_error("pib_get_rows: this matrix keeps only its tensor-core tiles"); return PIB_ERR_UNSUPP; }
     if (w->type == PIB_TYPE_Q3_K) return pib_get_rows_q3k(w, ids_dev, n, out_dev, (cudaStream_t) s);
     if (w->type == PIB_TYPE_Q5_K) return pib_get_rows_q5k(w, ids_dev, n, out_dev, (cudaStream_t) s);

@@ -12,7 +12,7 @@
 //   Q6_K:  qs  192 B [N][K/256]      hdr 32 B [N][K/256]     {ql[128], qh[64]} and {int8 scales[16], fp16 d, pad}
 //
 // The tensor-core GEMV additionally builds fragment-major tiles from these planes (gemv_mma.cu).
-#include "pib_common.cuh"
+#include "f8_block.cuh"
 
 #include <string.h>
 
@@ -99,6 +99,7 @@ static int block_geom(int type, int * elems, int * bytes) {
 
 static pib_weight * alloc_weight(int type, int64_t N, int64_t K) {
     int be, bb;
+    if (type == PIB_TYPE_F8) { pib_set_error("pib_weight: scales of 8-bit floating point rows come with pib_weight_upload_f8 / pib_weight_from_device_f8"); return nullptr; }
     if (block_geom(type, &be, &bb) != 0 || N <= 0 || K <= 0 || K % be != 0) {
         pib_set_error("pib_weight: unsupported type %d or shape %lld x %lld", type, (long long) N, (long long) K);
         return nullptr;
@@ -210,6 +211,7 @@ extern "C" void pib_weight_free(pib_weight * w) {
     if (!w) return;
     if (w->owns && w->base) cudaFree(w->base);
     if (w->tiles) cudaFree(w->tiles);
+    free(w->map);
     free(w);
 }
 
@@ -226,6 +228,7 @@ extern "C" size_t pib_weight_bytes(const pib_weight * w) { return w ? w->bytes :
 
 extern "C" int pib_weight_row_blocks(const pib_weight * w, int64_t row, void * out) {
     if (!w || row < 0 || row >= w->N) { pib_set_error("pib_weight_row_blocks: bad row"); return PIB_ERR_ARG; }
+    if (w->type == PIB_TYPE_F8) return pib_f8_row(w, row, out);
     if (!w->qs) { pib_set_error("pib_weight_row_blocks: this matrix keeps only its tensor-core tiles"); return PIB_ERR_UNSUPP; }
     uint8_t * o = (uint8_t *) out;
     if (w->type == PIB_TYPE_Q5_K) {

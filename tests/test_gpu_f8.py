@@ -1,0 +1,250 @@
+"""8-bit floating point weights with a scale per 128 x 128 block (csrc/f8_quant.cu, f8_gemv.cu, f8_gemm.cu) against float64: sizes that fill no block, no tile and no share, every number of
+tokens where another kernel or tile begins, zero and tiny blocks, infinities and numbers that are none in one token, fused prologues, captured calls, other streams."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+F8 = 64
+
+
+@pytest.fixture(scope="module")
+def pib():
+    from pipeinfer_b200 import lib as pib
+    pib.load().init(0)
+    return pib
+
+
+@pytest.fixture(scope="module")
+def torch():
+    return pytest.importorskip("torch")
+
+
+def blocks(n):
+    return (n + 127) // 128
+
+
+def matrix(torch, N, K, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = (torch.randn(N, K, device="cuda", generator=g) * 96).clamp(-448, 448).to(torch.float8_e4m3fn)
+    s = (torch.rand(blocks(N), blocks(K), device="cuda", generator=g) + 0.5) / 96
+    return q, s, g
+
+
+def rows(torch, b, K, g):
+    x = torch.randn(b, K, device="cuda", generator=g)
+    x[:, ::37] *= 20
+    return x
+
+
+def quantised(torch, x):
+    """e4m3 values and scales, by their definition"""
+    b, K = x.shape
+    p = torch.zeros(b, blocks(K) * 128, device="cuda")
+    p[:, :K] = x
+    v = p.reshape(b, -1, 128)
+    d = v.abs().amax(-1).clamp(min=2.0 ** -100) * float(np.float32(1) / np.float32(448))
+    return (v / d.unsqueeze(-1)).to(torch.float8_e4m3fn).reshape(b, -1), d
+
+
+def dense(torch, q, s):
+    N, K = q.shape
+    return q.double() * s.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+
+
+def want(torch, q, s, x):
+    """float64 outputs and the bound of an output's error: a block's 128 products are added in four steps of the tensor core, which may cut instead of round (2^-22 each), the blocks
+    by KB fused multiply-adds with a factor of one rounding (2^-24 each)"""
+    a, d = quantised(torch, x)
+    K = x.shape[1]
+    X = (a.double() * d.double().repeat_interleave(128, 1))[:, :K]
+    W = dense(torch, q, s)
+    return X @ W.T, (X.abs() @ W.abs().T) * (4 * 2.0 ** -22 + (blocks(K) + 3) * 2.0 ** -24) + 1e-36
+
+
+def product(torch, pib, w, x, how, stream=0):
+    lib, (b, K) = pib.load(), x.shape
+    y = torch.full((b, w.N), float("nan"), device="cuda")
+    if how == "fused":
+        lib.gemv_fused(w, x.data_ptr(), b, y.data_ptr(), stream)
+        return y
+    act = torch.empty(lib.act_bytes(F8, K, b), dtype=torch.uint8, device="cuda")
+    (lib.quantize_act_dev if how == "gemv" else lib.quantize_act_rows)(F8, x.data_ptr(), b, K, act.data_ptr(), stream)
+    if how == "gemv":
+        lib.gemv(w, act.data_ptr(), b, y.data_ptr(), stream)
+    else:
+        lib.gemm(w, act.data_ptr(), b, y.data_ptr(), None, stream)
+        lib.gemm_check(stream)
+    return y
+
+
+@pytest.mark.parametrize("b,K", [(1, 1), (1, 128), (3, 127), (5, 129), (16, 1000), (17, 4096), (300, 260)])
+def test_quantiser(torch, pib, b, K):
+    """bytes and scales as defined; blocks of zeros, of values whose quotients with 448 are no normal numbers, of the largest floats"""
+    lib = pib.load()
+    g = torch.Generator(device="cuda").manual_seed(b * 7 + K)
+    x = rows(torch, b, K, g)
+    if b >= 3:
+        x[1, :128] = 0
+        x[2, :128] *= 1e-38
+        x[0, :128] = x[0, :128].clamp(-2, 2) * 1.5e38
+    act = torch.empty(lib.act_bytes(F8, K, b), dtype=torch.uint8, device="cuda")
+    lib.quantize_act_rows(F8, x.data_ptr(), b, K, act.data_ptr())
+    out = np.zeros((b, blocks(K), 132), np.uint8)
+    lib.check(lib.L.pib_act_to_blocks(F8, act.data_ptr(), b, K, out.ctypes.data))
+    a, d = quantised(torch, x)
+    assert np.array_equal(out[:, :, :4].copy().view(np.float32)[..., 0], d.cpu().numpy())
+    got = torch.from_numpy(out[:, :, 4:].copy()).view(torch.float8_e4m3fn).float()
+    assert torch.equal(got, a.float().cpu().reshape(b, -1, 128))      # as values: the two zeros are one
+
+
+@pytest.mark.parametrize("b,K", [(1, 128), (4, 1000), (16, 5632)])
+def test_quantiser_behind_a_norm(torch, pib, b, K):
+    lib = pib.load()
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x, w = rows(torch, b, K, g), torch.rand(K, device="cuda", generator=g) + 0.5
+    act, xn = torch.empty(lib.act_bytes(F8, K, b), dtype=torch.uint8, device="cuda"), torch.empty(b, K, device="cuda")
+    lib.check(lib.L.pib_norm_quantize_act(F8, 1, x.data_ptr(), w.data_ptr(), 1e-5, b, K, act.data_ptr(), xn.data_ptr(), None))
+    torch.cuda.synchronize()
+    ref = x.double() / (x.double().pow(2).mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    # the mean's sum of K / 256 + 8 fp32 additions in a thread's chain, halved by the root; three roundings behind it
+    assert ((xn.double() - ref).abs() <= ref.abs() * ((K / 256 + 16) / 2 + 6) * 2.0 ** -24).all()
+    out = np.zeros((b, blocks(K), 132), np.uint8)
+    lib.check(lib.L.pib_act_to_blocks(F8, act.data_ptr(), b, K, out.ctypes.data))
+    a, d = quantised(torch, xn)
+    assert np.array_equal(out[:, :, 4:].copy().reshape(b, -1) & 127, a.view(torch.uint8).cpu().numpy() & 127)
+    assert np.array_equal(out[:, :, :4].copy().view(np.float32)[..., 0], d.cpu().numpy())
+
+
+SIZES = [(1, 1), (16, 128), (17, 129), (127, 1000), (128, 256), (129, 2048), (1000, 5700), (2560, 2048), (10000, 640)]
+
+
+@pytest.mark.parametrize("N,K", SIZES)
+@pytest.mark.parametrize("b", [1, 2, 7, 8, 9, 13, 16])
+def test_decode_batches(torch, pib, N, K, b):
+    q, s, g = matrix(torch, N, K, N + K)
+    x = rows(torch, b, K, g)
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), N, K)
+    y, lim = want(torch, q, s, x)
+    for how in ["gemv"] + (["fused"] if b <= 8 else []):
+        err = (product(torch, pib, w, x, how).double() - y).abs()
+        assert (err <= lim).all(), (how, float((err / lim).max()))
+
+
+@pytest.mark.parametrize("N,K,b", [(1, 1, 1), (16, 128, 20), (130, 129, 33), (128, 256, 16), (257, 1000, 65), (300, 5700, 100), (2560, 2048, 129), (1000, 640, 256), (640, 1300, 257), (384, 8192, 40),
+                                   (1100, 2000, 700), (20000, 256, 31), (19000, 128, 300), (5000, 3000, 513)])
+def test_prompts(torch, pib, N, K, b):
+    q, s, g = matrix(torch, N, K, N + K)
+    x = rows(torch, b, K, g)
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), N, K)
+    y, lim = want(torch, q, s, x)
+    got = product(torch, pib, w, x, "gemm")
+    err = (got.double() - y).abs()
+    assert (err <= lim).all(), float((err / lim).max())
+    for _ in range(3):
+        assert torch.equal(product(torch, pib, w, x, "gemm"), got)
+
+
+@pytest.mark.parametrize("how,b", [("fused", 3), ("gemv", 11), ("gemm", 50)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 0.0])
+def test_one_bad_token(torch, pib, how, b, bad):
+    """an infinity or a number that is none spoils its own token alone; a token of zeros gives zeros"""
+    q, s, g = matrix(torch, 200, 700, 5)
+    x = rows(torch, b, 700, g)
+    if bad == 0.0:
+        x[1] = 0
+    else:
+        x[1, 333] = bad
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), 200, 700)
+    got = product(torch, pib, w, x, how)
+    y, lim = want(torch, q, s, x)
+    others = [t for t in range(b) if t != 1]
+    assert ((got[others].double() - y[others]).abs() <= lim[others]).all()
+    assert (got[1] == 0).all() if bad == 0.0 else torch.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("K,xstride", [(1024, 0), (1000, 1003), (2048, 4096)])
+def test_fused_prologues(torch, pib, K, xstride):
+    lib, b, N = pib.load(), 4, 300
+    q, s, g = matrix(torch, N, K, K)
+    ld = xstride or K
+    x, x2 = torch.randn(b, ld, device="cuda", generator=g), torch.randn(b, ld, device="cuda", generator=g)
+    add, nw = torch.randn(b, K, device="cuda", generator=g), torch.rand(K, device="cuda", generator=g) + 0.5
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), N, K)
+    y, out = torch.empty(b, N, device="cuda"), torch.empty(b, K, device="cuda")
+
+    def close(ref_in):
+        # the prologue's own roundings move a value across an e4m3 border now and then: one step (2^-4 of the value, half of it either way from the border) of one element at a time
+        ref, lim = want(torch, q, s, ref_in.float().contiguous())
+        step = (ref_in.abs().amax(1, keepdim=True) / 448 * 32) * dense(torch, q, s).abs().amax()
+        assert ((y.double() - ref).abs() <= lim + 2 * step).all()
+        assert ((y.double() - ref).abs() <= lim).double().mean() > 0.5
+
+    lib.gemv_fused(w, x.data_ptr(), b, y.data_ptr(), prologue=1, x2=nw.data_ptr(), addend=add.data_ptr(), sum_out=out.data_ptr(), xstride=xstride, eps=1e-6)
+    sm = x[:, :K] + add
+    torch.cuda.synchronize()
+    assert torch.equal(out, sm)
+    close(sm.double() / (sm.double().pow(2).mean(1, keepdim=True) + 1e-6).sqrt() * nw.double())
+    lib.gemv_fused(w, x.data_ptr(), b, y.data_ptr(), prologue=2, x2=x2.data_ptr(), xstride=xstride)
+    close((x.double() / (1 + torch.exp(-x.double())) * x2.double())[:, :K])
+    lib.gemv_fused(w, x.data_ptr(), b, y.data_ptr(), xstride=xstride)
+    ref, lim = want(torch, q, s, x[:, :K].contiguous())
+    torch.cuda.synchronize()
+    assert ((y.double() - ref).abs() <= lim).all()
+
+
+def test_rows_and_host_forms(torch, pib):
+    lib, N, K = pib.load(), 300, 1001
+    q, s, g = matrix(torch, N, K, 9)
+    W = dense(torch, q, s)
+    qh, sh = q.view(torch.uint8).cpu().numpy(), s.cpu().numpy()
+    h = lib.L.pib_weight_upload_f8(qh.ctypes.data, sh.ctypes.data, N, K)
+    assert h and lib.L.pib_weight_bytes(h) == N * K + 4 * sh.size
+    for r in (0, 127, 128, 299):
+        raw = np.zeros(K + 4 * blocks(K), np.uint8)
+        lib.check(lib.L.pib_weight_row_blocks(h, r, raw.ctypes.data))
+        assert np.array_equal(raw[:K], qh[r]) and np.array_equal(raw[K:].copy().view(np.float32), sh[r // 128])
+    ids = [0, 299, 128, 5, 5]
+    assert np.array_equal(lib.get_rows(h, ids, K), W[ids].float().cpu().numpy())
+    for b, fn in ((5, lambda x, y: lib.L.pib_mul_mat_host(h, x.ctypes.data, x.shape[0], y.ctypes.data, 0)), (40, lambda x, y: lib.L.pib_gemm_host(h, x.ctypes.data, x.shape[0], y.ctypes.data))):
+        x = rows(torch, b, K, g)
+        y = np.zeros((b, N), np.float32)
+        lib.check(fn(x.cpu().numpy(), y))
+        ref, lim = want(torch, q, s, x)
+        assert (np.abs(y - ref.cpu().numpy()) <= lim.cpu().numpy()).all()
+    lib.L.pib_weight_free(h)
+
+
+@pytest.mark.parametrize("how,b", [("fused", 2), ("gemv", 9), ("gemm", 70)])
+def test_captured_and_on_another_stream(torch, pib, how, b):
+    """the first call on a stream may be a captured one; replays follow new inputs; a call on a stream is ordered with what is on it"""
+    lib, N, K = pib.load(), 520, 900
+    q, s, g = matrix(torch, N, K, 3)
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), N, K)
+    x, y = rows(torch, b, K, g), torch.zeros(b, N, device="cuda")
+    act = torch.empty(lib.act_bytes(F8, K, b), dtype=torch.uint8, device="cuda")
+
+    def call(stream):
+        if how == "fused":
+            return lib.gemv_fused(w, x.data_ptr(), b, y.data_ptr(), stream)
+        lib.quantize_act_rows(F8, x.data_ptr(), b, K, act.data_ptr(), stream)
+        lib.gemv(w, act.data_ptr(), b, y.data_ptr(), stream) if how == "gemv" else lib.gemm(w, act.data_ptr(), b, y.data_ptr(), None, stream)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        call(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        x.copy_(rows(torch, b, K, g))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, lim = want(torch, q, s, x)
+        assert ((y.double() - ref).abs() <= lim).all()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        x.mul_(0.5)
+        y.zero_()
+        call(torch.cuda.current_stream().cuda_stream)
+        z = y * 2
+    torch.cuda.synchronize()
+    assert ((z.double() - ref).abs() <= lim).all()
