@@ -4,7 +4,8 @@
 //
 // The scales change from block to block, so a block's product is one accumulator in tensor memory (four MMAs of K 32) that is read back, scaled and added up in fp32 registers, while the
 // tensor core works on the next blocks' accumulators (512 / NB of them take turns).
-//   warp 0       streams a block of both operands by TMA (a row's 128 bytes are a line of the 128-byte swizzle) through a ring, and the block's activation scales through a ring of their own
+//   warp 0       streams blocks of both operands by TMA (a row's 128 bytes are a line of the 128-byte swizzle) through a ring
+//   warp 10      streams the blocks' activation scales through a ring of their own
 //   warp 1       issues the MMAs; a commit hands the operands back, another says that the accumulator is there
 //   warps 2..9   two groups of four, half of the columns each: a thread owns a weight row (lane) and adds acc[c] += P[c] (s d[c])
 // The CTAs walk the tiles (128 rows x NB tokens).  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks each and add their sums up through
@@ -17,12 +18,12 @@
 
 #include <algorithm>
 
-#define FT_THREADS 320
+#define FT_THREADS 352
 #define FT_BM      128
 #define FT_A_TILE  (FT_BM * 128)
 #define FT_RING    (192 * 1024)
 #define FT_STAGES  10                       // at most
-#define FT_DRING   8                        // scale rows under way
+#define FT_DRING   8                        // scale rows under way (an even number)
 #define FT_BARS    (2 * FT_STAGES + 2 * FT_DRING + 2 * 16)
 #define FT_SMEM    ((size_t) FT_RING + FT_DRING * 1024 + FT_BARS * 8 + 32 + 1024)
 
@@ -37,6 +38,9 @@ __device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
 }
 __device__ __forceinline__ void ft_tma_2d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void ft_tma_3d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(z) : "memory");
 }
 __device__ __forceinline__ void ft_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -58,7 +62,8 @@ struct ft_args {
 template <int NB>
 __global__ void __launch_bounds__(FT_THREADS, 1)
 f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ ft_args A) {
-    constexpr int STAGE = FT_A_TILE + NB * 128, STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / NB < 8 ? 512 / NB : 8, HALF = NB / 2;
+    // KPS blocks a stage: a copy costs the producer as much as some 10 KB take
+    constexpr int KPS = NB <= 64 ? 2 : 1, STAGE = KPS * (FT_A_TILE + NB * 128), STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / NB < 8 ? 512 / NB : 8, HALF = NB / 2;
     extern __shared__ __align__(1024) uint8_t ft_dsm[];
     uint8_t *  sm  = ft_dsm + ((1024u - (dt_smem(ft_dsm) & 1023u)) & 1023u);
     float *    dsc = reinterpret_cast<float *>(sm + FT_RING);                            // scale rows, 256 floats a place
@@ -68,6 +73,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FT_STAGES * 8, bar_d = bar_e + FT_STAGES * 8, bar_g = bar_d + FT_DRING * 8, bar_t = bar_g + FT_DRING * 8, bar_r = bar_t + 16 * 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = A.shares, share = S > 1 ? (int) ft_rank() : 0;
     const int unit = blockIdx.x / S, units = gridDim.x / S;
+    const int tile0 = (int) ((int64_t) A.tiles * unit / units), tile1 = (int) ((int64_t) A.tiles * (unit + 1) / units);
     const int k0 = (int) ((int64_t) A.KB * share / S), nk = (int) ((int64_t) A.KB * (share + 1) / S) - k0;
     const uint32_t sm0 = dt_smem(sm);
 
@@ -91,40 +97,53 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     bool ok = true;
 
     if (warp == 0) {
-        int s = 0, ds = 0;
-        uint32_t ph = 1, dph = 1;                                // the first round finds its places free
-        for (int tile = unit; tile < A.tiles && ok; tile += units) {
-            const int n0 = tile / A.tiles_m * FT_BM, m0 = tile % A.tiles_m * NB;
+        int s = 0;
+        uint32_t ph = 1;                                         // the first round finds its places free
+        for (int tile = tile0; tile < tile1 && ok && lane == 0; tile++) {
+            const int n_tile = tile / A.tiles_m, m0 = tile % A.tiles_m * NB;
+            for (int kt = 0; kt < nk; kt += KPS) {
+                ok = dt_mbar_wait(bar_e + s * 8, ph, abort_s);
+                if (!ok) break;
+                // what a share's last copy takes of the next blocks is not used
+                dt_mbar_expect_tx(bar_f + s * 8, STAGE);
+                ft_tma_2d(sm0 + s * STAGE, &wmap, bar_f + s * 8, 0, (n_tile * A.KB + k0 + kt) * 128);
+                ft_tma_3d(sm0 + s * STAGE + KPS * FT_A_TILE, &xmap, bar_f + s * 8, m0, k0 + kt);
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        int ds = 0;
+        uint32_t dph = 1;
+        for (int tile = tile0; tile < tile1 && ok && lane == 0; tile++) {
+            const int m0 = tile % A.tiles_m * NB;
             const uint32_t dbytes = (uint32_t) min(NB, A.bp - m0) * 4;
             for (int kt = 0; kt < nk; kt++) {
-                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_e + s * 8, ph, abort_s) && dt_mbar_wait(bar_g + ds * 8, dph, abort_s));
+                ok = dt_mbar_wait(bar_g + ds * 8, dph, abort_s);
                 if (!ok) break;
-                if (lane == 0) {
-                    dt_mbar_expect_tx(bar_f + s * 8, STAGE);
-                    ft_tma_2d(sm0 + s * STAGE, &wmap, bar_f + s * 8, (k0 + kt) * 128, n0);
-                    ft_tma_2d(sm0 + s * STAGE + FT_A_TILE, &xmap, bar_f + s * 8, (k0 + kt) * 128, m0);
-                    dt_mbar_expect_tx(bar_d + ds * 8, dbytes);
-                    ft_bulk(dt_smem(dsc + ds * 256), A.ad + (int64_t) (k0 + kt) * A.bp + m0, dbytes, bar_d + ds * 8);
-                }
-                __syncwarp();
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                dt_mbar_expect_tx(bar_d + ds * 8, dbytes);
+                ft_bulk(dt_smem(dsc + ds * 256), A.ad + (int64_t) (k0 + kt) * A.bp + m0, dbytes, bar_d + ds * 8);
                 if (++ds == FT_DRING) { ds = 0; dph ^= 1; }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         const uint64_t d0 = dt_desc(sm0);
         int s = 0, a = 0;
         uint32_t ph = 0, aph = 1;
-        for (int tile = unit; tile < A.tiles && ok; tile += units)
+        for (int tile = tile0; tile < tile1 && ok; tile++)
             for (int kt = 0; kt < nk; kt++) {
-                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && dt_mbar_wait(bar_f + s * 8, ph, abort_s));
+                const int j = kt % KPS;
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && (j || dt_mbar_wait(bar_f + s * 8, ph, abort_s)));
                 if (!ok) break;
                 dt_fence_after();
-                const uint64_t ad = d0 + (uint64_t) (s * STAGE >> 4);
-                ft_mma(tmem + a * NB, ad, ad + (FT_A_TILE >> 4), ft_idesc(FT_BM, NB));
-                dt_commit(bar_e + s * 8);
+                const uint64_t ad = d0 + (uint64_t) ((s * STAGE + j * FT_A_TILE) >> 4), bd = d0 + (uint64_t) ((s * STAGE + KPS * FT_A_TILE + j * NB * 128) >> 4);
+                ft_mma(tmem + a * NB, ad, bd, ft_idesc(FT_BM, NB));
                 dt_commit(bar_t + a * 8);
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (j == KPS - 1 || kt == nk - 1) {
+                    dt_commit(bar_e + s * 8);
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                }
                 if (++a == ACCS) { a = 0; aph ^= 1; }
             }
     } else {
@@ -133,7 +152,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         float acc[HALF];
         int a = 0, ds = 0;
         uint32_t aph = 0, dph = 0;
-        for (int tile = unit; tile < A.tiles && ok; tile += units) {
+        for (int tile = tile0; tile < tile1 && ok; tile++) {
             const int64_t n = (int64_t) (tile / A.tiles_m) * FT_BM + q4 * 32 + lane;
             const int m0 = tile % A.tiles_m * NB + hf * HALF;
             const float * ws = A.ws + (int64_t) (tile / A.tiles_m) * A.KB + k0;
@@ -187,7 +206,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     __syncwarp();
     if (S > 1) {
         ft_cluster_sync();
-        if (warp >= 2 && !*abort_s) {
+        if (warp >= 2 && warp < 10 && !*abort_s) {
             const int q4 = warp & 3, hf = (warp - 2) >> 2;
             const int64_t n = (int64_t) (unit / A.tiles_m) * FT_BM + q4 * 32 + lane;
             const int m0 = unit % A.tiles_m * NB;
@@ -226,16 +245,29 @@ static ft_encode_fn ft_encode() {
     }();
     return fn;
 }
-// rows of Kp bytes, boxes of 128 bytes x `box` rows, 128-byte swizzle
-static int ft_map(CUtensorMap * map, const void * base, int64_t Kp, int64_t rows, int box) {
+static int ft_map(CUtensorMap * map, const void * base, int dims, const cuuint64_t * size, const cuuint64_t * stride, const cuuint32_t * box) {
     ft_encode_fn enc = ft_encode();
     if (!enc) { pib_set_error("tensor map: cuTensorMapEncodeTiled not available"); return PIB_ERR_UNSUPP; }
-    const cuuint64_t gdim[2] = { (cuuint64_t) Kp, (cuuint64_t) rows }, gstr[1] = { (cuuint64_t) Kp };
-    const cuuint32_t bx[2] = { 128, (cuuint32_t) box }, es[2] = { 1, 1 };
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint32_t es[4] = { 1, 1, 1, 1 };
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t) dims, const_cast<void *>(base), size, stride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { pib_set_error("tensor map: cuTensorMapEncodeTiled failed (%d)", (int) r); return PIB_ERR_UNSUPP; }
     return PIB_OK;
+}
+int pib_f8_map(CUtensorMap * map, const void * base, int64_t rows, int box) {
+    const cuuint64_t size[2] = { 128, (cuuint64_t) rows }, stride[1] = { 128 };
+    const cuuint32_t bx[2] = { 128, (cuuint32_t) box };
+    return ft_map(map, base, 2, size, stride, bx);
+}
+int pib_f8_map3(CUtensorMap * map, const void * base, int64_t rows, int64_t groups, int64_t group_bytes, int box_rows, int box_groups) {
+    const cuuint64_t size[3] = { 128, (cuuint64_t) rows, (cuuint64_t) groups }, stride[2] = { 128, (cuuint64_t) group_bytes };
+    const cuuint32_t bx[3] = { 128, (cuuint32_t) box_rows, (cuuint32_t) box_groups };
+    return ft_map(map, base, 3, size, stride, bx);
+}
+int pib_f8_map4(CUtensorMap * map, const void * base, int64_t KB, int64_t NB, int box_rows, int box_kb) {
+    const cuuint64_t size[4] = { 128, 128, (cuuint64_t) KB, (cuuint64_t) NB }, stride[3] = { 128, 128 * 128, (cuuint64_t) KB * 128 * 128 };
+    const cuuint32_t bx[4] = { 128, (cuuint32_t) box_rows, (cuuint32_t) box_kb, 1 };
+    return ft_map(map, base, 4, size, stride, bx);
 }
 
 template <int NB> static int ft_launch(const CUtensorMap & wmap, const CUtensorMap & xmap, ft_args A, cudaStream_t st) {
@@ -263,7 +295,7 @@ int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     while (A.shares < 8 && A.tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
     if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
     CUtensorMap wmap, xmap;
-    if ((rc = ft_map(&wmap, w->qs, L.Kp, pib_f8_blocks(w->N) * PIB_F8_BLOCK, FT_BM)) != PIB_OK || (rc = ft_map(&xmap, act, L.Kp, b, NB)) != PIB_OK) return rc;
+    if ((rc = pib_f8_map(&wmap, w->qs, pib_f8_blocks(w->N) * L.Kp, FT_BM * (NB <= 64 ? 2 : 1))) != PIB_OK || (rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, NB, NB <= 64 ? 2 : 1)) != PIB_OK) return rc;
     switch (NB) {
         case 32:  return ft_launch<32>(wmap, xmap, A, st);
         case 64:  return ft_launch<64>(wmap, xmap, A, st);

@@ -13,12 +13,13 @@ static __global__ void f8_pad_kernel(const uint8_t * __restrict__ src, uint8_t *
         __align__(16) uint8_t v[16];
 #pragma unroll
         for (int j = 0; j < 16; j++) v[j] = r0 + r < N && k + j < K ? src[r * K + k + j] : 0;
-        *reinterpret_cast<int4 *>(dst + (r0 + r) * Kp + k) = *reinterpret_cast<const int4 *>(v);
+        *reinterpret_cast<int4 *>(dst + pib_f8_at(r0 + r, k, Kp >> 7)) = *reinterpret_cast<const int4 *>(v);
     }
 }
 
 static pib_weight * f8_alloc(int64_t N, int64_t K) {
-    if (N <= 0 || K <= 0 || N > 0x7fffff00 || K > 0x7fffff00) {
+    // the rows of 128 bytes are counted in 32 bits
+    if (N <= 0 || K <= 0 || N > 0x7fffff00 || K > 0x7fffff00 || pib_f8_blocks(N) * pib_f8_blocks(K) > 0x7fffffff / PIB_F8_BLOCK) {
         pib_set_error("pib_weight: bad shape %lld x %lld", (long long) N, (long long) K);
         return nullptr;
     }
@@ -84,7 +85,9 @@ extern "C" pib_weight * pib_weight_upload_f8(const void * q_host, const float * 
 
 int pib_f8_row(const pib_weight * w, int64_t row, void * out) {
     const int64_t KB = pib_f8_blocks(w->K);
-    PIB_CHECK(cudaMemcpy(out, w->qs + row * KB * PIB_F8_BLOCK, (size_t) w->K, cudaMemcpyDeviceToHost));
+    const size_t  full = (size_t) (w->K / PIB_F8_BLOCK), tail = (size_t) (w->K % PIB_F8_BLOCK);
+    if (full) PIB_CHECK(cudaMemcpy2D(out, PIB_F8_BLOCK, w->qs + pib_f8_at(row, 0, KB), PIB_F8_BLOCK * PIB_F8_BLOCK, PIB_F8_BLOCK, full, cudaMemcpyDeviceToHost));
+    if (tail) PIB_CHECK(cudaMemcpy((uint8_t *) out + full * PIB_F8_BLOCK, w->qs + pib_f8_at(row, (int64_t) full * PIB_F8_BLOCK, KB), tail, cudaMemcpyDeviceToHost));
     PIB_CHECK(cudaMemcpy((uint8_t *) out + w->K, (const float *) w->d + row / PIB_F8_BLOCK * KB, (size_t) KB * 4, cudaMemcpyDeviceToHost));
     return PIB_OK;
 }
@@ -96,7 +99,7 @@ static __global__ void f8_rows_kernel(const uint8_t * __restrict__ qs, const flo
     pib_pdl_trigger();
     const int64_t row = ids[blockIdx.x];
     for (int64_t k = (int64_t) blockIdx.y * blockDim.x + threadIdx.x; k < K; k += (int64_t) gridDim.y * blockDim.x)
-        out[(int64_t) blockIdx.x * K + k] = __fmul_rn(f8_value(qs[row * KB * PIB_F8_BLOCK + k]), d[row / PIB_F8_BLOCK * KB + k / PIB_F8_BLOCK]);
+        out[(int64_t) blockIdx.x * K + k] = __fmul_rn(f8_value(qs[pib_f8_at(row, k, KB)]), d[row / PIB_F8_BLOCK * KB + k / PIB_F8_BLOCK]);
 }
 
 int pib_f8_get_rows(const pib_weight * w, const int32_t * ids, int n, float * out, cudaStream_t st) {
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(256) f8_quant_kernel(const float * __restrict_
                     if (xnorm) xnorm[row * K + k + j] = v[j];
                 }
         const float s = f8_scale(warp_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))));
-        reinterpret_cast<uint32_t *>(qs)[u * 32 + lane] = f8_pack4(v[0], v[1], v[2], v[3], s);
+        reinterpret_cast<uint32_t *>(qs)[(kb * b + row) * 32 + lane] = f8_pack4(v[0], v[1], v[2], v[3], s);
         if (lane == 0) d[kb * bp + row] = s;
     }
 }
@@ -178,7 +181,7 @@ int pib_f8_act_blocks(const void * act_dev, int b, int64_t K, void * out) {
     for (int64_t t = 0; t < b; t++)
         for (int64_t kb = 0; kb < A.KB; kb++, o += 4 + PIB_F8_BLOCK) {
             memcpy(o, h + A.d_off + (size_t) (kb * A.bp + t) * 4, 4);
-            memcpy(o + 4, h + (size_t) t * A.Kp + kb * PIB_F8_BLOCK, PIB_F8_BLOCK);
+            memcpy(o + 4, h + (size_t) (kb * b + t) * PIB_F8_BLOCK, PIB_F8_BLOCK);
         }
     free(h);
     return PIB_OK;
