@@ -35,6 +35,7 @@ int pib_f8_get_rows(const pib_weight * w, const int32_t * ids, int n, float * ou
 int pib_f8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st);
 int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st);
 int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st);
+int pib_f8_gemm_pair(const pib_weight * w, const void * act, int b, float * y, int * err, cudaStream_t st);
 int pib_f8_gemm_host(const pib_weight * w, const float * x_host, int b, float * y_host);
 int pib_f8_map(CUtensorMap * map, const void * base, int64_t rows, int box);                   // f8_gemm.cu: rows of 128 bytes, boxes of `box` rows, 128-byte swizzle (these three)
 int pib_f8_map3(CUtensorMap * map, const void * base, int64_t rows, int64_t groups, int64_t group_bytes, int box_rows, int box_groups);      // groups of rows of 128 bytes

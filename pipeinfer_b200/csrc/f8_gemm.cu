@@ -1,9 +1,9 @@
-// f8_gemm.cu -- 8-bit floating point weights with block scales times any number of tokens on tcgen05 (kind::f8f6f4), fp32 accumulation.
+// f8_gemm.cu -- 8-bit floating point weights with block scales times up to 128 tokens (f8_gemm_pair.cu beyond) on tcgen05 (kind::f8f6f4), fp32 accumulation.
 //
 //   y[t][n] = sum over kb of (s[n/128][kb] d[kb][t]) P_kb[n][t],  P_kb = the product of the block's 128 columns
 //
 // The scales change from block to block, so a block's product is one accumulator in tensor memory (four MMAs of K 32) that is read back, scaled and added up in fp32 registers, while the
-// tensor core works on the next blocks' accumulators (512 / NB of them take turns).
+// tensor core works on the next blocks' accumulators.
 //   warp 0       streams blocks of both operands by TMA (a row's 128 bytes are a line of the 128-byte swizzle) through a ring
 //   warp 10      streams the blocks' activation scales through a ring of their own
 //   warp 1       issues the MMAs; a commit hands the operands back, another says that the accumulator is there
@@ -23,9 +23,10 @@
 #define FT_A_TILE  (FT_BM * 128)
 #define FT_RING    (192 * 1024)
 #define FT_STAGES  10                       // at most
-#define FT_DRING   8                        // scale rows under way (an even number)
+#define FT_KPS     2                        // blocks of a stage, and of a hand-over between the warps: fewer and larger ones (57344 x 8192, 4 tokens: 133 us with 1, 89 with 2)
+#define FT_DRING   8                        // stages whose scale rows are under way
 #define FT_BARS    (2 * FT_STAGES + 2 * FT_DRING + 2 * 16)
-#define FT_SMEM    ((size_t) FT_RING + FT_DRING * 1024 + FT_BARS * 8 + 32 + 1024)
+#define FT_SMEM    ((size_t) FT_RING + FT_DRING * FT_KPS * 512 + FT_BARS * 8 + 32 + 1024)
 
 __device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
     // a block: four MMAs of K 32, 32 bytes further along both operands each; the first one starts the accumulator
@@ -62,12 +63,11 @@ struct ft_args {
 template <int NB>
 __global__ void __launch_bounds__(FT_THREADS, 1)
 f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ ft_args A) {
-    // KPS blocks a stage: a copy costs the producer as much as some 10 KB take
-    constexpr int KPS = NB <= 64 ? 2 : 1, STAGE = KPS * (FT_A_TILE + NB * 128), STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / NB < 8 ? 512 / NB : 8, HALF = NB / 2;
+    constexpr int KPS = FT_KPS, STAGE = KPS * (FT_A_TILE + NB * 128), STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / (KPS * NB), HALF = NB / 2;
     extern __shared__ __align__(1024) uint8_t ft_dsm[];
     uint8_t *  sm  = ft_dsm + ((1024u - (dt_smem(ft_dsm) & 1023u)) & 1023u);
-    float *    dsc = reinterpret_cast<float *>(sm + FT_RING);                            // scale rows, 256 floats a place
-    uint64_t * bar = reinterpret_cast<uint64_t *>(sm + FT_RING + FT_DRING * 1024);       // operands there / read, scales there / read, accumulator there / read
+    float *    dsc = reinterpret_cast<float *>(sm + FT_RING);                            // scale rows, KPS of 128 floats a place
+    uint64_t * bar = reinterpret_cast<uint64_t *>(sm + FT_RING + FT_DRING * FT_KPS * 512);       // operands there / read, scales there / read, accumulator there / read
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + FT_BARS);
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FT_STAGES * 8, bar_d = bar_e + FT_STAGES * 8, bar_g = bar_d + FT_DRING * 8, bar_t = bar_g + FT_DRING * 8, bar_r = bar_t + 16 * 8;
@@ -118,11 +118,12 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         for (int tile = tile0; tile < tile1 && ok && lane == 0; tile++) {
             const int m0 = tile % A.tiles_m * NB;
             const uint32_t dbytes = (uint32_t) min(NB, A.bp - m0) * 4;
-            for (int kt = 0; kt < nk; kt++) {
+            for (int kt = 0; kt < nk; kt += KPS) {
                 ok = dt_mbar_wait(bar_g + ds * 8, dph, abort_s);
                 if (!ok) break;
-                dt_mbar_expect_tx(bar_d + ds * 8, dbytes);
-                ft_bulk(dt_smem(dsc + ds * 256), A.ad + (int64_t) (k0 + kt) * A.bp + m0, dbytes, bar_d + ds * 8);
+                const int n = min(KPS, nk - kt);
+                dt_mbar_expect_tx(bar_d + ds * 8, n * dbytes);
+                for (int j = 0; j < n; j++) ft_bulk(dt_smem(dsc + (ds * KPS + j) * 128), A.ad + (int64_t) (k0 + kt + j) * A.bp + m0, dbytes, bar_d + ds * 8);
                 if (++ds == FT_DRING) { ds = 0; dph ^= 1; }
             }
         }
@@ -132,18 +133,18 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         int s = 0, a = 0;
         uint32_t ph = 0, aph = 1;
         for (int tile = tile0; tile < tile1 && ok; tile++)
-            for (int kt = 0; kt < nk; kt++) {
-                const int j = kt % KPS;
-                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && (j || dt_mbar_wait(bar_f + s * 8, ph, abort_s)));
+            for (int kt = 0; kt < nk; kt += KPS) {
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && dt_mbar_wait(bar_f + s * 8, ph, abort_s));
                 if (!ok) break;
                 dt_fence_after();
-                const uint64_t ad = d0 + (uint64_t) ((s * STAGE + j * FT_A_TILE) >> 4), bd = d0 + (uint64_t) ((s * STAGE + KPS * FT_A_TILE + j * NB * 128) >> 4);
-                ft_mma(tmem + a * NB, ad, bd, ft_idesc(FT_BM, NB));
-                dt_commit(bar_t + a * 8);
-                if (j == KPS - 1 || kt == nk - 1) {
-                    dt_commit(bar_e + s * 8);
-                    if (++s == STAGES) { s = 0; ph ^= 1; }
+#pragma unroll
+                for (int j = 0; j < KPS; j++) {
+                    const uint64_t ad = d0 + (uint64_t) ((s * STAGE + j * FT_A_TILE) >> 4), bd = d0 + (uint64_t) ((s * STAGE + KPS * FT_A_TILE + j * NB * 128) >> 4);
+                    if (kt + j < nk) ft_mma(tmem + (a * KPS + j) * NB, ad, bd, ft_idesc(FT_BM, NB));
                 }
+                dt_commit(bar_t + a * 8);
+                dt_commit(bar_e + s * 8);
+                if (++s == STAGES) { s = 0; ph ^= 1; }
                 if (++a == ACCS) { a = 0; aph ^= 1; }
             }
     } else {
@@ -158,30 +159,37 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             const float * ws = A.ws + (int64_t) (tile / A.tiles_m) * A.KB + k0;
 #pragma unroll
             for (int c = 0; c < HALF; c++) acc[c] = 0.f;
-            for (int kt = 0; kt < nk; kt++) {
-                const float w = __ldg(ws + kt);
+            for (int kt = 0; kt < nk; kt += KPS) {
+                float w[KPS];
+#pragma unroll
+                for (int j = 0; j < KPS; j++) w[j] = kt + j < nk ? __ldg(ws + kt + j) : 0.f;
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_d + ds * 8, dph, abort_s) && dt_mbar_wait(bar_t + a * 8, aph, abort_s));
                 if (!ok) break;
                 dt_fence_after();
-                const float4 * dv = reinterpret_cast<const float4 *>(dsc + ds * 256 + hf * HALF);
                 constexpr int STEP = HALF < 32 ? HALF : 32;
 #pragma unroll
-                for (int c0 = 0; c0 < HALF; c0 += STEP) {
-                    uint32_t v[32];
-                    if (STEP == 32) dt_ld32(tmem + lanes + a * NB + hf * HALF + c0, v);
-                    else {
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                                       "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(tmem + lanes + a * NB + hf * HALF + c0) : "memory");
-                    }
-                    dt_wait_ld();
+                for (int j = 0; j < KPS; j++) {
+                    if (kt + j >= nk) break;
+                    const float4 * dv = reinterpret_cast<const float4 *>(dsc + (ds * KPS + j) * 128 + hf * HALF);
+                    const uint32_t at = tmem + lanes + (a * KPS + j) * NB + hf * HALF;
 #pragma unroll
-                    for (int c = 0; c < STEP; c += 4) {
-                        const float4 d = dv[(c0 + c) / 4];
-                        acc[c0 + c]     = fmaf(__uint_as_float(v[c]), w * d.x, acc[c0 + c]);
-                        acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), w * d.y, acc[c0 + c + 1]);
-                        acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), w * d.z, acc[c0 + c + 2]);
-                        acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), w * d.w, acc[c0 + c + 3]);
+                    for (int c0 = 0; c0 < HALF; c0 += STEP) {
+                        uint32_t v[32];
+                        if (STEP == 32) dt_ld32(at + c0, v);
+                        else {
+                            asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                                           "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at + c0) : "memory");
+                        }
+                        dt_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < STEP; c += 4) {
+                            const float4 d = dv[(c0 + c) / 4];
+                            acc[c0 + c]     = fmaf(__uint_as_float(v[c]), w[j] * d.x, acc[c0 + c]);
+                            acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), w[j] * d.y, acc[c0 + c + 1]);
+                            acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), w[j] * d.z, acc[c0 + c + 2]);
+                            acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), w[j] * d.w, acc[c0 + c + 3]);
+                        }
                     }
                 }
                 dt_fence_before();
@@ -283,7 +291,10 @@ int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     if (rc != PIB_OK) return rc;
     if ((uintptr_t) act & 15) { pib_set_error("pib_gemm: act_dev needs 16-byte alignment"); return PIB_ERR_ARG; }
     const pib_f8_act L = pib_f8_act_of(w->K, b);
-    const int NB = b <= 32 ? 32 : b <= 64 ? 64 : b <= 128 ? 128 : 256;
+    int * err = pib_tc_error_word(st);
+    if (!err) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
+    if (b > 128) return pib_f8_gemm_pair(w, act, b, y, err, st);
+    const int NB = b <= 32 ? 32 : b <= 64 ? 64 : 128;
     ft_args A;
     A.b = b; A.KB = L.KB; A.bp = L.bp; A.N = w->N; A.y = y;
     A.ws = (const float *) w->d; A.ad = (const float *) ((const uint8_t *) act + L.d_off);
@@ -293,13 +304,12 @@ int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     A.tiles = (int) tiles;
     A.shares = 1;
     while (A.shares < 8 && A.tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
-    if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
+    A.err = err;
     CUtensorMap wmap, xmap;
-    if ((rc = pib_f8_map(&wmap, w->qs, pib_f8_blocks(w->N) * L.Kp, FT_BM * (NB <= 64 ? 2 : 1))) != PIB_OK || (rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, NB, NB <= 64 ? 2 : 1)) != PIB_OK) return rc;
+    if ((rc = pib_f8_map(&wmap, w->qs, pib_f8_blocks(w->N) * L.Kp, FT_BM * FT_KPS)) != PIB_OK || (rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, NB, FT_KPS)) != PIB_OK) return rc;
     switch (NB) {
         case 32:  return ft_launch<32>(wmap, xmap, A, st);
         case 64:  return ft_launch<64>(wmap, xmap, A, st);
-        case 128: return ft_launch<128>(wmap, xmap, A, st);
-        default:  return ft_launch<256>(wmap, xmap, A, st);
+        default:  return ft_launch<128>(wmap, xmap, A, st);
     }
 }
