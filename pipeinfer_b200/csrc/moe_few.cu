@@ -2,67 +2,146 @@
 //
 //   z = R x;  chosen: the `top` largest score + correction;  h_e = silu(G_e x) * U_e x;  y = residual + sum_e w_e D_e h_e   (shared experts: w = 1)
 //
-// moe_logits_kernel   a block per router output, all tokens; also clears the counters of the second launch
+// moe_logits_kernel   a block per router output, all tokens; one per token that splits its row into parts (below); also clears the counters of the second launch
 // moe_few_kernel      every block chooses the experts by itself (fewer steps than sharing the choice would take), then takes items by ticket: first the up items (expert, 16 gate rows and
 //                     their 16 up rows), behind them the down items (expert, 32 output rows).  A down item waits for its expert's up items, which have lower tickets: whoever holds one is running
 //                     and waits for nothing behind it, so the waits end however few blocks the GPU runs at a time.  The block that finishes the last expert of 32 output rows
 //                     adds the experts up, in the order of the token's choices: no sum depends on which block came first.
 //
-// Products: mma.m16n8k16, expert rows as M, the expert's tokens as N.  Weights enter exactly: e4m3 as fp16 (times the block's scale in fp32 behind the block's sum), bfloat16 as it
-// is.  The fp32 activations enter as parts: two fp16 (of the block's values times a power of two that brings the largest to 2^14 .. 2^15: 22 bits) with e4m3 weights, three bfloat16 (24
-// bits) with bfloat16 ones; a line of 128 bytes of a weight row is summed by the tensor core and then added up in fp32.  Lane t of a row takes 16 neighbouring bytes of 64 (f8_gemv.cu).
+//   producer warp     takes the tickets and streams the items' rows in pieces of up to 24 KB (6 lines of 128 bytes of 32 rows, in one piece of memory) through a ring that runs on across
+//                     items, a down item's weights ahead of its wait
+//   six consumer warps take a line of a piece each and meet in shared memory at the item's end, in warp order
+//   publisher warp    makes an item's results known to the other blocks and adds up finished rows: fences and atomics that the consumers would stand still for
+//
+// Products: mma.m16n8k16, expert rows as M, the expert's tokens as N.  Weights enter exactly: e4m3 as fp16 (times the block's scale in fp32 behind the sum), bfloat16 as it is.  The fp32
+// activations enter as parts: with e4m3 weights two fp16 of the row times a power of two that brings its largest to 2^14 .. 2^15 (22 bits, to 2^-39 of the largest), with bfloat16 weights
+// three bfloat16 (24 bits).  (h is split where it is made, before the rest of its row is there: its power of two brings a bound of the row, the largest norms of the expert's gate and up
+// rows times the token's squared norm, to 2^14 .. 2^15; the bound lies some 2^9 above the largest, which leaves 2^-31 of it.)  Half a line's sums are made by the tensor core, scaled and added up in fp32.  Four tokens' two parts (eight tokens' one of three) share
+// the eight columns of one MMA; an expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which
+// costs less than a second form of the kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
+// a row (lane t) are four values each of four (two) neighbouring tiles of 16, the k of an MMA, and the parts lie in that order too.
+// What bounds it: ??
 #include <cuda_bf16.h>
 
 #include "f8_block.cuh"
-#include "hybrid.cuh"
+#include "tc_common.cuh"
 
 #include <algorithm>
 
-#define MF_WARPS 8
-#define MF_SPIN  (1u << 22)
+#define MF_WARPS   6                          // consumers; with the producer and the publisher eight warps, and 128 registers a thread in two blocks per SM
+#define MF_THREADS (MF_WARPS * 32 + 64)
+#define MF_SPIN    (1u << 22)
+#define MF_LINE    4096                       // 128 bytes of 32 rows
+#define MF_STAGE   (MF_WARPS * MF_LINE)
+#define MF_STAGES  3
+#define mf_bar()   asm volatile("bar.sync 1, 192;" ::: "memory")          // the consumers
 
 struct pib_moe {
     pib_moe_shape s;
     int   dev, KB1, KB2, T1, T2;         // lines of 128 bytes in a row of W1, W2; up and down items of an expert
     uint8_t * base;
     float * router, * corr;              // corr: null without a correction
-    uint8_t * w1, * w2;                  // [experts + shared][T1][16 gate rows, 16 up rows][KB1 * 128 bytes], [..][T2 * 32 rows][KB2 * 128 bytes], zero behind the matrices
+    uint8_t * w1, * w2;                  // [experts + shared][T1][KB1][16 gate rows, 16 up rows][128 bytes], [..][T2][KB2][32 rows][128 bytes], zero behind the matrices; the 16-byte pieces of a row
+                                         // lie at their number xor (row & 7): lanes of neighbouring rows read different banks
     float * s1, * s2;                    // F8: [..][gate, up][rows / 128][KB1], [..][rows / 128][KB2]
+    float * norms;                       // [..][gate, up]: the largest squared norm of a row
 };
 struct mf_args {
-    int b, E, shared, top, score, renorm, has_corr, T1, T2, KB1, KB2, nb1, nb2, vec;
+    int b, E, shared, top, score, renorm, has_corr, T1, T2, KB1, KB2, nb1, nb2;
     float scale;
-    int64_t D, F, Fk, Dr;
+    int64_t D, Dr;
     const float * corr, * z;
     const uint8_t * w1, * w2;
     const float * s1, * s2;
-    const float * x, * res; int64_t ldx, ldr, ldy;
-    float * y, * h, * part;
-    int * cnt, * err;                    // cnt: ticket, abort, up items done per active expert, experts done per 32 output rows
+    const float * res; int64_t ldr, ldy;
+    const uint16_t * xp; const float * xm;                   // parts of the tokens' rows, their largest |x| and squared norm
+    uint16_t * hp;                                           // parts of the pairs' rows of h
+    const float * norms;
+    float * y, * part;
+    int * cnt, * err;                    // cnt: ticket, abort, up items done per entry of the list, entries done per 32 output rows
 };
-struct mf_layout { size_t z, h, part, total; int64_t Fk, Dr; int n_cnt; };
+struct mf_layout { size_t z, xm, xp, hp, part, total; int64_t Dr; int n_cnt; };
+// a row's parts: [part][line][lane t][tile of the line][4] 16-bit numbers; 64 (F8) or 32 bytes per line, part and lane
+__host__ __device__ static inline int64_t mf_row_of(bool f8, int KB) { return (int64_t) KB * (f8 ? 2 * 128 : 3 * 64); }
 static mf_layout mf_of(const pib_moe * m, int b) {
     const int64_t P = (int64_t) b * (m->s.top + m->s.shared);
+    const bool    f8 = m->s.type == PIB_TYPE_F8;
     auto al = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     mf_layout L;
-    L.Fk = (m->s.ff + 15) / 16 * 16; L.Dr = (int64_t) m->T2 * 32;
-    L.n_cnt = 2 + m->s.experts + m->s.shared + m->T2;
-    L.z = al((size_t) L.n_cnt * 4);
-    L.h = L.z + al((size_t) b * m->s.experts * 4);
-    L.part = L.h + al((size_t) (P * L.Fk) * 4);
+    L.Dr = (int64_t) m->T2 * 32;
+    L.n_cnt = 2 + (int) P + m->T2;
+    L.xm = al((size_t) L.n_cnt * 4);
+    L.z = L.xm + al((size_t) b * 8);
+    L.xp = L.z + al((size_t) b * m->s.experts * 4);
+    L.hp = L.xp + al((size_t) (b * mf_row_of(f8, m->KB1)) * 2);
+    L.part = L.hp + al((size_t) (P * mf_row_of(f8, m->KB2)) * 2);
     L.total = L.part + al((size_t) (P * L.Dr) * 4);
     return L;
 }
 
-// ---- router logits ------------------------------------------------------------------------------------------------------------------
-template <int NT> __global__ void __launch_bounds__(256) moe_logits_kernel(const float * __restrict__ R, const float * __restrict__ x, int64_t ldx, int b, int E, int64_t D, int vec, float * __restrict__ z,
-                                                                           int * __restrict__ cnt, int n_cnt) {
+__device__ __forceinline__ void mf_mma_h(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mf_mma_b(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two e4m3 as two fp16, exact
+__device__ __forceinline__ uint32_t mf_half2(uint32_t q, int hi) {
+    uint32_t h;
+    asm volatile("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short) (hi ? q >> 16 : q)));
+    return h;
+}
+// the exponent field of the power of two that brings a number to 2^14 .. 2^15; 254 less it is the inverse's
+__device__ __forceinline__ int mf_exponent(float v) { return min(253, 268 - (__float_as_int(v) >> 23 & 255)); }
+__device__ __forceinline__ float mf_pow2(int field) { return __uint_as_float((uint32_t) field << 23); }
+// parts of value v times `up` (F8), to place r of tile `tile` of a row
+template <bool F8> __device__ __forceinline__ void mf_store(float v, float up, int tile, int r, int KB, uint16_t * row) {
+    constexpr int Q = F8 ? 8 : 4;
+    const int plane = KB * Q * 16, at = ((tile / Q * 4 + (r >> 2)) * Q + tile % Q) * 4 + (r & 3);
+    if (F8) {
+        const float  p  = v * up;
+        const __half hi = __float2half_rn(p), lo = __float2half_rn(p - __half2float(hi));
+        __stcg(row + at, __half_as_ushort(hi));
+        __stcg(row + plane + at, __half_as_ushort(lo));
+    } else {
+#pragma unroll
+        for (int part = 0; part < 3; part++) {
+            const __nv_bfloat16 h = __float2bfloat16_rn(v);
+            v -= __bfloat162float(h);
+            __stcg(row + part * plane + at, __bfloat16_as_ushort(h));
+        }
+    }
+}
+
+// ---- router logits, parts of the tokens ---------------------------------------------------------------------------------------------
+template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_kernel(const float * __restrict__ R, const float * __restrict__ x, int64_t ldx, int b, int E, int64_t D, int vec,
+                                                                                    float * __restrict__ z, int * __restrict__ cnt, int n_cnt, int KB, uint16_t * __restrict__ xp, float * __restrict__ xm) {
     __shared__ float red[8][NT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float * r = R + (int64_t) blockIdx.x * D;
     pib_pdl_wait();
     pib_pdl_trigger();
     if (blockIdx.x == 0) for (int i = threadIdx.x; i < n_cnt; i += 256) cnt[i] = 0;
+    if (blockIdx.x >= E) {
+        const int t = blockIdx.x - E;
+        float up = 1.f;
+        if (F8) {
+            __shared__ float sq[8];
+            float m = 0.f, n = 0.f;
+            for (int64_t k = threadIdx.x; k < D; k += 256) { const float v = x[t * ldx + k]; m = fmaxf(m, fabsf(v)); n = fmaf(v, v, n); }
+            m = warp_max(m); n = warp_sum(n);
+            if (lane == 0) { red[warp][0] = m; sq[warp] = n; }
+            __syncthreads();
+            n = 0.f;
+            for (int i = 0; i < 8; i++) { m = fmaxf(m, red[i][0]); n += sq[i]; }
+            up = mf_pow2(mf_exponent(m));
+            if (threadIdx.x == 0) { xm[2 * t] = m; xm[2 * t + 1] = n; }
+        }
+        for (int u = threadIdx.x; u < KB * (F8 ? 128 : 64); u += 256) mf_store<F8>(u < D ? x[t * ldx + u] : 0.f, up, u >> 4, u & 15, KB, xp + t * mf_row_of(F8, KB));
+        return;
+    }
+    const float * r = R + (int64_t) blockIdx.x * D;
     float acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = 0.f;
@@ -97,328 +176,408 @@ template <int NT> __global__ void __launch_bounds__(256) moe_logits_kernel(const
 }
 
 // ---- the layer ----------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void mf_mma_h(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mf_mma_b(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// two e4m3 as two fp16, exact
-__device__ __forceinline__ uint32_t mf_half2(uint32_t q, int hi) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (hi ? q >> 16 : q), __NV_E4M3);
-    return (uint32_t) h.x | (uint32_t) h.y << 16;
-}
-__device__ __forceinline__ uint32_t mf_pack_h(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
-__device__ __forceinline__ float2   mf_unpack_h(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
-__device__ __forceinline__ uint32_t mf_pack_b(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
-__device__ __forceinline__ float2   mf_unpack_b(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
-
-// N floats from p on, of which those behind `left` are zero; p is written by other blocks of this launch: cached in L2 only
-template <int N> __device__ __forceinline__ void mf_row(const float * p, int64_t left, int vec, float (&v)[N]) {
-    if (vec && left >= N) {
-#pragma unroll
-        for (int j = 0; j < N / 4; j++) {
-            const float4 f = __ldcg(reinterpret_cast<const float4 *>(p) + j);
-            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-        }
-    } else
-#pragma unroll
-        for (int j = 0; j < N; j++) v[j] = j < left ? __ldcg(p + j) : 0.f;
-}
-
-// acc[column tile][half][..] = 32 rows of W (two tiles of 16; lines kb of this warp) times the columns' rows.  row: the lane's weight row (g) and 16 bytes (t) of it, Kp bytes a row;
-// src: the lane's column's values or null, K of them; sa, sb: scales of the two tiles' blocks
-template <bool F8, int NT>
-__device__ __forceinline__ void mf_product(const uint8_t * __restrict__ row, int64_t Kp, int KB, int warp, int t, const float * const (&src)[NT], int64_t K, int vec, const float * __restrict__ sa,
-                                           const float * __restrict__ sb, float (&acc)[NT][2][4]) {
-    constexpr int LINE = F8 ? 128 : 64;                          // values of a line
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[i][m][j] = 0.f;
-#pragma unroll 1
-    for (int kb = warp; kb < KB; kb += MF_WARPS) {
-        int4 w[2][2][2];
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) w[m][h][c] = ld_stream_v4(row + (int64_t) (m * 16 + h * 8) * Kp + kb * 128 + c * 64);
-        const float wa = F8 ? __ldg(sa + kb) : 1.f, wb = F8 ? __ldg(sb + kb) : 1.f;
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-            float v[2][LINE / 8];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int64_t k = (int64_t) kb * LINE + c * (LINE / 2) + t * (LINE / 8);
-                mf_row(src[i] + k, src[i] ? K - k : 0, vec, v[c]);
-            }
-            float c[2][4];
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) c[m][j] = 0.f;
-            if (F8) {
-                float amax = 0.f;
-#pragma unroll
-                for (int j = 0; j < 32; j++) amax = fmaxf(amax, fabsf(v[j / 16][j % 16]));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int   e  = min(253, 268 - (int) (__float_as_uint(amax) >> 23));
-                const float up = __uint_as_float((uint32_t) e << 23), down = __uint_as_float((uint32_t) (254 - e) << 23);
-#pragma unroll
-                for (int q = 0; q < 8; q++) {                    // 16 values of k each
-                    const float * p = &v[q / 4][q % 4 * 4];
-                    const float p0 = p[0] * up, p1 = p[1] * up, p2 = p[2] * up, p3 = p[3] * up;
-                    const uint32_t h0 = mf_pack_h(p0, p1), h1 = mf_pack_h(p2, p3);
-                    const float2 f0 = mf_unpack_h(h0), f1 = mf_unpack_h(h1);
-                    const uint32_t l0 = mf_pack_h(p0 - f0.x, p1 - f0.y), l1 = mf_pack_h(p2 - f1.x, p3 - f1.y);
-#pragma unroll
-                    for (int m = 0; m < 2; m++) {
-                        const uint32_t r0 = (uint32_t) (&w[m][0][q / 4].x)[q % 4], r1 = (uint32_t) (&w[m][1][q / 4].x)[q % 4];
-                        const uint32_t a0 = mf_half2(r0, 0), a1 = mf_half2(r1, 0), a2 = mf_half2(r0, 1), a3 = mf_half2(r1, 1);
-                        mf_mma_h(c[m], a0, a1, a2, a3, h0, h1);
-                        mf_mma_h(c[m], a0, a1, a2, a3, l0, l1);
-                    }
-                }
-                const float d0 = __shfl_sync(0xffffffffu, down, t * 8), d1 = __shfl_sync(0xffffffffu, down, t * 8 + 4);
-#pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    const float s0 = (m ? wb : wa) * d0, s1 = (m ? wb : wa) * d1;
-                    acc[i][m][0] = fmaf(c[m][0], s0, acc[i][m][0]);
-                    acc[i][m][1] = fmaf(c[m][1], s1, acc[i][m][1]);
-                    acc[i][m][2] = fmaf(c[m][2], s0, acc[i][m][2]);
-                    acc[i][m][3] = fmaf(c[m][3], s1, acc[i][m][3]);
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    float p[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) p[j] = v[q / 2][q % 2 * 4 + j];
-#pragma unroll
-                    for (int part = 0; part < 3; part++) {
-                        const uint32_t b0 = mf_pack_b(p[0], p[1]), b1 = mf_pack_b(p[2], p[3]);
-                        const float2 f0 = mf_unpack_b(b0), f1 = mf_unpack_b(b1);
-                        p[0] -= f0.x; p[1] -= f0.y; p[2] -= f1.x; p[3] -= f1.y;
-#pragma unroll
-                        for (int m = 0; m < 2; m++) {
-                            const uint32_t * r0 = reinterpret_cast<const uint32_t *>(&w[m][0][q / 2]) + q % 2 * 2, * r1 = reinterpret_cast<const uint32_t *>(&w[m][1][q / 2]) + q % 2 * 2;
-                            mf_mma_b(c[m], r0[0], r1[0], r0[1], r1[1], b0, b1);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int m = 0; m < 2; m++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][m][j] += c[m][j];
-            }
-        }
-    }
-}
-
 struct mf_shared {
     float    wts[16][16];
     int      ids[16][16], at[16][16];     // chosen experts of a token; its row of h and of the experts' outputs
-    uint32_t mask[PIB_MOE_MAX_EXPERTS + 16];
-    int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[257], n_act, ticket, next, last;
-    float    red[MF_WARPS][16][33];       // also the choice values of a warp's token
+    uint32_t mask[PIB_MOE_MAX_EXPERTS + 16], tokens[256];        // of an expert, of an entry of the list
+    int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[256], n_act, item[MF_STAGES], pub[2], abort;
+    uint64_t bars[2 * MF_STAGES + 4];     // a piece there / read, an item's results written / published
+    float    red[2][MF_WARPS][9][33];     // two items' turns; also the choice values of a warp's token
 };
 static_assert(sizeof(((mf_shared *) 0)->red) >= MF_WARPS * PIB_MOE_MAX_EXPERTS * 4, "choice values");
+#define MF_RING (((int) sizeof(mf_shared) + 127) & ~127)          // behind it the ring
+#define MF_SMEM ((size_t) MF_RING + MF_STAGES * MF_STAGE)
+extern __shared__ __align__(128) uint8_t mf_dsm[];               // named here, so that the compiler knows a shared address in every function
+
+struct mf_place { int s; uint32_t ph; };       // a place of the ring and its phase
+
+// order-preserving key of a choice value; what is no number comes last, a chosen one is 0
+__device__ __forceinline__ uint32_t mf_key(float v) { const uint32_t u = __float_as_uint(v + 0.0f); return v != v ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u; }
 
 // the choice, by every block for itself
-__device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, int warp, int lane) {
+template <int COLS> __device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, int warp, int lane) {      // COLS: tokens of an entry of the list
     const int E = A.E;
-    float * cv = &S.red[0][0][0] + warp * PIB_MOE_MAX_EXPERTS;
+    uint32_t * cv = reinterpret_cast<uint32_t *>(&S.red[0][0][0][0]) + warp * PIB_MOE_MAX_EXPERTS;
     for (int tk = warp; tk < A.b; tk += MF_WARPS) {
         const float * z = A.z + tk * E;
-        float mx = -INFINITY, sum = 0.f;
-        for (int i = lane; i < E; i += 32) mx = fmaxf(mx, z[i]);
-        mx = warp_max(mx);
-        for (int i = lane; i < E; i += 32) { const float s = A.score == PIB_MOE_SIGMOID ? 1.0f / (1.0f + expf(-z[i])) : expf(z[i] - mx); cv[i] = s; sum += s; }
-        sum = warp_sum(sum);
-        // softmax without a correction is chosen by the logits themselves: no two of them become equal on the way
-        const bool by_z = !A.has_corr;
-        for (int i = lane; i < E; i += 32) cv[i] = by_z ? z[i] : (A.score == PIB_MOE_SIGMOID ? cv[i] : cv[i] / sum) + A.corr[i];
+        float mx = -INFINITY, sum = 1.f;
+        if (A.score == PIB_MOE_SOFTMAX) {
+            for (int i = lane; i < E; i += 32) mx = fmaxf(mx, z[i]);
+            mx = warp_max(mx);
+            if (!A.renorm || A.has_corr) {                       // else the sum cancels
+                sum = 0.f;
+                for (int i = lane; i < E; i += 32) sum += expf(z[i] - mx);
+                sum = warp_sum(sum);
+            }
+        }
+        auto score = [&](float v) { return A.score == PIB_MOE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : expf(v - mx) / sum; };
+        // without a correction chosen by the logits themselves: no two of them become equal on the way
+        uint32_t best = 0;
+        int      at = 0x7fffffff;
+        for (int i = lane; i < E; i += 32) {
+            const uint32_t k = mf_key(A.has_corr ? score(z[i]) + A.corr[i] : z[i]);
+            cv[i] = k;
+            if (k > best) { best = k; at = i; }
+        }
         float tot = 0.f, mine = 0.f;
         int   id = 0;
         for (int k = 0; k < A.top; k++) {
-            float bv = -INFINITY;
-            int   bi = 0x7fffffff;
-            for (int i = lane; i < E; i += 32) { const float v = cv[i]; if (v > bv || (v == bv && v > -INFINITY && i < bi)) { bv = v; bi = i; } }      // a lane reads back only what it wrote
-            for (int o = 16; o > 0; o >>= 1) {
-                const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-                const int   oi = __shfl_xor_sync(0xffffffffu, bi, o);
-                if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
+            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+            const int bi = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+            if (at == bi) {                                      // the owner looks for its next
+                cv[bi] = 0; best = 0; at = 0x7fffffff;
+                for (int i = lane; i < E; i += 32) if (cv[i] > best) { best = cv[i]; at = i; }
             }
-            if (bi >= E) {                                       // nothing comparable is left (logits that are no numbers): the first output that is not chosen yet
-                for (bi = 0; __any_sync(0xffffffffu, lane < k && id == bi); bi++) {}
-            }
-            if ((bi & 31) == lane) cv[bi] = -INFINITY;
-            const float s = A.score == PIB_MOE_SIGMOID ? 1.0f / (1.0f + expf(-z[bi])) : expf(z[bi] - mx) / sum;
-            if (lane == k) { id = bi; mine = s; }
-            tot += s;
+            const float v = score(z[bi]);
+            if (lane == k) { id = bi; mine = v; }
+            tot += v;
         }
         if (lane < A.top) { S.ids[tk][lane] = id; S.wts[tk][lane] = A.scale * (A.renorm ? mine / (tot + 1e-20f) : mine); }
         else if (lane < A.top + A.shared) { S.ids[tk][lane] = E + lane - A.top; S.wts[tk][lane] = 1.f; }
     }
     const int all = E + A.shared, per = A.top + A.shared;
     for (int i = threadIdx.x; i < all; i += MF_WARPS * 32) S.mask[i] = 0;
-    __syncthreads();
+    mf_bar();
     for (int i = threadIdx.x; i < A.b * per; i += MF_WARPS * 32) atomicOr(&S.mask[S.ids[i / per][i % per]], 1u << i / per);
-    __syncthreads();
+    mf_bar();
     if (warp == 0) {                                             // the experts with tokens, in order; the first row of each one's tokens
         int n = 0, rows = 0;
         for (int i0 = 0; i0 < all; i0 += 32) {
             const uint32_t m = i0 + lane < all ? S.mask[i0 + lane] : 0;
-            const unsigned has = __ballot_sync(0xffffffffu, m != 0), before = has & ((1u << lane) - 1);
-            int r = __popc(m), s = r;
+            const unsigned has = __ballot_sync(0xffffffffu, m != 0);
+            if (!has) continue;
+            const int r = __popc(m), k = (r + COLS - 1) / COLS;
+            int s = r | k << 16;
             for (int o = 1; o < 32; o <<= 1) { const int p = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += p; }
-            if (m) { const int a = n + __popc(before); S.act[a] = i0 + lane; S.base[a] = rows + s - r; S.slot[i0 + lane] = a; }
-            n += __popc(has);
-            rows += __shfl_sync(0xffffffffu, s, 31);
+            if (m) {
+                int      a = n + (s >> 16) - k, row = rows + (s & 0xffff) - r;
+                uint32_t left = m;
+                S.slot[i0 + lane] = a;
+                for (; left; a++) {
+                    uint32_t few = 0;
+                    for (int j = 0; j < COLS && left; j++) { few |= left & (0u - left); left &= left - 1; }
+                    S.act[a] = i0 + lane; S.base[a] = row; S.tokens[a] = few;
+                    row += __popc(few);
+                }
+            }
+            s = __shfl_sync(0xffffffffu, s, 31);
+            n += s >> 16;
+            rows += s & 0xffff;
         }
         if (lane == 0) S.n_act = n;
     }
-    __syncthreads();
+    mf_bar();
     for (int i = threadIdx.x; i < A.b * per; i += MF_WARPS * 32) {
         const int tk = i / per, e = S.ids[tk][i % per];
         S.at[tk][i % per] = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
     }
-    __syncthreads();
 }
 
 __device__ __forceinline__ int mf_nth_bit(uint32_t m, int n) {
     for (; n > 0; n--) m &= m - 1;
     return __ffs((int) m) - 1;
 }
+__device__ __forceinline__ uint4 mf_ld(const uint16_t * p) { return __ldcg(reinterpret_cast<const uint4 *>(p)); }
 
-template <bool F8, int NT>
-__device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, bool up, int a, int i, int warp, int lane) {
-    const int g = lane >> 2, t = lane & 3, e = S.act[a], base = S.base[a];
-    const uint32_t mask = S.mask[e];
-    const int n = __popc(mask);
-    const float * src[NT];
+// What a lane holds of a line's activations for one column tile: PARTS pieces of the row of column g (PACK: of token g & 3, part g >> 2)
+template <bool F8, bool PACK> struct mf_b {
+    static constexpr int PARTS = F8 ? (PACK ? 1 : 2) : 3, WORDS = F8 ? 4 : 2;
+    uint4 v[PARTS][WORDS];
+};
+template <bool F8, bool PACK> __device__ __forceinline__ void mf_ask(mf_b<F8, PACK> & B, const uint16_t * row, int plane, int kb, int t) {
+    constexpr int P = mf_b<F8, PACK>::PARTS, W = mf_b<F8, PACK>::WORDS;
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int c = j * 8 + g;
-        src[j] = c >= n ? nullptr : up ? A.x + mf_nth_bit(mask, c) * A.ldx : A.h + (int64_t) (base + c) * A.Fk;
+    for (int part = 0; part < P; part++)
+#pragma unroll
+        for (int w = 0; w < W; w++) B.v[part][w] = row ? mf_ld(row + part * plane + (kb * 4 + t) * (W * 8) + w * 8) : make_uint4(0, 0, 0, 0);
+}
+// half c of a line of a piece times eight columns: acc[tile of 16 rows].  f: what a sum of the tile of rows is worth, per column that the lane holds
+template <bool F8, bool PACK> __device__ __forceinline__ void mf_half(const uint8_t * line, int c, int lane, const mf_b<F8, PACK> & B, const float (&f)[2][2], float (&acc)[2][4]) {
+    constexpr int P = mf_b<F8, PACK>::PARTS;
+    const int g = lane >> 2, t = lane & 3, gp = (g >> 1) | (g & 1) << 2;
+    int4  w[2][2];
+    float s[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) w[m][h] = *reinterpret_cast<const int4 *>(line + (m * 16 + h * 8 + gp) * 128 + ((c * 4 + t) ^ gp) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[m][j] = 0.f;
     }
-    float acc[NT][2][4];
-    if (up) {
-        const float * s = A.s1 + ((int64_t) e * 2 * A.nb1 + i / 8) * A.KB1;
-        mf_product<F8, NT>(A.w1 + (((int64_t) e * A.T1 + i) * 32 + g) * (A.KB1 * 128LL) + t * 16, A.KB1 * 128LL, A.KB1, warp, t, src, A.D, A.vec, s, s + (int64_t) A.nb1 * A.KB1, acc);
+    if (F8) {
+#pragma unroll
+        for (int q = 0; q < 4; q++)                              // 16 values of k each
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                const uint32_t r0 = (uint32_t) (q == 0 ? w[m][0].x : q == 1 ? w[m][0].y : q == 2 ? w[m][0].z : w[m][0].w), r1 = (uint32_t) (q == 0 ? w[m][1].x : q == 1 ? w[m][1].y : q == 2 ? w[m][1].z : w[m][1].w);
+                const uint32_t a0 = mf_half2(r0, 0), a1 = mf_half2(r1, 0), a2 = mf_half2(r0, 1), a3 = mf_half2(r1, 1);
+#pragma unroll
+                for (int part = P - 1; part >= 0; part--) {      // the small ones first
+                    const uint4 b = B.v[part][c * 2 + (q >> 1)];
+                    mf_mma_h(s[m], a0, a1, a2, a3, q & 1 ? b.z : b.x, q & 1 ? b.w : b.y);
+                }
+            }
     } else {
-        const float * s = A.s2 + ((int64_t) e * A.nb2 + i / 4) * A.KB2;
-        mf_product<F8, NT>(A.w2 + (((int64_t) e * A.T2 + i) * 32 + g) * (A.KB2 * 128LL) + t * 16, A.KB2 * 128LL, A.KB2, warp, t, src, A.Fk, 1, s, s, acc);
+#pragma unroll
+        for (int part = P - 1; part >= 0; part--) {
+            const uint4 b = B.v[part][c];
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                mf_mma_b(s[m], w[m][0].x, w[m][1].x, w[m][0].y, w[m][1].y, b.x, b.y);
+                mf_mma_b(s[m], w[m][0].z, w[m][1].z, w[m][0].w, w[m][1].w, b.z, b.w);
+            }
+        }
     }
 #pragma unroll
-    for (int j = 0; j < NT; j++)
+    for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int j = 0; j < 4; j++) acc[m][j] = F8 ? fmaf(s[m][j], f[m][j & 1], acc[m][j]) : acc[m][j] + s[m][j];
+}
+
+// An item, by the consumers: the warp's lines of its pieces, the meeting, the results.  turn: the item's turn at the places of the sums
+template <bool F8, bool UP>
+__device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const uint8_t * ring, uint32_t bar_f, uint32_t bar_e, mf_place & at, int turn, int a, int i) {
+    constexpr bool PACK = F8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, e = S.act[a], base = S.base[a], KB = UP ? A.KB1 : A.KB2;
+    const uint32_t mask = S.tokens[a];
+    const int n = __popc(mask), stride = (int) mf_row_of(F8, KB), plane = KB * (F8 ? 128 : 64);
+    // row of a column, -1: none
+    auto row_of = [&](int c) { c = PACK ? c & 3 : c; return c >= n ? -1 : UP ? mf_nth_bit(mask, c) : base + c; };
+    // the power of two of a token's row of x or h, as its exponent field
+    auto field_x = [&](int tk) { return mf_exponent(__ldcg(A.xm + 2 * tk)); };
+    auto field_h = [&](int tk) { return mf_exponent(1.01f * sqrtf(__ldg(A.norms + 2 * e)) * sqrtf(__ldg(A.norms + 2 * e + 1)) * __ldcg(A.xm + 2 * tk + 1)); };
+    const int r = row_of(g);
+    const uint16_t * row = r < 0 ? nullptr : (UP ? A.xp : A.hp) + (int64_t) r * stride + (PACK && g >= 4 ? plane : 0);
+    float d[2] = { 1.f, 1.f };
+    if (F8)
 #pragma unroll
-            for (int q = 0; q < 4; q++) S.red[warp][j * 8 + t * 2 + (q & 1)][m * 16 + g + (q >> 1) * 8] = acc[j][m][q];
-    __syncthreads();
-    if (up) {
+        for (int k = 0; k < 2; k++) {
+            const int c = (t * 2 + k) & 3, tk = c >= n ? -1 : mf_nth_bit(mask, c);
+            d[k] = tk < 0 ? 1.f : mf_pow2(254 - (UP ? field_x(tk) : field_h(tk)));
+        }
+    const float * sa = nullptr, * sb = nullptr;
+    if (F8) {
+        sa = UP ? A.s1 + ((int64_t) e * 2 * A.nb1 + i / 8) * A.KB1 : A.s2 + ((int64_t) e * A.nb2 + i / 4) * A.KB2;
+        sb = UP ? sa + (int64_t) A.nb1 * A.KB1 : sa;
+    }
+    float acc[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) acc[m][q] = 0.f;
+#pragma unroll 1
+    for (int st = 0; st < KB; st += MF_WARPS) {
+        const int  kb = st + warp;
+        const bool in = kb < KB;
+        mf_b<F8, PACK> B;
+        float wa = 1.f, wb = 1.f;
+        if (F8 && in) { wa = __ldg(sa + kb); wb = UP ? __ldg(sb + kb) : wa; }
+        if (in) mf_ask<F8, PACK>(B, row, plane, kb, t);          // ahead of the wait
+        if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_f + at.s * 8, at.ph, (volatile int *) &S.abort))) break;
+        if (in) {
+            const uint8_t * line = ring + at.s * MF_STAGE + warp * MF_LINE;
+            const float f[2][2] = { { wa * d[0], wa * d[1] }, { wb * d[0], wb * d[1] } };
+            mf_half<F8, PACK>(line, 0, lane, B, f, acc);
+            mf_half<F8, PACK>(line, 1, lane, B, f, acc);
+        }
+        __syncwarp();
+        if (lane == 0) dt_arrive(bar_e + at.s * 8);
+        if (++at.s == MF_STAGES) { at.s = 0; at.ph ^= 1; }
+    }
+    const int gp = (g >> 1) | (g & 1) << 2;
+    auto & red = S.red[turn];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) red[warp][t * 2 + (q & 1)][m * 16 + gp + (q >> 1) * 8] = acc[m][q];
+    mf_bar();
+    auto sum = [&](int c, int k) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < MF_WARPS; w++) x += PACK ? red[w][c][k] + red[w][c + 4][k] : red[w][c][k];
+        return x;
+    };
+    if (UP) {
+        const int last = i == A.T1 - 1 ? A.KB2 * (F8 ? 8 : 4) : i + 1;           // behind the last tile zeros, to the end of its line
         for (int q = threadIdx.x; q < n * 16; q += MF_WARPS * 32) {
-            const int c = q >> 4, r = q & 15;
-            float gt = 0.f, u = 0.f;
-#pragma unroll
-            for (int w = 0; w < MF_WARPS; w++) { gt += S.red[w][c][r]; u += S.red[w][c][16 + r]; }
-            __stcg(A.h + (int64_t) (base + c) * A.Fk + i * 16 + r, gt / (1.0f + expf(-gt)) * u);
+            const int c = q >> 4, k = q & 15;
+            const float gt = sum(c, k), u = sum(c, 16 + k), h = gt / (1.0f + expf(-gt)) * u;
+            uint16_t *  hrow = A.hp + (int64_t) (base + c) * mf_row_of(F8, A.KB2);
+            mf_store<F8>(h, F8 ? mf_pow2(field_h(mf_nth_bit(mask, c))) : 1.f, i, k, A.KB2, hrow);
+            for (int z = i + 1; z < last; z++) mf_store<F8>(0.f, 1.f, z, k, A.KB2, hrow);
         }
-    } else {
-        for (int q = threadIdx.x; q < n * 32; q += MF_WARPS * 32) {
-            const int c = q >> 5, r = q & 31;
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < MF_WARPS; w++) v += S.red[w][c][r];
-            __stcg(A.part + (int64_t) (base + c) * A.Dr + i * 32 + r, v);
-        }
-    }
+    } else
+        for (int q = threadIdx.x; q < n * 32; q += MF_WARPS * 32) __stcg(A.part + (int64_t) (base + (q >> 5)) * A.Dr + i * 32 + (q & 31), sum(q >> 5, q & 31));
 }
 
 template <bool F8>
-__global__ void __launch_bounds__(MF_WARPS * 32, 2) moe_few_kernel(const __grid_constant__ mf_args A) {
-    __shared__ mf_shared S;
+__global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_constant__ mf_args A) {
+    mf_shared & S = *reinterpret_cast<mf_shared *>(mf_dsm);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t * ring = mf_dsm + MF_RING;
+    const uint32_t bar_f = dt_smem(S.bars), bar_e = bar_f + MF_STAGES * 8, bar_w = bar_e + MF_STAGES * 8, bar_p = bar_w + 16;
+    volatile int * abort_s = (volatile int *) &S.abort;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MF_STAGES; s++) { dt_mbar_init(bar_f + s * 8, 1); dt_mbar_init(bar_e + s * 8, MF_WARPS); }
+        for (int s = 0; s < 2; s++) { dt_mbar_init(bar_w + s * 8, MF_WARPS); dt_mbar_init(bar_p + s * 8, 1); }
+        S.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     pib_pdl_wait();
     pib_pdl_trigger();
-    if (threadIdx.x == 0) S.next = atomicAdd(A.cnt, 1);
-    mf_route(A, S, warp, lane);
+    int ticket = 0;
+    if (warp == MF_WARPS && lane == 0) ticket = atomicAdd(A.cnt, 1);
+    if (warp < MF_WARPS) mf_route<F8 ? 4 : 8>(A, S, warp, lane);
+    __syncthreads();
     const int per = A.top + A.shared, ups = S.n_act * A.T1, items = ups + S.n_act * A.T2;
-    int * done_up = A.cnt + 2, * done_rows = done_up + A.E + A.shared;
-    for (;;) {
-        const int item = S.next;
-        __syncthreads();
-        if (item >= items) break;
-        int next = 0;
-        if (threadIdx.x == 0) next = atomicAdd(A.cnt, 1);
-        const bool up = item < ups;
-        const int  a = up ? item / A.T1 : (item - ups) / A.T2, i = up ? item % A.T1 : (item - ups) % A.T2;
-        if (!up) {
-            if (threadIdx.x == 0) {
-                int ok = 0;
-                for (uint32_t it = 0; it < MF_SPIN && !ok; it++) {
-                    int v, stop;
-                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done_up + a) : "memory");
-                    ok = v >= A.T1;
-                    if (!ok && (it & 63) == 63) {
-                        asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(stop) : "l"(A.cnt + 1) : "memory");
-                        if (stop) break;
-                    }
+    int * done_up = A.cnt + 2, * done_rows = done_up + A.b * per;
+    if (warp == MF_WARPS) {
+        if (lane == 0) {
+            int s = 0, item = ticket;
+            uint32_t ph = 1;
+            bool ok = true;
+            while (item < items && ok) {
+                const int  next = atomicAdd(A.cnt, 1);
+                const bool up = item < ups;
+                const int  a = up ? item / A.T1 : (item - ups) / A.T2, i = up ? item % A.T1 : (item - ups) % A.T2, KB = up ? A.KB1 : A.KB2;
+                const uint8_t * src = up ? A.w1 + ((int64_t) S.act[a] * A.T1 + i) * KB * MF_LINE : A.w2 + ((int64_t) S.act[a] * A.T2 + i) * KB * MF_LINE;
+                for (int st = 0; st < KB; st += MF_WARPS) {
+                    ok = dt_mbar_wait(bar_e + s * 8, ph, abort_s);
+                    if (!ok) break;
+                    const uint32_t bytes = (uint32_t) min(MF_WARPS, KB - st) * MF_LINE;
+                    S.item[s] = item;
+                    dt_mbar_expect_tx(bar_f + s * 8, bytes);
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                 ::"r"(dt_smem(ring) + s * MF_STAGE), "l"(src + (int64_t) st * MF_LINE), "r"(bytes), "r"(bar_f + s * 8) : "memory");
+                    if (++s == MF_STAGES) { s = 0; ph ^= 1; }
                 }
-                if (!ok) { atomicExch(A.cnt + 1, 1); atomicExch(A.err, 1 + (int) blockIdx.x); }
-                S.last = ok;
+                item = next;
             }
-            __syncthreads();
-            if (!S.last) break;                                  // a wait ran out: every block gives up at its own
+            if (ok && dt_mbar_wait(bar_e + s * 8, ph, abort_s)) { S.item[s] = -1; dt_arrive(bar_f + s * 8); }
         }
-        if (__popc(S.mask[S.act[a]]) > 8) mf_item<F8, 2>(A, S, up, a, i, warp, lane);
-        else                              mf_item<F8, 1>(A, S, up, a, i, warp, lane);
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            if (up) atomicAdd(done_up + a, 1);
-            else    S.last = atomicAdd(done_rows + i, 1) == S.n_act - 1;
-            S.next = next;
-            __threadfence();
-        }
-        __syncthreads();
-        if (!up && S.last) {
-            for (int q = threadIdx.x; q < A.b * 32; q += MF_WARPS * 32) {
-                const int tk = q >> 5;
-                const int64_t row = i * 32 + (q & 31);
-                if (row >= A.D) continue;
-                float v = A.res ? A.res[tk * A.ldr + row] : 0.f;
-                for (int k = 0; k < per; k++) v = fmaf(S.wts[tk][k], __ldcg(A.part + (int64_t) S.at[tk][k] * A.Dr + row), v);
-                A.y[tk * A.ldy + row] = v;
+    } else if (warp == MF_WARPS + 1) {
+        // publisher: in the order of the block's items
+        int turn = 0;
+        uint32_t ph = 0;
+        for (;;) {
+            if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_w + turn * 8, ph, abort_s))) break;
+            const int item = S.pub[turn];
+            if (item < 0) break;
+            const bool up = item < ups;
+            const int  i = (item - ups) % A.T2;
+            bool last = false;
+            if (lane == 0) {
+                __threadfence();                                 // the consumers' writes too: they lie in front of their arrivals
+                if (up) atomicAdd(done_up + item / A.T1, 1);
+                else    last = atomicAdd(done_rows + i, 1) == S.n_act - 1;
+                dt_arrive(bar_p + turn * 8);
             }
+            if (__shfl_sync(0xffffffffu, last, 0)) {
+                __threadfence();
+                const int64_t row = i * 32 + lane;
+                if (row < A.D)
+                    for (int tk = 0; tk < A.b; tk++) {
+                        float v = A.res ? A.res[tk * A.ldr + row] : 0.f, p[PIB_MOE_MAX_TOP];
+#pragma unroll
+                        for (int k = 0; k < PIB_MOE_MAX_TOP; k++) p[k] = k < per ? __ldcg(A.part + (int64_t) S.at[tk][k] * A.Dr + row) : 0.f;
+#pragma unroll
+                        for (int k = 0; k < PIB_MOE_MAX_TOP; k++) if (k < per) v = fmaf(S.wts[tk][k], p[k], v);
+                        A.y[tk * A.ldy + row] = v;
+                    }
+            }
+            if (turn ^= 1) continue;
+            ph ^= 1;
         }
+    } else {
+        int turn = 0;
+        mf_place at = { 0, 0 };
+        uint32_t pph = 1;                                        // the first two turns find their places free
+        for (;;) {
+            bool ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_f + at.s * 8, at.ph, abort_s) && dt_mbar_wait(bar_p + turn * 8, pph, abort_s));
+            const int item = ok ? S.item[at.s] : items;             // a wait that ran out: through the barrier with the others, then out
+            if (item < 0) {
+                __syncwarp();
+                if (lane == 0) { if (warp == 0) S.pub[turn] = -1; dt_arrive(bar_w + turn * 8); }
+                break;
+            }
+            const bool up = item < ups;
+            const int  a = !ok ? 0 : up ? item / A.T1 : (item - ups) / A.T2, i = !ok ? 0 : up ? item % A.T1 : (item - ups) % A.T2;
+            if (!up && ok) {
+                if (lane == 0) {
+                    ok = false;
+                    for (uint32_t it = 0; it < MF_SPIN && !ok; it++) {
+                        int v, stop;
+                        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done_up + a) : "memory");
+                        ok = v >= A.T1;
+                        if (!ok && (it & 63) == 63) {
+                            asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(stop) : "l"(A.cnt + 1) : "memory");
+                            if (stop) break;
+                        }
+                    }
+                    if (!ok) { *abort_s = 1; atomicExch(A.cnt + 1, 1); }
+                }
+                __syncwarp();
+            }
+            if (up) mf_item<F8, true>(A, S, ring, bar_f, bar_e, at, turn, a, i);
+            else    mf_item<F8, false>(A, S, ring, bar_f, bar_e, at, turn, a, i);
+            if (*abort_s) break;                                 // raised in front of mf_item's barrier: every warp sees it and leaves here
+            __syncwarp();
+            if (lane == 0) { if (warp == 0) S.pub[turn] = item; dt_arrive(bar_w + turn * 8); }
+            if (!(turn ^= 1)) pph ^= 1;
+        }
+    }
+    __syncthreads();
+    if (*abort_s) {                                              // say so, give copies still in flight time to land (bounded)
+        if (threadIdx.x == 0) { atomicExch(A.cnt + 1, 1); atomicExch(A.err, 1 + (int) blockIdx.x); }
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
     }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------------
-// rows of `bytes` bytes into rows of Kp, zero behind them; with `pairs` the source rows are tiles of 16 that land 32 apart (behind `off`)
-static __global__ void mf_pack_kernel(const uint8_t * __restrict__ src, uint8_t * __restrict__ dst, int64_t rows, int64_t bytes, int64_t rows_p, int64_t Kp, int64_t dst_rows, int pairs, int off, int64_t n) {
+// rows of `bytes` bytes into the items' lines; with `pairs` an item holds 16 of them, behind `off`, else 32.  A thread per 16 bytes: lane t, four (two) tiles
+static __global__ void mf_pack_kernel(const uint8_t * __restrict__ src, uint8_t * __restrict__ dst, int64_t rows, int64_t bytes, int64_t rows_p, int KB, int eb, int pairs, int off, int64_t n) {
     for (int64_t u = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; u < n; u += (int64_t) gridDim.x * blockDim.x) {
-        const int64_t k = u % (Kp / 16) * 16, r = u / (Kp / 16) % rows_p, e = u / (Kp / 16) / rows_p;
+        const int64_t j = u & 7, kb = (u >> 3) % KB, r = (u >> 3) / KB % rows_p, e = (u >> 3) / KB / rows_p;
+        const int     t = (int) (j & 3), tiles = 4 / eb;         // of half a line
         __align__(16) uint8_t v[16];
-        const uint8_t * p = src + (e * rows + r) * bytes + k;
+        const uint8_t * p = src + (e * rows + r) * bytes;
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = r < rows && k + j < bytes ? p[j] : 0;
-        *reinterpret_cast<int4 *>(dst + (e * dst_rows + (pairs ? r / 16 * 32 + off + r % 16 : r)) * Kp + k) = *reinterpret_cast<const int4 *>(v);
+        for (int q = 0; q < 16; q++) {
+            const int64_t k = (kb * (128 / eb) + ((j >> 2) * tiles + q / (4 * eb)) * 16 + t * 4) * eb + q % (4 * eb);
+            v[q] = r < rows && k < bytes ? p[k] : 0;
+        }
+        const int     per = pairs ? 16 : 32, in = (int) (r % per) + off;
+        const int64_t tile = e * (rows_p / per) + r / per;
+        *reinterpret_cast<int4 *>(dst + (tile * KB + kb) * MF_LINE + in * 128 + ((j ^ (in & 7)) * 16)) = *reinterpret_cast<const int4 *>(v);
     }
 }
-static cudaError_t mf_pack(const void * src, uint8_t * dst, int64_t E, int64_t rows, int64_t bytes, int64_t rows_p, int64_t Kp, int64_t dst_rows, int pairs, int off) {
-    const int64_t n = E * rows_p * (Kp / 16);
-    mf_pack_kernel<<<(unsigned) std::min<int64_t>((n + 255) / 256, 1 << 16), 256>>>((const uint8_t *) src, dst, rows, bytes, rows_p, Kp, dst_rows, pairs, off, n);
+static cudaError_t mf_pack(const void * src, uint8_t * dst, int64_t E, int64_t rows, int64_t bytes, int64_t rows_p, int KB, int eb, int pairs, int off) {
+    const int64_t n = E * rows_p * KB * 8;
+    mf_pack_kernel<<<(unsigned) std::min<int64_t>((n + 255) / 256, 1 << 16), 256>>>((const uint8_t *) src, dst, rows, bytes, rows_p, KB, eb, pairs, off, n);
     return cudaGetLastError();
+}
+
+// the largest squared norm of an expert's rows, a block per expert and matrix; scales of gate and up are neighbours (pib_moe::s1)
+static __global__ void __launch_bounds__(256) mf_norms_kernel(const uint8_t * __restrict__ gate, const uint8_t * __restrict__ up, const float * __restrict__ s1, int64_t F, int64_t D, int nb1, int KB1,
+                                                              float * __restrict__ norms) {
+    __shared__ float red[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t e = blockIdx.x;
+    const uint8_t * w = (blockIdx.y ? up : gate) + e * F * D;
+    float most = 0.f;
+    for (int64_t r = warp; r < F; r += 8) {
+        const float * s = s1 + ((e * 2 + blockIdx.y) * nb1 + r / 128) * KB1;
+        float n = 0.f;
+        for (int64_t k = lane; k < D; k += 32) { const float v = __half2float(__half(__nv_cvt_fp8_to_halfraw(w[r * D + k], __NV_E4M3))) * s[k / 128]; n = fmaf(v, v, n); }
+        most = fmaxf(most, warp_sum(n));
+    }
+    if (lane == 0) red[warp] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; i++) most = fmaxf(most, red[i]);
+        norms[e * 2 + blockIdx.y] = most;
+    }
 }
 
 extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float * router, const float * correction, const void * gate, const float * gate_scales, const void * up,
@@ -439,9 +598,9 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
     m->T1 = (int) ((F + 15) / 16); m->T2 = (int) ((D + 31) / 32);
     auto al = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     const size_t n_r = al((size_t) (sh->experts * D) * 4), n_c = al((size_t) sh->experts * 4), n_1 = (size_t) E * m->T1 * 32 * m->KB1 * 128, n_2 = (size_t) E * m->T2 * 32 * m->KB2 * 128;
-    const size_t n_s1 = f8 ? al((size_t) (E * 2 * pib_f8_blocks(F) * m->KB1) * 4) : 0, n_s2 = f8 ? al((size_t) (E * pib_f8_blocks(D) * m->KB2) * 4) : 0;
-    if (cudaGetDevice(&m->dev) != cudaSuccess || cudaMalloc(&m->base, n_r + n_c + n_1 + n_2 + n_s1 + n_s2) != cudaSuccess) {
-        pib_set_error("pib_moe_from_device: cudaMalloc of %zu bytes failed", n_r + n_c + n_1 + n_2 + n_s1 + n_s2);
+    const size_t n_s1 = f8 ? al((size_t) (E * 2 * pib_f8_blocks(F) * m->KB1) * 4) : 0, n_s2 = f8 ? al((size_t) (E * pib_f8_blocks(D) * m->KB2) * 4) : 0, n_n = f8 ? al((size_t) E * 8) : 0;
+    if (cudaGetDevice(&m->dev) != cudaSuccess || cudaMalloc(&m->base, n_r + n_c + n_1 + n_2 + n_s1 + n_s2 + n_n) != cudaSuccess) {
+        pib_set_error("pib_moe_from_device: cudaMalloc of %zu bytes failed", n_r + n_c + n_1 + n_2 + n_s1 + n_s2 + n_n);
         cudaGetLastError();
         free(m);
         return nullptr;
@@ -449,16 +608,20 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
     m->router = (float *) m->base;
     m->corr = correction ? (float *) (m->base + n_r) : nullptr;
     m->w1 = m->base + n_r + n_c; m->w2 = m->w1 + n_1;
-    m->s1 = (float *) (m->w2 + n_2); m->s2 = (float *) (m->w2 + n_2 + n_s1);
+    m->s1 = (float *) (m->w2 + n_2); m->s2 = (float *) (m->w2 + n_2 + n_s1); m->norms = (float *) (m->w2 + n_2 + n_s1 + n_s2);
     cudaError_t e = cudaMemcpyAsync(m->router, router, (size_t) (sh->experts * D) * 4, cudaMemcpyDeviceToDevice, 0);
     if (e == cudaSuccess && correction) e = cudaMemcpyAsync(m->corr, correction, (size_t) sh->experts * 4, cudaMemcpyDeviceToDevice, 0);
-    if (e == cudaSuccess) e = mf_pack(gate, m->w1, E, F, D * eb, m->T1 * 16LL, m->KB1 * 128LL, m->T1 * 32LL, 1, 0);
-    if (e == cudaSuccess) e = mf_pack(up, m->w1, E, F, D * eb, m->T1 * 16LL, m->KB1 * 128LL, m->T1 * 32LL, 1, 16);
-    if (e == cudaSuccess) e = mf_pack(down, m->w2, E, D, F * eb, m->T2 * 32LL, m->KB2 * 128LL, m->T2 * 32LL, 0, 0);
+    if (e == cudaSuccess) e = mf_pack(gate, m->w1, E, F, D * eb, m->T1 * 16LL, m->KB1, eb, 1, 0);
+    if (e == cudaSuccess) e = mf_pack(up, m->w1, E, F, D * eb, m->T1 * 16LL, m->KB1, eb, 1, 16);
+    if (e == cudaSuccess) e = mf_pack(down, m->w2, E, D, F * eb, m->T2 * 32LL, m->KB2, eb, 0, 0);
     if (f8) {
         const size_t row1 = (size_t) pib_f8_blocks(F) * m->KB1 * 4;                      // gate and up scales of an expert become neighbours
         if (e == cudaSuccess) e = cudaMemcpy2DAsync(m->s1, 2 * row1, gate_scales, row1, row1, (size_t) E, cudaMemcpyDeviceToDevice, 0);
         if (e == cudaSuccess) e = cudaMemcpy2DAsync((uint8_t *) m->s1 + row1, 2 * row1, up_scales, row1, row1, (size_t) E, cudaMemcpyDeviceToDevice, 0);
+        if (e == cudaSuccess) {
+            mf_norms_kernel<<<dim3((unsigned) E, 2), 256>>>((const uint8_t *) gate, (const uint8_t *) up, m->s1, F, D, (int) pib_f8_blocks(F), m->KB1, m->norms);
+            e = cudaGetLastError();
+        }
         if (e == cudaSuccess) e = cudaMemcpyAsync(m->s2, down_scales, (size_t) (E * pib_f8_blocks(D) * m->KB2) * 4, cudaMemcpyDeviceToDevice, 0);
     }
     if (e == cudaSuccess) e = cudaStreamSynchronize(0);
@@ -497,20 +660,28 @@ extern "C" int pib_moe_forward(const pib_moe * m, const float * x, int64_t ldx, 
     memset(&A, 0, sizeof(A));
     A.b = b; A.E = m->s.experts; A.shared = m->s.shared; A.top = m->s.top; A.score = m->s.score; A.renorm = m->s.renorm; A.scale = m->s.scale; A.has_corr = m->corr != nullptr; A.corr = m->corr;
     A.T1 = m->T1; A.T2 = m->T2; A.KB1 = m->KB1; A.KB2 = m->KB2; A.nb1 = (int) pib_f8_blocks(m->s.ff); A.nb2 = (int) pib_f8_blocks(D);
-    A.D = D; A.F = m->s.ff; A.Fk = L.Fk; A.Dr = L.Dr;
-    A.vec = ldx % 4 == 0 && !((uintptr_t) x & 15);
+    A.D = D; A.Dr = L.Dr;
     A.w1 = m->w1; A.w2 = m->w2; A.s1 = m->s1; A.s2 = m->s2;
-    A.x = x; A.res = residual; A.ldx = ldx; A.ldr = ldr; A.ldy = ldy; A.y = y;
-    A.cnt = (int *) sc; A.z = (const float *) (sc + L.z); A.h = (float *) (sc + L.h); A.part = (float *) (sc + L.part);
-    if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_moe_forward: no memory for the error word"); return PIB_ERR_NOMEM; }
-    const dim3 rg((unsigned) A.E), rb(256);
-    const int  rv = A.vec && D % 4 == 0;
+    A.res = residual; A.ldr = ldr; A.ldy = ldy; A.y = y;
     float *    z = (float *) (sc + L.z);
-    if (b == 1)      PIB_CHECK(pib_launch(moe_logits_kernel<1>, rg, rb, 0, st, m->router, x, ldx, b, A.E, D, rv, z, A.cnt, L.n_cnt));
-    else if (b <= 4) PIB_CHECK(pib_launch(moe_logits_kernel<4>, rg, rb, 0, st, m->router, x, ldx, b, A.E, D, rv, z, A.cnt, L.n_cnt));
-    else             PIB_CHECK(pib_launch(moe_logits_kernel<16>, rg, rb, 0, st, m->router, x, ldx, b, A.E, D, rv, z, A.cnt, L.n_cnt));
-    const dim3 grid((unsigned) (2 * pib_num_sms())), block(MF_WARPS * 32);
-    if (m->s.type == PIB_TYPE_F8) PIB_CHECK(pib_launch(moe_few_kernel<true>, grid, block, 0, st, A));
-    else                          PIB_CHECK(pib_launch(moe_few_kernel<false>, grid, block, 0, st, A));
+    float *    xm = (float *) (sc + L.xm);
+    uint16_t * xp = (uint16_t *) (sc + L.xp);
+    A.cnt = (int *) sc; A.z = z; A.xp = xp; A.xm = xm; A.norms = m->norms; A.hp = (uint16_t *) (sc + L.hp); A.part = (float *) (sc + L.part);
+    if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_moe_forward: no memory for the error word"); return PIB_ERR_NOMEM; }
+    const dim3 rg((unsigned) (A.E + b)), rb(256);
+    const int  vec = ldx % 4 == 0 && !((uintptr_t) x & 15) && D % 4 == 0;
+    const bool f8 = m->s.type == PIB_TYPE_F8;
+#define MF_LOGITS(F8, NT) PIB_CHECK(pib_launch(moe_logits_kernel<F8, NT>, rg, rb, 0, st, m->router, x, ldx, b, A.E, D, vec, z, A.cnt, L.n_cnt, A.KB1, xp, xm))
+    if (f8) { if (b == 1) MF_LOGITS(true, 1); else if (b <= 4) MF_LOGITS(true, 4); else MF_LOGITS(true, 16); }
+    else    { if (b == 1) MF_LOGITS(false, 1); else if (b <= 4) MF_LOGITS(false, 4); else MF_LOGITS(false, 16); }
+#undef MF_LOGITS
+    const dim3 grid((unsigned) (2 * pib_num_sms())), block(MF_THREADS);
+    static pib_per_device attrs;
+    PIB_CHECK(attrs.once([&] {
+        const cudaError_t e = cudaFuncSetAttribute(moe_few_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) MF_SMEM);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(moe_few_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) MF_SMEM);
+    }));
+    if (f8) PIB_CHECK(pib_launch(moe_few_kernel<true>, grid, block, MF_SMEM, st, A));
+    else    PIB_CHECK(pib_launch(moe_few_kernel<false>, grid, block, MF_SMEM, st, A));
     return PIB_OK;
 }
