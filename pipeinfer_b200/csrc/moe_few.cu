@@ -177,7 +177,8 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
 
 // ---- the layer ----------------------------------------------------------------------------------------------------------------------
 struct mf_shared {
-    float    wts[16][16];
+    float    wts[16][16], xm[16][2];
+    int      px[256], ph[256];            // of a pair
     int      ids[16][16], at[16][16];     // chosen experts of a token; its row of h and of the experts' outputs
     uint32_t mask[PIB_MOE_MAX_EXPERTS + 16], tokens[256];        // of an expert, of an entry of the list
     int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[256], n_act, item[MF_STAGES], pub[2], abort;
@@ -195,45 +196,53 @@ struct mf_place { int s; uint32_t ph; };       // a place of the ring and its ph
 __device__ __forceinline__ uint32_t mf_key(float v) { const uint32_t u = __float_as_uint(v + 0.0f); return v != v ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u; }
 
 // the choice, by every block for itself
-template <int COLS> __device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, int warp, int lane) {      // COLS: tokens of an entry of the list
+template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, int warp, int lane) {
+    constexpr int COLS = F8 ? 4 : 8;                             // tokens of an entry of the list
     const int E = A.E;
-    uint32_t * cv = reinterpret_cast<uint32_t *>(&S.red[0][0][0][0]) + warp * PIB_MOE_MAX_EXPERTS;
+    float * sv = &S.red[0][0][0][0] + warp * PIB_MOE_MAX_EXPERTS;        // the token's logits, then its scores
     for (int tk = warp; tk < A.b; tk += MF_WARPS) {
         const float * z = A.z + tk * E;
         float mx = -INFINITY, sum = 1.f;
+        for (int i = lane; i < E; i += 32) { const float v = __ldcg(z + i); sv[i] = v; mx = fmaxf(mx, v); }
         if (A.score == PIB_MOE_SOFTMAX) {
-            for (int i = lane; i < E; i += 32) mx = fmaxf(mx, z[i]);
             mx = warp_max(mx);
-            if (!A.renorm || A.has_corr) {                       // else the sum cancels
-                sum = 0.f;
-                for (int i = lane; i < E; i += 32) sum += expf(z[i] - mx);
-                sum = warp_sum(sum);
-            }
+            sum = 0.f;
+            for (int i = lane; i < E; i += 32) { const float v = expf(sv[i] - mx); sum += v; }
+            sum = warp_sum(sum);
         }
         auto score = [&](float v) { return A.score == PIB_MOE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : expf(v - mx) / sum; };
-        // without a correction chosen by the logits themselves: no two of them become equal on the way
-        uint32_t best = 0;
+        // Without a correction chosen by the logits themselves: no two of them become equal on the way.  Keys of outputs lane + 32 j stay in registers, 0 once chosen; the
+        // tests on E are the same in all lanes
+        constexpr int PL = PIB_MOE_MAX_EXPERTS / 32;
+        uint32_t key[PL], best = 0;
         int      at = 0x7fffffff;
-        for (int i = lane; i < E; i += 32) {
-            const uint32_t k = mf_key(A.has_corr ? score(z[i]) + A.corr[i] : z[i]);
-            cv[i] = k;
-            if (k > best) { best = k; at = i; }
+#pragma unroll
+        for (int j = 0; j < PL; j++) {
+            key[j] = 0;
+            if (j * 32 >= E) break;
+            const int i = j * 32 + lane;
+            if (i < E) key[j] = mf_key(A.has_corr ? score(sv[i]) + __ldg(A.corr + i) : sv[i]);
+            if (key[j] > best) { best = key[j]; at = i; }
         }
-        float tot = 0.f, mine = 0.f;
-        int   id = 0;
+        int id = 0;
         for (int k = 0; k < A.top; k++) {
             const uint32_t top = __reduce_max_sync(0xffffffffu, best);
             const int bi = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
-            if (at == bi) {                                      // the owner looks for its next
-                cv[bi] = 0; best = 0; at = 0x7fffffff;
-                for (int i = lane; i < E; i += 32) if (cv[i] > best) { best = cv[i]; at = i; }
+            if (lane == k) id = bi;
+            const bool mine = at == bi;
+            if (mine) { best = 0; at = 0x7fffffff; }
+#pragma unroll
+            for (int j = 0; j < PL; j++) {
+                if (j * 32 >= E) break;
+                const int i = j * 32 + lane;
+                if (i == bi) key[j] = 0;
+                if (mine && key[j] > best) { best = key[j]; at = i; }
             }
-            const float v = score(z[bi]);
-            if (lane == k) { id = bi; mine = v; }
-            tot += v;
         }
+        const float mine = lane < A.top ? score(sv[id]) : 0.f, tot = warp_sum(mine);
         if (lane < A.top) { S.ids[tk][lane] = id; S.wts[tk][lane] = A.scale * (A.renorm ? mine / (tot + 1e-20f) : mine); }
         else if (lane < A.top + A.shared) { S.ids[tk][lane] = E + lane - A.top; S.wts[tk][lane] = 1.f; }
+        if (F8 && lane < 2) S.xm[tk][lane] = __ldcg(A.xm + 2 * tk + lane);
     }
     const int all = E + A.shared, per = A.top + A.shared;
     for (int i = threadIdx.x; i < all; i += MF_WARPS * 32) S.mask[i] = 0;
@@ -269,7 +278,12 @@ template <int COLS> __device__ __forceinline__ void mf_route(const mf_args & A, 
     mf_bar();
     for (int i = threadIdx.x; i < A.b * per; i += MF_WARPS * 32) {
         const int tk = i / per, e = S.ids[tk][i % per];
-        S.at[tk][i % per] = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
+        const int at = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
+        S.at[tk][i % per] = at;
+        if (F8) {                                                // the exponent fields of the powers of two of the pair's rows of x and h
+            S.px[at] = mf_exponent(S.xm[tk][0]);
+            S.ph[at] = mf_exponent(1.01f * sqrtf(__ldg(A.norms + 2 * e)) * sqrtf(__ldg(A.norms + 2 * e + 1)) * S.xm[tk][1]);
+        }
     }
 }
 
@@ -343,23 +357,28 @@ __device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const 
     const int n = __popc(mask), stride = (int) mf_row_of(F8, KB), plane = KB * (F8 ? 128 : 64);
     // row of a column, -1: none
     auto row_of = [&](int c) { c = PACK ? c & 3 : c; return c >= n ? -1 : UP ? mf_nth_bit(mask, c) : base + c; };
-    // the power of two of a token's row of x or h, as its exponent field
-    auto field_x = [&](int tk) { return mf_exponent(__ldcg(A.xm + 2 * tk)); };
-    auto field_h = [&](int tk) { return mf_exponent(1.01f * sqrtf(__ldg(A.norms + 2 * e)) * sqrtf(__ldg(A.norms + 2 * e + 1)) * __ldcg(A.xm + 2 * tk + 1)); };
     const int r = row_of(g);
     const uint16_t * row = r < 0 ? nullptr : (UP ? A.xp : A.hp) + (int64_t) r * stride + (PACK && g >= 4 ? plane : 0);
     float d[2] = { 1.f, 1.f };
     if (F8)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const int c = (t * 2 + k) & 3, tk = c >= n ? -1 : mf_nth_bit(mask, c);
-            d[k] = tk < 0 ? 1.f : mf_pow2(254 - (UP ? field_x(tk) : field_h(tk)));
+            const int c = (t * 2 + k) & 3;
+            d[k] = c < n ? mf_pow2(254 - (UP ? S.px : S.ph)[base + c]) : 1.f;
         }
     const float * sa = nullptr, * sb = nullptr;
     if (F8) {
         sa = UP ? A.s1 + ((int64_t) e * 2 * A.nb1 + i / 8) * A.KB1 : A.s2 + ((int64_t) e * A.nb2 + i / 4) * A.KB2;
         sb = UP ? sa + (int64_t) A.nb1 * A.KB1 : sa;
     }
+    // the scales of 32 of the warp's lines, one a lane
+    float ha = 0.f, hb = 0.f;
+    auto scales = [&](int j) {
+        const int kb = (j + lane) * MF_WARPS + warp;
+        ha = kb < KB ? __ldg(sa + kb) : 0.f;
+        hb = UP && kb < KB ? __ldg(sb + kb) : 0.f;
+    };
+    if (F8) scales(0);
     float acc[2][4];
 #pragma unroll
     for (int m = 0; m < 2; m++)
@@ -371,7 +390,12 @@ __device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const 
         const bool in = kb < KB;
         mf_b<F8, PACK> B;
         float wa = 1.f, wb = 1.f;
-        if (F8 && in) { wa = __ldg(sa + kb); wb = UP ? __ldg(sb + kb) : wa; }
+        if (F8) {
+            const int j = st / MF_WARPS;
+            if (j && (j & 31) == 0) scales(j);
+            wa = __shfl_sync(0xffffffffu, ha, j & 31);
+            wb = UP ? __shfl_sync(0xffffffffu, hb, j & 31) : wa;
+        }
         if (in) mf_ask<F8, PACK>(B, row, plane, kb, t);          // ahead of the wait
         if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_f + at.s * 8, at.ph, (volatile int *) &S.abort))) break;
         if (in) {
@@ -403,7 +427,7 @@ __device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const 
             const int c = q >> 4, k = q & 15;
             const float gt = sum(c, k), u = sum(c, 16 + k), h = gt / (1.0f + expf(-gt)) * u;
             uint16_t *  hrow = A.hp + (int64_t) (base + c) * mf_row_of(F8, A.KB2);
-            mf_store<F8>(h, F8 ? mf_pow2(field_h(mf_nth_bit(mask, c))) : 1.f, i, k, A.KB2, hrow);
+            mf_store<F8>(h, F8 ? mf_pow2(S.ph[base + c]) : 1.f, i, k, A.KB2, hrow);
             for (int z = i + 1; z < last; z++) mf_store<F8>(0.f, 1.f, z, k, A.KB2, hrow);
         }
     } else
@@ -418,7 +442,7 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
     const uint32_t bar_f = dt_smem(S.bars), bar_e = bar_f + MF_STAGES * 8, bar_w = bar_e + MF_STAGES * 8, bar_p = bar_w + 16;
     volatile int * abort_s = (volatile int *) &S.abort;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MF_STAGES; s++) { dt_mbar_init(bar_f + s * 8, 1); dt_mbar_init(bar_e + s * 8, MF_WARPS); }
+        for (int s = 0; s < MF_STAGES; s++) { dt_mbar_init(bar_f + s * 8, 2); dt_mbar_init(bar_e + s * 8, MF_WARPS); }
         for (int s = 0; s < 2; s++) { dt_mbar_init(bar_w + s * 8, MF_WARPS); dt_mbar_init(bar_p + s * 8, 1); }
         S.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -428,7 +452,7 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
     pib_pdl_trigger();
     int ticket = 0;
     if (warp == MF_WARPS && lane == 0) ticket = atomicAdd(A.cnt, 1);
-    if (warp < MF_WARPS) mf_route<F8 ? 4 : 8>(A, S, warp, lane);
+    if (warp < MF_WARPS) mf_route<F8>(A, S, warp, lane);
     __syncthreads();
     const int per = A.top + A.shared, ups = S.n_act * A.T1, items = ups + S.n_act * A.T2;
     int * done_up = A.cnt + 2, * done_rows = done_up + A.b * per;
@@ -450,11 +474,26 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
                     dt_mbar_expect_tx(bar_f + s * 8, bytes);
                     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                                  ::"r"(dt_smem(ring) + s * MF_STAGE), "l"(src + (int64_t) st * MF_LINE), "r"(bytes), "r"(bar_f + s * 8) : "memory");
+                    // the second arrival says that what a down item multiplies with is there
+                    if (!up && st == 0) {
+                        ok = false;
+                        for (uint32_t it = 0; it < MF_SPIN && !ok; it++) {
+                            int v, stop;
+                            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done_up + a) : "memory");
+                            ok = v >= A.T1;
+                            if (!ok && (it & 63) == 63) {
+                                asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(stop) : "l"(A.cnt + 1) : "memory");
+                                if (stop || *abort_s) break;
+                            }
+                        }
+                        if (!ok) { *abort_s = 1; atomicExch(A.cnt + 1, 1); break; }
+                    }
+                    dt_arrive(bar_f + s * 8);
                     if (++s == MF_STAGES) { s = 0; ph ^= 1; }
                 }
                 item = next;
             }
-            if (ok && dt_mbar_wait(bar_e + s * 8, ph, abort_s)) { S.item[s] = -1; dt_arrive(bar_f + s * 8); }
+            if (ok && dt_mbar_wait(bar_e + s * 8, ph, abort_s)) { S.item[s] = -1; dt_arrive(bar_f + s * 8); dt_arrive(bar_f + s * 8); }
         }
     } else if (warp == MF_WARPS + 1) {
         // publisher: in the order of the block's items
@@ -503,22 +542,6 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
             }
             const bool up = item < ups;
             const int  a = !ok ? 0 : up ? item / A.T1 : (item - ups) / A.T2, i = !ok ? 0 : up ? item % A.T1 : (item - ups) % A.T2;
-            if (!up && ok) {
-                if (lane == 0) {
-                    ok = false;
-                    for (uint32_t it = 0; it < MF_SPIN && !ok; it++) {
-                        int v, stop;
-                        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done_up + a) : "memory");
-                        ok = v >= A.T1;
-                        if (!ok && (it & 63) == 63) {
-                            asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(stop) : "l"(A.cnt + 1) : "memory");
-                            if (stop) break;
-                        }
-                    }
-                    if (!ok) { *abort_s = 1; atomicExch(A.cnt + 1, 1); }
-                }
-                __syncwarp();
-            }
             if (up) mf_item<F8, true>(A, S, ring, bar_f, bar_e, at, turn, a, i);
             else    mf_item<F8, false>(A, S, ring, bar_f, bar_e, at, turn, a, i);
             if (*abort_s) break;                                 // raised in front of mf_item's barrier: every warp sees it and leaves here
