@@ -20,7 +20,9 @@
 // the eight columns of one MMA; an expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which
 // costs less than a second form of the kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
 // a row (lane t) are four values each of four (two) neighbouring tiles of 16, the k of an MMA, and the parts lie in that order too.
-// What bounds it: ??
+// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in 316 us (0.76 of the copy rate; the choice takes some 10 us of it, the turns of 48 KB down items the
+// rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 31 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
+// way to memory and back each.  Sharing the choice among the blocks would save none of it: the launch's first 4 us are mostly the way of its code into the caches.
 #include <cuda_bf16.h>
 
 #include "f8_block.cuh"
@@ -35,6 +37,12 @@
 #define MF_STAGE   (MF_WARPS * MF_LINE)
 #define MF_STAGES  3
 #define mf_bar()   asm volatile("bar.sync 1, 192;" ::: "memory")          // the consumers
+// the same; true in all of them if it is in one: they leave together or not at all
+__device__ __forceinline__ bool mf_bar_or(bool v) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 192, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t) v) : "memory");
+    return any != 0;
+}
 
 struct pib_moe {
     pib_moe_shape s;
@@ -348,9 +356,9 @@ template <bool F8, bool PACK> __device__ __forceinline__ void mf_half(const uint
         for (int j = 0; j < 4; j++) acc[m][j] = F8 ? fmaf(s[m][j], f[m][j & 1], acc[m][j]) : acc[m][j] + s[m][j];
 }
 
-// An item, by the consumers: the warp's lines of its pieces, the meeting, the results.  turn: the item's turn at the places of the sums
+// An item, by the consumers: the warp's lines of its pieces, the meeting, the results.  turn: the item's turn at the places of the sums.  False: the block gives up
 template <bool F8, bool UP>
-__device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const uint8_t * ring, uint32_t bar_f, uint32_t bar_e, mf_place & at, int turn, int a, int i) {
+__device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const uint8_t * ring, uint32_t bar_f, uint32_t bar_e, mf_place & at, int turn, int a, int i) {
     constexpr bool PACK = F8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, e = S.act[a], base = S.base[a], KB = UP ? A.KB1 : A.KB2;
     const uint32_t mask = S.tokens[a];
@@ -414,7 +422,7 @@ __device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const 
     for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int q = 0; q < 4; q++) red[warp][t * 2 + (q & 1)][m * 16 + gp + (q >> 1) * 8] = acc[m][q];
-    mf_bar();
+    if (mf_bar_or(*(volatile int *) &S.abort)) return false;
     auto sum = [&](int c, int k) {
         float x = 0.f;
 #pragma unroll
@@ -432,6 +440,7 @@ __device__ __forceinline__ void mf_item(const mf_args & A, mf_shared & S, const 
         }
     } else
         for (int q = threadIdx.x; q < n * 32; q += MF_WARPS * 32) __stcg(A.part + (int64_t) (base + (q >> 5)) * A.Dr + i * 32 + (q & 31), sum(q >> 5, q & 31));
+    return true;
 }
 
 template <bool F8>
@@ -538,13 +547,13 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
             if (item < 0) {
                 __syncwarp();
                 if (lane == 0) { if (warp == 0) S.pub[turn] = -1; dt_arrive(bar_w + turn * 8); }
+                mf_bar_or(false);                                // a warp whose wait ran out stands in mf_item's
                 break;
             }
             const bool up = item < ups;
             const int  a = !ok ? 0 : up ? item / A.T1 : (item - ups) / A.T2, i = !ok ? 0 : up ? item % A.T1 : (item - ups) % A.T2;
-            if (up) mf_item<F8, true>(A, S, ring, bar_f, bar_e, at, turn, a, i);
-            else    mf_item<F8, false>(A, S, ring, bar_f, bar_e, at, turn, a, i);
-            if (*abort_s) break;                                 // raised in front of mf_item's barrier: every warp sees it and leaves here
+            const bool go = up ? mf_item<F8, true>(A, S, ring, bar_f, bar_e, at, turn, a, i) : mf_item<F8, false>(A, S, ring, bar_f, bar_e, at, turn, a, i);
+            if (!go) break;
             __syncwarp();
             if (lane == 0) { if (warp == 0) S.pub[turn] = item; dt_arrive(bar_w + turn * 8); }
             if (!(turn ^= 1)) pph ^= 1;

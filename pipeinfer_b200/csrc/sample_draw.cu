@@ -16,7 +16,8 @@
 //   4  the weights' sums of what is kept, per chunk, and the walk through one chunk (not where step 3 gathered everything that is kept)
 // Among gathered tokens each finds what lies ahead of it by comparing with all.  Where a list would be too long (thousands of equal logits, say) sd_select narrows the threshold
 // down by histograms over the order's own bits instead.
-// What bounds it: ??
+// What bounds it: the arithmetic and shared memory of an SM's walks over its slice, not the memory (64 rows of 128 256: 61 us with mixed settings, the bytes take 5).  64 rows of 128 256
+// with a block each: greedy (one walk) 15 us, top-k 32, min-p 41, no truncation 54 (a dozen fp64 steps for a weight), top-p 130 (three walks that form weights, one with atomics beside it).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -32,6 +33,7 @@
 #define SD_PER     256.0f                     // bins for a difference of 1
 #define SD_LIST    2048
 #define SD_POW     1024
+#define SD_SLICE   4096                       // ids of a block at least, where a row is divided
 #define SD_CHUNK   256
 #define SD_CHUNKS  (PIB_SAMPLE_MAX_VOCAB / SD_CHUNK + 1)
 
@@ -767,8 +769,12 @@ template <typename T>
 static int sd_launch(const void * logits, int64_t ld, int rows, int V, const pib_sample_params * params, const float * u, int32_t * ids, float * p, int32_t * kept, cudaStream_t st) {
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(sample_draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) sizeof(sd_shared)); }));
+    // Blocks of a row: as many as run at a time (two per SM), a slice holding 4096 ids or more.  us for 1, 2, 4, 8 blocks, top-p 0.9 and top-k 40:
+    //   1 row of 32 000      47 34 27 24   15 15 14 16        64 rows of 128 256   130  80  69  97   32 27 26 46
+    //   64 rows of 32 000    48 36 35 64   15 17 18 39        300 rows of 50 257   143 146 193 330   46 61 94 194
+    //   40 rows of 8 000     28 25 28 53   11 14 17 36        100 rows of 128 256  132 108 111 163   35 33 47 81
     int P = 1;
-    while (P < 8 && (int64_t) rows * P * 2 <= 2 * pib_num_sms() && V >= P * 4 * SD_THREADS) P <<= 1;
+    while (P < 8 && (int64_t) rows * P * 2 <= 2 * pib_num_sms() && V >= P * 2 * SD_SLICE) P <<= 1;
     for (int r0 = 0; r0 < rows; r0 += 1 << 20) {
         const int n = rows - r0 < 1 << 20 ? rows - r0 : 1 << 20;
         PIB_CHECK(pib_launch_cluster(sample_draw_kernel<T>, dim3((unsigned) n, (unsigned) P), dim3(SD_THREADS), dim3(1, (unsigned) P, 1), sizeof(sd_shared), st, (const T *) logits + r0 * ld, ld, V,
