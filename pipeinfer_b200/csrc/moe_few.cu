@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #define MF_WARPS   6                          // consumers; with the producer and the publisher eight warps, and 128 registers a thread in two blocks per SM
+#define MF_LT      4                          // tokens of a block of router outputs, where there are several
 #define MF_THREADS (MF_WARPS * 32 + 64)
 #define MF_SPIN    (1u << 22)
 #define MF_LINE    4096                       // 128 bytes of 32 rows
@@ -128,11 +129,15 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
                                                                                     float * __restrict__ z, int * __restrict__ cnt, int n_cnt, int KB, uint16_t * __restrict__ xp, float * __restrict__ xm) {
     __shared__ float red[8][NT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int out = blockIdx.x % E, t0 = blockIdx.x / E * NT, groups = (b + NT - 1) / NT;
+    const bool split = (int) blockIdx.x >= groups * E;
+    const float * r = R + (int64_t) out * D;
+    if (!split) for (int64_t k = (int64_t) threadIdx.x * 32; k < D; k += 256 * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + k));     // the layer's own, ahead of the wait
     pib_pdl_wait();
     pib_pdl_trigger();
     if (blockIdx.x == 0) for (int i = threadIdx.x; i < n_cnt; i += 256) cnt[i] = 0;
-    if (blockIdx.x >= E) {
-        const int t = blockIdx.x - E;
+    if (split) {
+        const int t = blockIdx.x - groups * E;
         float up = 1.f;
         if (F8) {
             __shared__ float sq[8];
@@ -149,25 +154,25 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
         for (int u = threadIdx.x; u < KB * (F8 ? 128 : 64); u += 256) mf_store<F8>(u < D ? x[t * ldx + u] : 0.f, up, u >> 4, u & 15, KB, xp + t * mf_row_of(F8, KB));
         return;
     }
-    const float * r = R + (int64_t) blockIdx.x * D;
+    // a token behind the last is the last one again: no branch between the loads (with one per token a row of 4096 took 12 us for 16 tokens)
     float acc[NT];
+    const float * xt[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = 0.f;
+    for (int t = 0; t < NT; t++) { acc[t] = 0.f; xt[t] = x + min(t0 + t, b - 1) * ldx; }
     if (vec) {
         for (int64_t k = threadIdx.x * 4; k < D; k += 1024) {
             const float4 w = *reinterpret_cast<const float4 *>(r + k);
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                if (t < b) {
-                    const float4 v = *reinterpret_cast<const float4 *>(x + t * ldx + k);
-                    acc[t] = fmaf(w.x, v.x, fmaf(w.y, v.y, fmaf(w.z, v.z, fmaf(w.w, v.w, acc[t]))));
-                }
+            for (int t = 0; t < NT; t++) {
+                const float4 v = *reinterpret_cast<const float4 *>(xt[t] + k);
+                acc[t] = fmaf(w.x, v.x, fmaf(w.y, v.y, fmaf(w.z, v.z, fmaf(w.w, v.w, acc[t]))));
+            }
         }
     } else {
         for (int64_t k = threadIdx.x; k < D; k += 256) {
             const float w = r[k];
 #pragma unroll
-            for (int t = 0; t < NT; t++) if (t < b) acc[t] = fmaf(w, x[t * ldx + k], acc[t]);
+            for (int t = 0; t < NT; t++) acc[t] = fmaf(w, xt[t][k], acc[t]);
         }
     }
 #pragma unroll
@@ -176,17 +181,19 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
         if (lane == 0) red[warp][t] = acc[t];
     }
     __syncthreads();
-    if (threadIdx.x < b) {
+    if (threadIdx.x < NT && t0 + threadIdx.x < b) {
         float s = 0.f;
+#pragma unroll
         for (int i = 0; i < 8; i++) s += red[i][threadIdx.x];
-        z[threadIdx.x * E + blockIdx.x] = s;
+        z[(t0 + threadIdx.x) * E + out] = s;
     }
 }
 
 // ---- the layer ----------------------------------------------------------------------------------------------------------------------
 struct mf_shared {
-    float    wts[16][16], xm[16][2];
-    int      px[256], ph[256];            // of a pair
+    float    wts[16][16];
+    uint16_t pf[16][16];                  // of a choice; px, ph: of a pair (a row)
+    int      px[256], ph[256];
     int      ids[16][16], at[16][16];     // chosen experts of a token; its row of h and of the experts' outputs
     uint32_t mask[PIB_MOE_MAX_EXPERTS + 16], tokens[256];        // of an expert, of an entry of the list
     int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[256], n_act, item[MF_STAGES], pub[2], abort;
@@ -210,6 +217,8 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
     float * sv = &S.red[0][0][0][0] + warp * PIB_MOE_MAX_EXPERTS;        // the token's logits, then its scores
     for (int tk = warp; tk < A.b; tk += MF_WARPS) {
         const float * z = A.z + tk * E;
+        float xmax = 0.f, xsum = 0.f;
+        if (F8) { xmax = __ldcg(A.xm + 2 * tk); xsum = __ldcg(A.xm + 2 * tk + 1); }
         float mx = -INFINITY, sum = 1.f;
         for (int i = lane; i < E; i += 32) { const float v = __ldcg(z + i); sv[i] = v; mx = fmaxf(mx, v); }
         if (A.score == PIB_MOE_SOFTMAX) {
@@ -247,10 +256,17 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
                 if (mine && key[j] > best) { best = key[j]; at = i; }
             }
         }
+        if (lane >= A.top) id = E + lane - A.top;
+        const bool has = lane < A.top + A.shared;
+        float ng = 0.f, nu = 0.f;
+        if (F8 && has) { ng = __ldg(A.norms + 2 * id); nu = __ldg(A.norms + 2 * id + 1); }
         const float mine = lane < A.top ? score(sv[id]) : 0.f, tot = warp_sum(mine);
-        if (lane < A.top) { S.ids[tk][lane] = id; S.wts[tk][lane] = A.scale * (A.renorm ? mine / (tot + 1e-20f) : mine); }
-        else if (lane < A.top + A.shared) { S.ids[tk][lane] = E + lane - A.top; S.wts[tk][lane] = 1.f; }
-        if (F8 && lane < 2) S.xm[tk][lane] = __ldcg(A.xm + 2 * tk + lane);
+        if (has) {
+            S.ids[tk][lane] = id;
+            S.wts[tk][lane] = lane < A.top ? A.scale * (A.renorm ? mine / (tot + 1e-20f) : mine) : 1.f;
+            // the exponent fields of the powers of two of the pair's rows of x and h
+            if (F8) S.pf[tk][lane] = (uint16_t) (mf_exponent(xmax) | mf_exponent(1.01f * sqrtf(ng) * sqrtf(nu) * xsum) << 8);
+        }
     }
     const int all = E + A.shared, per = A.top + A.shared;
     for (int i = threadIdx.x; i < all; i += MF_WARPS * 32) S.mask[i] = 0;
@@ -288,10 +304,7 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
         const int tk = i / per, e = S.ids[tk][i % per];
         const int at = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
         S.at[tk][i % per] = at;
-        if (F8) {                                                // the exponent fields of the powers of two of the pair's rows of x and h
-            S.px[at] = mf_exponent(S.xm[tk][0]);
-            S.ph[at] = mf_exponent(1.01f * sqrtf(__ldg(A.norms + 2 * e)) * sqrtf(__ldg(A.norms + 2 * e + 1)) * S.xm[tk][1]);
-        }
+        if (F8) { S.px[at] = S.pf[tk][i % per] & 255; S.ph[at] = S.pf[tk][i % per] >> 8; }
     }
 }
 
@@ -700,12 +713,12 @@ extern "C" int pib_moe_forward(const pib_moe * m, const float * x, int64_t ldx, 
     uint16_t * xp = (uint16_t *) (sc + L.xp);
     A.cnt = (int *) sc; A.z = z; A.xp = xp; A.xm = xm; A.norms = m->norms; A.hp = (uint16_t *) (sc + L.hp); A.part = (float *) (sc + L.part);
     if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_moe_forward: no memory for the error word"); return PIB_ERR_NOMEM; }
-    const dim3 rg((unsigned) (A.E + b)), rb(256);
-    const int  vec = ldx % 4 == 0 && !((uintptr_t) x & 15) && D % 4 == 0;
+    const int  vec = ldx % 4 == 0 && !((uintptr_t) x & 15) && D % 4 == 0, nt = b == 1 ? 1 : MF_LT;
+    const dim3 rg((unsigned) (A.E * ((b + nt - 1) / nt) + b)), rb(256);
     const bool f8 = m->s.type == PIB_TYPE_F8;
 #define MF_LOGITS(F8, NT) PIB_CHECK(pib_launch(moe_logits_kernel<F8, NT>, rg, rb, 0, st, m->router, x, ldx, b, A.E, D, vec, z, A.cnt, L.n_cnt, A.KB1, xp, xm))
-    if (f8) { if (b == 1) MF_LOGITS(true, 1); else if (b <= 4) MF_LOGITS(true, 4); else MF_LOGITS(true, 16); }
-    else    { if (b == 1) MF_LOGITS(false, 1); else if (b <= 4) MF_LOGITS(false, 4); else MF_LOGITS(false, 16); }
+    if (f8) { if (b == 1) MF_LOGITS(true, 1); else MF_LOGITS(true, MF_LT); }
+    else    { if (b == 1) MF_LOGITS(false, 1); else MF_LOGITS(false, MF_LT); }
 #undef MF_LOGITS
     const dim3 grid((unsigned) (2 * pib_num_sms())), block(MF_THREADS);
     static pib_per_device attrs;
