@@ -37,6 +37,9 @@ int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const floa
 int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st);
 int pib_f8_gemm_pair(const pib_weight * w, const void * act, int b, float * y, int * err, cudaStream_t st);
 int pib_f8_gemm_host(const pib_weight * w, const float * x_host, int b, float * y_host);
+// the tensor maps of a matrix, made with it (pib_weight::map): boxes of 32, 64, 96 and 128 rows of a block, 128 rows of two blocks (f8_gemm.cu), 16 rows of 16 blocks (f8_gemv.cu), 128 rows (f8_gemm_pair.cu)
+struct pib_f8_runs { CUtensorMap m[5]; };
+struct pib_f8_maps { pib_f8_runs runs; CUtensorMap stage, block; };
 int pib_f8_map(CUtensorMap * map, const void * base, int64_t rows, int box);                   // f8_gemm.cu: rows of 128 bytes, boxes of `box` rows, 128-byte swizzle (these three)
 int pib_f8_map3(CUtensorMap * map, const void * base, int64_t rows, int64_t groups, int64_t group_bytes, int box_rows, int box_groups);      // groups of rows of 128 bytes
 int pib_f8_map4(CUtensorMap * map, const void * base, int64_t KB, int64_t NB, int box_rows, int box_kb);      // the weights' blocks: boxes of some rows of some blocks of one row block

@@ -8,8 +8,11 @@
 //   warp 10      streams the blocks' activation scales through a ring of their own
 //   warp 1       issues the MMAs; a commit hands the operands back, another says that the accumulator is there
 //   warps 2..9   two groups of four, half of the columns each: a thread owns a weight row (lane) and adds acc[c] += P[c] (s d[c])
-// The CTAs walk the tiles (128 rows x NB tokens).  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks each and add their sums up through
-// distributed shared memory, in share order.
+// The CTAs walk tiles of up to 128 rows, all the tokens wide (NB: 16 .. 128, the smallest that holds them), each CTA a part of the rows (ft_grain).  Where the tiles leave most SMs idle, 2, 4 or 8
+// CTAs of a cluster take a share of the blocks each and add their sums up through distributed shared memory, in share order.  (Clusters that share every tile of a longer walk lose: a meeting
+// costs 3 us, 21 999 x 5700 with 13 tokens takes 36 us on pairs and 41 on fours instead of 29.)
+// What bounds it: up to 48 tokens the weights' way from memory and an uneven last tile (57344 x 8192, 13 tokens: 88 us, 0.83 of the copy rate; 10240 x 8192, 40 tokens: 23 us on 80 SMs, 19 without
+// any sums); beyond, reading the accumulators and adding them up (28672 x 8192, 128 tokens: 70 us, 1 000 clocks a block, of which the MMAs take 256).
 // Every wait is bounded (tc_common.cuh).
 #include "f8_block.cuh"
 #include "tc_common.cuh"
@@ -40,6 +43,9 @@ __device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
 __device__ __forceinline__ void ft_tma_2d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void ft_tma_4d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int y, int z, int u) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(z), "r"(u) : "memory");
+}
 __device__ __forceinline__ void ft_tma_3d(uint32_t dst, const CUtensorMap * map, uint32_t bar, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y), "r"(z) : "memory");
 }
@@ -49,21 +55,34 @@ __device__ __forceinline__ void ft_bulk(uint32_t dst, const void * src, uint32_t
 __device__ __forceinline__ uint32_t ft_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t ft_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
 __device__ __forceinline__ void ft_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void ft_ld(uint32_t at, uint32_t (&v)[N]) {
+    if constexpr (N == 32) dt_ld32(at, v);
+    else if constexpr (N == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                       "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at) : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(at) : "memory");
+}
 // M x N outputs of e4m3 x e4m3, fp32 accumulators, both operands K-major
 __host__ __device__ constexpr uint32_t ft_idesc(int M, int N) { return (1u << 4) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
 
 struct ft_args {
-    int b, KB, bp, tiles_m, tiles, shares;
+    int b, KB, bp, runs, shares;                                 // runs: of 32 rows, in all
     int64_t N;
     const float * ws, * ad;
     float * y;
     int * err;
 };
 
+// A CTA's rows begin at a multiple of so many runs of 32.  One divides the rows more evenly, four leave the weights' scales the same in all warps.  us with 1, with 4:
+//   21 999 x 5700, 13 tokens  29.6  32.4      28 672 x 8192, 64 tokens  52  49      10 240 x 8192, 40 tokens  23.9  23.0      28 672 x 8192, 128 tokens  73  69
+__host__ __device__ constexpr int ft_grain(int NB) { return NB <= 32 ? 1 : 4; }
 template <int NB>
 __global__ void __launch_bounds__(FT_THREADS, 1)
-f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ ft_args A) {
-    constexpr int KPS = FT_KPS, STAGE = KPS * (FT_A_TILE + NB * 128), STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, ACCS = 512 / (KPS * NB), HALF = NB / 2;
+f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ ft_args A) {
+    constexpr int KPS = FT_KPS, STAGE = KPS * (FT_A_TILE + NB * 128), STAGES = FT_RING / STAGE < FT_STAGES ? FT_RING / STAGE : FT_STAGES, PITCH = NB <= 16 ? 16 : NB <= 32 ? 32 : NB <= 64 ? 64 : 128, ACCS = 512 / (KPS * PITCH), HALF = NB / 2, GRAIN = ft_grain(NB);
     extern __shared__ __align__(1024) uint8_t ft_dsm[];
     uint8_t *  sm  = ft_dsm + ((1024u - (dt_smem(ft_dsm) & 1023u)) & 1023u);
     float *    dsc = reinterpret_cast<float *>(sm + FT_RING);                            // scale rows, KPS of 128 floats a place
@@ -72,8 +91,10 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FT_STAGES * 8, bar_d = bar_e + FT_STAGES * 8, bar_g = bar_d + FT_DRING * 8, bar_t = bar_g + FT_DRING * 8, bar_r = bar_t + 16 * 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = A.shares, share = S > 1 ? (int) ft_rank() : 0;
+    // the rows of a CTA (cluster) are neighbours, in runs of 32; its tiles take up to four runs each, as alike as can be
     const int unit = blockIdx.x / S, units = gridDim.x / S;
-    const int tile0 = (int) ((int64_t) A.tiles * unit / units), tile1 = (int) ((int64_t) A.tiles * (unit + 1) / units);
+    const int grains = (A.runs + GRAIN - 1) / GRAIN, r0 = (int) ((int64_t) grains * unit / units) * GRAIN;
+    const int runs = min(A.runs, (int) ((int64_t) grains * (unit + 1) / units) * GRAIN) - r0, tiles = (runs + 3) / 4, each = runs / tiles, more = runs % tiles;
     const int k0 = (int) ((int64_t) A.KB * share / S), nk = (int) ((int64_t) A.KB * (share + 1) / S) - k0;
     const uint32_t sm0 = dt_smem(sm);
 
@@ -99,15 +120,22 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     if (warp == 0) {
         int s = 0;
         uint32_t ph = 1;                                         // the first round finds its places free
-        for (int tile = tile0; tile < tile1 && ok && lane == 0; tile++) {
-            const int n_tile = tile / A.tiles_m, m0 = tile % A.tiles_m * NB;
+        for (int tile = 0; tile < tiles && ok && lane == 0; tile++) {
+            // rows of the tile in one block of the weights' layout, and in the next
+            const int t0 = r0 + tile * each + min(tile, more), n = each + (tile < more), n1 = GRAIN == 4 ? n : min(n, 4 - (t0 & 3)), n2 = n - n1;
             for (int kt = 0; kt < nk; kt += KPS) {
                 ok = dt_mbar_wait(bar_e + s * 8, ph, abort_s);
                 if (!ok) break;
-                // what a share's last copy takes of the next blocks is not used
-                dt_mbar_expect_tx(bar_f + s * 8, STAGE);
-                ft_tma_2d(sm0 + s * STAGE, &wmap, bar_f + s * 8, 0, (n_tile * A.KB + k0 + kt) * 128);
-                ft_tma_3d(sm0 + s * STAGE + KPS * FT_A_TILE, &xmap, bar_f + s * 8, m0, k0 + kt);
+                const int      ks = n1 == 4 ? KPS : min(KPS, nk - kt);         // (what a share's last copies take of the next block is not used)
+                const uint32_t to = sm0 + s * STAGE;
+                dt_mbar_expect_tx(bar_f + s * 8, ks * n * 4096 + KPS * NB * 128);
+                static_assert(KPS == 2, "a copy of whole blocks");
+                if (n1 == 4) ft_tma_2d(to, &wmaps.m[4], bar_f + s * 8, 0, (t0 / 4 * A.KB + k0 + kt) * 128);
+                else for (int j = 0; j < ks; j++) {
+                    ft_tma_4d(to + j * FT_A_TILE, &wmaps.m[n1 - 1], bar_f + s * 8, t0 % 4 * 32, k0 + kt + j, t0 / 4);
+                    if (n2) ft_tma_4d(to + j * FT_A_TILE + n1 * 4096, &wmaps.m[n2 - 1], bar_f + s * 8, 0, k0 + kt + j, t0 / 4 + 1);
+                }
+                ft_tma_3d(to + KPS * FT_A_TILE, &xmap, bar_f + s * 8, 0, k0 + kt);
                 if (++s == STAGES) { s = 0; ph ^= 1; }
             }
         }
@@ -115,15 +143,14 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     } else if (warp == 10) {
         int ds = 0;
         uint32_t dph = 1;
-        for (int tile = tile0; tile < tile1 && ok && lane == 0; tile++) {
-            const int m0 = tile % A.tiles_m * NB;
-            const uint32_t dbytes = (uint32_t) min(NB, A.bp - m0) * 4;
+        const uint32_t dbytes = (uint32_t) min(NB, A.bp) * 4;
+        for (int tile = 0; tile < tiles && ok && lane == 0; tile++) {
             for (int kt = 0; kt < nk; kt += KPS) {
                 ok = dt_mbar_wait(bar_g + ds * 8, dph, abort_s);
                 if (!ok) break;
                 const int n = min(KPS, nk - kt);
                 dt_mbar_expect_tx(bar_d + ds * 8, n * dbytes);
-                for (int j = 0; j < n; j++) ft_bulk(dt_smem(dsc + (ds * KPS + j) * 128), A.ad + (int64_t) (k0 + kt + j) * A.bp + m0, dbytes, bar_d + ds * 8);
+                for (int j = 0; j < n; j++) ft_bulk(dt_smem(dsc + (ds * KPS + j) * 128), A.ad + (int64_t) (k0 + kt + j) * A.bp, dbytes, bar_d + ds * 8);
                 if (++ds == FT_DRING) { ds = 0; dph ^= 1; }
             }
         }
@@ -132,7 +159,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         const uint64_t d0 = dt_desc(sm0);
         int s = 0, a = 0;
         uint32_t ph = 0, aph = 1;
-        for (int tile = tile0; tile < tile1 && ok; tile++)
+        for (int tile = 0; tile < tiles && ok; tile++)
             for (int kt = 0; kt < nk; kt += KPS) {
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_r + a * 8, aph, abort_s) && dt_mbar_wait(bar_f + s * 8, ph, abort_s));
                 if (!ok) break;
@@ -140,7 +167,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 #pragma unroll
                 for (int j = 0; j < KPS; j++) {
                     const uint64_t ad = d0 + (uint64_t) ((s * STAGE + j * FT_A_TILE) >> 4), bd = d0 + (uint64_t) ((s * STAGE + KPS * FT_A_TILE + j * NB * 128) >> 4);
-                    if (kt + j < nk) ft_mma(tmem + (a * KPS + j) * NB, ad, bd, ft_idesc(FT_BM, NB));
+                    if (kt + j < nk) ft_mma(tmem + (a * KPS + j) * PITCH, ad, bd, ft_idesc(FT_BM, NB));
                 }
                 dt_commit(bar_t + a * 8);
                 dt_commit(bar_e + s * 8);
@@ -153,10 +180,14 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         float acc[HALF];
         int a = 0, ds = 0;
         uint32_t aph = 0, dph = 0;
-        for (int tile = tile0; tile < tile1 && ok; tile++) {
-            const int64_t n = (int64_t) (tile / A.tiles_m) * FT_BM + q4 * 32 + lane;
-            const int m0 = tile % A.tiles_m * NB + hf * HALF;
-            const float * ws = A.ws + (int64_t) (tile / A.tiles_m) * A.KB + k0;
+        for (int tile = 0; tile < tiles && ok; tile++) {
+            const int  t0 = r0 + tile * each + min(tile, more), run = t0 + q4;      // the warp's rows
+            const bool in  = q4 < each + (tile < more);
+            const int64_t n = (int64_t) run * 32 + lane;
+            int m0 = hf * HALF;
+            asm volatile("" : "+r"(m0));                         // keeps the outputs' addresses from being made, and held, ahead of the tiles
+            // (a warp without rows goes along: a branch of its own in front of tcgen05.ld costs the others a tenth)
+            const float * ws = A.ws + (int64_t) (GRAIN == 4 ? t0 / 4 : in ? run / 4 : 0) * A.KB + k0;
 #pragma unroll
             for (int c = 0; c < HALF; c++) acc[c] = 0.f;
             for (int kt = 0; kt < nk; kt += KPS) {
@@ -166,21 +197,16 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_d + ds * 8, dph, abort_s) && dt_mbar_wait(bar_t + a * 8, aph, abort_s));
                 if (!ok) break;
                 dt_fence_after();
-                constexpr int STEP = HALF < 32 ? HALF : 32;
+                constexpr int STEP = HALF % 32 == 0 ? 32 : HALF % 16 == 0 ? 16 : 8;
 #pragma unroll
                 for (int j = 0; j < KPS; j++) {
                     if (kt + j >= nk) break;
                     const float4 * dv = reinterpret_cast<const float4 *>(dsc + (ds * KPS + j) * 128 + hf * HALF);
-                    const uint32_t at = tmem + lanes + (a * KPS + j) * NB + hf * HALF;
+                    const uint32_t at = tmem + lanes + (a * KPS + j) * PITCH + hf * HALF;
 #pragma unroll
                     for (int c0 = 0; c0 < HALF; c0 += STEP) {
-                        uint32_t v[32];
-                        if (STEP == 32) dt_ld32(at + c0, v);
-                        else {
-                            asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                                           "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at + c0) : "memory");
-                        }
+                        uint32_t v[STEP];
+                        ft_ld<STEP>(at + c0, v);
                         dt_wait_ld();
 #pragma unroll
                         for (int c = 0; c < STEP; c += 4) {
@@ -200,7 +226,7 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             }
             if (!ok) break;
             if (S == 1) {
-                if (n < A.N)
+                if (in && n < A.N)
 #pragma unroll
                     for (int c = 0; c < HALF; c++) if (m0 + c < A.b) A.y[(int64_t) (m0 + c) * A.N + n] = acc[c];
             } else {
@@ -216,16 +242,15 @@ f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         ft_cluster_sync();
         if (warp >= 2 && warp < 10 && !*abort_s) {
             const int q4 = warp & 3, hf = (warp - 2) >> 2;
-            const int64_t n = (int64_t) (unit / A.tiles_m) * FT_BM + q4 * 32 + lane;
-            const int m0 = unit % A.tiles_m * NB;
-            for (int c = share * 2 + hf; c < NB && m0 + c < A.b; c += S * 2) {
+            const int64_t n = (int64_t) (r0 + q4) * 32 + lane;
+            for (int c = share * 2 + hf; c < NB && c < A.b; c += S * 2) {
                 float v = 0.f;
                 for (int sh = 0; sh < S; sh++) {
                     float o;
                     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(ft_mapa(sm0 + (uint32_t) (c * FT_BM + q4 * 32 + lane) * 4, (uint32_t) sh)) : "memory");
                     v += o;
                 }
-                if (n < A.N) A.y[(int64_t) (m0 + c) * A.N + n] = v;
+                if (q4 < runs && n < A.N) A.y[(int64_t) c * A.N + n] = v;
             }
         }
     }
@@ -278,11 +303,11 @@ int pib_f8_map4(CUtensorMap * map, const void * base, int64_t KB, int64_t NB, in
     return ft_map(map, base, 4, size, stride, bx);
 }
 
-template <int NB> static int ft_launch(const CUtensorMap & wmap, const CUtensorMap & xmap, ft_args A, cudaStream_t st) {
+template <int NB> static int ft_launch(const pib_f8_runs & wmaps, const CUtensorMap & xmap, ft_args A, cudaStream_t st) {
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(f8_gemm_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) FT_SMEM); }));
-    const int units = A.shares > 1 ? A.tiles : std::min(A.tiles, pib_num_sms());
-    PIB_CHECK(pib_launch_cluster(f8_gemm_kernel<NB>, dim3((unsigned) (units * A.shares)), dim3(FT_THREADS), dim3((unsigned) A.shares, 1, 1), FT_SMEM, st, wmap, xmap, A));
+    const int units = A.shares > 1 ? (A.runs + 3) / 4 : std::min((A.runs + ft_grain(NB) - 1) / ft_grain(NB), pib_num_sms());
+    PIB_CHECK(pib_launch_cluster(f8_gemm_kernel<NB>, dim3((unsigned) (units * A.shares)), dim3(FT_THREADS), dim3((unsigned) A.shares, 1, 1), FT_SMEM, st, wmaps, xmap, A));
     return PIB_OK;
 }
 
@@ -294,22 +319,24 @@ int pib_f8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     int * err = pib_tc_error_word(st);
     if (!err) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
     if (b > 128) return pib_f8_gemm_pair(w, act, b, y, err, st);
-    const int NB = b <= 32 ? 32 : b <= 64 ? 64 : 128;
+    const int NB = b <= 16 ? 16 : b <= 32 ? 32 : b <= 48 ? 48 : b <= 64 ? 64 : b <= 96 ? 96 : 128;
     ft_args A;
     A.b = b; A.KB = L.KB; A.bp = L.bp; A.N = w->N; A.y = y;
     A.ws = (const float *) w->d; A.ad = (const float *) ((const uint8_t *) act + L.d_off);
-    A.tiles_m = (b + NB - 1) / NB;
-    const int64_t tiles = pib_f8_blocks(w->N) * A.tiles_m;
-    if (tiles > 0x3fffffff) { pib_set_error("pib_gemm: %lld x %d outputs are too many", (long long) w->N, b); return PIB_ERR_ARG; }
-    A.tiles = (int) tiles;
+    A.runs = (int) ((w->N + 31) / 32);
+    const int tiles = (A.runs + 3) / 4;
     A.shares = 1;
-    while (A.shares < 8 && A.tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
+    while (A.shares < 8 && tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
     A.err = err;
-    CUtensorMap wmap, xmap;
-    if ((rc = pib_f8_map(&wmap, w->qs, pib_f8_blocks(w->N) * L.Kp, FT_BM * FT_KPS)) != PIB_OK || (rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, NB, FT_KPS)) != PIB_OK) return rc;
+    const pib_f8_runs & wmaps = ((const pib_f8_maps *) w->map)->runs;
+    CUtensorMap xmap;
+    if ((rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, NB, FT_KPS)) != PIB_OK) return rc;
     switch (NB) {
-        case 32:  return ft_launch<32>(wmap, xmap, A, st);
-        case 64:  return ft_launch<64>(wmap, xmap, A, st);
-        default:  return ft_launch<128>(wmap, xmap, A, st);
+        case 16:  return ft_launch<16>(wmaps, xmap, A, st);
+        case 32:  return ft_launch<32>(wmaps, xmap, A, st);
+        case 48:  return ft_launch<48>(wmaps, xmap, A, st);
+        case 64:  return ft_launch<64>(wmaps, xmap, A, st);
+        case 96:  return ft_launch<96>(wmaps, xmap, A, st);
+        default:  return ft_launch<128>(wmaps, xmap, A, st);
     }
 }

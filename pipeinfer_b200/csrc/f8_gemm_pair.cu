@@ -234,11 +234,11 @@ int pib_f8_gemm_pair(const pib_weight * w, const void * act, int b, float * y, i
     A.wide = w->N % 8 == 0 && !((uintptr_t) y & 31) ? 8 : 1;
     A.tiles_m = (b + 255) / 256;
     A.tiles = (A.NB + 1) / 2 * A.tiles_m;
-    CUtensorMap xmap, wmap;
+    CUtensorMap xmap;
     int rc;
-    if ((rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, 128, 1)) != PIB_OK || (rc = pib_f8_map(&wmap, w->qs, (int64_t) A.NB * L.Kp, 128)) != PIB_OK) return rc;
+    if ((rc = pib_f8_map3(&xmap, act, b, L.KB, (int64_t) b * PIB_F8_BLOCK, 128, 1)) != PIB_OK) return rc;
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(f8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) FP_SMEM); }));
-    PIB_CHECK(pib_launch_cluster(f8_gemm_pair_kernel, dim3((unsigned) (2 * std::min(A.tiles, pib_num_sms() / 2))), dim3(FP_THREADS), dim3(2, 1, 1), FP_SMEM, st, xmap, wmap, A));
+    PIB_CHECK(pib_launch_cluster(f8_gemm_pair_kernel, dim3((unsigned) (2 * std::min(A.tiles, pib_num_sms() / 2))), dim3(FP_THREADS), dim3(2, 1, 1), FP_SMEM, st, xmap, ((const pib_f8_maps *) w->map)->block, A));
     return PIB_OK;
 }

@@ -231,14 +231,14 @@ __global__ void __launch_bounds__(FG_THREADS, 1) f8_gemv_kernel(const __grid_con
 // shared memory: the ring, and beside it the activations and their scales where they are resident
 static size_t fg_resident(int b, int64_t Kp) { return (size_t) b * Kp + (size_t) (Kp / PIB_F8_BLOCK) * ((b + 1) & ~1) * 4; }
 
-static int fg_of(fg_args & A, CUtensorMap & wmap, const pib_weight * w, int b, float * y, cudaStream_t st) {
+static int fg_of(fg_args & A, const pib_weight * w, int b, float * y, cudaStream_t st) {
     memset(&A, 0, sizeof(A));
     A.KB = (int) pib_f8_blocks(w->K);
     A.Kp = (int64_t) A.KB * PIB_F8_BLOCK;
     A.tiles = (int) ((w->N + 15) / 16);
     A.ws = (const float *) w->d; A.N = w->N; A.K = w->K; A.b = b; A.y = y;
     if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_gemv: no memory for the error word"); return PIB_ERR_NOMEM; }
-    return pib_f8_map4(&wmap, w->qs, A.KB, pib_f8_blocks(w->N), 16, 16);
+    return PIB_OK;
 }
 template <int PRO> static int fg_launch(const CUtensorMap & wmap, const CUtensorMap & amap, fg_args A, cudaStream_t st) {
     const size_t stage = PRO == FG_RING ? FG_STAGE + 16 * 1024 : FG_STAGE, fixed = FG_WARPS * 8 * 17 * 4 + 512 + 1024, res = PRO == FG_RING ? 0 : fg_resident(A.b, A.Kp);
@@ -256,8 +256,9 @@ int pib_f8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaSt
     const pib_f8_act L = pib_f8_act_of(w->K, b);
     if (b > 8) return pib_f8_gemm(w, act, b, y, st);
     fg_args A;
-    CUtensorMap wmap, amap;
-    if ((rc = fg_of(A, wmap, w, b, y, st)) != PIB_OK) return rc;
+    const CUtensorMap & wmap = ((const pib_f8_maps *) w->map)->stage;
+    CUtensorMap amap;
+    if ((rc = fg_of(A, w, b, y, st)) != PIB_OK) return rc;
     A.a = (const uint8_t *) act; A.ad = (const float *) (A.a + L.d_off); A.bp = L.bp;
     // resident activations leave room for three stages at least
     if (fg_resident(b, A.Kp) <= 104 * 1024) return fg_launch<FG_RES>(wmap, wmap, A, st);
@@ -269,8 +270,8 @@ int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const floa
     if (b < 1 || b > 8 || w->K > 8192) { pib_set_error("pib_gemv_fused: unsupported matrix / batch"); return PIB_ERR_UNSUPP; }
     if (pro == 1 && sum_out && (sum_out == x || sum_out == addend)) { pib_set_error("pib_gemv_fused: sum_out_dev is an input that other blocks still read"); return PIB_ERR_ARG; }
     fg_args A;
-    CUtensorMap wmap;
-    const int rc = fg_of(A, wmap, w, b, y, st);
+    const CUtensorMap & wmap = ((const pib_f8_maps *) w->map)->stage;
+    const int rc = fg_of(A, w, b, y, st);
     if (rc != PIB_OK) return rc;
     A.x = x; A.x2 = pro ? x2 : nullptr; A.addend = pro == 1 ? addend : nullptr; A.sum_out = pro == 1 ? sum_out : nullptr;
     A.xs = xstride ? xstride : w->K; A.eps = eps;

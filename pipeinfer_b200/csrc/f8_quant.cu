@@ -39,6 +39,14 @@ static pib_weight * f8_alloc(int64_t N, int64_t K) {
     w->qs   = (uint8_t *) w->base;
     w->d    = (uint16_t *) (w->qs + plane);
     w->owns = 1;
+    pib_f8_maps * m = (pib_f8_maps *) aligned_alloc(64, (sizeof(pib_f8_maps) + 63) / 64 * 64);
+    w->map = m;
+    if (!m) pib_set_error("pib_weight: no host memory");
+    int rc = m ? pib_f8_map(&m->block, w->qs, NB * KB * PIB_F8_BLOCK, PIB_F8_BLOCK) : PIB_ERR_NOMEM;
+    if (rc == PIB_OK) rc = pib_f8_map4(&m->stage, w->qs, KB, NB, 16, 16);
+    for (int i = 0; i < 4 && rc == PIB_OK; i++) rc = pib_f8_map4(&m->runs.m[i], w->qs, KB, NB, (i + 1) * 32, 1);
+    if (rc == PIB_OK) rc = pib_f8_map(&m->runs.m[4], w->qs, NB * KB * PIB_F8_BLOCK, 2 * PIB_F8_BLOCK);
+    if (rc != PIB_OK) { pib_weight_free(w); return nullptr; }
     return w;
 }
 

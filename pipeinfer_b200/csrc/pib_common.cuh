@@ -137,7 +137,7 @@ struct pib_weight {
     uint8_t * tiles;
     size_t    tile_bytes;
     int       owns;
-    void *    map;      // F8: the tensor map of the rows (CUtensorMap in host memory, f8_gemm.cu)
+    void *    map;      // F8: pib_f8_maps in host memory (f8_block.cuh)
 };
 
 // Dynamic shared memory of decode-matmul CTAs of which an SM takes two: where there is one per SM or fewer, so much that it takes one.  (Launched while the quantiser in front still
