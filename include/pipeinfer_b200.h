@@ -154,7 +154,7 @@ int    pib_quantize_act_rows(int wtype, const float * x_dev, int b, int64_t K, v
 
 /* ---- K3: embedding rows ---------------------------------------------------------------------------------------- */
 /* out_dev float [n][K] = dequantised rows `ids` of W.  Replaces: ggml_compute_forward_get_rows_q (ggml.c:10161) with
- * dequantize_row_q4_0 / q8_0 / q4_K (ggml-quants.c:1074, 1168, 1917). */
+ * dequantize_row_q4_0 / q8_0 / q4_K (ggml-quants.c:1074, 1168, 1917).  Of a PIB_TYPE_F8 matrix a row that it has not is zeros. */
 int pib_get_rows(const pib_weight * w, const int32_t * ids_dev, int n, float * out_dev, pib_stream s);
 
 /* ---- a whole mixture layer for a few tokens ----------------------------------------------------------------------- */

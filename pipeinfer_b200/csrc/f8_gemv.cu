@@ -269,6 +269,7 @@ int pib_f8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaSt
 int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st) {
     if (b < 1 || b > 8 || w->K > 8192) { pib_set_error("pib_gemv_fused: unsupported matrix / batch"); return PIB_ERR_UNSUPP; }
     if (pro == 1 && sum_out && (sum_out == x || sum_out == addend)) { pib_set_error("pib_gemv_fused: sum_out_dev is an input that other blocks still read"); return PIB_ERR_ARG; }
+    if (((uintptr_t) x | (uintptr_t) x2 | (uintptr_t) addend | (uintptr_t) sum_out | (uintptr_t) y) & 3) { pib_set_error("pib_gemv_fused: fp32 rows need 4-byte alignment"); return PIB_ERR_ARG; }
     fg_args A;
     const CUtensorMap & wmap = ((const pib_f8_maps *) w->map)->stage;
     const int rc = fg_of(A, w, b, y, st);

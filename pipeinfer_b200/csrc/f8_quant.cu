@@ -102,16 +102,16 @@ int pib_f8_row(const pib_weight * w, int64_t row, void * out) {
 
 __device__ __forceinline__ float f8_value(uint8_t q) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3))); }
 
-static __global__ void f8_rows_kernel(const uint8_t * __restrict__ qs, const float * __restrict__ d, int64_t K, int64_t KB, const int32_t * __restrict__ ids, float * __restrict__ out) {
+static __global__ void f8_rows_kernel(const uint8_t * __restrict__ qs, const float * __restrict__ d, int64_t N, int64_t K, int64_t KB, const int32_t * __restrict__ ids, float * __restrict__ out) {
     pib_pdl_wait();
     pib_pdl_trigger();
     const int64_t row = ids[blockIdx.x];
     for (int64_t k = (int64_t) blockIdx.y * blockDim.x + threadIdx.x; k < K; k += (int64_t) gridDim.y * blockDim.x)
-        out[(int64_t) blockIdx.x * K + k] = __fmul_rn(f8_value(qs[pib_f8_at(row, k, KB)]), d[row / PIB_F8_BLOCK * KB + k / PIB_F8_BLOCK]);
+        out[(int64_t) blockIdx.x * K + k] = row < 0 || row >= N ? 0.f : __fmul_rn(f8_value(qs[pib_f8_at(row, k, KB)]), d[row / PIB_F8_BLOCK * KB + k / PIB_F8_BLOCK]);
 }
 
 int pib_f8_get_rows(const pib_weight * w, const int32_t * ids, int n, float * out, cudaStream_t st) {
-    PIB_CHECK(pib_launch(f8_rows_kernel, dim3((unsigned) n, (unsigned) std::min<int64_t>((w->K + 255) / 256, 64)), dim3(256), 0, st, w->qs, (const float *) w->d, w->K, pib_f8_blocks(w->K), ids, out));
+    PIB_CHECK(pib_launch(f8_rows_kernel, dim3((unsigned) n, (unsigned) std::min<int64_t>((w->K + 255) / 256, 64)), dim3(256), 0, st, w->qs, (const float *) w->d, w->N, w->K, pib_f8_blocks(w->K), ids, out));
     return PIB_OK;
 }
 
@@ -165,6 +165,10 @@ int pib_f8_quantize(const float * x, const float * norm_w, float eps, int b, int
         pib_set_error("act quantise: bad arguments (8-bit floating point, b %d, K %lld)", b, (long long) K);
         return PIB_ERR_ARG;
     }
+    if (((uintptr_t) act & 15) || (((uintptr_t) x | (uintptr_t) norm_w | (uintptr_t) xnorm) & 3)) {
+        pib_set_error("act quantise: act_dev needs 16-byte alignment, fp32 rows 4-byte alignment");
+        return PIB_ERR_ARG;
+    }
     const pib_f8_act A = pib_f8_act_of(K, b);
     uint8_t * q = (uint8_t *) act;
     float *   d = (float *) (q + A.d_off);
@@ -196,8 +200,8 @@ int pib_f8_act_blocks(const void * act_dev, int b, int64_t K, void * out) {
 }
 
 int pib_f8_rows_ok(const char * who, const pib_weight * w, const void * in, const void * out, int b, int max_b) {
-    if (w && in && out && b >= 1 && b <= max_b) return PIB_OK;
-    pib_set_error("%s: bad arguments (b = %d, limit %d)", who, b, max_b);
+    if (w && in && out && b >= 1 && b <= max_b && !((uintptr_t) out & 3)) return PIB_OK;
+    pib_set_error("%s: bad arguments (b = %d, limit %d; fp32 rows need 4-byte alignment)", who, b, max_b);
     return PIB_ERR_ARG;
 }
 

@@ -630,7 +630,8 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
     const bool f8 = sh && sh->type == PIB_TYPE_F8;
     if (!sh || !router || !gate || !up || !down || (!f8 && sh->type != PIB_TYPE_BF16) || (f8 && (!gate_scales || !up_scales || !down_scales)) || sh->experts < 1 || sh->experts > PIB_MOE_MAX_EXPERTS ||
         sh->top < 1 || sh->top > sh->experts || sh->shared < 0 || sh->shared > PIB_MOE_MAX_TOP || sh->top + sh->shared > PIB_MOE_MAX_TOP || (sh->score != PIB_MOE_SOFTMAX && sh->score != PIB_MOE_SIGMOID) ||
-        sh->width < 1 || sh->ff < 1 || sh->width > (1 << 20) || sh->ff > (1 << 20)) {
+        sh->width < 1 || sh->ff < 1 || sh->width > (1 << 20) || sh->ff > (1 << 20) ||
+        (((uintptr_t) router | (uintptr_t) correction | (f8 ? (uintptr_t) gate_scales | (uintptr_t) up_scales | (uintptr_t) down_scales : 0)) & 3)) {
         pib_set_error("pib_moe_from_device: bad arguments");
         return nullptr;
     }
@@ -688,7 +689,7 @@ extern "C" void pib_moe_free(pib_moe * m) {
 extern "C" size_t pib_moe_scratch_bytes(const pib_moe * m, int b) { return m && b >= 1 && b <= PIB_MAX_BATCH ? mf_of(m, b).total : 0; }
 
 extern "C" int pib_moe_forward(const pib_moe * m, const float * x, int64_t ldx, int b, const float * residual, int64_t ldr, float * y, int64_t ldy, void * scratch, pib_stream s) {
-    if (!m || !x || !y || !scratch || b < 1 || b > PIB_MAX_BATCH || (const float *) y == x || ((uintptr_t) scratch & 255)) {
+    if (!m || !x || !y || !scratch || b < 1 || b > PIB_MAX_BATCH || (const float *) y == x || ((uintptr_t) scratch & 255) || (((uintptr_t) x | (uintptr_t) residual | (uintptr_t) y) & 3)) {
         pib_set_error("pib_moe_forward: bad arguments (b = %d, limit %d)", b, PIB_MAX_BATCH);
         return PIB_ERR_ARG;
     }

@@ -785,7 +785,8 @@ static int sd_launch(const void * logits, int64_t ld, int rows, int V, const pib
 
 extern "C" int pib_sample(int type, const void * logits, int64_t ld, int rows, int n_vocab, const pib_sample_params * params, const float * u, int32_t * ids, float * p, int32_t * kept, pib_stream s) {
     if (rows == 0) return PIB_OK;
-    if ((type != PIB_TYPE_F32 && type != PIB_TYPE_BF16) || !logits || !params || !u || !ids || rows < 0 || n_vocab < 1 || n_vocab > PIB_SAMPLE_MAX_VOCAB || (rows > 1 && ld < n_vocab)) {
+    if ((type != PIB_TYPE_F32 && type != PIB_TYPE_BF16) || !logits || !params || !u || !ids || rows < 0 || n_vocab < 1 || n_vocab > PIB_SAMPLE_MAX_VOCAB || (rows > 1 && ld < n_vocab) ||
+        ((uintptr_t) logits & (type == PIB_TYPE_F32 ? 3 : 1)) || (((uintptr_t) params | (uintptr_t) u | (uintptr_t) ids | (uintptr_t) p | (uintptr_t) kept) & 3)) {
         pib_set_error("pib_sample: bad arguments (type %d, %d rows of %d, %lld apart; at most %d tokens)", type, rows, n_vocab, (long long) ld, PIB_SAMPLE_MAX_VOCAB);
         return PIB_ERR_ARG;
     }

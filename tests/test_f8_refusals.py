@@ -78,3 +78,18 @@ def test_sampling(L):
 def test_products_without_a_weight(L):
     assert refused(L, L.pib_gemv(None, P, 1, P, 0, None), "pib_gemv")
     assert refused(L, L.pib_gemm(None, P, 1, P, P, None), "pib_gemm")
+
+
+def test_alignment(L):
+    """pointers that no load of their type could read"""
+    assert refused(L, L.pib_quantize_act_rows(F8, P + 2, 1, 128, P, None), "act quantise")
+    assert refused(L, L.pib_quantize_act_rows(F8, P, 1, 128, P + 8, None), "act quantise")
+    for i, off in ((0, 2), (1, 1), (3, 2), (5, 1), (7, 3)):
+        args = [P] * 8
+        args[i] += off
+        assert not L.pib_moe_from_device(C.byref(shape()), *args) and b"bad arguments" in L.pib_last_error()
+    for i in range(6):
+        ptr = [P] * 6
+        ptr[i] += 2
+        assert refused(L, L.pib_sample(0, ptr[0], 100, 2, 100, ptr[1], ptr[2], ptr[3], ptr[4], ptr[5], None), "pib_sample")
+    assert refused(L, L.pib_sample(30, P + 1, 100, 2, 100, P, P, P, None, None, None), "pib_sample")

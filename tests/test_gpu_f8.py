@@ -248,3 +248,29 @@ def test_captured_and_on_another_stream(torch, pib, how, b):
         z = y * 2
     torch.cuda.synchronize()
     assert ((z.double() - ref).abs() <= lim).all()
+
+
+def test_rows_that_are_not_there(torch, pib):
+    lib, N, K = pib.load(), 300, 260
+    q, s, g = matrix(torch, N, K, 11)
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), N, K)
+    ids = torch.tensor([-1, 0, N, 299, 0x7fffffff, -0x80000000], dtype=torch.int32, device="cuda")
+    out = torch.full((6, K), float("nan"), device="cuda")
+    lib.check(lib.L.pib_get_rows(w.h, ids.data_ptr(), 6, out.data_ptr(), None))
+    torch.cuda.synchronize()
+    W = dense(torch, q, s)
+    assert torch.equal(out[[1, 3]], W[[0, 299]].float()) and not out[[0, 2, 4, 5]].any()
+
+
+# outputs that fill the last CTA's, the last tile's or the last run's rows by one, and few rows in many shares
+@pytest.mark.parametrize("N,K,b", [(148 * 32 + 1, 300, 9), (148 * 96 - 31, 257, 16), (148 * 160 + 5, 130, 17), (19000, 129, 32), (148 * 128 + 1, 260, 33), (148 * 128 - 127, 128, 48), (20001, 385, 49), (31, 4100, 96),
+                                     (33, 2049, 97), (9500, 1100, 128)])
+def test_divided_rows(torch, pib, N, K, b):
+    q, s, g = matrix(torch, N, K, N + b)
+    x = rows(torch, b, K, g)
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), N, K)
+    ref, lim = want(torch, q, s, x)
+    y = product(torch, pib, w, x, "gemm")
+    torch.cuda.synchronize()
+    assert ((y.double() - ref).abs() <= lim).all()
+    assert torch.equal(product(torch, pib, w, x, "gemm"), y)
