@@ -95,6 +95,9 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
     const int unit = blockIdx.x / S, units = gridDim.x / S;
     const int grains = (A.runs + GRAIN - 1) / GRAIN, r0 = (int) ((int64_t) grains * unit / units) * GRAIN;
     const int runs = min(A.runs, (int) ((int64_t) grains * (unit + 1) / units) * GRAIN) - r0, tiles = (runs + 3) / 4, each = runs / tiles, more = runs % tiles;
+    // a tile's first run, and how many; where rows go by blocks of four runs no tile reaches into the next
+    auto run_of  = [&](int tile) { return r0 + (GRAIN == 4 ? tile * 4 : tile * each + min(tile, more)); };
+    auto runs_of = [&](int tile) { return GRAIN == 4 ? min(4, runs - tile * 4) : each + (tile < more); };
     const int k0 = (int) ((int64_t) A.KB * share / S), nk = (int) ((int64_t) A.KB * (share + 1) / S) - k0;
     const uint32_t sm0 = dt_smem(sm);
 
@@ -122,7 +125,7 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
         uint32_t ph = 1;                                         // the first round finds its places free
         for (int tile = 0; tile < tiles && ok && lane == 0; tile++) {
             // rows of the tile in one block of the weights' layout, and in the next
-            const int t0 = r0 + tile * each + min(tile, more), n = each + (tile < more), n1 = GRAIN == 4 ? n : min(n, 4 - (t0 & 3)), n2 = n - n1;
+            const int t0 = run_of(tile), n = runs_of(tile), n1 = GRAIN == 4 ? n : min(n, 4 - (t0 & 3)), n2 = n - n1;
             for (int kt = 0; kt < nk; kt += KPS) {
                 ok = dt_mbar_wait(bar_e + s * 8, ph, abort_s);
                 if (!ok) break;
@@ -181,8 +184,8 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
         int a = 0, ds = 0;
         uint32_t aph = 0, dph = 0;
         for (int tile = 0; tile < tiles && ok; tile++) {
-            const int  t0 = r0 + tile * each + min(tile, more), run = t0 + q4;      // the warp's rows
-            const bool in  = q4 < each + (tile < more);
+            const int  t0 = run_of(tile), run = t0 + q4;      // the warp's rows
+            const bool in  = q4 < runs_of(tile);
             const int64_t n = (int64_t) run * 32 + lane;
             int m0 = hf * HALF;
             asm volatile("" : "+r"(m0));                         // keeps the outputs' addresses from being made, and held, ahead of the tiles
