@@ -5,18 +5,19 @@
 // A pair forms 256 tokens x 256 outputs, tokens as M: each CTA brings its own 128 tokens and half of the weight rows, the tensor cores of both read both halves.
 //   warp 0       streams a block of both operands by TMA through a ring; both CTAs' copies complete on the first CTA's barrier
 //   warp 1       of the first CTA issues the MMAs of both: a block is one accumulator, two of them take turns
-//   warp 10      makes the factors f = d s of a block's tokens and both weight blocks
-//   warps 2..9   a thread owns a token (lane) and the outputs of one weight block (half): acc[c] += P[c] f with ONE factor f = d s for its 128 outputs
+//   warp 2       makes the factors f = d s of a block's tokens and both weight blocks
+//   warps 3..18  a thread owns a token (lane) and half of the outputs of one weight block: acc[c] += P[c] f with ONE factor f = d s for its 64 outputs
 // That the factor is one number per thread is why the tokens are M here (f8_gemm.cu has them as N: a factor per column, whose product costs as much as the sum).
-// What bounds it: the warps that add up, 1 300 clocks a block (loads from tensor memory, one accumulator of 128 columns held in registers beside 128 sums) of which the MMAs take 512: 28672 x 8192
-// at 1 999 tokens takes 561 us (1.67 PFLOP/s); copies and MMAs alone took 292.
+// What bounds it: an accumulator's round -- MMAs, their commit to both CTAs, reading it, handing it back -- with two of them in tensor memory, and the sums between the reads: 28672 x 8192 at
+// 1 999 tokens takes 526 us (1.79 PFLOP/s) in a short burst, 404 without sums, 292 without reads.  Eight warps of 128 columns, which hold 128 sums a thread, take 562; four accumulators of
+// 128 columns 562, since MMAs that narrow read the tokens twice.
 // Every wait is bounded (tc_common.cuh).
 #include "f8_block.cuh"
 #include "tc_common.cuh"
 
 #include <algorithm>
 
-#define FP_THREADS 352
+#define FP_THREADS 608
 #define FP_FRING   8                          // factor rows under way
 #define FP_TILE    (128 * 128)
 #define FP_STAGE   (2 * FP_TILE)
@@ -53,6 +54,11 @@ __device__ __forceinline__ unsigned long long fp_fma2(unsigned long long a, unsi
 }
 __device__ __forceinline__ unsigned long long fp_pack(uint32_t lo, uint32_t hi) { return (unsigned long long) hi << 32 | lo; }
 
+__device__ __forceinline__ void fp_ld16(uint32_t at, uint32_t * v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at) : "memory");
+}
 struct fp_args {
     int b, KB, NB, bp, tiles_m, tiles, wide;         // wide: floats that a store may take (8, 4 or 1)
     int64_t N;
@@ -74,8 +80,8 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < FP_STAGES; s++) { dt_mbar_init(bar_f + s * 8, 1); dt_mbar_init(bar_e + s * 8, 1); }
-        for (int a = 0; a < 2; a++) { dt_mbar_init(bar_t + a * 8, 1); dt_mbar_init(bar_r + a * 8, 16); }
-        for (int f = 0; f < FP_FRING; f++) { dt_mbar_init(bar_d + f * 8, 1); dt_mbar_init(bar_g + f * 8, 8); }
+        for (int a = 0; a < 2; a++) { dt_mbar_init(bar_t + a * 8, 1); dt_mbar_init(bar_r + a * 8, 32); }
+        for (int f = 0; f < FP_FRING; f++) { dt_mbar_init(bar_d + f * 8, 1); dt_mbar_init(bar_g + f * 8, 16); }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -121,7 +127,7 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
                     if (++a == 2) { a = 0; aph ^= 1; }
                 }
         }
-    } else if (warp == 10) {
+    } else if (warp == 2) {
         // four tokens a lane, four blocks under way in registers that keep their places
         int fs = 0;
         uint32_t fph = 1;
@@ -155,16 +161,16 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
                     }
         }
     } else {
-        const int q4 = warp & 3, hf = (warp - 2) >> 2;
-        const uint32_t at = tmem + ((uint32_t) (q4 * 32) << 16) + hf * 128;
-        unsigned long long acc[64];
+        const int q4 = warp & 3, part = (warp - 3) >> 2, hf = part >> 1;       // 64 columns
+        const uint32_t at = tmem + ((uint32_t) (q4 * 32) << 16) + part * 64;
+        unsigned long long acc[32];
         int a = 0, fs = 0;
         uint32_t aph = 0, fph = 0;
         for (int tile = pair; tile < A.tiles && ok; tile += pairs) {
             const int  tk = tile % A.tiles_m * 256 + rank * 128 + q4 * 32 + lane, nb = tile / A.tiles_m * 2 + hf;
             const bool in = tk < A.b && nb < A.NB;
 #pragma unroll
-            for (int c = 0; c < 64; c++) acc[c] = 0;
+            for (int c = 0; c < 32; c++) acc[c] = 0;
             for (int kb = 0; kb < A.KB; kb++) {
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_d + fs * 8, fph, abort_s));
                 if (!ok) break;
@@ -173,40 +179,38 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar_t + a * 8, aph, abort_s));
                 if (!ok) break;
                 dt_fence_after();
-                uint32_t v[2][32];
-                dt_ld32(at + a * 256, v[0]);
-                dt_wait_ld();
+                uint32_t v[16];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {                    // the next 32 columns are under way while these are added
-                    if (c < 3) dt_ld32(at + a * 256 + (c + 1) * 32, v[(c + 1) & 1]);
-                    else {                                       // all read: the accumulator goes back in front of the last sums
+                for (int c = 0; c < 4; c++) {
+                    fp_ld16(at + a * 256 + c * 16, v);
+                    dt_wait_ld();
+                    if (c == 3) {                                // all read: the accumulator goes back in front of the last sums
                         dt_fence_before();
                         __syncwarp();
-                        // relaxed: no memory is handed over with it (a release at cluster scope in its place: 1 190 us instead of 650)
+                        // relaxed: no memory is handed over with it (a release at cluster scope in its place took twice the time)
                         if (lane == 0) {
                             asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_r + a * 8) : "memory");
                             dt_arrive(bar_g + fs * 8);
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j++) acc[c * 16 + j] = fp_fma2(fp_pack(v[c & 1][2 * j], v[c & 1][2 * j + 1]), ff, acc[c * 16 + j]);
-                    if (c < 3) dt_wait_ld();
+                    for (int j = 0; j < 8; j++) acc[c * 8 + j] = fp_fma2(fp_pack(v[2 * j], v[2 * j + 1]), ff, acc[c * 8 + j]);
                 }
                 if (++a == 2) { a = 0; aph ^= 1; }
                 if (++fs == FP_FRING) { fs = 0; fph ^= 1; }
             }
             if (!ok) break;
             if (!in) continue;
-            const int64_t n0 = (int64_t) nb * 128;
+            const int64_t n0 = (int64_t) nb * 128 + (part & 1) * 64;
             float * y = A.y + (int64_t) tk * A.N + n0;
-            const int left = (int) min((int64_t) 128, A.N - n0);
-            if (A.wide == 8 && left == 128) {
+            const int left = (int) min((int64_t) 64, A.N - n0);
+            if (A.wide == 8 && left == 64) {
 #pragma unroll
-                for (int c = 0; c < 64; c += 4)
+                for (int c = 0; c < 32; c += 4)
                     asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(y + c * 2), "l"(acc[c]), "l"(acc[c + 1]), "l"(acc[c + 2]), "l"(acc[c + 3]) : "memory");
             } else {
 #pragma unroll
-                for (int c = 0; c < 64; c++) {
+                for (int c = 0; c < 32; c++) {
                     if (2 * c < left)     y[2 * c]     = __uint_as_float((uint32_t) acc[c]);
                     if (2 * c + 1 < left) y[2 * c + 1] = __uint_as_float((uint32_t) (acc[c] >> 32));
                 }
