@@ -198,9 +198,9 @@ struct mf_shared {
     uint32_t mask[PIB_MOE_MAX_EXPERTS + 16], tokens[256];        // of an expert, of an entry of the list
     int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[256], n_act, item[MF_STAGES], pub[2], abort;
     uint64_t bars[2 * MF_STAGES + 4];     // a piece there / read, an item's results written / published
-    float    red[2][MF_WARPS][9][33];     // two items' turns; also the choice values of a warp's token
+    float    red[2][MF_WARPS][9][33];     // two items' turns
 };
-static_assert(sizeof(((mf_shared *) 0)->red) >= MF_WARPS * PIB_MOE_MAX_EXPERTS * 4, "choice values");
+static_assert(MF_STAGES * MF_STAGE >= MF_THREADS / 32 * PIB_MOE_MAX_EXPERTS * 4, "a token's logits for every warp");
 #define MF_RING (((int) sizeof(mf_shared) + 127) & ~127)          // behind it the ring
 #define MF_SMEM ((size_t) MF_RING + MF_STAGES * MF_STAGE)
 extern __shared__ __align__(128) uint8_t mf_dsm[];               // named here, so that the compiler knows a shared address in every function
@@ -211,11 +211,11 @@ struct mf_place { int s; uint32_t ph; };       // a place of the ring and its ph
 __device__ __forceinline__ uint32_t mf_key(float v) { const uint32_t u = __float_as_uint(v + 0.0f); return v != v ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u; }
 
 // the choice, by every block for itself
-template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, int warp, int lane) {
+template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, mf_shared & S, uint8_t * ring, int warp, int lane) {
     constexpr int COLS = F8 ? 4 : 8;                             // tokens of an entry of the list
     const int E = A.E;
-    float * sv = &S.red[0][0][0][0] + warp * PIB_MOE_MAX_EXPERTS;        // the token's logits, then its scores
-    for (int tk = warp; tk < A.b; tk += MF_WARPS) {
+    float * sv = reinterpret_cast<float *>(ring) + warp * PIB_MOE_MAX_EXPERTS;             // the token's logits
+    for (int tk = warp; tk < A.b; tk += MF_THREADS / 32) {
         const float * z = A.z + tk * E;
         float xmax = 0.f, xsum = 0.f;
         if (F8) { xmax = __ldcg(A.xm + 2 * tk); xsum = __ldcg(A.xm + 2 * tk + 1); }
@@ -269,10 +269,10 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
         }
     }
     const int all = E + A.shared, per = A.top + A.shared;
-    for (int i = threadIdx.x; i < all; i += MF_WARPS * 32) S.mask[i] = 0;
-    mf_bar();
-    for (int i = threadIdx.x; i < A.b * per; i += MF_WARPS * 32) atomicOr(&S.mask[S.ids[i / per][i % per]], 1u << i / per);
-    mf_bar();
+    for (int i = threadIdx.x; i < all; i += MF_THREADS) S.mask[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.b * per; i += MF_THREADS) atomicOr(&S.mask[S.ids[i / per][i % per]], 1u << i / per);
+    __syncthreads();
     if (warp == 0) {                                             // the experts with tokens, in order; the first row of each one's tokens
         int n = 0, rows = 0;
         for (int i0 = 0; i0 < all; i0 += 32) {
@@ -299,8 +299,8 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
         }
         if (lane == 0) S.n_act = n;
     }
-    mf_bar();
-    for (int i = threadIdx.x; i < A.b * per; i += MF_WARPS * 32) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.b * per; i += MF_THREADS) {
         const int tk = i / per, e = S.ids[tk][i % per];
         const int at = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
         S.at[tk][i % per] = at;
@@ -474,7 +474,8 @@ __global__ void __launch_bounds__(MF_THREADS, 2) moe_few_kernel(const __grid_con
     pib_pdl_trigger();
     int ticket = 0;
     if (warp == MF_WARPS && lane == 0) ticket = atomicAdd(A.cnt, 1);
-    if (warp < MF_WARPS) mf_route<F8>(A, S, warp, lane);
+    mf_route<F8>(A, S, ring, warp, lane);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the choice's values in the ring lie ahead of the copies
     __syncthreads();
     const int per = A.top + A.shared, ups = S.n_act * A.T1, items = ups + S.n_act * A.T2;
     int * done_up = A.cnt + 2, * done_rows = done_up + A.b * per;
