@@ -20,7 +20,7 @@
 // the eight columns of one MMA; an expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which
 // costs less than a second form of the kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
 // a row (lane t) are four values each of four (two) neighbouring tiles of 16, the k of an MMA, and the parts lie in that order too.
-// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in 316 us (0.76 of the copy rate; the choice takes some 10 us of it, the turns of 48 KB down items the
+// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in 312 us (0.77 of the copy rate; the choice takes some 8 us of it, the turns of 48 KB down items the
 // rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 31 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
 // way to memory and back each.  Sharing the choice among the blocks would save none of it: the launch's first 4 us are mostly the way of its code into the caches.
 #include <cuda_bf16.h>
