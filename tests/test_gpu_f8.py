@@ -274,3 +274,26 @@ def test_divided_rows(torch, pib, N, K, b):
     torch.cuda.synchronize()
     assert ((y.double() - ref).abs() <= lim).all()
     assert torch.equal(product(torch, pib, w, x, "gemm"), y)
+
+
+def test_more_than_four_gigabytes(torch, pib):
+    """offsets of rows, and of outputs, that 32 bits do not hold"""
+    lib, N, K = pib.load(), 530000, 8192
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randint(0, 120, (N, K), device="cuda", generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    s = (torch.rand(blocks(N), blocks(K), device="cuda", generator=g) + 0.5) / 96
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), N, K)
+    for how, b in (("fused", 1), ("gemv", 3), ("gemm", 20), ("gemm", 70), ("gemm", 200)):
+        x = rows(torch, b, K, g)
+        y = product(torch, pib, w, x, how)
+        torch.cuda.synchronize()
+        for r0 in (0, 262144 - 128, N // 128 * 128 - 256):        # whole blocks of rows
+            r1 = min(N, r0 + 512)
+            ref, lim = want(torch, q[r0:r1], s[r0 // 128:blocks(r1)], x)
+            assert ((y[:, r0:r1].double() - ref).abs() <= lim).all(), (how, b, r0)
+    ids = torch.tensor([N - 1, 262144, 524289], dtype=torch.int32, device="cuda")
+    out = torch.empty(3, K, device="cuda")
+    lib.check(lib.L.pib_get_rows(w.h, ids.data_ptr(), 3, out.data_ptr(), None))
+    torch.cuda.synchronize()
+    for i, r in enumerate(ids.tolist()):
+        assert torch.equal(out[i], dense(torch, q[r:r + 1], s[r // 128:r // 128 + 1])[0].float())

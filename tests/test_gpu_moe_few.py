@@ -222,3 +222,13 @@ def test_captured_and_at_the_same_time(torch, pib):
             check(L, xs[i], rs[i], ys[i])
         check(L, xs[0], rs[1], y3)
     pib.load().gemm_check(third.cuda_stream)
+
+
+def test_more_than_four_gigabytes(torch, pib):
+    """experts whose weights lie beyond what 32 bits address"""
+    L = Layer(torch, pib, F8, 256, 1, 3, 4096, 2048, correction=True)
+    L.w["correction"].copy_(torch.where(torch.arange(256, device="cuda") % 83 == 5, 50.0, 0.0))          # 5, 88, 171, 254
+    L.moe = pib.Moe(pib.load(), F8, 256, 1, 3, 4096, 2048, renorm=True, **{k: v.data_ptr() for k, v in L.w.items()})
+    x = torch.randn(5, 4096, device="cuda", generator=L.g)
+    res = torch.randn(5, 4096, device="cuda", generator=L.g)
+    check(L, x, res, L.run(x, res))

@@ -196,3 +196,25 @@ def test_captured_and_on_another_stream(pib):
         got = ids.clone()
     torch.cuda.synchronize()
     assert [int(v) for v in got] == [want(x[r].cpu().numpy(), (0.8, 0, 0.9, 0.0), float(u[r]))[0] for r in range(rows)]
+
+
+def test_rows_far_apart(pib):
+    """rows whose distance passes 32 bits, against the same rows side by side"""
+    torch = pytest.importorskip("torch")
+    lib, rows, V, ld = pib.load(), 4, 40001, 1500000001
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = (torch.randn(rows, V, device="cuda", generator=g) * 3).bfloat16()
+    far = torch.empty((rows - 1) * ld + V, dtype=torch.bfloat16, device="cuda")
+    for r in range(rows):
+        far[r * ld:r * ld + V] = x[r]
+    p = np.array([(0.8, 40, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0, 1.0, 0.1), (1.0, 0, 1.0, 0.0)], [("temp", "f4"), ("top_k", "i4"), ("top_p", "f4"), ("min_p", "f4")])
+    p = torch.from_numpy(p.view(np.uint8).copy()).cuda()
+    u = torch.rand(rows, device="cuda", generator=g)
+    out = []
+    for t, d in ((x, V), (far, ld)):
+        ids, pr, kept = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        lib.sample(lib.TYPE_BF16, t.data_ptr(), d, rows, V, p.data_ptr(), u.data_ptr(), ids.data_ptr(), pr.data_ptr(), kept.data_ptr(), 0)
+        torch.cuda.synchronize()
+        out.append((ids.tolist(), pr.tolist(), kept.tolist()))
+    assert out[0] == out[1] and min(out[0][0]) >= 0
