@@ -21,16 +21,14 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
-#include <float.h>
 #include <limits.h>
 
 #include "engine.cuh"
+#include "sample_border.cuh"
 
 #define SD_THREADS 512
 #define SD_WARPS   (SD_THREADS / 32)
 #define SD_BINS    2048                       // of a level of sd_select
-#define SD_FINE    8192                       // of l_max - l
-#define SD_PER     256.0f                     // bins for a difference of 1
 #define SD_LIST    2048
 #define SD_POW     1024
 #define SD_SLICE   4096                       // ids of a block at least, where a row is divided
@@ -136,7 +134,6 @@ template <typename T, typename F> __device__ __forceinline__ void sd_walk(const 
         if (more) f(c + SD_WARPS, i + SD_WARPS * SD_CHUNK, b);
     }
 }
-__device__ __forceinline__ int sd_fine(float l, float mx) { return (int) fminf((mx - l) * SD_PER, (float) (SD_FINE - 1)); }
 
 // members of a level: bin0 of l_max - l, and the order's leading bits
 struct sd_level { int bin0, shift; sd_u64 prefix; };
@@ -281,14 +278,6 @@ __device__ __noinline__ void sd_select(sd_shared & S, const sd_row<T> & R, cg::c
 __device__ __forceinline__ sd_u64 sd_need(float top_p, sd_u64 mass) {
     const sd_u64 n = (sd_u64) ceil((double) top_p * (double) mass);
     return n < 1 ? 1 : n > mass ? mass : n;
-}
-// the lowest logit of bin b of l_max - l: sd_fine does not grow with the logit
-__device__ __forceinline__ float sd_bin_floor(int b, float mx) {
-    float f = mx - (float) (b + 1) / SD_PER;
-    if (b == SD_FINE - 1) return -FLT_MAX;
-    while (sd_fine(f, mx) > b) f = nextafterf(f, INFINITY);
-    for (float d = nextafterf(f, -INFINITY); sd_fine(d, mx) <= b; d = nextafterf(f, -INFINITY)) f = d;
-    return f;
 }
 // what a block has in all its warps: S.own
 __device__ __forceinline__ void sd_block_sum(sd_shared & S, int warp, int lane, uint32_t n, sd_u64 m) {

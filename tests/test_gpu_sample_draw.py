@@ -218,3 +218,27 @@ def test_rows_far_apart(pib):
         torch.cuda.synchronize()
         out.append((ids.tolist(), pr.tolist(), kept.tolist()))
     assert out[0] == out[1] and min(out[0][0]) >= 0
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [1000, 20000, 70000])
+def test_borders_beside_zero(pib, V, bf16):
+    """thresholds in the bins above and below logit 0 behind a positive maximum, where 10^8 floats have the same difference to it: equal zeros, denormal numbers, some ulps and whole bins either side"""
+    rng = np.random.default_rng(V)
+    n = 900                                                      # tokens beside 0, as far apart as they go; the rest weighs nothing
+    around = [np.zeros(n), rng.integers(-3, 4, n) * 1e-40, rng.integers(-2000, 2000, n) * 2.0 ** -24, (rng.random(n) - 0.5) / 64, rng.integers(-1, 2, n) / 256.0]
+    x, params = [], []
+    for mx, top_p in ((0.5, 0.5), (3.0, 0.5), (8.0, 0.9), (12.25, 0.998), (20.0, 0.999999)):
+        for a in around:
+            row = np.full(V, -1000.0)
+            at = rng.permutation(V)[:n + 1]
+            row[at[:n]], row[at[n]] = a, mx
+            for p in ((1.0, 0, top_p, 0.0), (0.7, 600, 1.0, 0.0), (1.0, 700, top_p, 1e-9)):
+                x.append(row)
+                params.append(p)
+    x = np.array(x, np.float32)
+    if bf16:
+        x = (x.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+    u = rng.random(len(params), np.float32)
+    for r in range(0, len(params), 25):                          # few rows at a time, so that long ones are divided
+        compare(pib, x[r:r + 25], params[r:r + 25], u[r:r + 25], bf16=bf16)
