@@ -48,3 +48,13 @@ SD_HD_CALL float sd_bin_floor(int b, float mx) {
     if (b == SD_FINE - 1) return -FLT_MAX;
     return sd_least(mx - (float) (b + 1) / SD_PER, mx, [=](float l) { return sd_fine(l, mx) <= b; });
 }
+
+// the smallest logit with e^(l - l_max) >= min_p, 0 < min_p <= 1; the exponential is formed only where the logarithm leaves it open
+SD_HD bool sd_enough(float l, float mx, double min_p, double log_p) {
+    const double rel = (double) l - (double) mx;
+    return rel >= log_p + 1e-12 || (rel > log_p - 1e-12 && exp(rel) >= min_p);
+}
+SD_HD_CALL float sd_min_p(float min_p, float mx) {
+    const double p = (double) min_p, log_p = log(p);
+    return sd_least((float) ((double) mx + log_p), mx, [=](float l) { return sd_enough(l, mx, p, log_p); });
+}

@@ -424,14 +424,7 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
     // what is kept: logits above kl, and those equal to it up to id ki
     float kl = -INFINITY;
     int   ki = INT_MIN;
-    if (q.min_p > 0.f) {                                         // the smallest logit with e^(l - l_max) >= min_p
-        const double min_p = (double) q.min_p, log_p = log(min_p);
-        auto enough = [&](float l) { const double rel = (double) l - R.one.mx; return rel >= log_p + 1e-12 || (rel > log_p - 1e-12 && exp(rel) >= min_p); };
-        kl = fminf((float) (R.one.mx + log_p), mx);
-        while (!enough(kl)) kl = nextafterf(kl, INFINITY);
-        for (float d = nextafterf(kl, -INFINITY); enough(d); d = nextafterf(kl, -INFINITY)) kl = d;
-        ki = 0x7fffffff;
-    }
+    if (q.min_p > 0.f) { kl = sd_min_p(q.min_p, mx); ki = 0x7fffffff; }
     auto kept = [&](float v, int i) { return v > kl || (v == kl && i <= ki); };
     auto by_id = [&](uint32_t a, uint32_t b) { return (uint32_t) S.list[a] > (uint32_t) S.list[b]; };           // inverted ids: larger is lower
     auto by_place = [&](uint32_t a, uint32_t b) { return S.list[a] > S.list[b]; };

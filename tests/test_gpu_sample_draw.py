@@ -242,3 +242,27 @@ def test_borders_beside_zero(pib, V, bf16):
     u = rng.random(len(params), np.float32)
     for r in range(0, len(params), 25):                          # few rows at a time, so that long ones are divided
         compare(pib, x[r:r + 25], params[r:r + 25], u[r:r + 25], bf16=bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [700, 33000])
+def test_min_p_beside_zero(pib, V, bf16):
+    """min_p 1 and just below behind a maximum of 0 (shifted logits, a row of zeros, some infinities) and next to it, and borders at 0 behind a positive maximum"""
+    rng = np.random.default_rng(V + 1)
+    x = np.full((9, V), -7.0, np.float32)
+    x[:, 5::7] = rng.random((9, len(range(5, V, 7)))) * -1e-3
+    x[0, [3, 40, 600]] = 0.0
+    x[1] = 0.0
+    x[2, [9, 99, 350]] = np.inf
+    x[3, 50] = 1e-38; x[3, 60] = -1e-38; x[3, 61] = 0.0
+    x[4] = -0.0; x[4, ::3] = 0.0
+    x[5, 11] = 0.0; x[5, 12:40] = -1e-17; x[5, 40:60] = -1e-45
+    x[6, 7] = 1.0; x[6, 20:40] = 0.0
+    x[7, 7] = 0.6931472; x[7, 20:40] = 0.0
+    x[8, 7] = 2.0 ** -24; x[8, 20:40] = 0.0
+    if bf16:
+        x = (x.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+    u = rng.random(9, np.float32)
+    for m in (1.0, 0.99999994, 0.3678, 0.36788, 0.4999):
+        for k, p in ((0, 1.0), (300, 1.0), (0, 0.7), (500, 0.8)):
+            compare(pib, x, [(0.9, k, p, m)] * 9, u, bf16=bf16)

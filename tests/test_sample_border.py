@@ -13,7 +13,15 @@ PROGRAM = r"""
 static long tests;
 template <typename F> struct counted { F f; bool operator()(float v) const { tests++; return f(v); } };
 template <typename F> static counted<F> count(F f) { return { f }; }
-int main(int argc, char ** argv) {      // maxima: for each the most floats looked at for a border, and wrong borders
+int main(int argc, char ** argv) {      // maxima, or "min_p", a number and a maximum: for each the most floats looked at for a border, and wrong borders
+    if (!strcmp(argv[1], "min_p")) {
+        const float min_p = strtof(argv[2], nullptr), mx = strtof(argv[3], nullptr);
+        const double p = min_p, log_p = log(p);
+        auto in = [=](float l) { return sd_enough(l, mx, p, log_p); };
+        const float f = sd_least((float) ((double) mx + log_p), mx, count(in));
+        printf("%ld %d\n", tests, f != sd_min_p(min_p, mx) || !in(f) || in(sd_of_rank(sd_rank(f) - 1)));
+        return 0;
+    }
     for (int i = 1; i < argc; i++) {
         const float mx = strtof(argv[i], nullptr);
         long most = 0, wrong = 0;
@@ -47,3 +55,11 @@ MAXIMA = ["3", "5", "8", "20", "7.5", "10", "12.25", "31.75", "0.5", "0.50390625
 def test_bins(program, mx):
     most, wrong = (int(v) for v in subprocess.run([program, mx], check=True, capture_output=True, text=True, timeout=60).stdout.split())
     assert wrong == 0 and most <= 64
+
+
+# 1 behind a maximum of 0 (logits less their maximum, rows of zeros, rows with an infinity): every float down to -5e-17 has e^l = 1; a border that lands at or near 0
+@pytest.mark.parametrize("min_p", ["1", "0.99999994", "0.999", "0.5", "0.36787945", "0.1", "1e-20", "1e-38", "1e-45"])
+@pytest.mark.parametrize("mx", MAXIMA + ["0.69314718", "1.0", "5.9604645e-08"])
+def test_min_p(program, min_p, mx):
+    tests, wrong = (int(v) for v in subprocess.run([program, "min_p", min_p, mx], check=True, capture_output=True, text=True, timeout=60).stdout.split())
+    assert wrong == 0 and tests <= 64
