@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
     const int chunks = (V + R.shift + SD_CHUNK - 1) / SD_CHUNK;
     R.c0 = chunks * R.part / R.P; R.c1 = chunks * (R.part + 1) / R.P;
     R.lo = max(0, R.c0 * SD_CHUNK - R.shift); R.hi = min(V, R.c1 * SD_CHUNK - R.shift);
+    if (R.P > 1) cl.barrier_arrive();                            // this block has started: waited for ahead of the first store to another one's shared memory
     for (int j = tid; j < SD_POW; j += SD_THREADS) S.pow[j] = exp2((double) j / SD_POW);
     for (int i = tid; i < SD_FINE; i += SD_THREADS) S.fine[i] = 0;
     pib_pdl_wait();
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
         if (m > mx) { mx = m; arg = i; }
     });
     const bool first = !(q.temp > 0.f) || q.top_k == 1 || q.min_p > 1.f || !(q.top_p > 0.f || q.top_p != q.top_p), by_k = q.top_k > 0 && q.top_k < V, by_p = q.top_p < 1.f;
+    if (R.P > 1) cl.barrier_wait();
     if (by_k) cl.map_shared_rank(&S, 0)->tmax[R.part * SD_THREADS + tid] = mx;
     const float best = warp_max(mx);
     arg = __reduce_min_sync(0xffffffffu, mx == best ? arg : 0x7fffffff);
