@@ -48,7 +48,7 @@ struct sd_shared {
     sd_u64   chunk[SD_CHUNKS];
     double   pow[SD_POW];                                        // 2^(j / 1024)
     sd_u64   wsum[SD_WARPS], sum;                                // of a block's warps, of the block
-    double   wbound[SD_WARPS], bound;
+    sd_u64   wbound[SD_WARPS], bound;
     uint32_t wcnt[SD_WARPS], cnt, n_list;
     float    bound_k;                                            // at least top_k tokens reach it
     float    wmax[SD_WARPS], max;
@@ -459,11 +459,12 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
         const uint32_t k = by_k ? min((uint32_t) q.top_k, n) : 0;
         const double want = (double) need;
         const int per = SD_FINE / R.P, each = per / SD_THREADS, b0 = R.part * per + tid * each;
-        // a token of bin b weighs at most 2^44 e^(-b / 256), rounded: from bin to bin by a factor (a weight formed for each bin: 300 rows of 50 257 with top-p 142 us instead of 139)
+        // a token of bin b weighs at most 2^44 e^(-b / 256), rounded: from bin to bin by a factor (a weight formed for each bin: 300 rows of 50 257 with top-p 142 us instead of 139).  The sums are
+        // whole numbers: wherever a thread's or a block's bins begin they are the same, and one thread of the cluster finds each border
         const double fall = 0.99610136947011749, edge = by_k ? 0.0 : exp(-(double) b0 / 256.0) * 17592186044416.0;
-        auto most_of = [&](double w, uint32_t c) { return (double) c * (w + 0.5); };
+        auto most_of = [&](double w, uint32_t c) { return (sd_u64) c * ((sd_u64) __double_as_longlong(w + (4503599627370496.0 + 1.0)) - SD_BITS52); };
         uint32_t sc = 0;
-        double   sb = 0.0;
+        sd_u64   sb = 0;
         // (loops that are not unrolled: most of a short row's time is code that runs once, and its way from memory)
         double w = edge;
 #pragma unroll 1
@@ -481,11 +482,11 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
             w *= fall;
         }
         const uint32_t mine = sc;
-        const double   mine_b = sb;
+        const sd_u64   mine_b = sb;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t pc = __shfl_up_sync(0xffffffffu, sc, o);
-            const double   pb = __shfl_up_sync(0xffffffffu, sb, o);
+            const sd_u64   pb = __shfl_up_sync(0xffffffffu, sb, o);
             if (lane >= o) { sc += pc; sb += pb; }
         }
         __syncthreads();
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
         if (tid == 0) { S.first = S.last = SD_FINE; S.n_list = 0; S.n_first = S.n_last = 0; }
         sd_sync(cl, R.P);
         sc -= mine; sb -= mine_b;
-        double most = 0.0;
+        sd_u64 most = 0;
         for (int p = 0; p < R.P; p++) {
             const sd_shared * o = cl.map_shared_rank(&S, p);
             if (p < R.part) { sc += o->cnt; sb += o->bound; }
@@ -505,15 +506,15 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
         // The bins between which the threshold lies.  What lies up to a bin weighs at most the sum of the bounds, `b`; at least e^(-1/256) of it, and at least all less the bounds behind it.
         // (4.1e-6: l_max - l is rounded to fp32, half a unit of 2^-19 at most; weights to integers, one unit for each of 2^18 tokens where the first alone weighs 2^44.  The last bin holds what lies
         // further away too, which weighs less than a unit each)
-        auto least = [&](double b) { return fmax(b * (0.99610136947 * (1.0 - 4.1e-6)), (double) mass - (most - b) * (1.0 + 4.1e-6)); };
+        auto least = [&](sd_u64 b) { return fmax((double) b * (0.99610136947 * (1.0 - 4.1e-6)), (double) mass - (double) (most - b) * (1.0 + 4.1e-6)); };
         const double reach = want * (1.0 - 4.1e-6);
         w = edge;
 #pragma unroll 1
         for (int b = b0; b < b0 + each; b++, w *= fall) {
             const uint32_t c = S.fine[b];
             if (!c) continue;
-            const double nb = sb + most_of(w, c);
-            const bool   f = by_k ? sc < k && sc + c >= k : sb < reach && nb >= reach, l = by_k ? f : (sc == 0 || least(sb) < want) && least(nb) >= want;
+            const sd_u64 nb = sb + most_of(w, c);
+            const bool   f = by_k ? sc < k && sc + c >= k : (double) sb < reach && (double) nb >= reach, l = by_k ? f : (sc == 0 || least(sb) < want) && least(nb) >= want;
             if (f || l)
                 for (int p = 0; p < R.P; p++) {
                     sd_shared * o = cl.map_shared_rank(&S, p);
