@@ -217,6 +217,7 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
     float * sv = reinterpret_cast<float *>(ring) + warp * PIB_MOE_MAX_EXPERTS;             // the token's logits
     for (int tk = warp; tk < A.b; tk += MF_THREADS / 32) {
         const float * z = A.z + tk * E;
+        __syncwarp();                                            // the last token's logits have been read
         float xmax = 0.f, xsum = 0.f;
         if (F8) { xmax = __ldcg(A.xm + 2 * tk); xsum = __ldcg(A.xm + 2 * tk + 1); }
         float mx = -INFINITY, sum = 1.f;
@@ -257,6 +258,7 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
             }
         }
         if (lane >= A.top) id = E + lane - A.top;
+        __syncwarp();                                            // other lanes' logits, read below, are there
         const bool has = lane < A.top + A.shared;
         float ng = 0.f, nu = 0.f;
         if (F8 && has) { ng = __ldg(A.norms + 2 * id); nu = __ldg(A.norms + 2 * id + 1); }
