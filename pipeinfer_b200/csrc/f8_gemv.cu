@@ -25,6 +25,12 @@ __device__ __forceinline__ void fg_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the consumers meet; true in all of them if it is in one: they leave together or not at all
+__device__ __forceinline__ bool fg_bar_or(bool v) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t) v) : "memory");
+    return any != 0;
+}
 // the row of a swizzled tile that MMA row (or column) g stands for: the rows of neighbouring g lie in different halves of the banks
 __device__ __forceinline__ int fg_perm(int g) { return (g >> 1) | (g & 1) << 2; }
 
@@ -207,9 +213,8 @@ __global__ void __launch_bounds__(FG_THREADS, 1) f8_gemv_kernel(const __grid_con
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) red[warp][RING ? fg_perm(t * 2 + (j & 1)) : t * 2 + (j & 1)][gp + (j >> 1) * 8] = acc[j];
-            asm volatile("bar.sync 1, 512;" ::: "memory");
+            if (fg_bar_or(*abort_s)) break;
             if (steps <= 32) w32 = w32_next;
-            if (*abort_s) break;                                 // raised in front of the barrier: every warp sees it and leaves here
             for (int e = threadIdx.x; e < A.b * 16; e += FG_WARPS * 32) {
                 const int     tk = e >> 4;
                 const int64_t n  = (int64_t) tile * 16 + (e & 15);
