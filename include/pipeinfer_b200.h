@@ -68,7 +68,8 @@ pib_weight * pib_weight_upload(int type, const void * host_blocks, int64_t N, in
 pib_weight * pib_weight_from_device(int type, const void * dev_blocks, int64_t N, int64_t K);
 /* PIB_TYPE_F8: q [N][K] e4m3 bytes, scales fp32 [ceil(N/128)][ceil(K/128)]; element (n, k) stands for scales[n/128][k/128] * q[n][k].  From host or device memory (the latter in the order of the
  * legacy default stream; it waits).  Such a weight goes through the calls below like any other: pib_act_bytes, pib_quantize_act, pib_norm_quantize_act, pib_quantize_act_rows with
- * wtype PIB_TYPE_F8, pib_gemv, pib_gemv_fused, pib_gemm, pib_get_rows and the host forms.  pib_weight_row_blocks writes a row's K e4m3 bytes and behind them its
+ * wtype PIB_TYPE_F8, pib_gemv, pib_gemv_fused, pib_gemm, pib_get_rows and the host forms.  Waits inside the three products' kernels are bounded and reported by pib_gemm_check(stream);
+ * the host forms ask it themselves.  pib_weight_row_blocks writes a row's K e4m3 bytes and behind them its
  * ceil(K/128) scales (4 bytes each, not aligned); pib_act_to_blocks blocks of {float d, 128 e4m3}, zero behind column K. */
 pib_weight * pib_weight_upload_f8(const void * q_host, const float * scales_host, int64_t N, int64_t K);
 pib_weight * pib_weight_from_device_f8(const void * q_dev, const float * scales_dev, int64_t N, int64_t K);

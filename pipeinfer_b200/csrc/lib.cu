@@ -189,6 +189,7 @@ extern "C" int pib_mul_mat_host(const pib_weight * w, const float * x_host, int 
     if (cudaMemcpy(x, x_host, xb, cudaMemcpyHostToDevice) != cudaSuccess) rc = PIB_ERR_CUDA;
     if (rc == PIB_OK) rc = pib_quantize_act(pib_act_family(w->type), x, b, w->K, act, nullptr);
     if (rc == PIB_OK) rc = pib_gemv(w, act, b, y, variant, nullptr);
+    if (rc == PIB_OK && w->type == PIB_TYPE_F8 && (rc = pib_gemm_check(nullptr)) != PIB_OK) { cudaFree(buf); return rc; }      // its kernels' waits are bounded
     if (rc == PIB_OK && cudaMemcpy(y_host, y, yb, cudaMemcpyDeviceToHost) != cudaSuccess) rc = PIB_ERR_CUDA;
     if (rc == PIB_ERR_CUDA) pib_set_error("pib_mul_mat_host: %s", cudaGetErrorString(cudaGetLastError()));
     cudaFree(buf);

@@ -297,3 +297,21 @@ def test_more_than_four_gigabytes(torch, pib):
     torch.cuda.synchronize()
     for i, r in enumerate(ids.tolist()):
         assert torch.equal(out[i], dense(torch, q[r:r + 1], s[r // 128:r // 128 + 1])[0].float())
+
+
+@pytest.mark.parametrize("b", [3, 12])
+def test_host_forms_report_a_wait_that_ran_out(torch, pib, b):
+    """the error word of the stream is written here in a kernel's place"""
+    import subprocess
+    lib = pib.load()
+    names = subprocess.run(["nm", "-D", "--defined-only", pib.SO_PATH], capture_output=True, text=True, check=True).stdout.split()
+    word = getattr(lib.L, next(n for n in names if "pib_tc_error_word" in n))
+    word.restype, word.argtypes = C.c_void_p, [C.c_void_p]
+    q, s, g = matrix(torch, 300, 260, 5)
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), 300, 260)
+    x, y, seven = np.ones((b, 260), np.float32), np.zeros((b, 300), np.float32), np.array([7], np.int32)
+    for fn in (lambda: lib.L.pib_mul_mat_host(w.h, x.ctypes.data, b, y.ctypes.data, 0), lambda: lib.L.pib_gemm_host(w.h, x.ctypes.data, b, y.ctypes.data)):
+        assert fn() == 0
+        lib.check(lib.L.pib_memcpy_h2d(word(None), seven.ctypes.data, 4, None))
+        assert fn() == -1 and b"block 6" in lib.L.pib_last_error()
+        assert fn() == 0
