@@ -124,7 +124,7 @@ int pib_gemv_direct_splits(int64_t N, int64_t K);
  *   prologue 0: x                                             (quantize_row_q8_K of the attention output)
  *   prologue 1: rmsnorm(x [+ addend]) * x2, eps               (ggml_add, ggml_rms_norm ggml.c:9028, ggml_mul; sum_out, if given, receives x + addend)
  *   prologue 2: silu(x) * x2                                  (ggml_silu through the fp16 table ggml.c:1490, ggml_mul; x and x2 rows xstride apart)
- * F8 weights (same b and K; any prologue): silu(x) = x / (1 + e^-x) in fp32.
+ * F8 weights (same b and K; any prologue): silu(x) = x / (1 + e^-x) in fp32; y and sum_out lie over none of the inputs (every block reads the inputs for itself).
  * Device pointers; x [b][xstride or K] fp32, y [b][N] fp32.  Same values as pib_quantize_act / pib_norm_quantize_act followed by pib_gemv
  * up to the order of the fp32 additions. */
 int pib_gemv_fused(const pib_weight * w, int prologue, const float * x_dev, const float * x2_dev, const float * addend_dev, float * sum_out_dev,

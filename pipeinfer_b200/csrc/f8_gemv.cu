@@ -273,14 +273,27 @@ int pib_f8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaSt
 
 int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st) {
     if (b < 1 || b > 8 || w->K > 8192) { pib_set_error("pib_gemv_fused: unsupported matrix / batch"); return PIB_ERR_UNSUPP; }
-    if (pro == 1 && sum_out && (sum_out == x || sum_out == addend)) { pib_set_error("pib_gemv_fused: sum_out_dev is an input that other blocks still read"); return PIB_ERR_ARG; }
+    const int64_t xs = xstride ? xstride : w->K;
+    if (xs < 0) { pib_set_error("pib_gemv_fused: bad arguments"); return PIB_ERR_ARG; }
+    auto over = [&](const float * o, int64_t n, const float * in, int64_t stride) {            // n floats at o, rows of K at in
+        for (int t = 0; t < b; t++) if (o && in && o < in + t * stride + w->K && in + t * stride < o + n) return true;
+        return false;
+    };
+    const float * out[2] = { y, pro == 1 ? sum_out : nullptr };
+    for (int i = 0; i < 2; i++) {
+        const int64_t n = b * (i ? w->K : w->N);
+        if (over(out[i], n, x, xs) || (pro && over(out[i], n, x2, pro == 2 ? xs : 0)) || (pro == 1 && over(out[i], n, addend, w->K))) {
+            pib_set_error("pib_gemv_fused: an output lies over an input that other blocks still read");
+            return PIB_ERR_ARG;
+        }
+    }
     if (((uintptr_t) x | (uintptr_t) x2 | (uintptr_t) addend | (uintptr_t) sum_out | (uintptr_t) y) & 3) { pib_set_error("pib_gemv_fused: fp32 rows need 4-byte alignment"); return PIB_ERR_ARG; }
     fg_args A;
     const CUtensorMap & wmap = ((const pib_f8_maps *) w->map)->stage;
     const int rc = fg_of(A, w, b, y, st);
     if (rc != PIB_OK) return rc;
     A.x = x; A.x2 = pro ? x2 : nullptr; A.addend = pro == 1 ? addend : nullptr; A.sum_out = pro == 1 ? sum_out : nullptr;
-    A.xs = xstride ? xstride : w->K; A.eps = eps;
+    A.xs = xs; A.eps = eps;
     A.vec = w->K % 4 == 0 && A.xs % 4 == 0 && !(((uintptr_t) A.x | (uintptr_t) A.x2 | (uintptr_t) A.addend) & 15);
     switch (pro) {
         case 0:  return fg_launch<0>(wmap, wmap, A, st);

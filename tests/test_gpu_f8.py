@@ -315,3 +315,18 @@ def test_host_forms_report_a_wait_that_ran_out(torch, pib, b):
         lib.check(lib.L.pib_memcpy_h2d(word(None), seven.ctypes.data, 4, None))
         assert fn() == -1 and b"block 6" in lib.L.pib_last_error()
         assert fn() == 0
+
+
+def test_fused_outputs_over_inputs_are_refused(torch, pib):
+    lib, N, K, b = pib.load(), 256, 256, 3
+    q, s, g = matrix(torch, N, K, 9)
+    w = pib.F8Weight(lib, q.data_ptr(), s.data_ptr(), N, K)
+    buf = torch.randn(8, b, 400, device="cuda", generator=g)
+    x, x2, add, out, y = (buf[i].data_ptr() for i in range(5))
+    call = lambda pro, x, x2, add, out, y, xs=400: lib.L.pib_gemv_fused(w.h, pro, x, x2, add, out, xs, 1e-5, b, y, None)
+    for args in ((0, x, None, None, None, x), (0, x, None, None, None, x + 255 * 4), (0, x, None, None, None, x + 801 * 4), (0, x + 800 * 4, None, None, None, x + 33 * 4), (1, x, x2, add, out, x2 + 1020),
+                 (1, x, x2, add, out, add), (1, x, x2, add, x + 4, y), (1, x, x2, add, add, y), (1, x, x2, add, x2, y), (2, x, x2, None, None, x2 + 1200 * 4 - 600), (0, x, None, None, None, y, -400)):
+        assert call(*args) == -2 and b"pib_gemv_fused" in lib.L.pib_last_error(), args
+    for args in ((0, x, None, None, None, x + 1200 * 4), (1, x, x2, add, out, y), (2, x, x2, None, None, y), (0, x, None, None, None, x + 256 * 4, 1100)):          # the last one between two rows of x
+        assert call(*args) == 0, args
+    torch.cuda.synchronize()
