@@ -161,7 +161,9 @@ int pib_get_rows(const pib_weight * w, const int32_t * ids_dev, int n, float * o
 /* ---- a whole mixture layer for a few tokens ----------------------------------------------------------------------- */
 /* y[t] = residual[t] + sum over the chosen experts e of w_e D_e (silu(G_e x[t]) * U_e x[t]) + sum over the shared experts s of D_s (silu(G_s x[t]) * U_s x[t])
  * z = R x, score = softmax(z) or sigmoid(z) per output; chosen are the `top` largest score + correction (the lower index among equals); w = scale * score,
- * divided by (the chosen scores' sum + 1e-20) with renorm.  Everything is fp32 but the experts' matrices, which are e4m3 with block scales (PIB_TYPE_F8) or bfloat16. */
+ * divided by (the chosen scores' sum + 1e-20) with renorm.  The experts' matrices are e4m3 with block scales (PIB_TYPE_F8) or bfloat16, all else is fp32; sums are fp32.  Into the products with
+ * e4m3 a token's x enters with 22 bits of each value down to 2^-16 of the row's largest (below that to 2^-39 of the largest), silu(..) * .. the same way for each 16 neighbouring values; into
+ * those with bfloat16 both enter with 24 bits. */
 #define PIB_MOE_SOFTMAX 0
 #define PIB_MOE_SIGMOID 1
 #define PIB_MOE_MAX_EXPERTS 512   /* router outputs */

@@ -14,14 +14,15 @@
 //   publisher warp    makes an item's results known to the other blocks and adds up finished rows: fences and atomics that the consumers would stand still for
 //
 // Products: mma.m16n8k16, expert rows as M, the expert's tokens as N.  Weights enter exactly: e4m3 as fp16 (times the block's scale in fp32 behind the sum), bfloat16 as it is.  The fp32
-// activations enter as parts: with e4m3 weights two fp16 of the row times a power of two that brings its largest to 2^14 .. 2^15 (22 bits, to 2^-39 of the largest), with bfloat16 weights
-// three bfloat16 (24 bits).  (h is split where it is made, before the rest of its row is there: its power of two brings a bound of the row, the largest norms of the expert's gate and up
-// rows times the token's squared norm, to 2^14 .. 2^15; the bound lies some 2^9 above the largest, which leaves 2^-31 of it.)  Half a line's sums are made by the tensor core, scaled and added up in fp32.  Four tokens' two parts (eight tokens' one of three) share
-// the eight columns of one MMA; an expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which
-// costs less than a second form of the kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
+// activations enter as parts: with e4m3 weights two fp16 of the values times a power of two that brings the largest of them to 2^14 .. 2^15 (22 bits, down to 2^-39 of the largest), with bfloat16
+// weights three bfloat16 (24 bits).  x has a power of two a row; h is split where it is made, 16 values of a row, so each such tile has its own: the k of one MMA, whose sum is scaled by it.
+// (A bound of the row, which is there before the row is, in its place: where an expert's rows differ by a factor of 300 that left 2^-12 of the layer's output.)
+// Half a line's sums (F8 with h: a tile's) are made by the tensor core, scaled and added up in fp32.  Four tokens' two parts (eight tokens' one of three) share the eight columns of one MMA; an
+// expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which costs less than a second form of the
+// kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
 // a row (lane t) are four values each of four (two) neighbouring tiles of 16, the k of an MMA, and the parts lie in that order too.
-// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in 312 us (0.77 of the copy rate; the choice takes some 8 us of it, the turns of 48 KB down items the
-// rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 31 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
+// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in some 335 us (0.72 of the copy rate; the choice takes some 8 us of it, a power of two for each tile of h
+// some 10, the turns of 48 KB down items the rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 30 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
 // way to memory and back each.  Sharing the choice among the blocks would save none of it: the launch's first 4 us are mostly the way of its code into the caches.
 #include <cuda_bf16.h>
 
@@ -37,8 +38,7 @@
 #define MF_LINE    4096                       // 128 bytes of 32 rows
 #define MF_STAGE   (MF_WARPS * MF_LINE)
 #define MF_STAGES  3
-#define mf_bar()   asm volatile("bar.sync 1, 192;" ::: "memory")          // the consumers
-// the same; true in all of them if it is in one: they leave together or not at all
+// the consumers meet; true in all of them if it is in one: they leave together or not at all
 __device__ __forceinline__ bool mf_bar_or(bool v) {
     uint32_t any;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 192, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t) v) : "memory");
@@ -53,7 +53,6 @@ struct pib_moe {
     uint8_t * w1, * w2;                  // [experts + shared][T1][KB1][16 gate rows, 16 up rows][128 bytes], [..][T2][KB2][32 rows][128 bytes], zero behind the matrices; the 16-byte pieces of a row
                                          // lie at their number xor (row & 7): lanes of neighbouring rows read different banks
     float * s1, * s2;                    // F8: [..][gate, up][rows / 128][KB1], [..][rows / 128][KB2]
-    float * norms;                       // [..][gate, up]: the largest squared norm of a row
 };
 struct mf_args {
     int b, E, shared, top, score, renorm, has_corr, T1, T2, KB1, KB2, nb1, nb2;
@@ -63,13 +62,12 @@ struct mf_args {
     const uint8_t * w1, * w2;
     const float * s1, * s2;
     const float * res; int64_t ldr, ldy;
-    const uint16_t * xp; const float * xm;                   // parts of the tokens' rows, their largest |x| and squared norm
-    uint16_t * hp;                                           // parts of the pairs' rows of h
-    const float * norms;
+    const uint16_t * xp; const float * xm;                   // parts of the tokens' rows, their largest |x|
+    uint16_t * hp, * hx;                                     // parts of the pairs' rows of h; F8: the power of two that brings a tile of 16 back, its upper half
     float * y, * part;
     int * cnt, * err;                    // cnt: ticket, abort, up items done per entry of the list, entries done per 32 output rows
 };
-struct mf_layout { size_t z, xm, xp, hp, part, total; int64_t Dr; int n_cnt; };
+struct mf_layout { size_t z, xm, xp, hp, hx, part, total; int64_t Dr; int n_cnt; };
 // a row's parts: [part][line][lane t][tile of the line][4] 16-bit numbers; 64 (F8) or 32 bytes per line, part and lane
 __host__ __device__ static inline int64_t mf_row_of(bool f8, int KB) { return (int64_t) KB * (f8 ? 2 * 128 : 3 * 64); }
 static mf_layout mf_of(const pib_moe * m, int b) {
@@ -80,10 +78,11 @@ static mf_layout mf_of(const pib_moe * m, int b) {
     L.Dr = (int64_t) m->T2 * 32;
     L.n_cnt = 2 + (int) P + m->T2;
     L.xm = al((size_t) L.n_cnt * 4);
-    L.z = L.xm + al((size_t) b * 8);
+    L.z = L.xm + al((size_t) b * 4);
     L.xp = L.z + al((size_t) b * m->s.experts * 4);
     L.hp = L.xp + al((size_t) (b * mf_row_of(f8, m->KB1)) * 2);
-    L.part = L.hp + al((size_t) (P * mf_row_of(f8, m->KB2)) * 2);
+    L.hx = L.hp + al((size_t) (P * mf_row_of(f8, m->KB2)) * 2);
+    L.part = L.hx + (f8 ? al((size_t) P * m->KB2 * 16) : 0);
     L.total = L.part + al((size_t) (P * L.Dr) * 4);
     return L;
 }
@@ -91,6 +90,15 @@ static mf_layout mf_of(const pib_moe * m, int b) {
 __device__ __forceinline__ void mf_mma_h(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two fp32 at a time
+__device__ __forceinline__ uint64_t mf_pair(float lo, float hi) { return (uint64_t) __float_as_uint(hi) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ uint64_t mf_mul2(uint64_t a, uint64_t b) { uint64_t d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ uint64_t mf_fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+// mf_mma_h without sums before it
+__device__ __forceinline__ void mf_mma_h0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mf_mma_b(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -140,16 +148,14 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
         const int t = blockIdx.x - groups * E;
         float up = 1.f;
         if (F8) {
-            __shared__ float sq[8];
-            float m = 0.f, n = 0.f;
-            for (int64_t k = threadIdx.x; k < D; k += 256) { const float v = x[t * ldx + k]; m = fmaxf(m, fabsf(v)); n = fmaf(v, v, n); }
-            m = warp_max(m); n = warp_sum(n);
-            if (lane == 0) { red[warp][0] = m; sq[warp] = n; }
+            float m = 0.f;
+            for (int64_t k = threadIdx.x; k < D; k += 256) m = fmaxf(m, fabsf(x[t * ldx + k]));
+            m = warp_max(m);
+            if (lane == 0) red[warp][0] = m;
             __syncthreads();
-            n = 0.f;
-            for (int i = 0; i < 8; i++) { m = fmaxf(m, red[i][0]); n += sq[i]; }
+            for (int i = 0; i < 8; i++) m = fmaxf(m, red[i][0]);
             up = mf_pow2(mf_exponent(m));
-            if (threadIdx.x == 0) { xm[2 * t] = m; xm[2 * t + 1] = n; }
+            if (threadIdx.x == 0) xm[t] = m;
         }
         for (int u = threadIdx.x; u < KB * (F8 ? 128 : 64); u += 256) mf_store<F8>(u < D ? x[t * ldx + u] : 0.f, up, u >> 4, u & 15, KB, xp + t * mf_row_of(F8, KB));
         return;
@@ -192,8 +198,7 @@ template <bool F8, int NT> __global__ void __launch_bounds__(256) moe_logits_ker
 // ---- the layer ----------------------------------------------------------------------------------------------------------------------
 struct mf_shared {
     float    wts[16][16];
-    uint16_t pf[16][16];                  // of a choice; px, ph: of a pair (a row)
-    int      px[256], ph[256];
+    int      px[16];                      // the exponent field of a token's power of two
     int      ids[16][16], at[16][16];     // chosen experts of a token; its row of h and of the experts' outputs
     uint32_t mask[PIB_MOE_MAX_EXPERTS + 16], tokens[256];        // of an expert, of an entry of the list
     int      slot[PIB_MOE_MAX_EXPERTS + 16], act[256], base[256], n_act, item[MF_STAGES], pub[2], abort;
@@ -218,8 +223,7 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
     for (int tk = warp; tk < A.b; tk += MF_THREADS / 32) {
         const float * z = A.z + tk * E;
         __syncwarp();                                            // the last token's logits have been read
-        float xmax = 0.f, xsum = 0.f;
-        if (F8) { xmax = __ldcg(A.xm + 2 * tk); xsum = __ldcg(A.xm + 2 * tk + 1); }
+        const float xmax = F8 ? __ldcg(A.xm + tk) : 0.f;
         float mx = -INFINITY, sum = 1.f;
         for (int i = lane; i < E; i += 32) { const float v = __ldcg(z + i); sv[i] = v; mx = fmaxf(mx, v); }
         if (A.score == PIB_MOE_SOFTMAX) {
@@ -260,14 +264,11 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
         if (lane >= A.top) id = E + lane - A.top;
         __syncwarp();                                            // other lanes' logits, read below, are there
         const bool has = lane < A.top + A.shared;
-        float ng = 0.f, nu = 0.f;
-        if (F8 && has) { ng = __ldg(A.norms + 2 * id); nu = __ldg(A.norms + 2 * id + 1); }
         const float mine = lane < A.top ? score(sv[id]) : 0.f, tot = warp_sum(mine);
         if (has) {
             S.ids[tk][lane] = id;
             S.wts[tk][lane] = lane < A.top ? A.scale * (A.renorm ? mine / (tot + 1e-20f) : mine) : 1.f;
-            // the exponent fields of the powers of two of the pair's rows of x and h
-            if (F8) S.pf[tk][lane] = (uint16_t) (mf_exponent(xmax) | mf_exponent(1.01f * sqrtf(ng) * sqrtf(nu) * xsum) << 8);
+            if (F8 && lane == 0) S.px[tk] = mf_exponent(xmax);
         }
     }
     const int all = E + A.shared, per = A.top + A.shared;
@@ -304,9 +305,7 @@ template <bool F8> __device__ __forceinline__ void mf_route(const mf_args & A, m
     __syncthreads();
     for (int i = threadIdx.x; i < A.b * per; i += MF_THREADS) {
         const int tk = i / per, e = S.ids[tk][i % per];
-        const int at = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
-        S.at[tk][i % per] = at;
-        if (F8) { S.px[at] = S.pf[tk][i % per] & 255; S.ph[at] = S.pf[tk][i % per] >> 8; }
+        S.at[tk][i % per] = S.base[S.slot[e]] + __popc(S.mask[e] & ((1u << tk) - 1));
     }
 }
 
@@ -316,21 +315,22 @@ __device__ __forceinline__ int mf_nth_bit(uint32_t m, int n) {
 }
 __device__ __forceinline__ uint4 mf_ld(const uint16_t * p) { return __ldcg(reinterpret_cast<const uint4 *>(p)); }
 
-// What a lane holds of a line's activations for one column tile: PARTS pieces of the row of column g (PACK: of token g & 3, part g >> 2)
-template <bool F8, bool PACK> struct mf_b {
-    static constexpr int PARTS = F8 ? (PACK ? 1 : 2) : 3, WORDS = F8 ? 4 : 2;
+// What a lane holds of a line's activations: the row of column g (F8: of token g & 3, part g >> 2), three parts of it with bfloat16
+template <bool F8> struct mf_b {
+    static constexpr int PARTS = F8 ? 1 : 3, WORDS = F8 ? 4 : 2;
     uint4 v[PARTS][WORDS];
 };
-template <bool F8, bool PACK> __device__ __forceinline__ void mf_ask(mf_b<F8, PACK> & B, const uint16_t * row, int plane, int kb, int t) {
-    constexpr int P = mf_b<F8, PACK>::PARTS, W = mf_b<F8, PACK>::WORDS;
+template <bool F8> __device__ __forceinline__ void mf_ask(mf_b<F8> & B, const uint16_t * row, int plane, int kb, int t) {
+    constexpr int P = mf_b<F8>::PARTS, W = mf_b<F8>::WORDS;
 #pragma unroll
     for (int part = 0; part < P; part++)
 #pragma unroll
         for (int w = 0; w < W; w++) B.v[part][w] = row ? mf_ld(row + part * plane + (kb * 4 + t) * (W * 8) + w * 8) : make_uint4(0, 0, 0, 0);
 }
-// half c of a line of a piece times eight columns: acc[tile of 16 rows].  f: what a sum of the tile of rows is worth, per column that the lane holds
-template <bool F8, bool PACK> __device__ __forceinline__ void mf_half(const uint8_t * line, int c, int lane, const mf_b<F8, PACK> & B, const float (&f)[2][2], float (&acc)[2][4]) {
-    constexpr int P = mf_b<F8, PACK>::PARTS;
+// Half c of a line of a piece times eight columns: acc[tile of 16 rows].  f: what a sum of the tile of rows is worth, per column that the lane holds; x: what the sums of four
+// tiles of k are multiplied with besides (F8 with h), 16 bits each
+template <bool F8, bool UP> __device__ __forceinline__ void mf_half(const uint8_t * line, int c, int lane, const mf_b<F8> & B, const float (&f)[2][2], const uint2 (&x)[2], uint64_t (&acc)[2][2]) {
+    constexpr int P = mf_b<F8>::PARTS;
     const int g = lane >> 2, t = lane & 3, gp = (g >> 1) | (g & 1) << 2;
     int4  w[2][2];
     float s[2][4];
@@ -343,20 +343,30 @@ template <bool F8, bool PACK> __device__ __forceinline__ void mf_half(const uint
     }
     if (F8) {
 #pragma unroll
-        for (int q = 0; q < 4; q++)                              // 16 values of k each
+        for (int q = 0; q < 4; q++) {                            // 16 values of k each
+            const uint4    b = B.v[0][c * 2 + (q >> 1)];
+            const uint32_t b0 = q & 1 ? b.z : b.x, b1 = q & 1 ? b.w : b.y;
+            uint64_t d = 0;
+            if (!UP) {
+                const uint32_t x0 = q < 2 ? x[0].x : x[0].y, x1 = q < 2 ? x[1].x : x[1].y;
+                d = mf_mul2(mf_pair(f[0][0], f[0][1]), mf_pair(__uint_as_float(q & 1 ? x0 & 0xffff0000u : x0 << 16), __uint_as_float(q & 1 ? x1 & 0xffff0000u : x1 << 16)));
+            }
 #pragma unroll
             for (int m = 0; m < 2; m++) {
                 const uint32_t r0 = (uint32_t) (q == 0 ? w[m][0].x : q == 1 ? w[m][0].y : q == 2 ? w[m][0].z : w[m][0].w), r1 = (uint32_t) (q == 0 ? w[m][1].x : q == 1 ? w[m][1].y : q == 2 ? w[m][1].z : w[m][1].w);
                 const uint32_t a0 = mf_half2(r0, 0), a1 = mf_half2(r1, 0), a2 = mf_half2(r0, 1), a3 = mf_half2(r1, 1);
-#pragma unroll
-                for (int part = P - 1; part >= 0; part--) {      // the small ones first
-                    const uint4 b = B.v[part][c * 2 + (q >> 1)];
-                    mf_mma_h(s[m], a0, a1, a2, a3, q & 1 ? b.z : b.x, q & 1 ? b.w : b.y);
+                if (UP) mf_mma_h(s[m], a0, a1, a2, a3, b0, b1);
+                else {
+                    mf_mma_h0(s[m], a0, a1, a2, a3, b0, b1);
+                    acc[m][0] = mf_fma2(mf_pair(s[m][0], s[m][1]), d, acc[m][0]);
+                    acc[m][1] = mf_fma2(mf_pair(s[m][2], s[m][3]), d, acc[m][1]);
                 }
             }
+        }
+        if (!UP) return;
     } else {
 #pragma unroll
-        for (int part = P - 1; part >= 0; part--) {
+        for (int part = P - 1; part >= 0; part--) {              // the small ones first
             const uint4 b = B.v[part][c];
 #pragma unroll
             for (int m = 0; m < 2; m++) {
@@ -368,26 +378,28 @@ template <bool F8, bool PACK> __device__ __forceinline__ void mf_half(const uint
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[m][j] = F8 ? fmaf(s[m][j], f[m][j & 1], acc[m][j]) : acc[m][j] + s[m][j];
+        for (int j = 0; j < 2; j++) acc[m][j] = mf_fma2(mf_pair(s[m][2 * j], s[m][2 * j + 1]), F8 ? mf_pair(f[m][0], f[m][1]) : mf_pair(1.f, 1.f), acc[m][j]);
 }
 
 // An item, by the consumers: the warp's lines of its pieces, the meeting, the results.  turn: the item's turn at the places of the sums.  False: the block gives up
 template <bool F8, bool UP>
 __device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const uint8_t * ring, uint32_t bar_f, uint32_t bar_e, mf_place & at, int turn, int a, int i) {
-    constexpr bool PACK = F8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, e = S.act[a], base = S.base[a], KB = UP ? A.KB1 : A.KB2;
     const uint32_t mask = S.tokens[a];
     const int n = __popc(mask), stride = (int) mf_row_of(F8, KB), plane = KB * (F8 ? 128 : 64);
     // row of a column, -1: none
-    auto row_of = [&](int c) { c = PACK ? c & 3 : c; return c >= n ? -1 : UP ? mf_nth_bit(mask, c) : base + c; };
+    auto row_of = [&](int c) { c = F8 ? c & 3 : c; return c >= n ? -1 : UP ? mf_nth_bit(mask, c) : base + c; };
     const int r = row_of(g);
-    const uint16_t * row = r < 0 ? nullptr : (UP ? A.xp : A.hp) + (int64_t) r * stride + (PACK && g >= 4 ? plane : 0);
+    const uint16_t * row = r < 0 ? nullptr : (UP ? A.xp : A.hp) + (int64_t) r * stride + (F8 && g >= 4 ? plane : 0);
+    // of the lane's two columns: the inverse of x's power of two, and where those of h's tiles lie
     float d[2] = { 1.f, 1.f };
+    const uint16_t * hx[2] = { nullptr, nullptr };
     if (F8)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const int c = (t * 2 + k) & 3;
-            d[k] = c < n ? mf_pow2(254 - (UP ? S.px : S.ph)[base + c]) : 1.f;
+            const int rc = row_of(t * 2 + k);
+            if (UP && rc >= 0) d[k] = mf_pow2(254 - S.px[rc]);
+            if (!UP) hx[k] = rc < 0 ? nullptr : A.hx + (int64_t) rc * (KB * 8);
         }
     const float * sa = nullptr, * sb = nullptr;
     if (F8) {
@@ -402,16 +414,13 @@ __device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const 
         hb = UP && kb < KB ? __ldg(sb + kb) : 0.f;
     };
     if (F8) scales(0);
-    float acc[2][4];
-#pragma unroll
-    for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int q = 0; q < 4; q++) acc[m][q] = 0.f;
+    uint64_t acc[2][2] = { { 0, 0 }, { 0, 0 } };
 #pragma unroll 1
     for (int st = 0; st < KB; st += MF_WARPS) {
         const int  kb = st + warp;
         const bool in = kb < KB;
-        mf_b<F8, PACK> B;
+        mf_b<F8> B;
+        uint4 x[2] = { make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0) };
         float wa = 1.f, wb = 1.f;
         if (F8) {
             const int j = st / MF_WARPS;
@@ -419,13 +428,18 @@ __device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const 
             wa = __shfl_sync(0xffffffffu, ha, j & 31);
             wb = UP ? __shfl_sync(0xffffffffu, hb, j & 31) : wa;
         }
-        if (in) mf_ask<F8, PACK>(B, row, plane, kb, t);          // ahead of the wait
+        if (in) {                                                // ahead of the wait
+            mf_ask<F8>(B, row, plane, kb, t);
+            if (F8 && !UP)
+#pragma unroll
+                for (int k = 0; k < 2; k++) if (hx[k]) x[k] = mf_ld(hx[k] + kb * 8);
+        }
         if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_f + at.s * 8, at.ph, (volatile int *) &S.abort))) break;
         if (in) {
             const uint8_t * line = ring + at.s * MF_STAGE + warp * MF_LINE;
             const float f[2][2] = { { wa * d[0], wa * d[1] }, { wb * d[0], wb * d[1] } };
-            mf_half<F8, PACK>(line, 0, lane, B, f, acc);
-            mf_half<F8, PACK>(line, 1, lane, B, f, acc);
+            mf_half<F8, UP>(line, 0, lane, B, f, { make_uint2(x[0].x, x[0].y), make_uint2(x[1].x, x[1].y) }, acc);
+            mf_half<F8, UP>(line, 1, lane, B, f, { make_uint2(x[0].z, x[0].w), make_uint2(x[1].z, x[1].w) }, acc);
         }
         __syncwarp();
         if (lane == 0) dt_arrive(bar_e + at.s * 8);
@@ -436,12 +450,12 @@ __device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const 
 #pragma unroll
     for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) red[warp][t * 2 + (q & 1)][m * 16 + gp + (q >> 1) * 8] = acc[m][q];
+        for (int q = 0; q < 4; q++) red[warp][t * 2 + (q & 1)][m * 16 + gp + (q >> 1) * 8] = __uint_as_float((uint32_t) (acc[m][q >> 1] >> (q & 1) * 32));
     if (mf_bar_or(*(volatile int *) &S.abort)) return false;
     auto sum = [&](int c, int k) {
         float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < MF_WARPS; w++) x += PACK ? red[w][c][k] + red[w][c + 4][k] : red[w][c][k];
+        for (int w = 0; w < MF_WARPS; w++) x += F8 ? red[w][c][k] + red[w][c + 4][k] : red[w][c][k];
         return x;
     };
     if (UP) {
@@ -450,8 +464,20 @@ __device__ __forceinline__ bool mf_item(const mf_args & A, mf_shared & S, const 
             const int c = q >> 4, k = q & 15;
             const float gt = sum(c, k), u = sum(c, 16 + k), h = gt / (1.0f + expf(-gt)) * u;
             uint16_t *  hrow = A.hp + (int64_t) (base + c) * mf_row_of(F8, A.KB2);
-            mf_store<F8>(h, F8 ? mf_pow2(S.ph[base + c]) : 1.f, i, k, A.KB2, hrow);
-            for (int z = i + 1; z < last; z++) mf_store<F8>(0.f, 1.f, z, k, A.KB2, hrow);
+            uint16_t *  hx = A.hx + (int64_t) (base + c) * (A.KB2 * 8);
+            int field = 127;
+            if (F8) {                                            // 16 neighbouring lanes hold the tile
+                float m = fabsf(h);
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffu << (lane & 16), m, o));
+                field = mf_exponent(m);
+                if (k == 0) __stcg(hx + i, (uint16_t) ((254 - field) << 7));
+            }
+            mf_store<F8>(h, mf_pow2(field), i, k, A.KB2, hrow);
+            for (int z = i + 1; z < last; z++) {
+                mf_store<F8>(0.f, 1.f, z, k, A.KB2, hrow);
+                if (F8 && k == 0) __stcg(hx + z, (uint16_t) (127 << 7));
+            }
         }
     } else
         for (int q = threadIdx.x; q < n * 32; q += MF_WARPS * 32) __stcg(A.part + (int64_t) (base + (q >> 5)) * A.Dr + i * 32 + (q & 31), sum(q >> 5, q & 31));
@@ -606,28 +632,6 @@ static cudaError_t mf_pack(const void * src, uint8_t * dst, int64_t E, int64_t r
     return cudaGetLastError();
 }
 
-// the largest squared norm of an expert's rows, a block per expert and matrix; scales of gate and up are neighbours (pib_moe::s1)
-static __global__ void __launch_bounds__(256) mf_norms_kernel(const uint8_t * __restrict__ gate, const uint8_t * __restrict__ up, const float * __restrict__ s1, int64_t F, int64_t D, int nb1, int KB1,
-                                                              float * __restrict__ norms) {
-    __shared__ float red[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t e = blockIdx.x;
-    const uint8_t * w = (blockIdx.y ? up : gate) + e * F * D;
-    float most = 0.f;
-    for (int64_t r = warp; r < F; r += 8) {
-        const float * s = s1 + ((e * 2 + blockIdx.y) * nb1 + r / 128) * KB1;
-        float n = 0.f;
-        for (int64_t k = lane; k < D; k += 32) { const float v = __half2float(__half(__nv_cvt_fp8_to_halfraw(w[r * D + k], __NV_E4M3))) * s[k / 128]; n = fmaf(v, v, n); }
-        most = fmaxf(most, warp_sum(n));
-    }
-    if (lane == 0) red[warp] = most;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; i++) most = fmaxf(most, red[i]);
-        norms[e * 2 + blockIdx.y] = most;
-    }
-}
-
 extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float * router, const float * correction, const void * gate, const float * gate_scales, const void * up,
                                          const float * up_scales, const void * down, const float * down_scales) {
     const bool f8 = sh && sh->type == PIB_TYPE_F8;
@@ -647,9 +651,9 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
     m->T1 = (int) ((F + 15) / 16); m->T2 = (int) ((D + 31) / 32);
     auto al = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     const size_t n_r = al((size_t) (sh->experts * D) * 4), n_c = al((size_t) sh->experts * 4), n_1 = (size_t) E * m->T1 * 32 * m->KB1 * 128, n_2 = (size_t) E * m->T2 * 32 * m->KB2 * 128;
-    const size_t n_s1 = f8 ? al((size_t) (E * 2 * pib_f8_blocks(F) * m->KB1) * 4) : 0, n_s2 = f8 ? al((size_t) (E * pib_f8_blocks(D) * m->KB2) * 4) : 0, n_n = f8 ? al((size_t) E * 8) : 0;
-    if (cudaGetDevice(&m->dev) != cudaSuccess || cudaMalloc(&m->base, n_r + n_c + n_1 + n_2 + n_s1 + n_s2 + n_n) != cudaSuccess) {
-        pib_set_error("pib_moe_from_device: cudaMalloc of %zu bytes failed", n_r + n_c + n_1 + n_2 + n_s1 + n_s2 + n_n);
+    const size_t n_s1 = f8 ? al((size_t) (E * 2 * pib_f8_blocks(F) * m->KB1) * 4) : 0, n_s2 = f8 ? al((size_t) (E * pib_f8_blocks(D) * m->KB2) * 4) : 0;
+    if (cudaGetDevice(&m->dev) != cudaSuccess || cudaMalloc(&m->base, n_r + n_c + n_1 + n_2 + n_s1 + n_s2) != cudaSuccess) {
+        pib_set_error("pib_moe_from_device: cudaMalloc of %zu bytes failed", n_r + n_c + n_1 + n_2 + n_s1 + n_s2);
         cudaGetLastError();
         free(m);
         return nullptr;
@@ -657,7 +661,7 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
     m->router = (float *) m->base;
     m->corr = correction ? (float *) (m->base + n_r) : nullptr;
     m->w1 = m->base + n_r + n_c; m->w2 = m->w1 + n_1;
-    m->s1 = (float *) (m->w2 + n_2); m->s2 = (float *) (m->w2 + n_2 + n_s1); m->norms = (float *) (m->w2 + n_2 + n_s1 + n_s2);
+    m->s1 = (float *) (m->w2 + n_2); m->s2 = (float *) (m->w2 + n_2 + n_s1);
     cudaError_t e = cudaMemcpyAsync(m->router, router, (size_t) (sh->experts * D) * 4, cudaMemcpyDeviceToDevice, 0);
     if (e == cudaSuccess && correction) e = cudaMemcpyAsync(m->corr, correction, (size_t) sh->experts * 4, cudaMemcpyDeviceToDevice, 0);
     if (e == cudaSuccess) e = mf_pack(gate, m->w1, E, F, D * eb, m->T1 * 16LL, m->KB1, eb, 1, 0);
@@ -667,10 +671,6 @@ extern "C" pib_moe * pib_moe_from_device(const pib_moe_shape * sh, const float *
         const size_t row1 = (size_t) pib_f8_blocks(F) * m->KB1 * 4;                      // gate and up scales of an expert become neighbours
         if (e == cudaSuccess) e = cudaMemcpy2DAsync(m->s1, 2 * row1, gate_scales, row1, row1, (size_t) E, cudaMemcpyDeviceToDevice, 0);
         if (e == cudaSuccess) e = cudaMemcpy2DAsync((uint8_t *) m->s1 + row1, 2 * row1, up_scales, row1, row1, (size_t) E, cudaMemcpyDeviceToDevice, 0);
-        if (e == cudaSuccess) {
-            mf_norms_kernel<<<dim3((unsigned) E, 2), 256>>>((const uint8_t *) gate, (const uint8_t *) up, m->s1, F, D, (int) pib_f8_blocks(F), m->KB1, m->norms);
-            e = cudaGetLastError();
-        }
         if (e == cudaSuccess) e = cudaMemcpyAsync(m->s2, down_scales, (size_t) (E * pib_f8_blocks(D) * m->KB2) * 4, cudaMemcpyDeviceToDevice, 0);
     }
     if (e == cudaSuccess) e = cudaStreamSynchronize(0);
@@ -715,7 +715,7 @@ extern "C" int pib_moe_forward(const pib_moe * m, const float * x, int64_t ldx, 
     float *    z = (float *) (sc + L.z);
     float *    xm = (float *) (sc + L.xm);
     uint16_t * xp = (uint16_t *) (sc + L.xp);
-    A.cnt = (int *) sc; A.z = z; A.xp = xp; A.xm = xm; A.norms = m->norms; A.hp = (uint16_t *) (sc + L.hp); A.part = (float *) (sc + L.part);
+    A.cnt = (int *) sc; A.z = z; A.xp = xp; A.xm = xm; A.hp = (uint16_t *) (sc + L.hp); A.hx = (uint16_t *) (sc + L.hx); A.part = (float *) (sc + L.part);
     if (!(A.err = pib_tc_error_word(st))) { pib_set_error("pib_moe_forward: no memory for the error word"); return PIB_ERR_NOMEM; }
     const int  vec = ldx % 4 == 0 && !((uintptr_t) x & 15) && D % 4 == 0, nt = b == 1 ? 1 : MF_LT;
     const dim3 rg((unsigned) (A.E * ((b + nt - 1) / nt) + b)), rb(256);

@@ -232,3 +232,80 @@ def test_more_than_four_gigabytes(torch, pib):
     x = torch.randn(5, 4096, device="cuda", generator=L.g)
     res = torch.randn(5, 4096, device="cuda", generator=L.g)
     check(L, x, res, L.run(x, res))
+
+
+def layer_of(torch, pib, gate, up, down, gs, us, ds, shared=0):
+    """a layer of the given e4m3 values and block scales whose one chosen expert has the weight 1"""
+    n, F, D = gate.shape
+    L = Layer(torch, pib, F8, 1, n - 1, 1, D, F, renorm=False)
+    for k, v in dict(gate=gate, up=up, down=down, gate_scales=gs, up_scales=us, down_scales=ds).items():
+        assert L.w[k].shape == v.shape
+        L.w[k] = v.contiguous()
+    L.moe = pib.Moe(pib.load(), F8, 1, n - 1, 1, D, F, renorm=False, **{k: (v.data_ptr() if v is not None else None) for k, v in L.w.items()})
+    return L
+
+
+@pytest.mark.parametrize("b", [1, 4, 7, 16])
+def test_single_products(torch, pib, b):
+    """tokens with one value and rows of the down matrix with one weight: every output is one product of an h that is one product each of gate and up, so nothing but the operands' own roundings
+    shows.  Experts whose rows differ by 2^9 within a block and by 2^12 between blocks, gates that close, outputs that bring small h back to the size of large ones."""
+    t, F, D = torch, 700, 300
+    g = t.Generator(device="cuda").manual_seed(b)
+    e4 = lambda v: v.clamp(-448, 448).to(t.float8_e4m3fn)
+    sign = lambda *s: t.randint(0, 2, s, device="cuda", generator=g) * 2.0 - 1
+    gate = e4(sign(1, F, D) * 2.0 ** t.randint(-3, 9, (1, F, D), device="cuda", generator=g) * (1 + t.randint(0, 8, (1, F, D), device="cuda", generator=g) / 8))
+    up = e4(sign(1, F, D) * 2.0 ** t.randint(-3, 9, (1, F, D), device="cuda", generator=g))
+    j = t.randint(0, F, (D,), device="cuda", generator=g)                          # the h of each output
+    down = t.zeros(1, D, F, device="cuda")
+    down[0, t.arange(D, device="cuda"), j] = sign(D) * t.randint(1, 16, (D,), device="cuda", generator=g)
+    down = e4(down)
+    up_f = 2.0 ** t.randint(-6, 7, (blocks(F),), device="cuda", generator=g)       # of 128 rows of gate (up); of as many columns of down its inverse
+    us = up_f.view(1, -1, 1).expand(1, blocks(F), blocks(D)).contiguous()
+    ds = (1 / up_f).view(1, 1, -1).expand(1, blocks(D), blocks(F)).contiguous()
+    gs = t.full((1, blocks(F), blocks(D)), 2.0 ** -4, device="cuda")
+    L = layer_of(t, pib, gate, up, down, gs, us, ds)
+    x = t.zeros(b, D, device="cuda")
+    k = t.randint(0, D, (b,), device="cuda", generator=g)
+    x[t.arange(b, device="cuda"), k] = t.randn(b, device="cuda", generator=g)
+    got = L.run(x, None)
+    t.cuda.synchronize()
+    pib.load().gemm_check(0)
+    G, U, Dn = L.matrices(0)
+    gt, u = x.double() @ G.T, x.double() @ U.T
+    h = gt * t.sigmoid(gt) * u
+    y = h @ Dn.T
+    # x enters with 2^-22 of itself (two roundings to fp16), g and u with that and a step or two of fp32 (2^-24 each, three each); silu moves by at most (1 + |g|) times as much where the gate
+    # closes, and by the exponential's, the sum's and the quotient's roundings (2^-22 together); h's product; h enters with 2^-22, or with 2^-39 of its tile's largest; three steps of fp32 behind it
+    eps = (4 + 3) * EPS
+    dh = h.abs() * ((2 + gt.abs()) * eps + 4 * EPS + EPS)
+    p = t.nn.functional.pad(h.abs(), (0, (16 - F % 16) % 16)).view(b, -1, 16)
+    dh = dh + 4 * EPS * h.abs() + (p.amax(2, keepdim=True) * 2.0 ** -39).expand_as(p).reshape(b, -1)[:, :F]
+    lim = dh @ Dn.abs().T + 3 * EPS * y.abs() + 1e-35
+    err = (got.double() - y).abs()
+    assert (err <= lim).all(), float((err / lim).max())
+
+
+@pytest.mark.parametrize("down_too", [False, True])
+@pytest.mark.parametrize("c", [1.0, 10.0, 100.0, 300.0, 10000.0])
+def test_rows_of_unlike_size(torch, pib, c, down_too):
+    """one block of gate rows and one of up rows larger by c, and the columns of down that read them smaller by as much: the root mean square error over all outputs.  A sum's partial sums are no
+    larger than some three times their end; products of gate and up run through 4 steps of the tensor core that may cut (2^-22 each) and 20 fp32 steps at most, the same behind h:
+    2 * 3 * (4 * 2^-22 + 20 * 2^-24) and the operands' 2^-22 twice are below 2^-16.4, were all of one sign; they are not, so 2^-17"""
+    t, F, D = torch, 1408, 2048
+    L0 = Layer(t, pib, F8, 1, 0, 1, D, F)
+    w = {k: v.clone() for k, v in L0.w.items() if v is not None}
+    w["gate_scales"][:, 2] *= c
+    w["up_scales"][:, 5] *= c
+    if down_too:
+        w["down_scales"][:, :, 2] /= c
+        w["down_scales"][:, :, 5] /= c
+    L = layer_of(t, pib, w["gate"], w["up"], w["down"], w["gate_scales"], w["up_scales"], w["down_scales"])
+    x = t.randn(4, D, device="cuda", generator=L.g)
+    got = L.run(x, None)
+    G, U, Dn = L.matrices(0)
+    g = x.double() @ G.T
+    y = (g * t.sigmoid(g) * (x.double() @ U.T)) @ Dn.T
+    err = ((got.double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()).item()
+    print("c %g: 2^%.2f" % (c, __import__("math").log2(err)))
+    assert err <= 2.0 ** -17
+    check(L, x, t.zeros_like(x), got)
