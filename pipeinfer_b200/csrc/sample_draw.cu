@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(SD_THREADS, 2) sample_draw_kernel(const T * __
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 if (v[j] > -INFINITY) { n++; atomicAdd(&S.fine[sd_fine(v[j], mx)], 1u); }
-                if (!by_k) s += sd_weight52(S.pow, R.one, v[j]);
+                if (!by_k) s += sd_weight52(S.pow, R.one, fmaxf(v[j], -INFINITY));           // what is no number as -inf
             }
             if (!by_k) mass += s - 8 * SD_BITS52;
         });

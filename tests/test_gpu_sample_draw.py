@@ -266,3 +266,21 @@ def test_min_p_beside_zero(pib, V, bf16):
     for m in (1.0, 0.99999994, 0.3678, 0.36788, 0.4999):
         for k, p in ((0, 1.0), (300, 1.0), (0, 0.7), (500, 0.8)):
             compare(pib, x, [(0.9, k, p, m)] * 9, u, bf16=bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [777, 5000, 70000])
+def test_no_numbers_among_the_logits(pib, V, bf16):
+    """NaN of either sign and any payload takes no part: every truncation alone, thousands of equal logits, many NaN and few, at the borders of chunks"""
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal((6, V)) * 2).astype(np.float32)
+    x[2:4] = np.round(x[2:4])
+    x[4:] = 1.5
+    x = (x.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+    nans = np.array([0x7fc00000, 0xffc00000, 0x7f810000, 0xff810000, 0x7fff0000, 0xffff0000], np.uint32)
+    for r in range(6):
+        at = rng.permutation(V)[:V // 3] if r % 2 else [0, 7, 8, 255, 256, V - 1]
+        x.view(np.uint32)[r, at] = nans[rng.integers(0, 6, len(at))]
+    u = rng.random(6, np.float32)
+    for p in ((1.0, 0, 0.9, 0.0), (0.7, 0, 0.6, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 40, 1.0, 0.0), (0.8, 600, 0.9, 0.0), (1.2, 0, 1.0, 0.05), (1.0, 0, 0.99, 0.2), (0.0, 0, 0.5, 0.0)):
+        compare(pib, x, [p] * 6, u, bf16=bf16)
