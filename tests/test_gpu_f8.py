@@ -330,3 +330,30 @@ def test_fused_outputs_over_inputs_are_refused(torch, pib):
     for args in ((0, x, None, None, None, x + 1200 * 4), (1, x, x2, add, out, y), (2, x, x2, None, None, y), (0, x, None, None, None, x + 256 * 4, 1100)):          # the last one between two rows of x
         assert call(*args) == 0, args
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("N,K,b", [(50, 28672, 4), (300, 28672, 8), (2500, 13000, 8), (33, 26000, 5), (129, 66000, 1), (40, 66000, 2), (17, 66001, 8), (5000, 14336, 7), (60, 28672, 13), (60, 28672, 150)])
+def test_many_columns(torch, pib, N, K, b):
+    """decode batches whose activations do not fit beside the ring and come with the weights; more than 32 steps of a tile, whose scales are asked for again; the same columns for more tokens"""
+    q, s, g = matrix(torch, N, K, N + K)
+    x = rows(torch, b, K, g)
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), N, K)
+    y, lim = want(torch, q, s, x)
+    how = "gemv" if b <= 16 else "gemm"
+    got = product(torch, pib, w, x, how)
+    err = (got.double() - y).abs()
+    assert (err <= lim).all(), float((err / lim).max())
+    for _ in range(3):
+        assert torch.equal(product(torch, pib, w, x, how), got)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_one_bad_token_of_many_columns(torch, pib, bad):
+    q, s, g = matrix(torch, 70, 28672, 6)
+    x = rows(torch, 6, 28672, g)
+    x[2, 20000] = bad
+    w = pib.F8Weight(pib.load(), q.data_ptr(), s.data_ptr(), 70, 28672)
+    got = product(torch, pib, w, x, "gemv")
+    y, lim = want(torch, q, s, x)
+    others = [0, 1, 3, 4, 5]
+    assert ((got[others].double() - y[others]).abs() <= lim[others]).all() and torch.isnan(got[2]).all()
