@@ -164,9 +164,7 @@ dense_tc_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant_
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
-typedef CUresult (*dt_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static dt_encode_fn dt_encode() {
+dt_encode_fn pib_tma_encoder() {
     static dt_encode_fn fn = nullptr;
     if (!fn) {
         cudaDriverEntryPointQueryResult st;
@@ -207,7 +205,7 @@ static dt_scratch * dt_scratch_of(cudaStream_t st, size_t bytes) {
 }
 
 int pib_tma_map3(CUtensorMap * map, const void * base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1_bytes, uint64_t s2_bytes, uint32_t box1) {
-    dt_encode_fn enc = dt_encode();
+    dt_encode_fn enc = pib_tma_encoder();
     if (!enc) { pib_set_error("tensor map: cuTensorMapEncodeTiled not available"); return PIB_ERR_UNSUPP; }
     const cuuint64_t gdim[3] = { d0, d1, d2 };
     const cuuint64_t gstr[2] = { s1_bytes, s2_bytes };

@@ -25,9 +25,6 @@
 #define DP_BARS    (2 * DP_STAGES + 4)
 #define DP_SMEM    ((size_t) DP_RING + DP_BARS * 8 + 32 + 1024)
 
-__device__ __forceinline__ uint32_t dp_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t dp_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
-__device__ __forceinline__ void dp_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // What follows is called by a converged warp; one elected lane issues.  A k-step's instructions sit in one block behind one election: with an election each the producer and
 // the issuing warp took 0.29 us a step instead of 0.24, which is what a step of few tokens costs.
 // a stage of one operand: its two 64-wide tiles
@@ -115,7 +112,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + DP_BARS);
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + DP_STAGES * 8, bar_t = bar_e + DP_STAGES * 8, bar_r = bar_t + 16;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, crank = (int) dp_rank(), rank = crank & 1, S = A.shares, share = crank >> 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, crank = (int) dt_cluster_rank(), rank = crank & 1, S = A.shares, share = crank >> 1;
     const int unit = blockIdx.x / (2 * S), units = gridDim.x / (2 * S);                // a pair, or the cluster that shares a tile's K
     const uint32_t first = (uint32_t) (crank & ~1);                                    // the pair's first CTA
     const uint16_t both = (uint16_t) (3u << first);
@@ -129,8 +126,8 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    dp_cluster_sync();                                           // the other CTA's barriers exist
-    const uint32_t lead_f = dp_mapa(bar_f, first), sm0 = dt_smem(sm), bytes = 2 * (uint32_t) stage;
+    dt_cluster_sync();                                           // the other CTA's barriers exist
+    const uint32_t lead_f = dt_mapa(bar_f, first), sm0 = dt_smem(sm), bytes = 2 * (uint32_t) stage;
     // the weights of the first stages do not wait for the launch before this one, unless that made them
     const int early = A.w_made ? 0 : min(stages, n_ksteps);
     if (warp == 0)
@@ -149,7 +146,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
             dp_load2(sm0 + s * stage + 2 * DP_A_TILE, b_tile, &xmap, lead_f + s * 8, (k0 + s) * DP_BK, unit % A.tiles_m * A.NB + rank * half);
     dt_fence_before();
     __syncthreads();
-    dp_cluster_sync();                                           // the other CTA's tensor memory is there
+    dt_cluster_sync();                                           // the other CTA's tensor memory is there
     dt_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
@@ -190,7 +187,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
         }
     } else {
         const int q4 = warp & 3, hf = (warp - 2) >> 2;
-        const uint32_t lead_r = dp_mapa(bar_r, first);
+        const uint32_t lead_r = dt_mapa(bar_r, first);
         float * part = reinterpret_cast<float *>(sm);            // a share's sums, [token][row]: every MMA has completed, the ring is free
         int n = 0;
         for (int tile = unit; tile < A.tiles; tile += units, n++) {
@@ -216,13 +213,13 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     }
     __syncwarp();
     if (S > 1) {                                                 // one tile per cluster
-        dp_cluster_sync();
+        dt_cluster_sync();
         if (warp >= 2 && !*abort_s) {
             const int q4 = warp & 3, hf = (warp - 2) >> 2, w0 = unit / A.tiles_m * 256 + rank * 128 + q4 * 32, m0 = unit % A.tiles_m * A.NB;
             for (int c0 = (share * 2 + hf) * 8; c0 < A.NB && m0 + c0 < A.M; c0 += S * 16) {
                 float t[8];
                 for (int sh = 0; sh < S; sh++) {                 // in share order
-                    const uint32_t src = dp_mapa(sm0 + (uint32_t) (c0 * 128 + q4 * 32 + lane) * 4, (uint32_t) (sh * 2 + rank));
+                    const uint32_t src = dt_mapa(sm0 + (uint32_t) (c0 * 128 + q4 * 32 + lane) * 4, (uint32_t) (sh * 2 + rank));
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         float o;
@@ -245,7 +242,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    dp_cluster_sync();                                           // both CTAs have read their accumulators (and the shares' sums), nothing arrives at a barrier any more
+    dt_cluster_sync();                                           // both CTAs have read their accumulators (and the shares' sums), nothing arrives at a barrier any more
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 

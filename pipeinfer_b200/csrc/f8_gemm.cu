@@ -17,8 +17,6 @@
 #include "f8_block.cuh"
 #include "tc_common.cuh"
 
-#include <dlfcn.h>
-
 #include <algorithm>
 
 #define FT_THREADS 352
@@ -52,9 +50,6 @@ __device__ __forceinline__ void ft_tma_3d(uint32_t dst, const CUtensorMap * map,
 __device__ __forceinline__ void ft_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ uint32_t ft_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t ft_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
-__device__ __forceinline__ void ft_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void ft_ld(uint32_t at, uint32_t (&v)[N]) {
     if constexpr (N == 32) dt_ld32(at, v);
     else if constexpr (N == 16)
@@ -90,7 +85,7 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + FT_BARS);
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FT_STAGES * 8, bar_d = bar_e + FT_STAGES * 8, bar_g = bar_d + FT_DRING * 8, bar_t = bar_g + FT_DRING * 8, bar_r = bar_t + 16 * 8;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = A.shares, share = S > 1 ? (int) ft_rank() : 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, S = A.shares, share = S > 1 ? (int) dt_cluster_rank() : 0;
     // the rows of a CTA (cluster) are neighbours, in runs of 32; its tiles take up to four runs each, as alike as can be
     const int unit = blockIdx.x / S, units = gridDim.x / S;
     const int grains = (A.runs + GRAIN - 1) / GRAIN, r0 = (int) ((int64_t) grains * unit / units) * GRAIN;
@@ -242,7 +237,7 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
     }
     __syncwarp();
     if (S > 1) {
-        ft_cluster_sync();
+        dt_cluster_sync();
         if (warp >= 2 && warp < 10 && !*abort_s) {
             const int q4 = warp & 3, hf = (warp - 2) >> 2;
             const int64_t n = (int64_t) (r0 + q4) * 32 + lane;
@@ -250,7 +245,7 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
                 float v = 0.f;
                 for (int sh = 0; sh < S; sh++) {
                     float o;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(ft_mapa(sm0 + (uint32_t) (c * FT_BM + q4 * 32 + lane) * 4, (uint32_t) sh)) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(dt_mapa(sm0 + (uint32_t) (c * FT_BM + q4 * 32 + lane) * 4, (uint32_t) sh)) : "memory");
                     v += o;
                 }
                 if (q4 < runs && n < A.N) A.y[(int64_t) c * A.N + n] = v;
@@ -265,24 +260,13 @@ f8_gemm_kernel(const __grid_constant__ pib_f8_runs wmaps, const __grid_constant_
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    if (S > 1) ft_cluster_sync();                                // the shares' sums have been read
+    if (S > 1) dt_cluster_sync();                                // the shares' sums have been read
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
-typedef CUresult (*ft_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static ft_encode_fn ft_encode() {
-    static ft_encode_fn fn = [] {
-        void * p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) { cudaGetLastError(); p = nullptr; }
-        return (ft_encode_fn) p;
-    }();
-    return fn;
-}
 static int ft_map(CUtensorMap * map, const void * base, int dims, const cuuint64_t * size, const cuuint64_t * stride, const cuuint32_t * box) {
-    ft_encode_fn enc = ft_encode();
+    dt_encode_fn enc = pib_tma_encoder();
     if (!enc) { pib_set_error("tensor map: cuTensorMapEncodeTiled not available"); return PIB_ERR_UNSUPP; }
     const cuuint32_t es[4] = { 1, 1, 1, 1 };
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t) dims, const_cast<void *>(base), size, stride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -26,9 +26,6 @@
 #define FP_BARS    (2 * FP_STAGES + 4 + 2 * FP_FRING)
 #define FP_SMEM    ((size_t) FP_RING + FP_FRING * 1024 + FP_BARS * 8 + 32 + 1024)
 
-__device__ __forceinline__ uint32_t fp_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t fp_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
-__device__ __forceinline__ void fp_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // both operands of a block; called by a converged warp, one elected lane issues.  The first CTA (expect) announces the bytes of both CTAs' copies
 __device__ __forceinline__ void fp_load(uint32_t dst, const CUtensorMap * xmap, const CUtensorMap * wmap, uint32_t bar, int m, int kb, int wrow, uint32_t expect, uint32_t own_bar) {
     asm volatile("{\n\t.reg .pred q, e;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.and.b32 e, %8, 0, q;\n\t"
@@ -60,7 +57,7 @@ __device__ __forceinline__ void fp_ld16(uint32_t at, uint32_t * v) {
                    "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(at) : "memory");
 }
 struct fp_args {
-    int b, KB, NB, bp, tiles_m, tiles, wide;         // wide: floats that a store may take (8, 4 or 1)
+    int b, KB, NB, bp, tiles_m, tiles, wide;         // wide: rows that stores of eight floats may take
     int64_t N;
     const float * ws, * ad;
     float * y;
@@ -76,7 +73,7 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + FP_BARS);
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar_f = dt_smem(bar), bar_e = bar_f + FP_STAGES * 8, bar_t = bar_e + FP_STAGES * 8, bar_r = bar_t + 16, bar_d = bar_r + 16, bar_g = bar_d + FP_FRING * 8, sm0 = dt_smem(sm);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int) fp_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int) dt_cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < FP_STAGES; s++) { dt_mbar_init(bar_f + s * 8, 1); dt_mbar_init(bar_e + s * 8, 1); }
@@ -91,9 +88,9 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
     }
     dt_fence_before();
     __syncthreads();
-    fp_cluster_sync();                                           // the other CTA's barriers and tensor memory are there
+    dt_cluster_sync();                                           // the other CTA's barriers and tensor memory are there
     dt_fence_after();
-    const uint32_t tmem = *tmem_slot, lead_f = fp_mapa(bar_f, 0), lead_r = fp_mapa(bar_r, 0);
+    const uint32_t tmem = *tmem_slot, lead_f = dt_mapa(bar_f, 0), lead_r = dt_mapa(bar_r, 0);
     pib_pdl_wait();
     pib_pdl_trigger();
     bool ok = true;
@@ -204,7 +201,7 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
             const int64_t n0 = (int64_t) nb * 128 + (part & 1) * 64;
             float * y = A.y + (int64_t) tk * A.N + n0;
             const int left = (int) min((int64_t) 64, A.N - n0);
-            if (A.wide == 8 && left == 64) {
+            if (A.wide && left == 64) {
 #pragma unroll
                 for (int c = 0; c < 32; c += 4)
                     asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(y + c * 2), "l"(acc[c]), "l"(acc[c + 1]), "l"(acc[c + 2]), "l"(acc[c + 3]) : "memory");
@@ -226,7 +223,7 @@ f8_gemm_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_const
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
         __syncthreads();
     }
-    fp_cluster_sync();                                           // both CTAs have read their accumulators, nothing arrives at a barrier any more
+    dt_cluster_sync();                                           // both CTAs have read their accumulators, nothing arrives at a barrier any more
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
@@ -235,7 +232,7 @@ int pib_f8_gemm_pair(const pib_weight * w, const void * act, int b, float * y, i
     fp_args A;
     A.b = b; A.KB = L.KB; A.NB = (int) pib_f8_blocks(w->N); A.bp = L.bp; A.N = w->N; A.y = y; A.err = err;
     A.ws = (const float *) w->d; A.ad = (const float *) ((const uint8_t *) act + L.d_off);
-    A.wide = w->N % 8 == 0 && !((uintptr_t) y & 31) ? 8 : 1;
+    A.wide = w->N % 8 == 0 && !((uintptr_t) y & 31);
     A.tiles_m = (b + 255) / 256;
     A.tiles = (A.NB + 1) / 2 * A.tiles_m;
     CUtensorMap xmap;

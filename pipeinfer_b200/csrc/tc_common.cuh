@@ -48,6 +48,10 @@ __device__ __forceinline__ void dt_commit(uint32_t bar) {
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void dt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// thread-block clusters: this block's number, an address of shared memory in another block's, the meeting of all
+__device__ __forceinline__ uint32_t dt_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t dt_mapa(uint32_t a, uint32_t rank) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
+__device__ __forceinline__ void dt_cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // orders this thread's accesses to shared memory before and after it across proxies: loads and stores on one side, TMA, bulk copies and MMA operands on the other
 __device__ __forceinline__ void dt_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // 32 columns of this warp's 32 tensor-memory lanes, to and from registers (a lane's row each); the caller waits
@@ -75,6 +79,10 @@ __device__ __forceinline__ void dt_fence_after() { asm volatile("tcgen05.fence::
 // instruction descriptor: fp32 accumulators, bfloat16 x bfloat16, both operands K-major, M x N outputs
 __host__ __device__ constexpr uint32_t dt_idesc(int M, int N) { return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
 
+// dense_mma.cu: cuTensorMapEncodeTiled, null where the driver has none
+typedef CUresult (*dt_encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+dt_encode_fn pib_tma_encoder();
 // dense_mma.cu: a 3-D bfloat16 tensor map {d0, d1, d2} with boxes of 64 x box1 x 1 and 128-byte swizzle (strides in bytes)
 int   pib_tma_map3(CUtensorMap * map, const void * base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1_bytes, uint64_t s2_bytes, uint32_t box1);
 // dense_pair.cu: the dense matmul on pairs of SMs; tile width and shares of K for M rows and N outputs, and the launch for maps with boxes of 128 weight rows and half a tile of X rows
