@@ -195,8 +195,8 @@ int       pib_moe_forward(const pib_moe * m, const float * x_dev, int64_t ldx, i
 /* The chain of the reference's sampler with given random numbers (llama_sample_top_k, _top_p, _min_p, _temp, _token: llama.cpp:7048-7130, 7259, 7511), on the device.  A row's tokens are ordered by
  * logit, the lower id first among equals; -inf and what is no number take no part.  (1) the first top_k (<= 0: all); (2) the shortest run from the front whose probability among them
  * reaches top_p (>= 1: all); (3) of those the ones with at least min_p times the first one's probability (<= 0: all), the first in any case; (4) weights e^((l - l_max) / temp); temp <= 0: the
- * first token alone.  id = the first kept token, in the order of ids, at which the running sum of weights exceeds u times their total, 0 <= u < 1.  Sums are exact (64-bit fixed point), so equal
- * inputs give equal tokens, whatever the order of the threads. */
+ * first token alone.  id = the first kept token, in the order of ids, at which the running sum of weights exceeds u times their total, 0 <= u < 1.  A weight is formed to 2^-37 of itself and held
+ * in units of 2^-44 of the largest (below e^-31 of it a token is kept but not drawn); sums of them are exact (64-bit fixed point), so equal inputs give equal tokens, whatever the order of the threads. */
 #define PIB_SAMPLE_MAX_VOCAB 262144
 typedef struct pib_sample_params { float temp; int32_t top_k; float top_p; float min_p; } pib_sample_params;
 /* logits_dev [rows][n_vocab], rows ld elements apart, type PIB_TYPE_F32 or PIB_TYPE_BF16, not changed; params_dev and u_dev (float) one per row in device memory.  Results, one per row: ids_dev; p_dev

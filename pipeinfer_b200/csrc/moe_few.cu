@@ -21,8 +21,8 @@
 // expert with more tokens stands in the list of active ones once for each four (eight) of them, next to each other: its weights come from L2 again, which costs less than a second form of the
 // kernel (registers).  Which k a lane holds is free as long as both operands agree: the weights' columns are permuted within a line when they are packed, so that 16 bytes of
 // a row (lane t) are four values each of four (two) neighbouring tiles of 16, the k of an MMA, and the parts lie in that order too.
-// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in some 335 us (0.72 of the copy rate; the choice takes some 8 us of it, a power of two for each tile of h
-// some 10, the turns of 48 KB down items the rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 30 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
+// What bounds it: at 16 tokens of 128 experts (4096 x 1536, 8 each) the weights, 1.56 GB in 322 us (0.75 of the copy rate; the choice takes some 8 us of it, a power of two for each tile of h 11, the
+// turns of 48 KB down items the rest).  At one token (64 experts, 6 and 2 shared, 2048 x 1408: 30 us, the copies alone 11) latency: 6 us for the logits, 4 for the choice, then two rounds of items that are one
 // way to memory and back each.  Sharing the choice among the blocks would save none of it: the launch's first 4 us are mostly the way of its code into the caches.
 #include <cuda_bf16.h>
 

@@ -1,14 +1,15 @@
 // sample_draw.cu -- a token of each row of logits: top-k, top-p, min-p, temperature, drawn with a given number.
 //
 // A row's tokens are ordered by (logit descending, id ascending); every truncation keeps a run from the front of that order, so it is one threshold in it, and nothing is sorted.  With
-// w = e^(l - l_max) in 64 bits, rounded to a multiple of 2^-44: sums of up to 2^18 such numbers are exact in 64-bit integers, so no result depends on which thread or block added first.
+// w = e^(l - l_max), formed in fp64 to 2^-37 of itself and rounded to a multiple of 2^-44: sums of up to 2^18 such numbers are exact in 64-bit integers, so no result depends on which thread or
+// block added first.  (Below e^-31 a weight is 0: such a token is kept, and counted, but never drawn.)
 //   top-k   the threshold is the k-th token of the order
 //   top-p   the first token at which the running sum of w reaches top_p times that of what top-k left
 //   min-p   w >= min_p
 //   draw    weights e^((l - l_max) / temp) of what is kept, the first id at which their running sum exceeds u times the total
 // A row is divided over the P blocks of a thread-block cluster in slices of neighbouring ids; the blocks meet through distributed shared memory.  A slice is walked in chunks of 256 ids, eight
 // neighbours a lane (32 bytes of fp32, 16 of bfloat16, aligned wherever the row begins), two chunks of a warp under way; the row comes from memory once and from L2 after that:
-//   1  the maximum
+//   1  the maximum (behind it the cluster's blocks are known to have started)
 //   2  a histogram of l_max - l in 8192 bins 1/256 wide: counts alone, since the tokens of a bin weigh the same up to a factor of e^(1/256).  For top-p also the exact sum of all weights,
 //      in registers
 //   3  top-k: the tokens up to the bin of the k-th are gathered, and all that follows happens among them.  top-p: with the bounds that the counts give, the threshold lies in a few bins; their
