@@ -43,6 +43,11 @@ extern "C" {
 #define PIB_F8_BLOCK 128
 #define PIB_F8_MAX_ROWS 65536     /* tokens of one pib_quantize_act_rows / pib_gemm with such weights */
 
+/* 8-bit integer rows with one fp32 scale for each output (row); not a ggml type.  Activations: int8 with an fp32 scale for each token.  Any N, K up to PIB_I8_MAX_K. */
+#define PIB_TYPE_I8   65
+#define PIB_I8_MAX_K    131072    /* 128 * 127 * K stays below 2^31 */
+#define PIB_I8_MAX_ROWS 65536     /* tokens of one pib_quantize_act_rows / pib_gemm with such weights */
+
 #define PIB_MAX_BATCH 16          /* verification batch handled by the dequant-GEMV path (batch 1-16) */
 
 typedef struct pib_weight pib_weight;   /* a weight matrix repacked into HBM (layout private to the library) */
@@ -73,6 +78,12 @@ pib_weight * pib_weight_from_device(int type, const void * dev_blocks, int64_t N
  * ceil(K/128) scales (4 bytes each, not aligned); pib_act_to_blocks blocks of {float d, 128 e4m3}, zero behind column K. */
 pib_weight * pib_weight_upload_f8(const void * q_host, const float * scales_host, int64_t N, int64_t K);
 pib_weight * pib_weight_from_device_f8(const void * q_dev, const float * scales_dev, int64_t N, int64_t K);
+/* PIB_TYPE_I8: q [N][K] int8 (-128 .. 127), scales fp32 [N]; element (n, k) stands for scales[n] * q[n][k].  From host or device memory (the latter in the order of the legacy default stream; it
+ * waits).  Such a weight goes through the calls below like any other, as PIB_TYPE_F8 does: y[t][n] = fp32(sum of a q) * fp32(d[t] * scales[n]), the sum a whole number, each product rounded once, so that
+ * pib_gemv, pib_gemv_fused and pib_gemm give the same bits.  Waits inside the kernels are bounded and reported by pib_gemm_check(stream).  pib_weight_row_blocks writes a row's K bytes and behind
+ * them its scale (4 bytes, not aligned); pib_act_to_blocks a token's {float d, K int8 and zeros up to a multiple of 128}. */
+pib_weight * pib_weight_upload_i8(const void * q_host, const float * scales_host, int64_t N, int64_t K);
+pib_weight * pib_weight_from_device_i8(const void * q_dev, const float * scales_dev, int64_t N, int64_t K);
 void         pib_weight_free(pib_weight * w);
 size_t       pib_weight_bytes(const pib_weight * w);             /* algorithmic bytes: N * K * bits-per-weight / 8 */
 /* Copy row `row` back out in the reference block layout (inverse of the repack; for round-trip tests). */
@@ -80,8 +91,10 @@ int          pib_weight_row_blocks(const pib_weight * w, int64_t row, void * hos
 
 /* ---- K2: activation quantisation ------------------------------------------------------------------------------ */
 /* Bytes of the device buffer that holds `b` quantised activation rows of length K for weights of `wtype`. */
-size_t pib_act_bytes(int wtype, int64_t K, int b);          /* wtype: Q4_0 / Q8_0 / Q4_K; Q5_K and Q6_K weights use Q4_K's; F8 its own */
+size_t pib_act_bytes(int wtype, int64_t K, int b);          /* wtype: Q4_0 / Q8_0 / Q4_K; Q5_K and Q6_K weights use Q4_K's; F8 and I8 their own */
 /* F8: d = max(max |x| of the block, 2^-100) * fp32(1/448), e4m3(x / d); product, quotient and e4m3 each rounded to nearest (even).  A block with an infinity or a number that is none gives a token whose outputs are none. */
+/* I8: d = max(max |x| of the token, 2^-100) * fp32(1/127), a = x / d to the nearest whole number (even); product and quotient rounded once each.  A token with an infinity or a number that is none has
+ * outputs that are none. */
 /* x_dev float [b][K] -> act_dev.  Q8_0 blocks for Q4_0/Q8_0 weights, Q8_K super-blocks for Q4_K weights, with the
  * rounding of the reference's x86 build.  Replaces: quantize_row_q8_0 (ggml-quants.c:632, AVX2 branch :701-760) and
  * quantize_row_q8_K (ggml-quants.c:2329), called from the INIT phase of mul_mat (ggml.c:9493-9509). */
@@ -124,7 +137,7 @@ int pib_gemv_direct_splits(int64_t N, int64_t K);
  *   prologue 0: x                                             (quantize_row_q8_K of the attention output)
  *   prologue 1: rmsnorm(x [+ addend]) * x2, eps               (ggml_add, ggml_rms_norm ggml.c:9028, ggml_mul; sum_out, if given, receives x + addend)
  *   prologue 2: silu(x) * x2                                  (ggml_silu through the fp16 table ggml.c:1490, ggml_mul; x and x2 rows xstride apart)
- * F8 weights (same b and K; any prologue): silu(x) = x / (1 + e^-x) in fp32; y and sum_out lie over none of the inputs (every block reads the inputs for itself).
+ * F8 and I8 weights (same b and K; any prologue): silu(x) = x / (1 + e^-x) in fp32; y and sum_out lie over none of the inputs (every block reads the inputs for itself).
  * Device pointers; x [b][xstride or K] fp32, y [b][N] fp32.  Same values as pib_quantize_act / pib_norm_quantize_act followed by pib_gemv
  * up to the order of the fp32 additions. */
 int pib_gemv_fused(const pib_weight * w, int prologue, const float * x_dev, const float * x2_dev, const float * addend_dev, float * sum_out_dev,
@@ -142,7 +155,8 @@ int pib_gemm_host(const pib_weight * w, const float * x_host, int b, float * y_h
  * for the fp16 copy of the activations that the TMA loads from.  With b > 16 that copy is part of act_dev, written by the quantiser, so
  * act_dev has to come from a quantiser of this library called with the same b rows; scratch_dev is then not touched (but still asked
  * for).  With b <= 16 it is made in scratch_dev from the quants.
- * F8 weights: 1 <= b <= PIB_F8_MAX_ROWS rows of pib_quantize_act_rows(PIB_TYPE_F8, ...), 8-bit products summed in fp32 and scaled block by block; scratch_dev is not used and may be NULL. */
+ * F8 weights: 1 <= b <= PIB_F8_MAX_ROWS rows of pib_quantize_act_rows(PIB_TYPE_F8, ...), 8-bit products summed in fp32 and scaled block by block; scratch_dev is not used and may be NULL.
+ * I8 weights: 1 <= b <= PIB_I8_MAX_ROWS rows of pib_quantize_act_rows(PIB_TYPE_I8, ...), summed in 32-bit integers; scratch_dev as with F8. */
 size_t pib_gemm_scratch_bytes(int64_t K, int b);
 int    pib_gemm(const pib_weight * w, const void * act_dev, int b, float * y_dev, void * scratch_dev, pib_stream s);
 /* pib_gemm returns when the launch is made.  Every wait inside the kernel is bounded; one that runs out leaves y_dev unwritten in places and the stream's error
@@ -155,7 +169,7 @@ int    pib_quantize_act_rows(int wtype, const float * x_dev, int b, int64_t K, v
 
 /* ---- K3: embedding rows ---------------------------------------------------------------------------------------- */
 /* out_dev float [n][K] = dequantised rows `ids` of W.  Replaces: ggml_compute_forward_get_rows_q (ggml.c:10161) with
- * dequantize_row_q4_0 / q8_0 / q4_K (ggml-quants.c:1074, 1168, 1917).  Of a PIB_TYPE_F8 matrix a row that it has not is zeros. */
+ * dequantize_row_q4_0 / q8_0 / q4_K (ggml-quants.c:1074, 1168, 1917).  Of a PIB_TYPE_F8 or PIB_TYPE_I8 matrix a row that it has not is zeros. */
 int pib_get_rows(const pib_weight * w, const int32_t * ids_dev, int n, float * out_dev, pib_stream s);
 
 /* ---- a whole mixture layer for a few tokens ----------------------------------------------------------------------- */
@@ -204,6 +218,49 @@ typedef struct pib_sample_params { float temp; int32_t top_k; float top_p; float
  * to do.  One launch, no scratch. */
 int pib_sample(int type, const void * logits_dev, int64_t ld, int rows, int n_vocab, const pib_sample_params * params_dev, const float * u_dev, int32_t * ids_dev, float * p_dev, int32_t * kept_dev,
                pib_stream s);
+
+/* ---- a key / value cache in 4 bits, and attention over it ----------------------------------------------------------- */
+/* The cache of one layer: pages of PIB_KV4_PAGE cells, cell c the place c % PIB_KV4_PAGE of page c / PIB_KV4_PAGE; a cell holds a token's keys and values, [kv_heads][head_dim] each.  PIB_KV4_GROUP
+ * neighbouring channels share a lowest value m = fp16(min x) and a step d = fp16((max x - m) / 15) (x first brought to -60000 .. 60000); n = (x - m) / d to the nearest whole number (even), 0 .. 15, 0
+ * where d is 0; differences and quotients are fp32, rounded to the nearest.  A channel then stands for fp16(m + d n), rounded once: 5 bits a value, of which it is off by at most about d / 2.  A group with an infinity or a
+ * number that is none stands for numbers that are none.  New cells hold zeros.  Handles belong to the device that was current when they were made; calls on another one are refused. */
+#define PIB_KV4_PAGE       64
+#define PIB_KV4_GROUP      32
+#define PIB_KV4_MAX_WRITE  16384   /* tokens of one pib_kv4_write */
+#define PIB_KV4_MAX_TOKENS 65536   /* query tokens of one pib_kv4_attn */
+#define PIB_KV4_MAX_SEQS   1024
+#define PIB_KV4_MAX_HEADS  1024    /* query heads; head_dim is 64 or 128 */
+typedef struct pib_kv4 pib_kv4;
+pib_kv4 * pib_kv4_new(int64_t pages, int kv_heads, int head_dim);         /* NULL on failure */
+void      pib_kv4_free(pib_kv4 * kv);
+size_t    pib_kv4_bytes(const pib_kv4 * kv);                              /* device memory of the cells */
+/* Rounds n tokens' keys and values into cells.  k_dev, v_dev: rows of kv_heads * head_dim values, ldk and ldv elements apart (>= that), type PIB_TYPE_F32 or PIB_TYPE_BF16; cells_dev int32 [n]: a token
+ * whose cell is none of the cache's is left out, of several tokens with the same cell the last one stays.  n 0: nothing to do. */
+int       pib_kv4_write(pib_kv4 * kv, int type, const void * k_dev, int64_t ldk, const void * v_dev, int64_t ldv, const int32_t * cells_dev, int n, pib_stream s);
+/* The values that cells stand for, in fp32 (exact) or rounded to bfloat16; zeros for a cell that the cache has not.  k_dev or v_dev may be NULL; they do not overlap. */
+int       pib_kv4_read(const pib_kv4 * kv, int type, const int32_t * cells_dev, int n, void * k_dev, int64_t ldk, void * v_dev, int64_t ldv, pib_stream s);
+/* out = softmax(scale * q k) v for ragged sequences.  Sequence s has the query tokens starts[s] .. starts[s + 1] - 1 and lens[s] keys, those of its query tokens the last ones among them: the last query
+ * token stands at position lens[s] - 1.  A token at position p sees the keys j <= p, with a window > 0 of those j > p - window.  Key j lies in place j % PIB_KV4_PAGE of page
+ * pages[s * max_pages + j / PIB_KV4_PAGE]; several sequences may share pages.  Keys behind the table's row and on pages that the cache has not are not seen; a row that sees nothing is zeros.  Query head h
+ * reads key / value head h / (heads / kv_heads).  Rows of out behind starts[seqs] are left as they are.  Scores, softmax and sums are fp32; fp32 queries and weights enter the products with
+ * 22 bits, the weights of bfloat16 ones with 11. */
+typedef struct pib_kv4_batch {
+    int32_t type;                 /* of q and out: PIB_TYPE_F32 or PIB_TYPE_BF16 */
+    int32_t heads;                /* a multiple of the cache's */
+    int32_t tokens;               /* rows of q and out */
+    int32_t seqs;
+    int32_t max_tokens;           /* most query tokens of one sequence, 0: not known.  Chooses the kernels; results hold whatever it says */
+    int32_t max_pages;            /* entries of a row of pages_dev */
+    int32_t window;               /* 0: all keys */
+    float   scale;
+} pib_kv4_batch;
+/* scratch for such a call (a function of the batch and the device, not of the tables' contents); 0 where the batch is refused */
+size_t    pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * batch);
+/* q_dev and out_dev rows of heads * head_dim values, ldq and ldo elements apart; out does not overlap q.  starts_dev int32 [seqs + 1], not falling, from 0 to at most `tokens`; lens_dev int32 [seqs];
+ * pages_dev int32 [seqs][max_pages].  The tables are read on the device, in the order of the stream: a captured call follows them from replay to replay.  scratch_dev: 256-byte aligned, any
+ * contents; calls that may run at the same time need one each.  seqs or tokens 0: nothing to do.  Waits inside the kernels are bounded and reported by pib_gemm_check(stream). */
+int       pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * batch, const void * q_dev, int64_t ldq, const int32_t * starts_dev, const int32_t * lens_dev, const int32_t * pages_dev,
+                       void * out_dev, int64_t ldo, void * scratch_dev, pib_stream s);
 
 #ifdef __cplusplus
 }

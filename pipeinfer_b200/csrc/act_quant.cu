@@ -13,7 +13,7 @@
 //   PRO_LAYERNORM v = (x - mean) * 1/sqrtf(var + eps) * w + b   (ggml.c:8959-9020, two double sums)
 //   PRO_SILU_MUL  v = silu_f16lut(x) * x2                        (ggml.c:1490 table look-up, then ggml_mul; llama.cpp:3680)
 //   PRO_GELU      v = gelu_f16lut(x)                             (ggml.c:1433; falcon MLP)
-#include "f8_block.cuh"
+#include "i8_block.cuh"
 #include "q8k_quant.cuh"
 
 #include <algorithm>
@@ -331,22 +331,24 @@ static int check_args(int wtype, int b, int64_t K) {
 
 extern "C" size_t pib_act_bytes(int wtype, int64_t K, int b) {
     if (wtype == PIB_TYPE_F8) return pib_f8_act_of(K, b).total;
+    if (wtype == PIB_TYPE_I8) return pib_i8_act_of(K, b).total;
     return pib_act_layout_of(wtype, K, b).total;
 }
 
 extern "C" int pib_quantize_act(int wtype, const float * x_dev, int b, int64_t K, void * act_dev, pib_stream s) {
     if (wtype == PIB_TYPE_F8) return pib_f8_quantize(x_dev, nullptr, 0.f, b, K, act_dev, nullptr, (cudaStream_t) s);
+    if (wtype == PIB_TYPE_I8) return pib_i8_quantize(x_dev, nullptr, 0.f, b, K, act_dev, nullptr, (cudaStream_t) s);
     if (check_args(wtype, b, K) != PIB_OK) return PIB_ERR_ARG;
     return launch_aq<PRO_PLAIN>(wtype, x_dev, nullptr, 0, 0.f, b, K, act_dev, nullptr, nullptr, (cudaStream_t) s);
 }
 
 extern "C" int pib_norm_quantize_act(int wtype, int norm_kind, const float * x_dev, const float * norm_w_dev, float eps, int b,
                                      int64_t K, void * act_dev, float * xnorm_dev, pib_stream s) {
-    if (wtype != PIB_TYPE_F8 && check_args(wtype, b, K) != PIB_OK) return PIB_ERR_ARG;
+    if (wtype != PIB_TYPE_F8 && wtype != PIB_TYPE_I8 && check_args(wtype, b, K) != PIB_OK) return PIB_ERR_ARG;
     if (norm_kind != 1) { pib_set_error("pib_norm_quantize_act: only RMSNorm (1) is implemented"); return PIB_ERR_UNSUPP; }
-    if (wtype == PIB_TYPE_F8) {
+    if (wtype == PIB_TYPE_F8 || wtype == PIB_TYPE_I8) {
         if (!norm_w_dev) { pib_set_error("pib_norm_quantize_act: bad arguments"); return PIB_ERR_ARG; }
-        return pib_f8_quantize(x_dev, norm_w_dev, eps, b, K, act_dev, xnorm_dev, (cudaStream_t) s);
+        return (wtype == PIB_TYPE_F8 ? pib_f8_quantize : pib_i8_quantize)(x_dev, norm_w_dev, eps, b, K, act_dev, xnorm_dev, (cudaStream_t) s);
     }
     return launch_aq<PRO_RMSNORM>(wtype, x_dev, norm_w_dev, 0, eps, b, K, act_dev, xnorm_dev, nullptr, (cudaStream_t) s);
 }
@@ -393,6 +395,7 @@ int pib_gelu_quantize_act(int wtype, const float * x_dev, int b, int64_t K, void
 
 extern "C" int pib_act_to_blocks(int wtype, const void * act_dev, int b, int64_t K, void * out) {
     if (wtype == PIB_TYPE_F8) return pib_f8_act_blocks(act_dev, b, K, out);
+    if (wtype == PIB_TYPE_I8) return pib_i8_act_blocks(act_dev, b, K, out);
     if (check_args(wtype, b, K) != PIB_OK) return PIB_ERR_ARG;
     const pib_act_layout L = pib_act_layout_of(wtype, K, b);
     uint8_t * h = (uint8_t *) malloc(L.total);

@@ -28,6 +28,11 @@ static inline pib_f8_act pib_f8_act_of(int64_t K, int b) {
     return a;
 }
 
+// f8_quant.cu: a matrix of 8-bit values in the tiles above, without its scales (w->d, scale_bytes of them) and w->bytes; rows r0 .. r0 + rows from device memory, the whole matrix from the host's, a row back
+pib_weight * pib_tiles_alloc(int type, int64_t N, int64_t K, size_t scale_bytes);
+cudaError_t  pib_tiles_fill(pib_weight * w, const uint8_t * src, int64_t r0, int64_t rows);
+cudaError_t  pib_tiles_upload(pib_weight * w, const uint8_t * q_host);
+int          pib_tiles_row(const pib_weight * w, int64_t row, void * out);
 int pib_f8_quantize(const float * x, const float * norm_w, float eps, int b, int64_t K, void * act, float * xnorm, cudaStream_t st);
 int pib_f8_act_blocks(const void * act_dev, int b, int64_t K, void * out);
 int pib_f8_row(const pib_weight * w, int64_t row, void * out);
@@ -43,6 +48,8 @@ struct pib_f8_maps { pib_f8_runs runs; CUtensorMap stage, block; };
 int pib_f8_map(CUtensorMap * map, const void * base, int64_t rows, int box);                   // f8_gemm.cu: rows of 128 bytes, boxes of `box` rows, 128-byte swizzle (these three)
 int pib_f8_map3(CUtensorMap * map, const void * base, int64_t rows, int64_t groups, int64_t group_bytes, int box_rows, int box_groups);      // groups of rows of 128 bytes
 int pib_f8_map4(CUtensorMap * map, const void * base, int64_t KB, int64_t NB, int box_rows, int box_kb);      // the weights' blocks: boxes of some rows of some blocks of one row block
+// f8_gemv.cu: what both fused products refuse of their rows (an output that lies over an input, strides, alignment)
+int pib_fused_rows_ok(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, const float * sum_out, int64_t xstride, int b, const float * y);
 int pib_f8_rows_ok(const char * who, const pib_weight * w, const void * in, const void * out, int b, int max_b);
 
 // a block's scale: its largest value times 1/448 as fp32 has it

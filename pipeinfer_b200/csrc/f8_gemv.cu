@@ -271,8 +271,7 @@ int pib_f8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaSt
     return fg_launch<FG_RING>(wmap, amap, A, st);
 }
 
-int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st) {
-    if (b < 1 || b > 8 || w->K > 8192) { pib_set_error("pib_gemv_fused: unsupported matrix / batch"); return PIB_ERR_UNSUPP; }
+int pib_fused_rows_ok(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, const float * sum_out, int64_t xstride, int b, const float * y) {
     const int64_t xs = xstride ? xstride : w->K;
     if (xs < 0) { pib_set_error("pib_gemv_fused: bad arguments"); return PIB_ERR_ARG; }
     auto over = [&](const float * o, int64_t n, const float * in, int64_t stride) {            // n floats at o, rows of K at in
@@ -288,12 +287,18 @@ int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const floa
         }
     }
     if (((uintptr_t) x | (uintptr_t) x2 | (uintptr_t) addend | (uintptr_t) sum_out | (uintptr_t) y) & 3) { pib_set_error("pib_gemv_fused: fp32 rows need 4-byte alignment"); return PIB_ERR_ARG; }
+    return PIB_OK;
+}
+
+int pib_f8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st) {
+    if (b < 1 || b > 8 || w->K > 8192) { pib_set_error("pib_gemv_fused: unsupported matrix / batch"); return PIB_ERR_UNSUPP; }
+    int rc = pib_fused_rows_ok(w, pro, x, x2, addend, sum_out, xstride, b, y);
+    if (rc != PIB_OK) return rc;
     fg_args A;
     const CUtensorMap & wmap = ((const pib_f8_maps *) w->map)->stage;
-    const int rc = fg_of(A, w, b, y, st);
-    if (rc != PIB_OK) return rc;
+    if ((rc = fg_of(A, w, b, y, st)) != PIB_OK) return rc;
     A.x = x; A.x2 = pro ? x2 : nullptr; A.addend = pro == 1 ? addend : nullptr; A.sum_out = pro == 1 ? sum_out : nullptr;
-    A.xs = xs; A.eps = eps;
+    A.xs = xstride ? xstride : w->K; A.eps = eps;
     A.vec = w->K % 4 == 0 && A.xs % 4 == 0 && !(((uintptr_t) A.x | (uintptr_t) A.x2 | (uintptr_t) A.addend) & 15);
     switch (pro) {
         case 0:  return fg_launch<0>(wmap, wmap, A, st);

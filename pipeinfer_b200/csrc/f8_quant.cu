@@ -17,7 +17,7 @@ static __global__ void f8_pad_kernel(const uint8_t * __restrict__ src, uint8_t *
     }
 }
 
-static pib_weight * f8_alloc(int64_t N, int64_t K) {
+pib_weight * pib_tiles_alloc(int type, int64_t N, int64_t K, size_t scale_bytes) {
     // the rows of 128 bytes are counted in 32 bits
     if (N <= 0 || K <= 0 || N > 0x7fffff00 || K > 0x7fffff00 || pib_f8_blocks(N) * pib_f8_blocks(K) > 0x7fffffff / PIB_F8_BLOCK) {
         pib_set_error("pib_weight: bad shape %lld x %lld", (long long) N, (long long) K);
@@ -26,11 +26,10 @@ static pib_weight * f8_alloc(int64_t N, int64_t K) {
     const int64_t NB = pib_f8_blocks(N), KB = pib_f8_blocks(K);
     pib_weight *  w  = (pib_weight *) calloc(1, sizeof(pib_weight));
     if (!w) { pib_set_error("pib_weight: no host memory"); return nullptr; }
-    w->type = PIB_TYPE_F8;
+    w->type = type;
     w->N = N; w->K = K;
-    w->bytes = (size_t) N * K + (size_t) NB * KB * 4;
     const size_t plane = (size_t) NB * KB * PIB_F8_BLOCK * PIB_F8_BLOCK;
-    if (cudaMalloc(&w->base, plane + (size_t) NB * KB * 4 + 256) != cudaSuccess) {
+    if (cudaMalloc(&w->base, plane + scale_bytes + 256) != cudaSuccess) {
         pib_set_error("pib_weight: cudaMalloc of %zu bytes failed", plane);
         cudaGetLastError();
         free(w);
@@ -50,10 +49,40 @@ static pib_weight * f8_alloc(int64_t N, int64_t K) {
     return w;
 }
 
-static cudaError_t f8_pad(pib_weight * w, const uint8_t * src, int64_t r0, int64_t rows) {
+cudaError_t pib_tiles_fill(pib_weight * w, const uint8_t * src, int64_t r0, int64_t rows) {
     const int64_t Kp = pib_f8_blocks(w->K) * PIB_F8_BLOCK, n = rows * (Kp / 16);
     f8_pad_kernel<<<(unsigned) std::min<int64_t>((n + 255) / 256, 1 << 16), 256>>>(src, w->qs, w->N, w->K, Kp, r0, rows);
     return cudaGetLastError();
+}
+
+cudaError_t pib_tiles_upload(pib_weight * w, const uint8_t * q_host) {
+    // in pieces of whole rows, as the other formats: no second full-size buffer
+    const int64_t N = w->N, K = w->K, Np = pib_f8_blocks(N) * PIB_F8_BLOCK, per = std::max<int64_t>(1, std::min<int64_t>(N, (int64_t) (256u << 20) / K));
+    uint8_t *     stage = nullptr;
+    cudaError_t   e = cudaMalloc(&stage, (size_t) per * K);
+    for (int64_t r = 0; e == cudaSuccess && r < N; r += per) {
+        const int64_t rows = std::min(per, N - r);
+        if ((e = cudaMemcpy(stage, q_host + r * K, (size_t) (rows * K), cudaMemcpyHostToDevice)) != cudaSuccess) break;
+        if ((e = pib_tiles_fill(w, stage, r, r + rows == N ? Np - r : rows)) != cudaSuccess) break;
+        e = cudaStreamSynchronize(0);
+    }
+    cudaFree(stage);
+    return e;
+}
+
+int pib_tiles_row(const pib_weight * w, int64_t row, void * out) {
+    const int64_t KB = pib_f8_blocks(w->K);
+    const size_t  full = (size_t) (w->K / PIB_F8_BLOCK), tail = (size_t) (w->K % PIB_F8_BLOCK);
+    if (full) PIB_CHECK(cudaMemcpy2D(out, PIB_F8_BLOCK, w->qs + pib_f8_at(row, 0, KB), PIB_F8_BLOCK * PIB_F8_BLOCK, PIB_F8_BLOCK, full, cudaMemcpyDeviceToHost));
+    if (tail) PIB_CHECK(cudaMemcpy((uint8_t *) out + full * PIB_F8_BLOCK, w->qs + pib_f8_at(row, (int64_t) full * PIB_F8_BLOCK, KB), tail, cudaMemcpyDeviceToHost));
+    return PIB_OK;
+}
+
+static pib_weight * f8_alloc(int64_t N, int64_t K) {
+    const size_t sb = N > 0 && K > 0 ? (size_t) pib_f8_blocks(N) * pib_f8_blocks(K) * 4 : 0;
+    pib_weight * w  = pib_tiles_alloc(PIB_TYPE_F8, N, K, sb);
+    if (w) w->bytes = (size_t) N * K + sb;
+    return w;
 }
 
 extern "C" pib_weight * pib_weight_from_device_f8(const void * q_dev, const float * scales_dev, int64_t N, int64_t K) {
@@ -61,7 +90,7 @@ extern "C" pib_weight * pib_weight_from_device_f8(const void * q_dev, const floa
     pib_weight * w = f8_alloc(N, K);
     if (!w) return nullptr;
     const size_t sb = (size_t) pib_f8_blocks(N) * pib_f8_blocks(K) * 4;
-    if (f8_pad(w, (const uint8_t *) q_dev, 0, pib_f8_blocks(N) * PIB_F8_BLOCK) != cudaSuccess || cudaMemcpyAsync(w->d, scales_dev, sb, cudaMemcpyDeviceToDevice, 0) != cudaSuccess ||
+    if (pib_tiles_fill(w, (const uint8_t *) q_dev, 0, pib_f8_blocks(N) * PIB_F8_BLOCK) != cudaSuccess || cudaMemcpyAsync(w->d, scales_dev, sb, cudaMemcpyDeviceToDevice, 0) != cudaSuccess ||
         cudaStreamSynchronize(0) != cudaSuccess) {
         pib_set_error("pib_weight_from_device_f8: %s", cudaGetErrorString(cudaGetLastError()));
         pib_weight_free(w);
@@ -74,28 +103,18 @@ extern "C" pib_weight * pib_weight_upload_f8(const void * q_host, const float * 
     if (!q_host || !scales_host) { pib_set_error("pib_weight_upload_f8: bad arguments"); return nullptr; }
     pib_weight * w = f8_alloc(N, K);
     if (!w) return nullptr;
-    // in pieces of whole rows, as the other formats: no second full-size buffer
-    const int64_t Np = pib_f8_blocks(N) * PIB_F8_BLOCK, per = std::max<int64_t>(1, std::min<int64_t>(N, (int64_t) (256u << 20) / K));
-    const size_t  sb = (size_t) pib_f8_blocks(N) * pib_f8_blocks(K) * 4;
-    uint8_t *     stage = nullptr;
-    bool          ok = cudaMalloc(&stage, (size_t) per * K) == cudaSuccess;
-    for (int64_t r = 0; ok && r < N; r += per) {
-        const int64_t rows = std::min(per, N - r);
-        ok = cudaMemcpy(stage, (const uint8_t *) q_host + r * K, (size_t) (rows * K), cudaMemcpyHostToDevice) == cudaSuccess &&
-             f8_pad(w, stage, r, r + rows == N ? Np - r : rows) == cudaSuccess && cudaStreamSynchronize(0) == cudaSuccess;
-    }
+    const size_t sb = (size_t) pib_f8_blocks(N) * pib_f8_blocks(K) * 4;
+    bool         ok = pib_tiles_upload(w, (const uint8_t *) q_host) == cudaSuccess;
     ok = ok && cudaMemcpy(w->d, scales_host, sb, cudaMemcpyHostToDevice) == cudaSuccess;
     if (!ok) pib_set_error("pib_weight_upload_f8: %s", cudaGetErrorString(cudaGetLastError()));
-    cudaFree(stage);
     if (!ok) { pib_weight_free(w); return nullptr; }
     return w;
 }
 
 int pib_f8_row(const pib_weight * w, int64_t row, void * out) {
     const int64_t KB = pib_f8_blocks(w->K);
-    const size_t  full = (size_t) (w->K / PIB_F8_BLOCK), tail = (size_t) (w->K % PIB_F8_BLOCK);
-    if (full) PIB_CHECK(cudaMemcpy2D(out, PIB_F8_BLOCK, w->qs + pib_f8_at(row, 0, KB), PIB_F8_BLOCK * PIB_F8_BLOCK, PIB_F8_BLOCK, full, cudaMemcpyDeviceToHost));
-    if (tail) PIB_CHECK(cudaMemcpy((uint8_t *) out + full * PIB_F8_BLOCK, w->qs + pib_f8_at(row, (int64_t) full * PIB_F8_BLOCK, KB), tail, cudaMemcpyDeviceToHost));
+    const int     rc = pib_tiles_row(w, row, out);
+    if (rc != PIB_OK) return rc;
     PIB_CHECK(cudaMemcpy((uint8_t *) out + w->K, (const float *) w->d + row / PIB_F8_BLOCK * KB, (size_t) KB * 4, cudaMemcpyDeviceToHost));
     return PIB_OK;
 }

@@ -13,6 +13,8 @@ TYPE_Q5_K = 13
 TYPE_Q6_K = 14        # matmul only; multiplies with the same activations as Q4_K
 TYPE_F32, TYPE_BF16 = 0, 30
 TYPE_F8 = 64          # e4m3 with a scale per 128 x 128 block
+TYPE_I8 = 65          # int8 with a scale per output
+KV4_PAGE = 64         # cells of a page of a 4-bit key / value cache
 TYPES = {"q4_0": TYPE_Q4_0, "q8_0": TYPE_Q8_0, "q4_k": TYPE_Q4_K}
 BLOCK = {TYPE_Q4_0: (32, 18), TYPE_Q8_0: (32, 34), TYPE_Q4_K: (256, 144), TYPE_Q5_K: (256, 176), TYPE_Q6_K: (256, 210), TYPE_Q3_K: (256, 110)}
 ACT_BLOCK = {TYPE_Q4_0: (32, 34), TYPE_Q8_0: (32, 34), TYPE_Q4_K: (256, 292)}
@@ -25,6 +27,10 @@ class MoeShape(C.Structure):
 
 class SampleParams(C.Structure):
     _fields_ = [("temp", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
+
+
+class Kv4Batch(C.Structure):
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("tokens", C.c_int32), ("seqs", C.c_int32), ("max_tokens", C.c_int32), ("max_pages", C.c_int32), ("window", C.c_int32), ("scale", C.c_float)]
 
 
 class LibraryMissing(RuntimeError):
@@ -40,7 +46,7 @@ def _p(a):
 
 
 class Lib:
-    TYPE_F32, TYPE_BF16, TYPE_F8 = TYPE_F32, TYPE_BF16, TYPE_F8
+    TYPE_F32, TYPE_BF16, TYPE_F8, TYPE_I8 = TYPE_F32, TYPE_BF16, TYPE_F8, TYPE_I8
 
     def __init__(self, path=SO_PATH):
         if not os.path.exists(path):
@@ -73,7 +79,7 @@ class Lib:
         L.pib_gemv_q4k_noalloc.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
         L.pib_mul_mat_host.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int]
         L.pib_get_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
-        for name in ("pib_weight_upload_f8", "pib_weight_from_device_f8"):
+        for name in ("pib_weight_upload_f8", "pib_weight_from_device_f8", "pib_weight_upload_i8", "pib_weight_from_device_i8"):
             getattr(L, name).restype, getattr(L, name).argtypes = C.c_void_p, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64]
         L.pib_quantize_act_rows.argtypes = [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]
         L.pib_gemv_fused.argtypes = [C.c_void_p, C.c_int] + [C.c_void_p] * 4 + [C.c_int64, C.c_float, C.c_int, C.c_void_p, C.c_void_p]
@@ -84,6 +90,13 @@ class Lib:
         L.pib_moe_free.argtypes = [C.c_void_p]
         L.pib_moe_scratch_bytes.restype, L.pib_moe_scratch_bytes.argtypes = C.c_size_t, [C.c_void_p, C.c_int]
         L.pib_moe_forward.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+        L.pib_kv4_new.restype, L.pib_kv4_new.argtypes = C.c_void_p, [C.c_int64, C.c_int, C.c_int]
+        L.pib_kv4_free.argtypes = [C.c_void_p]
+        L.pib_kv4_bytes.restype, L.pib_kv4_bytes.argtypes = C.c_size_t, [C.c_void_p]
+        L.pib_kv4_write.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p]
+        L.pib_kv4_read.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]
+        L.pib_kv4_attn_scratch_bytes.restype, L.pib_kv4_attn_scratch_bytes.argtypes = C.c_size_t, [C.c_void_p, C.POINTER(Kv4Batch)]
+        L.pib_kv4_attn.argtypes = [C.c_void_p, C.POINTER(Kv4Batch), C.c_void_p, C.c_int64] + [C.c_void_p] * 4 + [C.c_int64, C.c_void_p, C.c_void_p]
         L.pib_sample.argtypes = [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int] + [C.c_void_p] * 6
 
     def check(self, rc):
@@ -198,16 +211,53 @@ class Lib:
 
 class F8Weight:
     """e4m3 rows [N][K] with fp32 scales [ceil(N/128)][ceil(K/128)], from device pointers; stands for the handle in Lib.gemv, gemv_fused and gemm"""
+    make = "pib_weight_from_device_f8"
 
     def __init__(self, lib, q, scales, N, K):
         self.lib, self.N, self.K = lib, N, K
-        self.h = lib.L.pib_weight_from_device_f8(q, scales, N, K)
+        self.h = getattr(lib.L, self.make)(q, scales, N, K)
         if not self.h:
             raise PibError(lib.L.pib_last_error().decode())
 
     def __del__(self):
         if getattr(self, "h", None):
             self.lib.L.pib_weight_free(self.h)
+            self.h = None
+
+
+class I8Weight(F8Weight):
+    """int8 rows [N][K] with fp32 scales [N], from device pointers; stands for the handle as F8Weight does"""
+    make = "pib_weight_from_device_i8"
+
+
+class Kv4:
+    """a layer's keys and values in 4 bits (pib_kv4_new), pages of KV4_PAGE cells; arrays as device pointers, cells, starts, lens and page tables int32"""
+
+    def __init__(self, lib, pages, kv_heads, head_dim):
+        self.lib = lib
+        self.h = lib.L.pib_kv4_new(pages, kv_heads, head_dim)
+        if not self.h:
+            raise PibError(lib.L.pib_last_error().decode())
+
+    def bytes(self):
+        return self.lib.L.pib_kv4_bytes(self.h)
+
+    def write(self, type_, k, ldk, v, ldv, cells, n, stream=None):
+        self.lib.check(self.lib.L.pib_kv4_write(self.h, type_, k, ldk, v, ldv, cells, n, stream))
+
+    def read(self, type_, cells, n, k, ldk, v, ldv, stream=None):
+        self.lib.check(self.lib.L.pib_kv4_read(self.h, type_, cells, n, k, ldk, v, ldv, stream))
+
+    def scratch_bytes(self, batch):
+        """batch: a Kv4Batch"""
+        return self.lib.L.pib_kv4_attn_scratch_bytes(self.h, C.byref(batch))
+
+    def attention(self, batch, q, ldq, starts, lens, pages, out, ldo, scratch, stream=None):
+        self.lib.check(self.lib.L.pib_kv4_attn(self.h, C.byref(batch), q, ldq, starts, lens, pages, out, ldo, scratch, stream))
+
+    def __del__(self):
+        if getattr(self, "h", None):
+            self.lib.L.pib_kv4_free(self.h)
             self.h = None
 
 
