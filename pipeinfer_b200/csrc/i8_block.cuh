@@ -27,6 +27,7 @@ int pib_i8_get_rows(const pib_weight * w, const int32_t * ids, int n, float * ou
 int pib_i8_gemv(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st);
 int pib_i8_gemv_fused(const pib_weight * w, int pro, const float * x, const float * x2, const float * addend, float * sum_out, int64_t xstride, float eps, int b, float * y, cudaStream_t st);
 int pib_i8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaStream_t st);
+int pib_i8_gemm_pair(const pib_weight * w, const void * act, int b, float * y, int * err, cudaStream_t st);
 int pib_i8_gemm_host(const pib_weight * w, const float * x_host, int b, float * y_host);
 
 // a token's scale from the bits of its largest magnitude, which order infinities and what is no number behind all numbers: a row with one of those has a scale, and outputs, that are none
