@@ -2,7 +2,8 @@
 //
 //   [page][key / value head] records of 80 * dim bytes, so that all that a page holds of a head is one copy:
 //     keys    [64 places][dim / 2] bytes, channel c the nibble c % 2 of byte c / 2; behind them [64][dim / 32] pairs of fp16 {step d, lowest value m}
-//     values  the same; with heads of 128 the 32-byte halves of a row change places where bit 1 of the place is set (kv4_flip), so that four neighbouring rows' quarters lie in different banks
+//     values  the same, with rows in another order: of eight places the even ones first (kv4_row), and with heads of 128 the 32-byte halves of a row change places where bit 1 of the row is set
+//             (kv4_flip).  The lanes of a matrix product's second operand read quarters of the places 0, 2, 4, 6 at a time: so they lie in different banks
 #pragma once
 
 #include <cuda_bf16.h>
@@ -20,7 +21,8 @@ struct pib_kv4 {
 __host__ __device__ constexpr int kv4_record(int dim) { return 80 * dim; }
 __host__ __device__ constexpr int kv4_half(int dim) { return 40 * dim; }          // the values' part begins here
 __host__ __device__ constexpr int kv4_steps(int dim) { return 32 * dim; }         // of either part: its steps and lowest values
-__host__ __device__ constexpr int kv4_flip(int dim, int place) { return dim == 128 ? (place >> 1 & 1) << 5 : 0; }
+__host__ __device__ constexpr int kv4_row(int place) { return (place & ~7) | (place >> 1 & 3) | (place & 1) << 2; }
+__host__ __device__ constexpr int kv4_flip(int dim, int row) { return dim == 128 ? (row >> 1 & 1) << 5 : 0; }
 
 // the device's answer: a wrong handle is refused before any launch
 static inline int kv4_ok(const char * who, const pib_kv4 * kv) {

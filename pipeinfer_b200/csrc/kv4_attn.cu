@@ -1,5 +1,6 @@
-// kv4_attn.cu -- attention of ragged sequences over a key / value cache in 4 bits (kv4.cuh): a warp per query token and head, one pass over its keys with the running maximum and sum.
+// kv4_attn.cu -- attention of ragged sequences over a key / value cache in 4 bits (kv4.cuh): one pass over the keys with the running maximum and sum.
 #include "kv4.cuh"
+#include "tc_common.cuh"
 
 #include <algorithm>
 
@@ -8,69 +9,514 @@
 struct ka_args {
     const uint8_t * base; int64_t pages; int kvh, rep, dim;
     const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
-    const void * q; void * out; int64_t ldq, ldo;
+    const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
+    int stages; float * pieces; struct ka_plan * plan; int * err;
 };
 
-template <typename T, int D>
-static __global__ void __launch_bounds__(128) kv4_attn_kernel(const __grid_constant__ ka_args A) {
+// n neighbouring values as floats, n a multiple of 8
+template <typename T, int N> __device__ __forceinline__ void ka_load(const T * p, bool wide, float (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) { const float4 f = *reinterpret_cast<const float4 *>(p + i); v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w; }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = p[i];
+    } else {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 8) {
+                const uint4 f = *reinterpret_cast<const uint4 *>(p + i);
+                const uint32_t w[4] = { f.x, f.y, f.z, f.w };
+#pragma unroll
+                for (int j = 0; j < 4; j++) { v[i + 2 * j] = __uint_as_float(w[j] << 16); v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = __bfloat162float(p[i]);
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, bool wide, const float (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) p[i] = v[i];
+    } else {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 8) {
+                __nv_bfloat162 h[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+                *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(h);
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) p[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+// ---- which keys a tile of rows sees ---------------------------------------------------------------------------------------------------
+// A sequence's rows, (token, head of the group) with the heads next to each other, are taken in tiles of RT; a tile of one key / value head is an item, its pages the units of work
+struct ka_seq { int n, len; };                      // query tokens and keys; both >= 0
+__device__ __forceinline__ ka_seq ka_load_seq(const ka_args & A, int s) {
+    const int a = min(max(A.starts[s], 0), A.tokens), b = min(max(A.starts[s + 1], 0), A.tokens);
+    return { max(b - a, 0), max(A.lens[s], 0) };
+}
+// pages [first, first + count) of tile r; keys behind the table's row are not there
+template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_seq q, int r, int & first) {
+    const int t0 = r * RT / A.rep, t1 = min(q.n - 1, ((r + 1) * RT - 1) / A.rep), p0 = q.len - q.n + t0, p1 = q.len - q.n + t1;
+    const int top = min(p1 < 0 ? -1 : p1 / KV4_P, A.max_pages - 1);
+    first = A.window > 0 ? max(0, p0 - A.window + 1) / KV4_P : 0;
+    return max(0, top - first + 1);
+}
+template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
+
+// what both kernels know of the work: behind the pieces in the scratch
+struct ka_plan { int64_t warps, prefix[PIB_KV4_MAX_SEQS + 1]; };          // warps that share the units; units in front of each sequence
+
+__device__ __forceinline__ void ka_mma(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ float2 ka_float2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+// what the rounding to fp16 took away
+__device__ __forceinline__ uint32_t ka_rest(float a, float b, uint32_t hi) { const float2 f = ka_float2(hi); return ka_pack(a - f.x, b - f.y); }
+__device__ __forceinline__ uint32_t ka_prmt(uint32_t a, uint32_t b, uint32_t sel) { uint32_t r; asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel)); return r; }
+__device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+#define KA_WARPS 8
+#define KA_LIFT  14.0f       // weights are e^(s - max) 2^14: fp16 then holds them down to 2^-38 of the largest
+
+// ---- decode and verification batches --------------------------------------------------------------------------------------------------
+// All (sequence, tile, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum and
+// sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
+//   scores   mma.m16n8k16, rows as M, eight keys as N: lane (g, t) has 16 or 32 neighbouring channels of key g, one load and one step and lowest value, four of them a product's k
+//   outputs  weights straight from the scores' registers as first operand, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
+// fp32 rows enter as fp16 part and remainder: rows 0..7 of a product's sixteen the parts, 8..15 the remainders, so that a row's sum is the sum of two registers of a lane.  bfloat16 rows are exact in fp16
+// (times a power of two of the row) and take all sixteen; their weights are one fp16 number.
+// An item that lies in one warp's run is written at once, pieces of others go to scratch and kv4_join_kernel adds them up, in the order of the keys.
+template <typename T, int D, int MT> struct ka_cfg {
+    static constexpr bool SPLIT = sizeof(T) == 4;
+    static constexpr int  RPM = SPLIT ? 8 : 16, RT = MT * RPM, NR = SPLIT ? 1 : 2, KS = D / 16, W = D / 32, NT = D / 8;
+    static constexpr bool QS = MT * KS > 8;                       // the queries' operands lie in shared memory
+    static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? KA_WARPS * MT * KS * 512 : 0;
+    static constexpr int  PIECE = RT * (D + 2);                   // floats
+};
+
+template <typename T, int D, int MT>
+static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
+    using C = ka_cfg<T, D, MT>;
+    extern __shared__ __align__(128) uint8_t ka_dsm[];
+    __shared__ uint64_t bars[KA_WARPS * 16];
+    __shared__ int64_t  part[KA_WARPS];
+    __shared__ int      abort_w;
+    volatile int * abort_s = &abort_w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, NST = A.stages;
+    uint8_t *  ring = ka_dsm + warp * NST * C::HALF;
+    uint4 *    qsm  = reinterpret_cast<uint4 *>(ka_dsm + KA_WARPS * NST * C::HALF) + warp * MT * C::KS * 32 + lane;
+    int64_t *  prefix = reinterpret_cast<int64_t *>(ka_dsm + KA_WARPS * NST * C::HALF + C::Q_BYTES);         // [seqs + 1]
+    ka_seq *   seq  = reinterpret_cast<ka_seq *>(prefix + A.seqs + 1);
+    const uint32_t bar0 = dt_smem(bars + warp * 16), ring0 = dt_smem(ring);
+    if (lane == 0) for (int i = 0; i < NST; i++) dt_mbar_init(bar0 + i * 8, 1);
+    if (threadIdx.x == 0) abort_w = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pib_pdl_wait();
     pib_pdl_trigger();
-    __shared__ float sq[4][D];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = A.kvh * A.rep;
-    const int64_t row = (int64_t) blockIdx.x * 4 + warp;
-    if (row >= (int64_t) A.tokens * heads) return;
-    const int t = (int) (row / heads), h = (int) (row % heads), kvh = h / A.rep;
-    // the last sequence that begins at or in front of t and has it
-    int s = -1;
-    for (int i = lane; i < A.seqs; i += 32) if (A.starts[i] <= t && t < A.starts[i + 1]) s = i;
-    s = __reduce_max_sync(0xffffffffu, s);
-    if (s < 0) return;
-    const int pos = A.lens[s] - (A.starts[s + 1] - t), first = A.window > 0 ? max(0, pos - A.window + 1) : 0;
-    const int last = min(pos, (int) min((int64_t) A.max_pages * KV4_P, (int64_t) 0x7fffffff) - 1);
-    const T * q = (const T *) A.q + (int64_t) t * A.ldq + (int64_t) h * D;
-    for (int c = lane; c < D; c += 32) sq[warp][c] = (float) q[c] * (A.scale * KA_LOG2E);
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o[D / 32] = {};
-    for (int j0 = first; j0 <= last; j0 += 32) {
-        const int j = j0 + lane;
-        const uint8_t * rec = nullptr;
-        float sc = -INFINITY;
-        if (j <= last) {
-            const int page = A.table[(int64_t) s * A.max_pages + j / KV4_P];
-            if (page >= 0 && page < A.pages) {
-                rec = A.base + ((int64_t) page * A.kvh + kvh) * kv4_record(D);
-                sc = 0.f;
-                for (int w = 0; w < D / 8; w++) {
-                    const __half2 dm = *reinterpret_cast<const __half2 *>(rec + kv4_steps(D) + ((j % KV4_P) * (D / 32) + w / 4) * 4);
-                    uint32_t p[4];
-                    kv4_pairs(*reinterpret_cast<const uint32_t *>(rec + (j % KV4_P) * (D / 2) + w * 4), __low2half2(dm), __high2half2(dm), p);
-                    for (int i = 0; i < 4; i++) { const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[i])); sc = fmaf(sq[warp][w * 8 + i], f.x, fmaf(sq[warp][w * 8 + i + 4], f.y, sc)); }
-                }
-            }
+
+    // units in front of each sequence: a thread's neighbouring sequences, then warps, then the block
+    {
+        const int per = (A.seqs + KA_WARPS * 32 - 1) / (KA_WARPS * 32), s0 = threadIdx.x * per;
+        int64_t sum = 0;
+        for (int s = s0; s < min(s0 + per, A.seqs); s++) {
+            const ka_seq q = ka_load_seq(A, s);
+            seq[s] = q;
+            prefix[s] = sum;
+            int first;
+            for (int r = 0; r < ka_tiles<C::RT>(A, q); r++) sum += (int64_t) ka_pages<C::RT>(A, q, r, first) * A.kvh;
         }
-        const float mn = fmaxf(m, warp_max(sc)), a = m == mn ? 1.f : exp2f(m - mn), p = rec ? exp2f(sc - mn) : 0.f;
-        l = l * a + warp_sum(p);
-        m = mn;
+        int64_t before = sum;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) o[i] *= a;
-        for (int k = 0; k < 32; k++) {
-            const uint8_t * r = (const uint8_t *) __shfl_sync(0xffffffffu, (unsigned long long) rec, k);
-            const float pk = __shfl_sync(0xffffffffu, p, k);
-            if (!r) continue;
-            const int place = (j0 + k) % KV4_P;
-            r += kv4_half(D);
-#pragma unroll
-            for (int i = 0; i < D / 32; i++) {
-                const int c = i * 32 + lane;
-                const __half2 dm = *reinterpret_cast<const __half2 *>(r + kv4_steps(D) + (place * (D / 32) + i) * 4);
-                const uint8_t b = r[place * (D / 2) + ((c / 2) ^ kv4_flip(D, place))];
-                o[i] = fmaf(pk, __half2float(__hfma(__int2half_rn(c & 1 ? b >> 4 : b & 15), __low2half(dm), __high2half(dm))), o[i]);
+        for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
+        if (lane == 31) part[warp] = before;
+        before -= sum;
+        __syncthreads();
+        int64_t all = 0;
+        for (int i = 0; i < KA_WARPS; i++) { if (i < warp) before += part[i]; all += part[i]; }
+        for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
+        if (threadIdx.x == 0) prefix[A.seqs] = all;
+    }
+    __syncthreads();
+    const int64_t U = prefix[A.seqs], warps = min((int64_t) gridDim.x * KA_WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) A.plan->warps = warps;
+        for (int s = threadIdx.x; s <= A.seqs; s += KA_WARPS * 32) A.plan->prefix[s] = prefix[s];
+    }
+    bool ok = true;
+    if (me < warps) {
+        const int64_t u0 = U * me / warps, u1 = U * (me + 1) / warps;
+        // a place among the units: page p of np from `first` on, of head h, of tile r, of sequence s
+        struct place { int s, r, h, p, np, first; };
+        auto enter = [&](place & c) { c.np = ka_pages<C::RT>(A, seq[c.s], c.r, c.first); };
+        auto next = [&](place & c) {                             // only called where there is a next unit
+            if (++c.p < c.np) return;
+            c.p = 0;
+            if (++c.h < A.kvh) return;
+            c.h = 0;
+            do {
+                if (++c.r >= ka_tiles<C::RT>(A, seq[c.s])) { c.r = 0; do c.s++; while (prefix[c.s + 1] == prefix[c.s]); }
+                enter(c);
+            } while (c.np == 0);
+        };
+        place at;
+        {
+            int lo = 0, hi = A.seqs;                             // the last sequence with prefix <= u0 that has units
+            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= u0) lo = mid; else hi = mid; }
+            int64_t rest = u0 - prefix[lo];
+            at.s = lo; at.r = 0;
+            for (enter(at); rest >= (int64_t) at.np * A.kvh; enter(at)) { rest -= (int64_t) at.np * A.kvh; at.r++; }
+            at.h = (int) (rest / at.np); at.p = (int) (rest % at.np);
+        }
+        // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
+        place    is = at;
+        int64_t  iu = u0;
+        int      ihalf = 0, ist = 0, id_s = -1, id_base = 0, ids = 0, id = 0;
+        uint32_t there = 0;                                      // of each stage: whether its page is one of the cache's
+        auto issue = [&]() {
+            if (iu >= u1) return;
+            if (!ihalf) {
+                const int pg = is.first + is.p;
+                if (is.s != id_s || pg < id_base || pg >= id_base + 32) {
+                    id_s = is.s; id_base = pg;
+                    ids = pg + lane < A.max_pages ? A.table[(int64_t) is.s * A.max_pages + pg + lane] : -1;
+                }
+                id = __shfl_sync(0xffffffffu, ids, pg - id_base);
             }
+            const bool in = id >= 0 && id < A.pages;
+            if (lane == 0) {
+                if (in) {
+                    dt_mbar_expect_tx(bar0 + ist * 8, C::HALF);
+                    ka_bulk(ring0 + ist * C::HALF, A.base + ((int64_t) id * A.kvh + is.h) * kv4_record(D) + ihalf * C::HALF, C::HALF, bar0 + ist * 8);
+                } else dt_arrive(bar0 + ist * 8);
+            }
+            there = in ? there | 1u << ist : there & ~(1u << ist);
+            if (++ist == NST) ist = 0;
+            if (ihalf) { iu++; if (iu < u1) next(is); }
+            ihalf ^= 1;
+        };
+        for (int i = 0; i < NST; i++) issue();
+
+        int st = 0;
+        uint32_t ph = 0;
+        int64_t u = u0;
+        while (u < u1 && ok) {
+            // ---- an item, or the piece of it in this warp's run
+            const ka_seq  q = seq[at.s];
+            const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = (int) min((int64_t) (at.np - at.p), u1 - u);
+            const bool    whole = at.p == 0 && pages == at.np;
+            const int     slot = 2 * (int) me + (at.p > 0 ? 0 : 1);
+            const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens);
+            const int     row0 = at.r * C::RT;
+            float qs[MT][C::NR], m[MT][C::NR], l[MT][C::NR], O[MT][C::NT][4];
+            int   lo[MT][C::NR], hi[MT][C::NR];
+            uint4 qf[C::QS ? 1 : MT][C::QS ? 1 : C::KS];
+            int   all_lo = 0, all_hi = 0x7fffffff;               // keys that all rows see
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                uint32_t w[2][C::KS][2];                         // [row or part][product][k low, k high]
+#pragma unroll
+                for (int nr = 0; nr < C::NR; nr++) {
+                    const int ri = mt * C::RPM + nr * 8 + g, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, pos = q.len - q.n + tk;
+                    hi[mt][nr] = pos;
+                    lo[mt][nr] = A.window > 0 ? max(0, pos - A.window + 1) : 0;
+                    const T * p = (const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4);
+                    float v[D / 4], top = 0.f;
+                    ka_load<T, D / 4>(p, A.wide_q, v);
+#pragma unroll
+                    for (int c = 0; c < D / 4; c++) top = fmaxf(top, fabsf(v[c]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+                    const float down = __uint_as_float((254u - e) << 23);
+                    qs[mt][nr] = __uint_as_float(e << 23) * (A.scale * KA_LOG2E);
+#pragma unroll
+                    for (int k = 0; k < C::KS; k++)
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {            // product k of word k / 2 takes channels 2 (k % 2) + b and four further
+                            const int   c = (k >> 1) * 8 + (k & 1) * 2 + b;
+                            const float x = v[c] * down, y = v[c + 4] * down;
+                            w[nr][k][b] = ka_pack(x, y);
+                            if (C::SPLIT) w[1][k][b] = ka_rest(x, y, w[nr][k][b]);
+                        }
+                    m[mt][nr] = -INFINITY; l[mt][nr] = 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < C::KS; k++) {
+                    const uint4 f = make_uint4(w[0][k][0], w[1][k][0], w[0][k][1], w[1][k][1]);
+                    if (C::QS) qsm[(mt * C::KS + k) * 32] = f; else qf[C::QS ? 0 : mt][C::QS ? 0 : k] = f;
+                }
+#pragma unroll
+                for (int i = 0; i < C::NT; i++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) O[mt][i][c] = 0.f;
+            }
+            all_hi = q.len - q.n + row0 / A.rep;                                     // the first token's last key, the last token's first one
+            all_lo = A.window > 0 ? q.len - q.n + (row0 + rows - 1) / A.rep - A.window + 1 : 0;
+
+            for (int i = 0; i < pages && ok; i++) {
+                const int key0 = (at.first + at.p + i) * KV4_P;
+                const bool in = there >> st & 1;
+                const uint32_t kst = st, kph = ph;
+                if (++st == NST) { st = 0; ph ^= 1; }
+                const uint32_t vst = st, vph = ph;
+                if (++st == NST) { st = 0; ph ^= 1; }
+                const uint8_t * kp = ring + kst * C::HALF, * vp = ring + vst * C::HALF;
+                const bool edge = key0 < all_lo || key0 + KV4_P - 1 > all_hi;
+                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + kst * 8, kph, abort_s));
+                if (!ok) break;
+                bool seen_v = false, bad_v = false;
+#pragma unroll 1
+                for (int kb = 0; kb < 2; kb++) {
+                    float S[4][MT][4];
+                    if (in) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                                for (int c = 0; c < 4; c++) S[j][mt][c] = 0.f;
+                            const int     r = kb * 32 + j * 8 + g;
+                            const __half2 dm = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                            const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
+                            uint32_t wv[C::W];
+                            if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[0] = x.x; wv[1] = x.y; wv[2] = x.z; wv[3] = x.w; }
+                            else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[0] = x.x; wv[1] = x.y; }
+#pragma unroll
+                            for (int w = 0; w < C::W; w++) {
+                                uint32_t o[4];
+                                kv4_pairs(wv[w], d2, m2, o);
+#pragma unroll
+                                for (int mt = 0; mt < MT; mt++) {
+                                    ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w], o[0], o[1]);
+                                    ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w + 1) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + 1], o[2], o[3]);
+                                }
+                            }
+                        }
+                    }
+                    if (kb == 1) {                               // the keys have been read
+                        __syncwarp();
+                        issue();
+                    }
+                    if (!in) continue;
+                    // ---- weights: the rows' maxima, exponentials, sums
+                    uint4 P[2][MT];
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+                        for (int nr = 0; nr < C::NR; nr++) {
+                            float s[4][2], top = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+#pragma unroll
+                                for (int c = 0; c < 2; c++) {
+                                    s[j][c] = (C::SPLIT ? S[j][mt][c] + S[j][mt][c + 2] : S[j][mt][nr * 2 + c]) * qs[mt][nr];
+                                    if (edge) {
+                                        const int key = key0 + kb * 32 + j * 8 + t * 2 + c;
+                                        if (key < lo[mt][nr] || key > hi[mt][nr]) s[j][c] = -INFINITY;
+                                    }
+                                    top = fmaxf(top, s[j][c]);
+                                }
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                            if (__any_sync(0xffffffffu, top > m[mt][nr])) {
+                                const float mn = fmaxf(m[mt][nr], top), a = mn == m[mt][nr] ? 1.f : ka_exp2(m[mt][nr] - mn);
+                                m[mt][nr] = mn;
+                                l[mt][nr] *= a;
+#pragma unroll
+                                for (int n = 0; n < C::NT; n++) {
+                                    O[mt][n][nr * 2] *= a; O[mt][n][nr * 2 + 1] *= a;
+                                    if (C::SPLIT) { O[mt][n][2] *= a; O[mt][n][3] *= a; }
+                                }
+                            }
+                            const float base = (m[mt][nr] == -INFINITY ? 0.f : m[mt][nr]) - KA_LIFT;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const float x = ka_exp2(s[j][0] - base), y = ka_exp2(s[j][1] - base);
+                                l[mt][nr] += x + y;
+                                const uint32_t h = ka_pack(x, y);
+                                uint32_t & at0 = j & 1 ? P[j >> 1][mt].z : P[j >> 1][mt].x, & at1 = j & 1 ? P[j >> 1][mt].w : P[j >> 1][mt].y;
+                                if (C::SPLIT) { at0 = h; at1 = ka_rest(x, y, h); }
+                                else if (nr == 0) at0 = h;
+                                else at1 = h;
+                            }
+                        }
+                    }
+                    if (!seen_v) {
+                        seen_v = true;
+                        ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
+                        if (!ok) break;
+                        if (edge) {                              // values that are none, on a page of which some row does not see all
+                            for (int k = lane; k < KV4_P * C::W; k += 32) bad_v |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + k * 4)));
+                            bad_v = __any_sync(0xffffffffu, bad_v);
+                        }
+                    }
+                    // ---- outputs
+#pragma unroll
+                    for (int i2 = 0; i2 < 2; i2++) {
+                        uint32_t a[2][C::W / 2], b[2][C::W / 2];               // this lane's channels of keys 2 t and 2 t + 1 of both groups of eight
+                        __half2  d2[2], m2[2];
+#pragma unroll
+                        for (int f = 0; f < 2; f++) {
+                            const int ra = kb * 32 + i2 * 16 + f * 8 + t, rb = ra + 4;         // kv4_row of the places 2 t and 2 t + 1
+                            __half2 da = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (ra * C::W + (g * C::W >> 3)) * 4);
+                            __half2 db = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (rb * C::W + (g * C::W >> 3)) * 4);
+                            if (bad_v) {                         // they enter as zeros here, and as what they are below
+                                if (__hisnan(__high2half(da))) da = __floats2half2_rn(0.f, 0.f);
+                                if (__hisnan(__high2half(db))) db = __floats2half2_rn(0.f, 0.f);
+                            }
+                            d2[f] = __lows2half2(da, db); m2[f] = __highs2half2(da, db);
+                            if constexpr (D == 128) {
+                                const uint2 x = *reinterpret_cast<const uint2 *>(vp + ra * 64 + ((g * 8) ^ kv4_flip(D, ra))), y = *reinterpret_cast<const uint2 *>(vp + rb * 64 + ((g * 8) ^ kv4_flip(D, rb)));
+                                a[f][0] = x.x; a[f][1] = x.y; b[f][0] = y.x; b[f][1] = y.y;
+                            } else { a[f][0] = *reinterpret_cast<const uint32_t *>(vp + ra * 32 + g * 4); b[f][0] = *reinterpret_cast<const uint32_t *>(vp + rb * 32 + g * 4); }
+                        }
+#pragma unroll
+                        for (int w = 0; w < C::W / 2; w++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                uint32_t x[4], y[4];
+                                kv4_pairs(ka_prmt(a[0][w], b[0][w], e ? 0x7632 : 0x5410), d2[0], m2[0], x);
+                                kv4_pairs(ka_prmt(a[1][w], b[1][w], e ? 0x7632 : 0x5410), d2[1], m2[1], y);
+#pragma unroll
+                                for (int n = 0; n < 4; n++)
+#pragma unroll
+                                    for (int mt = 0; mt < MT; mt++) ka_mma(O[mt][w * 8 + e * 4 + n], P[i2][mt], x[n], y[n]);
+                            }
+                    }
+                }
+                if (!ok) break;
+                if (in && bad_v)                                 // rows that see a value that is none: this lane's channels are of one group
+                    for (int k = 0; k < KV4_P; k++)
+                        if (__hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (t * C::W >> 2)) * 4))))
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                                for (int nr = 0; nr < C::NR; nr++)
+                                    if (key0 + k >= lo[mt][nr] && key0 + k <= hi[mt][nr])
+#pragma unroll
+                                        for (int n = 0; n < C::NT; n++) { O[mt][n][nr * 2] = __uint_as_float(0x7fc00000u); O[mt][n][nr * 2 + 1] = __uint_as_float(0x7fc00000u); }
+                if (!in) { ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s)); if (!ok) break; }
+                __syncwarp();
+                issue();                                         // the values have been read
+            }
+            if (!ok) break;
+            // ---- rows out: lane (g, t) has D / 4 neighbouring channels of its rows
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nr = 0; nr < C::NR; nr++) {
+                    float sum = l[mt][nr];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    const int ri = mt * C::RPM + nr * 8 + g;
+                    if (ri >= rows) continue;
+                    float v[D / 4];
+#pragma unroll
+                    for (int n = 0; n < C::NT; n++) {
+                        v[n]         = C::SPLIT ? O[mt][n][0] + O[mt][n][2] : O[mt][n][nr * 2];
+                        v[n + C::NT] = C::SPLIT ? O[mt][n][1] + O[mt][n][3] : O[mt][n][nr * 2 + 1];
+                    }
+                    if (whole) {
+                        const float inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
+#pragma unroll
+                        for (int c = 0; c < D / 4; c++) v[c] *= inv;
+                        const int rc = row0 + ri;
+                        ka_store<T, D / 4>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4), A.wide_o, v);
+                    } else {
+                        float * p = A.pieces + (int64_t) slot * C::PIECE;
+                        ka_store<float, D / 4>(p + ri * D + t * (D / 4), true, v);
+                        if (t == 0) { p[C::RT * D + ri] = m[mt][nr]; p[C::RT * D + C::RT + ri] = sum; }
+                    }
+                }
+            u += pages;
+            at.p += pages - 1;
+            if (u < u1) next(at);
         }
     }
-    T * out = (T *) A.out + (int64_t) t * A.ldo + (int64_t) h * D;
+    __syncthreads();
+    if (*abort_s) {                                              // a wait ran out: say so, give copies still in flight time to land (bounded)
+        if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+    }
+}
+
+// A block per (token, query head): rows of items that lay in several warps' runs get their pieces' sum, rows of items without pages zeros; the others are written already.
+template <typename T, int D, int MT>
+static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ ka_args A) {
+    using C = ka_cfg<T, D, MT>;
+    pib_pdl_wait();
+    pib_pdl_trigger();
+    __shared__ int   found;
+    __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = A.kvh * A.rep, t = blockIdx.x / heads, hq = blockIdx.x % heads, h = hq / A.rep;
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    for (int s = threadIdx.x; s < A.seqs; s += 256) if (A.starts[s] <= t && t < A.starts[s + 1]) atomicMax(&found, s);
+    __syncthreads();
+    const int s = found;
+    if (s < 0) return;
+    const ka_seq q = ka_load_seq(A, s);
+    const int tl = t - min(max(A.starts[s], 0), A.tokens), idx = tl * A.rep + hq % A.rep, r = idx / C::RT, ri = idx % C::RT;
+    if (tl >= q.n) return;
+    int     first;
+    int64_t ib = A.plan->prefix[s];
+    for (int i = 0; i < r; i++) ib += (int64_t) ka_pages<C::RT>(A, q, i, first) * A.kvh;
+    const int np = ka_pages<C::RT>(A, q, r, first);
+    ib += (int64_t) h * np;
+    T * out = (T *) A.out + (int64_t) t * A.ldo + (int64_t) hq * D;
+    if (np == 0) {
+        if (threadIdx.x < D) out[threadIdx.x] = (T) 0.f;
+        return;
+    }
+    const int64_t U = A.plan->prefix[A.seqs], W = A.plan->warps, wa = ((ib + 1) * W + U - 1) / U - 1, wb = ((ib + np) * W + U - 1) / U - 1;
+    if (wa == wb) return;
+    constexpr int CH = D / 32;
+    float m = -INFINITY, l = 0.f, o[CH];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) out[i * 32 + lane] = (T) (l > 0.f || l != l ? o[i] / l : 0.f);
+    for (int c = 0; c < CH; c++) o[c] = 0.f;
+#pragma unroll 2
+    for (int64_t w = wa + warp; w <= wb; w += 8) {
+        const float * p = A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE;
+        const float pm = p[C::RT * D + ri], pl = p[C::RT * D + C::RT + ri];
+        float v[CH];
+        if constexpr (CH == 4) { const float4 f = *reinterpret_cast<const float4 *>(p + ri * D + lane * 4); v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
+        else                   { const float2 f = *reinterpret_cast<const float2 *>(p + ri * D + lane * 2); v[0] = f.x; v[1] = f.y; }
+        const float mn = fmaxf(m, pm), a = m == mn ? 1.f : exp2f(m - mn), b = pm == mn ? 1.f : exp2f(pm - mn);
+        m = mn; l = l * a + pl * b;
+#pragma unroll
+        for (int c = 0; c < CH; c++) o[c] = o[c] * a + v[c] * b;
+    }
+    if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+#pragma unroll
+    for (int c = 0; c < CH; c++) sm_o[warp][lane * CH + c] = o[c];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    m = sm_m[0];
+    for (int i = 1; i < 8; i++) m = fmaxf(m, sm_m[i]);
+    float v = 0.f;
+    l = 0.f;
+    for (int i = 0; i < 8; i++) {
+        const float a = sm_m[i] == m ? 1.f : exp2f(sm_m[i] - m);
+        l += sm_l[i] * a; v += sm_o[i][threadIdx.x] * a;
+    }
+    out[threadIdx.x] = (T) (l > 0.f ? v / l : l != l ? l : 0.f);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
@@ -92,8 +538,28 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
+// tiles of two products' rows where a sequence has more rows than one product takes
+static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) {
+    const int most = b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens;
+    return (int64_t) most * (b->heads / kv->heads) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1;
+}
+static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
+    return (size_t) 2 * pib_num_sms() * KA_WARPS * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
+}
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    return ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) == PIB_OK ? 256 : 0;
+    if (ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) != PIB_OK) return 0;
+    return (ka_pieces(kv, b) + sizeof(ka_plan) + 255) & ~(size_t) 255;
+}
+
+template <typename T, int D, int MT> static int ka_go(ka_args A, cudaStream_t st) {
+    using C = ka_cfg<T, D, MT>;
+    const size_t table = ((size_t) (A.seqs + 1) * 8 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127, most = 224 * 1024;
+    A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (KA_WARPS * C::HALF));
+    static pib_per_device attrs;
+    PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
+    PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, MT>, dim3((unsigned) pib_num_sms()), dim3(KA_WARPS * 32), (size_t) KA_WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
+    PIB_CHECK(pib_launch(kv4_join_kernel<T, D, MT>, dim3((unsigned) ((int64_t) A.tokens * A.kvh * A.rep)), dim3(256), 0, st, A));
+    return PIB_OK;
 }
 
 extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const void * q, int64_t ldq, const int32_t * starts, const int32_t * lens, const int32_t * pages, void * out, int64_t ldo,
@@ -113,9 +579,21 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     A.base = kv->base; A.pages = kv->pages; A.kvh = kv->heads; A.rep = b->heads / kv->heads; A.dim = kv->dim;
     A.starts = starts; A.lens = lens; A.table = pages; A.tokens = b->tokens; A.seqs = b->seqs; A.max_pages = b->max_pages; A.window = b->window; A.scale = b->scale;
     A.q = q; A.out = out; A.ldq = ldq; A.ldo = ldo;
-    const dim3 grid((unsigned) (((int64_t) b->tokens * b->heads + 3) / 4));
+    A.wide_q = ((uintptr_t) q & 15) == 0 && ldq * size % 16 == 0;
+    A.wide_o = ((uintptr_t) out & 15) == 0 && ldo * size % 16 == 0;
+    A.pieces = (float *) scratch; A.plan = (ka_plan *) ((uint8_t *) scratch + ka_pieces(kv, b));
+    A.stages = 0;
+    if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;
-    if (size == 4) PIB_CHECK(pib_launch(kv->dim == 64 ? kv4_attn_kernel<float, 64> : kv4_attn_kernel<float, 128>, grid, dim3(128), 0, st, A));
-    else           PIB_CHECK(pib_launch(kv->dim == 64 ? kv4_attn_kernel<__nv_bfloat16, 64> : kv4_attn_kernel<__nv_bfloat16, 128>, grid, dim3(128), 0, st, A));
-    return PIB_OK;
+    const int form = (size == 4 ? 4 : 0) + (kv->dim == 128 ? 2 : 0) + (ka_mt(kv, b) == 2 ? 1 : 0);
+    switch (form) {
+        case 0:  return ka_go<__nv_bfloat16, 64, 1>(A, st);
+        case 1:  return ka_go<__nv_bfloat16, 64, 2>(A, st);
+        case 2:  return ka_go<__nv_bfloat16, 128, 1>(A, st);
+        case 3:  return ka_go<__nv_bfloat16, 128, 2>(A, st);
+        case 4:  return ka_go<float, 64, 1>(A, st);
+        case 5:  return ka_go<float, 64, 2>(A, st);
+        case 6:  return ka_go<float, 128, 1>(A, st);
+        default: return ka_go<float, 128, 2>(A, st);
+    }
 }

@@ -75,8 +75,9 @@ static __global__ void __launch_bounds__(KC_THREADS) kv4_write_kernel(uint8_t * 
         if (big >= 0x7f800000u) { d = __ushort_as_half(0); m = __ushort_as_half(0x7e00); q = 0; }
         if (u0 + (int) threadIdx.x >= all) continue;
         uint8_t * part = base + ((int64_t) (cell / KV4_P) * heads + head) * kv4_record(dim) + values * kv4_half(dim);
-        *reinterpret_cast<uint32_t *>(part + place * (dim / 2) + ((o * 4) ^ (values ? kv4_flip(dim, place) : 0))) = q;
-        if ((o & 3) == 0) *reinterpret_cast<__half2 *>(part + kv4_steps(dim) + (place * (dim / 32) + (o >> 2)) * 4) = __halves2half2(d, m);
+        const int row  = values ? kv4_row(place) : place;
+        *reinterpret_cast<uint32_t *>(part + row * (dim / 2) + ((o * 4) ^ (values ? kv4_flip(dim, row) : 0))) = q;
+        if ((o & 3) == 0) *reinterpret_cast<__half2 *>(part + kv4_steps(dim) + (row * (dim / 32) + (o >> 2)) * 4) = __halves2half2(d, m);
     }
 }
 
@@ -95,8 +96,9 @@ static __global__ void __launch_bounds__(KC_THREADS) kv4_read_kernel(const uint8
         uint32_t p[4] = { 0, 0, 0, 0 };
         if (there) {
             const uint8_t * part = base + ((int64_t) (cell / KV4_P) * heads + head) * kv4_record(dim) + values * kv4_half(dim);
-            const __half2   dm = *reinterpret_cast<const __half2 *>(part + kv4_steps(dim) + (place * (dim / 32) + (o >> 2)) * 4);
-            kv4_pairs(*reinterpret_cast<const uint32_t *>(part + place * (dim / 2) + ((o * 4) ^ (values ? kv4_flip(dim, place) : 0))), __low2half2(dm), __high2half2(dm), p);
+            const int       row = values ? kv4_row(place) : place;
+            const __half2   dm = *reinterpret_cast<const __half2 *>(part + kv4_steps(dim) + (row * (dim / 32) + (o >> 2)) * 4);
+            kv4_pairs(*reinterpret_cast<const uint32_t *>(part + row * (dim / 2) + ((o * 4) ^ (values ? kv4_flip(dim, row) : 0))), __low2half2(dm), __high2half2(dm), p);
         }
         float x[8];
 #pragma unroll
