@@ -35,12 +35,17 @@ static inline int kv4_ok(const char * who, const pib_kv4 * kv) {
 }
 static inline int kv4_type_size(int type) { return type == PIB_TYPE_F32 ? 4 : type == PIB_TYPE_BF16 ? 2 : 0; }
 
-// eight nibbles of a word as four pairs {n[i], n[i + 4]} of fp16 numbers.  A nibble or'ed into 1024's last bits is 1024 + n, into the bits above them 1024 + 16 n; both come off exactly
-__device__ __forceinline__ __half2 kv4_low(uint32_t w)  { const uint32_t v = (w & 0x000f000fu) | 0x64006400u; return __hsub2(*reinterpret_cast<const __half2 *>(&v), __floats2half2_rn(1024.f, 1024.f)); }
-__device__ __forceinline__ __half2 kv4_high(uint32_t w) {
-    const uint32_t v = (w & 0x00f000f0u) | 0x64006400u;
-    return __hfma2(*reinterpret_cast<const __half2 *>(&v), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-64.f, -64.f));
+// eight nibbles of a word as four pairs {n[i], n[i + 4]} of fp16 numbers.  A nibble or'ed into 1024's last bits is 1024 + n, into the bits above them 1024 + 16 n; both come off exactly.  (Constants by
+// their bits: a conversion of theirs stays in the loops.)
+__device__ __forceinline__ __half2 kv4_bits(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
+// (one instruction for and + or: as two operators they stay two, 256 more for a page and warp)
+__device__ __forceinline__ __half2 kv4_in(uint32_t w, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
+    return kv4_bits(r);
 }
+__device__ __forceinline__ __half2 kv4_low(uint32_t w)  { return __hadd2(kv4_in(w, 0x000f000fu), kv4_bits(0xe400e400u)); }
+__device__ __forceinline__ __half2 kv4_high(uint32_t w) { return __hfma2(kv4_in(w, 0x00f000f0u), kv4_bits(0x2c002c00u), kv4_bits(0xd400d400u)); }
 __device__ __forceinline__ void kv4_pairs(uint32_t w, __half2 d, __half2 m, uint32_t (&o)[4]) {
     const __half2 a = __hfma2(kv4_low(w), d, m), b = __hfma2(kv4_high(w), d, m), c = __hfma2(kv4_low(w >> 8), d, m), e = __hfma2(kv4_high(w >> 8), d, m);
     o[0] = *reinterpret_cast<const uint32_t *>(&a); o[1] = *reinterpret_cast<const uint32_t *>(&b);

@@ -92,8 +92,8 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-#define KA_WARPS 8
-#define KA_LIFT  14.0f       // weights are e^(s - max) 2^14: fp16 then holds them down to 2^-38 of the largest
+#define KA_LIFT  7.0f        // weights are e^(s - m) 2^7: fp16 then holds them down to 2^-31 of e^(s - m) = 1
+#define KA_LAZY  8.0f        // m follows the running maximum once that is 2^8 ahead: a weight is 2^15 at most, and few blocks of keys rescale the sums
 
 // ---- decode and verification batches --------------------------------------------------------------------------------------------------
 // All (sequence, tile, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum and
@@ -106,23 +106,24 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
 template <typename T, int D, int MT> struct ka_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RPM = SPLIT ? 8 : 16, RT = MT * RPM, NR = SPLIT ? 1 : 2, KS = D / 16, W = D / 32, NT = D / 8;
+    static constexpr int  WARPS = 8;
     static constexpr bool QS = MT * KS > 8;                       // the queries' operands lie in shared memory
-    static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? KA_WARPS * MT * KS * 512 : 0;
+    static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * MT * KS * 512 : 0;
     static constexpr int  PIECE = RT * (D + 2);                   // floats
 };
 
 template <typename T, int D, int MT>
-static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
+static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
     using C = ka_cfg<T, D, MT>;
     extern __shared__ __align__(128) uint8_t ka_dsm[];
-    __shared__ uint64_t bars[KA_WARPS * 16];
-    __shared__ int64_t  part[KA_WARPS];
+    __shared__ uint64_t bars[C::WARPS * 16];
+    __shared__ int64_t  part[C::WARPS];
     __shared__ int      abort_w;
     volatile int * abort_s = &abort_w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, NST = A.stages;
     uint8_t *  ring = ka_dsm + warp * NST * C::HALF;
-    uint4 *    qsm  = reinterpret_cast<uint4 *>(ka_dsm + KA_WARPS * NST * C::HALF) + warp * MT * C::KS * 32 + lane;
-    int64_t *  prefix = reinterpret_cast<int64_t *>(ka_dsm + KA_WARPS * NST * C::HALF + C::Q_BYTES);         // [seqs + 1]
+    uint4 *    qsm  = reinterpret_cast<uint4 *>(ka_dsm + C::WARPS * NST * C::HALF) + warp * MT * C::KS * 32 + lane;
+    int64_t *  prefix = reinterpret_cast<int64_t *>(ka_dsm + C::WARPS * NST * C::HALF + C::Q_BYTES);         // [seqs + 1]
     ka_seq *   seq  = reinterpret_cast<ka_seq *>(prefix + A.seqs + 1);
     const uint32_t bar0 = dt_smem(bars + warp * 16), ring0 = dt_smem(ring);
     if (lane == 0) for (int i = 0; i < NST; i++) dt_mbar_init(bar0 + i * 8, 1);
@@ -133,7 +134,7 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
 
     // units in front of each sequence: a thread's neighbouring sequences, then warps, then the block
     {
-        const int per = (A.seqs + KA_WARPS * 32 - 1) / (KA_WARPS * 32), s0 = threadIdx.x * per;
+        const int per = (A.seqs + C::WARPS * 32 - 1) / (C::WARPS * 32), s0 = threadIdx.x * per;
         int64_t sum = 0;
         for (int s = s0; s < min(s0 + per, A.seqs); s++) {
             const ka_seq q = ka_load_seq(A, s);
@@ -149,15 +150,15 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
         before -= sum;
         __syncthreads();
         int64_t all = 0;
-        for (int i = 0; i < KA_WARPS; i++) { if (i < warp) before += part[i]; all += part[i]; }
+        for (int i = 0; i < C::WARPS; i++) { if (i < warp) before += part[i]; all += part[i]; }
         for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
         if (threadIdx.x == 0) prefix[A.seqs] = all;
     }
     __syncthreads();
-    const int64_t U = prefix[A.seqs], warps = min((int64_t) gridDim.x * KA_WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
+    const int64_t U = prefix[A.seqs], warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) A.plan->warps = warps;
-        for (int s = threadIdx.x; s <= A.seqs; s += KA_WARPS * 32) A.plan->prefix[s] = prefix[s];
+        for (int s = threadIdx.x; s <= A.seqs; s += C::WARPS * 32) A.plan->prefix[s] = prefix[s];
     }
     bool ok = true;
     if (me < warps) {
@@ -244,8 +245,9 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-                    const float down = __uint_as_float((254u - e) << 23);
-                    qs[mt][nr] = __uint_as_float(e << 23) * (A.scale * KA_LOG2E);
+                    // the scale's sign goes to the queries: what scores are multiplied with is above zero, and -inf stays what it is
+                    const float down = A.scale == 0.f ? 0.f : copysignf(__uint_as_float((254u - e) << 23), A.scale);
+                    qs[mt][nr] = A.scale == 0.f ? 1.f : fminf(fmaxf(__uint_as_float(e << 23) * fabsf(A.scale * KA_LOG2E), 1.2e-38f), 3e38f);
 #pragma unroll
                     for (int k = 0; k < C::KS; k++)
 #pragma unroll
@@ -277,66 +279,103 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
                 if (++st == NST) { st = 0; ph ^= 1; }
                 const uint32_t vst = st, vph = ph;
                 if (++st == NST) { st = 0; ph ^= 1; }
-                const uint8_t * kp = ring + kst * C::HALF, * vp = ring + vst * C::HALF;
+                uint8_t * kp = ring + kst * C::HALF, * vp = ring + vst * C::HALF;
                 const bool edge = key0 < all_lo || key0 + KV4_P - 1 > all_hi;
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + kst * 8, kph, abort_s));
                 if (!ok) break;
-                bool seen_v = false, bad_v = false;
+                if (!in) {                                       // no page: nothing was copied
+                    issue();
+                    ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
+                    if (ok) issue();
+                    continue;
+                }
 #pragma unroll 1
                 for (int kb = 0; kb < 2; kb++) {
                     float S[4][MT][4];
-                    if (in) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
+                    for (int j = 0; j < 4; j++) {
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++)
+                        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                                for (int c = 0; c < 4; c++) S[j][mt][c] = 0.f;
-                            const int     r = kb * 32 + j * 8 + g;
-                            const __half2 dm = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
-                            const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
-                            uint32_t wv[C::W];
-                            if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[0] = x.x; wv[1] = x.y; wv[2] = x.z; wv[3] = x.w; }
-                            else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[0] = x.x; wv[1] = x.y; }
+                            for (int c = 0; c < 4; c++) S[j][mt][c] = 0.f;
+                        const int     r = kb * 32 + j * 8 + g;
+                        const __half2 dm = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                        const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
+                        uint32_t wv[C::W];
+                        if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[0] = x.x; wv[1] = x.y; wv[2] = x.z; wv[3] = x.w; }
+                        else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[0] = x.x; wv[1] = x.y; }
 #pragma unroll
-                            for (int w = 0; w < C::W; w++) {
-                                uint32_t o[4];
-                                kv4_pairs(wv[w], d2, m2, o);
+                        for (int w = 0; w < C::W; w++) {
+                            uint32_t o[4];
+                            kv4_pairs(wv[w], d2, m2, o);
 #pragma unroll
-                                for (int mt = 0; mt < MT; mt++) {
-                                    ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w], o[0], o[1]);
-                                    ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w + 1) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + 1], o[2], o[3]);
-                                }
+                            for (int mt = 0; mt < MT; mt++) {
+                                ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w], o[0], o[1]);
+                                ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w + 1) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + 1], o[2], o[3]);
                             }
                         }
                     }
                     if (kb == 1) {                               // the keys have been read
                         __syncwarp();
                         issue();
+                    } else {
+                        ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
+                        if (!ok) break;
                     }
-                    if (!in) continue;
+                    if (C::SPLIT)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) { S[j][mt][0] += S[j][mt][2]; S[j][mt][1] += S[j][mt][3]; }
+                    if (edge) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                            for (int nr = 0; nr < C::NR; nr++)
+#pragma unroll
+                                for (int j = 0; j < 4; j++)
+#pragma unroll
+                                    for (int c = 0; c < 2; c++) {
+                                        const int key = key0 + kb * 32 + j * 8 + t * 2 + c;
+                                        if (key < lo[mt][nr] || key > hi[mt][nr]) S[j][mt][nr * 2 + c] = -INFINITY;
+                                    }
+                        if (kb == 0) {
+                            // values that are none, on a page of which some row does not see all: the rows that see one are none in the channels of its group, and it takes part as zeros
+                            bool bad = false;
+                            for (int k = lane; k < KV4_P * C::W; k += 32) bad |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + k * 4)));
+                            if (__any_sync(0xffffffffu, bad)) {
+                                for (int k = 0; k < KV4_P; k++)
+                                    if (__hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (t * C::W >> 2)) * 4))))
+#pragma unroll
+                                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                                            for (int nr = 0; nr < C::NR; nr++)
+                                                if (key0 + k >= lo[mt][nr] && key0 + k <= hi[mt][nr])
+#pragma unroll
+                                                    for (int n = 0; n < C::NT; n++) { O[mt][n][nr * 2] = __uint_as_float(0x7fc00000u); O[mt][n][nr * 2 + 1] = __uint_as_float(0x7fc00000u); }
+                                __syncwarp();
+                                for (int k = lane; k < KV4_P * C::W; k += 32) {
+                                    __half2 * dm = reinterpret_cast<__half2 *>(vp + kv4_steps(D) + k * 4);
+                                    if (__hisnan(__high2half(*dm))) *dm = kv4_bits(0);
+                                }
+                                dt_fence_async();                // the ring's next copy comes behind these stores
+                                __syncwarp();
+                            }
+                        }
+                    }
                     // ---- weights: the rows' maxima, exponentials, sums
                     uint4 P[2][MT];
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
                         for (int nr = 0; nr < C::NR; nr++) {
-                            float s[4][2], top = -INFINITY;
+                            float top = -INFINITY;
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-#pragma unroll
-                                for (int c = 0; c < 2; c++) {
-                                    s[j][c] = (C::SPLIT ? S[j][mt][c] + S[j][mt][c + 2] : S[j][mt][nr * 2 + c]) * qs[mt][nr];
-                                    if (edge) {
-                                        const int key = key0 + kb * 32 + j * 8 + t * 2 + c;
-                                        if (key < lo[mt][nr] || key > hi[mt][nr]) s[j][c] = -INFINITY;
-                                    }
-                                    top = fmaxf(top, s[j][c]);
-                                }
+                            for (int j = 0; j < 4; j++) top = fmaxf(top, fmaxf(S[j][mt][nr * 2], S[j][mt][nr * 2 + 1]));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                            if (__any_sync(0xffffffffu, top > m[mt][nr])) {
-                                const float mn = fmaxf(m[mt][nr], top), a = mn == m[mt][nr] ? 1.f : ka_exp2(m[mt][nr] - mn);
+                            top = __fmul_rn(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), qs[mt][nr]);
+                            if (__any_sync(0xffffffffu, top > m[mt][nr] + KA_LAZY)) {
+                                const float mn = top > m[mt][nr] + KA_LAZY ? top : m[mt][nr], a = mn == m[mt][nr] ? 1.f : ka_exp2(m[mt][nr] - mn);
                                 m[mt][nr] = mn;
                                 l[mt][nr] *= a;
 #pragma unroll
@@ -345,10 +384,11 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
                                     if (C::SPLIT) { O[mt][n][2] *= a; O[mt][n][3] *= a; }
                                 }
                             }
-                            const float base = (m[mt][nr] == -INFINITY ? 0.f : m[mt][nr]) - KA_LIFT;
+                            const float base = KA_LIFT - (m[mt][nr] == -INFINITY ? 0.f : m[mt][nr]);
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                const float x = ka_exp2(s[j][0] - base), y = ka_exp2(s[j][1] - base);
+                                // (product and sum rounded one by one, as the maximum's product is: of scores beyond 2^24 the difference would be the product's rounding)
+                                const float x = ka_exp2(__fadd_rn(__fmul_rn(S[j][mt][nr * 2], qs[mt][nr]), base)), y = ka_exp2(__fadd_rn(__fmul_rn(S[j][mt][nr * 2 + 1], qs[mt][nr]), base));
                                 l[mt][nr] += x + y;
                                 const uint32_t h = ka_pack(x, y);
                                 uint32_t & at0 = j & 1 ? P[j >> 1][mt].z : P[j >> 1][mt].x, & at1 = j & 1 ? P[j >> 1][mt].w : P[j >> 1][mt].y;
@@ -356,15 +396,6 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
                                 else if (nr == 0) at0 = h;
                                 else at1 = h;
                             }
-                        }
-                    }
-                    if (!seen_v) {
-                        seen_v = true;
-                        ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
-                        if (!ok) break;
-                        if (edge) {                              // values that are none, on a page of which some row does not see all
-                            for (int k = lane; k < KV4_P * C::W; k += 32) bad_v |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + k * 4)));
-                            bad_v = __any_sync(0xffffffffu, bad_v);
                         }
                     }
                     // ---- outputs
@@ -375,12 +406,8 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
 #pragma unroll
                         for (int f = 0; f < 2; f++) {
                             const int ra = kb * 32 + i2 * 16 + f * 8 + t, rb = ra + 4;         // kv4_row of the places 2 t and 2 t + 1
-                            __half2 da = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (ra * C::W + (g * C::W >> 3)) * 4);
-                            __half2 db = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (rb * C::W + (g * C::W >> 3)) * 4);
-                            if (bad_v) {                         // they enter as zeros here, and as what they are below
-                                if (__hisnan(__high2half(da))) da = __floats2half2_rn(0.f, 0.f);
-                                if (__hisnan(__high2half(db))) db = __floats2half2_rn(0.f, 0.f);
-                            }
+                            const __half2 da = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (ra * C::W + (g * C::W >> 3)) * 4);
+                            const __half2 db = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (rb * C::W + (g * C::W >> 3)) * 4);
                             d2[f] = __lows2half2(da, db); m2[f] = __highs2half2(da, db);
                             if constexpr (D == 128) {
                                 const uint2 x = *reinterpret_cast<const uint2 *>(vp + ra * 64 + ((g * 8) ^ kv4_flip(D, ra))), y = *reinterpret_cast<const uint2 *>(vp + rb * 64 + ((g * 8) ^ kv4_flip(D, rb)));
@@ -402,17 +429,6 @@ static __global__ void __launch_bounds__(KA_WARPS * 32, 1) kv4_decode_kernel(con
                     }
                 }
                 if (!ok) break;
-                if (in && bad_v)                                 // rows that see a value that is none: this lane's channels are of one group
-                    for (int k = 0; k < KV4_P; k++)
-                        if (__hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (t * C::W >> 2)) * 4))))
-#pragma unroll
-                            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                                for (int nr = 0; nr < C::NR; nr++)
-                                    if (key0 + k >= lo[mt][nr] && key0 + k <= hi[mt][nr])
-#pragma unroll
-                                        for (int n = 0; n < C::NT; n++) { O[mt][n][nr * 2] = __uint_as_float(0x7fc00000u); O[mt][n][nr * 2 + 1] = __uint_as_float(0x7fc00000u); }
-                if (!in) { ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s)); if (!ok) break; }
                 __syncwarp();
                 issue();                                         // the values have been read
             }
@@ -544,7 +560,7 @@ static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) {
     return (int64_t) most * (b->heads / kv->heads) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1;
 }
 static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    return (size_t) 2 * pib_num_sms() * KA_WARPS * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
+    return (size_t) 2 * pib_num_sms() * 8 * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
 }
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
     if (ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) != PIB_OK) return 0;
@@ -554,10 +570,10 @@ extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_b
 template <typename T, int D, int MT> static int ka_go(ka_args A, cudaStream_t st) {
     using C = ka_cfg<T, D, MT>;
     const size_t table = ((size_t) (A.seqs + 1) * 8 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127, most = 224 * 1024;
-    A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (KA_WARPS * C::HALF));
+    A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
-    PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, MT>, dim3((unsigned) pib_num_sms()), dim3(KA_WARPS * 32), (size_t) KA_WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
+    PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, MT>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
     PIB_CHECK(pib_launch(kv4_join_kernel<T, D, MT>, dim3((unsigned) ((int64_t) A.tokens * A.kvh * A.rep)), dim3(256), 0, st, A));
     return PIB_OK;
 }
