@@ -79,8 +79,13 @@ template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_
 struct ka_plan { int64_t warps, prefix[PIB_KV4_MAX_SEQS + 1]; };          // warps that share the units; units in front of each sequence
 
 __device__ __forceinline__ void ka_mma(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// the first product of a sum
+__device__ __forceinline__ void ka_mma0(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
@@ -92,6 +97,10 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+#ifndef KA_W1
+#define KA_W1 12
+#define KA_QS 8
+#endif
 #define KA_LIFT  7.0f        // weights are e^(s - m) 2^7: fp16 then holds them down to 2^-31 of e^(s - m) = 1
 #define KA_LAZY  8.0f        // m follows the running maximum once that is 2^8 ahead: a weight is 2^15 at most, and few blocks of keys rescale the sums
 
@@ -106,8 +115,8 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
 template <typename T, int D, int MT> struct ka_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RPM = SPLIT ? 8 : 16, RT = MT * RPM, NR = SPLIT ? 1 : 2, KS = D / 16, W = D / 32, NT = D / 8;
-    static constexpr int  WARPS = 8;
-    static constexpr bool QS = MT * KS > 8;                       // the queries' operands lie in shared memory
+    static constexpr int  WARPS = MT == 1 ? KA_W1 : 8;               // registers for more of a tile, or more warps
+    static constexpr bool QS = MT * KS >= KA_QS;                       // the queries' operands lie in shared memory
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * MT * KS * 512 : 0;
     static constexpr int  PIECE = RT * (D + 2);                   // floats
 };
@@ -292,28 +301,34 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
 #pragma unroll 1
                 for (int kb = 0; kb < 2; kb++) {
                     float S[4][MT][4];
+                    uint32_t wv[4][C::W];
+                    __half2  dm[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
+                        const int r = kb * 32 + j * 8 + g;
+                        dm[j] = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                        if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[j][0] = x.x; wv[j][1] = x.y; wv[j][2] = x.z; wv[j][3] = x.w; }
+                        else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[j][0] = x.x; wv[j][1] = x.y; }
+                    }
+#pragma unroll
+                    for (int w = 0; w < C::W; w++) {
+                        uint4 f[MT][2];
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                            for (int c = 0; c < 4; c++) S[j][mt][c] = 0.f;
-                        const int     r = kb * 32 + j * 8 + g;
-                        const __half2 dm = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
-                        const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
-                        uint32_t wv[C::W];
-                        if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[0] = x.x; wv[1] = x.y; wv[2] = x.z; wv[3] = x.w; }
-                        else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[0] = x.x; wv[1] = x.y; }
+                            for (int e = 0; e < 2; e++) f[mt][e] = C::QS ? qsm[(mt * C::KS + 2 * w + e) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + e];
+                        uint32_t o[4][4];
 #pragma unroll
-                        for (int w = 0; w < C::W; w++) {
-                            uint32_t o[4];
-                            kv4_pairs(wv[w], d2, m2, o);
+                        for (int j = 0; j < 4; j++) {
+                            kv4_pairs(wv[j][w], __low2half2(dm[j]), __high2half2(dm[j]), o[j]);
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++) {
-                                ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w], o[0], o[1]);
-                                ka_mma(S[j][mt], C::QS ? qsm[(mt * C::KS + 2 * w + 1) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + 1], o[2], o[3]);
-                            }
+                            for (int mt = 0; mt < MT; mt++)
+                                if (w == 0) ka_mma0(S[j][mt], f[mt][0], o[j][0], o[j][1]); else ka_mma(S[j][mt], f[mt][0], o[j][0], o[j][1]);
                         }
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) ka_mma(S[j][mt], f[mt][1], o[j][2], o[j][3]);
                     }
                     if (kb == 1) {                               // the keys have been read
                         __syncwarp();
@@ -507,17 +522,23 @@ static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_const
     float m = -INFINITY, l = 0.f, o[CH];
 #pragma unroll
     for (int c = 0; c < CH; c++) o[c] = 0.f;
-#pragma unroll 2
-    for (int64_t w = wa + warp; w <= wb; w += 8) {
-        const float * p = A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE;
-        const float pm = p[C::RT * D + ri], pl = p[C::RT * D + C::RT + ri];
-        float v[CH];
-        if constexpr (CH == 4) { const float4 f = *reinterpret_cast<const float4 *>(p + ri * D + lane * 4); v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
-        else                   { const float2 f = *reinterpret_cast<const float2 *>(p + ri * D + lane * 2); v[0] = f.x; v[1] = f.y; }
-        const float mn = fmaxf(m, pm), a = m == mn ? 1.f : exp2f(m - mn), b = pm == mn ? 1.f : exp2f(pm - mn);
-        m = mn; l = l * a + pl * b;
+    // a warp takes every eighth piece, 32 of them at a time: their maxima and sums, a piece a lane, then their rows, whose loads wait for nothing
+    for (int64_t w0 = wa + warp; w0 <= wb; w0 += 256) {
+        const int n = (int) min((int64_t) 32, (wb - w0) / 8 + 1);
+        auto piece = [&](int k) { const int64_t w = w0 + 8 * k; return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
+        float pm = -INFINITY, pl = 0.f;
+        if (lane < n) { pm = piece(lane)[C::RT * D + ri]; pl = piece(lane)[C::RT * D + C::RT + ri]; }
+        const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
+        m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
 #pragma unroll
-        for (int c = 0; c < CH; c++) o[c] = o[c] * a + v[c] * b;
+        for (int c = 0; c < CH; c++) o[c] *= a;
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+            const float * p = piece(k) + ri * D;
+            const float   fk = __shfl_sync(0xffffffffu, f, k);
+            if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
+            else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
+        }
     }
     if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
 #pragma unroll
@@ -560,7 +581,7 @@ static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) {
     return (int64_t) most * (b->heads / kv->heads) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1;
 }
 static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    return (size_t) 2 * pib_num_sms() * 8 * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
+    return (size_t) 2 * pib_num_sms() * (ka_mt(kv, b) == 1 ? KA_W1 : 8) * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
 }
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
     if (ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) != PIB_OK) return 0;
