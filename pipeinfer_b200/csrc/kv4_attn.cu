@@ -1,82 +1,7 @@
 // kv4_attn.cu -- attention of ragged sequences over a key / value cache in 4 bits (kv4.cuh): one pass over the keys with the running maximum and sum.
-#include "kv4.cuh"
-#include "tc_common.cuh"
+#include "kv4_attn.cuh"
 
 #include <algorithm>
-
-#define KA_LOG2E 1.4426950408889634f
-
-struct ka_args {
-    const uint8_t * base; int64_t pages; int kvh, rep, dim;
-    const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
-    const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
-    int stages; float * pieces; struct ka_plan * plan; int * err;
-};
-
-// n neighbouring values as floats, n a multiple of 8
-template <typename T, int N> __device__ __forceinline__ void ka_load(const T * p, bool wide, float (&v)[N]) {
-    if constexpr (sizeof(T) == 4) {
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) { const float4 f = *reinterpret_cast<const float4 *>(p + i); v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w; }
-        } else
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = p[i];
-    } else {
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < N; i += 8) {
-                const uint4 f = *reinterpret_cast<const uint4 *>(p + i);
-                const uint32_t w[4] = { f.x, f.y, f.z, f.w };
-#pragma unroll
-                for (int j = 0; j < 4; j++) { v[i + 2 * j] = __uint_as_float(w[j] << 16); v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
-            }
-        } else
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = __bfloat162float(p[i]);
-    }
-}
-template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, bool wide, const float (&v)[N]) {
-    if constexpr (sizeof(T) == 4) {
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else
-#pragma unroll
-            for (int i = 0; i < N; i++) p[i] = v[i];
-    } else {
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < N; i += 8) {
-                __nv_bfloat162 h[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
-                *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(h);
-            }
-        } else
-#pragma unroll
-            for (int i = 0; i < N; i++) p[i] = __float2bfloat16_rn(v[i]);
-    }
-}
-
-// ---- which keys a tile of rows sees ---------------------------------------------------------------------------------------------------
-// A sequence's rows, (token, head of the group) with the heads next to each other, are taken in tiles of RT; a tile of one key / value head is an item, its pages the units of work
-struct ka_seq { int n, len; };                      // query tokens and keys; both >= 0
-__device__ __forceinline__ ka_seq ka_load_seq(const ka_args & A, int s) {
-    const int a = min(max(A.starts[s], 0), A.tokens), b = min(max(A.starts[s + 1], 0), A.tokens);
-    return { max(b - a, 0), max(A.lens[s], 0) };
-}
-// pages [first, first + count) of tile r; keys behind the table's row are not there
-template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_seq q, int r, int & first) {
-    const int t0 = r * RT / A.rep, t1 = min(q.n - 1, ((r + 1) * RT - 1) / A.rep), p0 = q.len - q.n + t0, p1 = q.len - q.n + t1;
-    const int top = min(p1 < 0 ? -1 : p1 / KV4_P, A.max_pages - 1);
-    first = A.window > 0 ? max(0, p0 - A.window + 1) / KV4_P : 0;
-    return max(0, top - first + 1);
-}
-template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
-
-// what both kernels know of the work: behind the pieces in the scratch
-struct ka_plan { int64_t warps, prefix[PIB_KV4_MAX_SEQS + 1]; };          // warps that share the units; units in front of each sequence
 
 __device__ __forceinline__ void ka_mma(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -87,23 +12,6 @@ __device__ __forceinline__ void ka_mma0(float (&c)[4], uint4 a, uint32_t b0, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
-__device__ __forceinline__ float2 ka_float2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-// what the rounding to fp16 took away
-__device__ __forceinline__ uint32_t ka_rest(float a, float b, uint32_t hi) { const float2 f = ka_float2(hi); return ka_pack(a - f.x, b - f.y); }
-__device__ __forceinline__ uint32_t ka_prmt(uint32_t a, uint32_t b, uint32_t sel) { uint32_t r; asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel)); return r; }
-__device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
-#ifndef KA_W1
-#define KA_W1 12
-#define KA_QS 8
-#endif
-#define KA_LIFT  7.0f        // weights are e^(s - m) 2^7: fp16 then holds them down to 2^-31 of e^(s - m) = 1
-#define KA_LAZY  8.0f        // m follows the running maximum once that is 2^8 ahead: a weight is 2^15 at most, and few blocks of keys rescale the sums
-
 // ---- decode and verification batches --------------------------------------------------------------------------------------------------
 // All (sequence, tile, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum and
 // sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
@@ -115,8 +23,8 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
 template <typename T, int D, int MT> struct ka_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RPM = SPLIT ? 8 : 16, RT = MT * RPM, NR = SPLIT ? 1 : 2, KS = D / 16, W = D / 32, NT = D / 8;
-    static constexpr int  WARPS = MT == 1 ? KA_W1 : 8;               // registers for more of a tile, or more warps
-    static constexpr bool QS = MT * KS >= KA_QS;                       // the queries' operands lie in shared memory
+    static constexpr int  WARPS = 8;
+    static constexpr bool QS = MT * KS >= 8;                       // the queries' operands lie in shared memory
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * MT * KS * 512 : 0;
     static constexpr int  PIECE = RT * (D + 2);                   // floats
 };
@@ -141,61 +49,16 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
     pib_pdl_wait();
     pib_pdl_trigger();
 
-    // units in front of each sequence: a thread's neighbouring sequences, then warps, then the block
-    {
-        const int per = (A.seqs + C::WARPS * 32 - 1) / (C::WARPS * 32), s0 = threadIdx.x * per;
-        int64_t sum = 0;
-        for (int s = s0; s < min(s0 + per, A.seqs); s++) {
-            const ka_seq q = ka_load_seq(A, s);
-            seq[s] = q;
-            prefix[s] = sum;
-            int first;
-            for (int r = 0; r < ka_tiles<C::RT>(A, q); r++) sum += (int64_t) ka_pages<C::RT>(A, q, r, first) * A.kvh;
-        }
-        int64_t before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
-        if (lane == 31) part[warp] = before;
-        before -= sum;
-        __syncthreads();
-        int64_t all = 0;
-        for (int i = 0; i < C::WARPS; i++) { if (i < warp) before += part[i]; all += part[i]; }
-        for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
-        if (threadIdx.x == 0) prefix[A.seqs] = all;
-    }
-    __syncthreads();
-    const int64_t U = prefix[A.seqs], warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
-    if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) A.plan->warps = warps;
-        for (int s = threadIdx.x; s <= A.seqs; s += C::WARPS * 32) A.plan->prefix[s] = prefix[s];
-    }
+    const int64_t U = ka_prefix<C::RT, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
+    const int64_t warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
+    ka_leave_plan<C::WARPS * 32>(A, prefix, warps);
+    auto seq_of = [&](int s) { return seq[s]; };
     bool ok = true;
     if (me < warps) {
         const int64_t u0 = U * me / warps, u1 = U * (me + 1) / warps;
-        // a place among the units: page p of np from `first` on, of head h, of tile r, of sequence s
-        struct place { int s, r, h, p, np, first; };
-        auto enter = [&](place & c) { c.np = ka_pages<C::RT>(A, seq[c.s], c.r, c.first); };
-        auto next = [&](place & c) {                             // only called where there is a next unit
-            if (++c.p < c.np) return;
-            c.p = 0;
-            if (++c.h < A.kvh) return;
-            c.h = 0;
-            do {
-                if (++c.r >= ka_tiles<C::RT>(A, seq[c.s])) { c.r = 0; do c.s++; while (prefix[c.s + 1] == prefix[c.s]); }
-                enter(c);
-            } while (c.np == 0);
-        };
-        place at;
-        {
-            int lo = 0, hi = A.seqs;                             // the last sequence with prefix <= u0 that has units
-            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= u0) lo = mid; else hi = mid; }
-            int64_t rest = u0 - prefix[lo];
-            at.s = lo; at.r = 0;
-            for (enter(at); rest >= (int64_t) at.np * A.kvh; enter(at)) { rest -= (int64_t) at.np * A.kvh; at.r++; }
-            at.h = (int) (rest / at.np); at.p = (int) (rest % at.np);
-        }
+        ka_place at = ka_find<C::RT>(A, prefix, seq_of, u0);
         // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
-        place    is = at;
+        ka_place is = at;
         int64_t  iu = u0;
         int      ihalf = 0, ist = 0, id_s = -1, id_base = 0, ids = 0, id = 0;
         uint32_t there = 0;                                      // of each stage: whether its page is one of the cache's
@@ -218,7 +81,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
             }
             there = in ? there | 1u << ist : there & ~(1u << ist);
             if (++ist == NST) ist = 0;
-            if (ihalf) { iu++; if (iu < u1) next(is); }
+            if (ihalf) { iu++; if (iu < u1) ka_next<C::RT>(A, prefix, seq_of, is); }
             ihalf ^= 1;
         };
         for (int i = 0; i < NST; i++) issue();
@@ -478,7 +341,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                 }
             u += pages;
             at.p += pages - 1;
-            if (u < u1) next(at);
+            if (u < u1) ka_next<C::RT>(A, prefix, seq_of, at);
         }
     }
     __syncthreads();
@@ -516,7 +379,7 @@ static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_const
         if (threadIdx.x < D) out[threadIdx.x] = (T) 0.f;
         return;
     }
-    const int64_t U = A.plan->prefix[A.seqs], W = A.plan->warps, wa = ((ib + 1) * W + U - 1) / U - 1, wb = ((ib + np) * W + U - 1) / U - 1;
+    const int64_t U = A.plan->prefix[A.seqs], W = A.plan->runs, wa = ((ib + 1) * W + U - 1) / U - 1, wb = ((ib + np) * W + U - 1) / U - 1;
     if (wa == wb) return;
     constexpr int CH = D / 32;
     float m = -INFINITY, l = 0.f, o[CH];
@@ -575,13 +438,13 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
-// tiles of two products' rows where a sequence has more rows than one product takes
-static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    const int most = b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens;
-    return (int64_t) most * (b->heads / kv->heads) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1;
-}
+// rows (token, head of the group) of the longest portion: up to one or two products' rows by the decode kernels, more than KA_FEW on tcgen05
+#define KA_FEW 64
+static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
+static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) { return ka_rows(kv, b) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1; }
 static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    return (size_t) 2 * pib_num_sms() * (ka_mt(kv, b) == 1 ? KA_W1 : 8) * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16) * (kv->dim + 2) * 4;
+    const size_t rows = ka_rows(kv, b) > KA_FEW ? KP_ROWS : (size_t) 8 * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16);
+    return (size_t) 2 * pib_num_sms() * rows * (kv->dim + 2) * 4;
 }
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
     if (ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) != PIB_OK) return 0;
@@ -622,6 +485,7 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     A.stages = 0;
     if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;
+    if (ka_rows(kv, b) > KA_FEW) return pib_kv4_prompt(A, size == 4, st);
     const int form = (size == 4 ? 4 : 0) + (kv->dim == 128 ? 2 : 0) + (ka_mt(kv, b) == 2 ? 1 : 0);
     switch (form) {
         case 0:  return ka_go<__nv_bfloat16, 64, 1>(A, st);

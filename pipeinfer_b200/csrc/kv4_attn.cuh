@@ -1,0 +1,152 @@
+// kv4_attn.cuh -- what the kernels of attention over a 4-bit cache share (kv4_attn.cu: decode and verification batches; kv4_prompt.cu: prompts): the work's division, rows in and out.
+#pragma once
+
+#include "kv4.cuh"
+#include "tc_common.cuh"
+
+#define KA_LOG2E 1.4426950408889634f
+
+struct ka_args {
+    const uint8_t * base; int64_t pages; int kvh, rep, dim;
+    const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
+    const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
+    int stages; float * pieces; struct ka_plan * plan; int * err;
+};
+
+// n neighbouring values as floats, n a multiple of 8
+template <typename T, int N> __device__ __forceinline__ void ka_load(const T * p, bool wide, float (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) { const float4 f = *reinterpret_cast<const float4 *>(p + i); v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w; }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = p[i];
+    } else {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 8) {
+                const uint4 f = *reinterpret_cast<const uint4 *>(p + i);
+                const uint32_t w[4] = { f.x, f.y, f.z, f.w };
+#pragma unroll
+                for (int j = 0; j < 4; j++) { v[i + 2 * j] = __uint_as_float(w[j] << 16); v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = __bfloat162float(p[i]);
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, bool wide, const float (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) p[i] = v[i];
+    } else {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < N; i += 8) {
+                __nv_bfloat162 h[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+                *reinterpret_cast<uint4 *>(p + i) = *reinterpret_cast<const uint4 *>(h);
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < N; i++) p[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+// ---- which keys a tile of rows sees ---------------------------------------------------------------------------------------------------
+// A sequence's rows, (token, head of the group) with the heads next to each other, are taken in tiles of RT; a tile of one key / value head is an item, its pages the units of work
+struct ka_seq { int n, len; };                      // query tokens and keys; both >= 0
+__device__ __forceinline__ ka_seq ka_load_seq(const ka_args & A, int s) {
+    const int a = min(max(A.starts[s], 0), A.tokens), b = min(max(A.starts[s + 1], 0), A.tokens);
+    return { max(b - a, 0), max(A.lens[s], 0) };
+}
+// pages [first, first + count) of tile r; keys behind the table's row are not there
+template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_seq q, int r, int & first) {
+    const int t0 = r * RT / A.rep, t1 = min(q.n - 1, ((r + 1) * RT - 1) / A.rep), p0 = q.len - q.n + t0, p1 = q.len - q.n + t1;
+    const int top = min(p1 < 0 ? -1 : p1 / KV4_P, A.max_pages - 1);
+    first = A.window > 0 ? max(0, p0 - A.window + 1) / KV4_P : 0;
+    return max(0, top - first + 1);
+}
+template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
+
+// what both kernels know of the work: behind the pieces in the scratch
+struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // runs of units; units in front of each sequence
+
+// A place among the units: page p of np from `first` on, of head h, of tile r, of sequence s.  prefix: units in front of each sequence; seq(s): its tokens and keys
+struct ka_place { int s, r, h, p, np, first; };
+template <int RT, typename Seq> __device__ __forceinline__ void ka_enter(const ka_args & A, const Seq & seq, ka_place & c) { c.np = ka_pages<RT>(A, seq(c.s), c.r, c.first); }
+// only called where there is a next unit
+template <int RT, typename Seq> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, const Seq & seq, ka_place & c) {
+    if (++c.p < c.np) return;
+    c.p = 0;
+    if (++c.h < A.kvh) return;
+    c.h = 0;
+    do {
+        if (++c.r >= ka_tiles<RT>(A, seq(c.s))) { c.r = 0; do c.s++; while (prefix[c.s + 1] == prefix[c.s]); }
+        ka_enter<RT>(A, seq, c);
+    } while (c.np == 0);
+}
+// unit u < prefix[seqs]
+template <int RT, typename Seq> __device__ __forceinline__ ka_place ka_find(const ka_args & A, const int64_t * prefix, const Seq & seq, int64_t u) {
+    int lo = 0, hi = A.seqs;                                     // the last sequence with prefix <= u: it has units
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= u) lo = mid; else hi = mid; }
+    int64_t  rest = u - prefix[lo];
+    ka_place c;
+    c.s = lo; c.r = 0;
+    for (ka_enter<RT>(A, seq, c); rest >= (int64_t) c.np * A.kvh; ka_enter<RT>(A, seq, c)) { rest -= (int64_t) c.np * A.kvh; c.r++; }
+    c.h = (int) (rest / c.np); c.p = (int) (rest % c.np);
+    return c;
+}
+// Units in front of each sequence, by all THREADS threads of a block: a thread's neighbouring sequences, then warps, then the block.  part: THREADS / 32 numbers.  Ends with a barrier; the first block leaves
+// them in the plan
+template <int RT, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, const Keep & keep) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (A.seqs + THREADS - 1) / THREADS, s0 = threadIdx.x * per;
+    int64_t sum = 0;
+    for (int s = s0; s < min(s0 + per, A.seqs); s++) {
+        const ka_seq q = ka_load_seq(A, s);
+        keep(s, q);
+        prefix[s] = sum;
+        int first;
+        for (int r = 0; r < ka_tiles<RT>(A, q); r++) sum += (int64_t) ka_pages<RT>(A, q, r, first) * A.kvh;
+    }
+    int64_t before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
+    if (lane == 31) part[warp] = before;
+    before -= sum;
+    __syncthreads();
+    int64_t all = 0;
+    for (int i = 0; i < THREADS / 32; i++) { if (i < warp) before += part[i]; all += part[i]; }
+    for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
+    if (threadIdx.x == 0) prefix[A.seqs] = all;
+    __syncthreads();
+    return all;
+}
+template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_args & A, const int64_t * prefix, int64_t runs) {
+    if (blockIdx.x != 0) return;
+    if (threadIdx.x == 0) A.plan->runs = runs;
+    for (int s = threadIdx.x; s <= A.seqs; s += THREADS) A.plan->prefix[s] = prefix[s];
+}
+
+#define KA_LIFT  7.0f        // weights are e^(s - m) 2^7: fp16 then holds them down to 2^-31 of e^(s - m) = 1
+#define KA_LAZY  8.0f        // m follows the running maximum once that is 2^8 ahead: a weight is 2^15 at most, and few blocks of keys rescale the sums
+
+__device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ float2 ka_float2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+// what the rounding to fp16 took away
+__device__ __forceinline__ uint32_t ka_rest(float a, float b, uint32_t hi) { const float2 f = ka_float2(hi); return ka_pack(a - f.x, b - f.y); }
+__device__ __forceinline__ uint32_t ka_prmt(uint32_t a, uint32_t b, uint32_t sel) { uint32_t r; asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel)); return r; }
+__device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// kv4_prompt.cu: launches; pieces in floats
+#define KP_ROWS 256
+int    pib_kv4_prompt(ka_args A, bool f32, cudaStream_t st);

@@ -1,0 +1,483 @@
+// kv4_prompt.cu -- attention of portions of prompts over a key / value cache in 4 bits (kv4.cuh) on tcgen05, scores, weights and outputs in tensor memory.
+//
+// A block takes 256 rows (token, head of the group) of one key / value head as two groups of 128 and walks the pages they see; pages of all such items lie in one row that the blocks of the GPU (one an
+// SM) divide evenly, whatever the sequences' lengths (kv4_attn.cuh).  An item that lies in one block's run is written at once; pieces of others go to scratch and kv4_prompt_join_kernel adds them up.
+//   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
+//   warps 2..5    write a page's keys [64][dim] and its values, turned, [dim][64] as fp16 into tiles of the 128-byte swizzle, two of each
+//   warp 1        issues the MMAs: scores S = Q K' of the next page, then O += P V of this one, for both groups
+//   warps 6..13   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 back into tensor memory, from where they enter the second product
+// fp32 queries and weights enter as fp16 part and remainder, two products each; bfloat16 queries are exact in fp16 (times a power of two of the row), their weights are one fp16 number.
+// Every wait is bounded (tc_common.cuh).
+#include "kv4_attn.cuh"
+
+#include <algorithm>
+
+#define KP_THREADS 448
+#define KP_BARS    32
+
+template <typename T, int D> struct kp_cfg {
+    static constexpr bool SPLIT = sizeof(T) == 4;
+    static constexpr int  RAW = SPLIT ? 2 : 3, W = D / 32, NC = D / 64;              // records under way; groups; 64-wide column chunks of a head
+    static constexpr int  Q_CHUNK = 128 * 128, Q_PART = 2 * NC * Q_CHUNK;            // both groups' rows: [group][chunk][128 rows][128 bytes]
+    static constexpr int  Q_BYTES = Q_PART * (SPLIT ? 2 : 1), K_CHUNK = 64 * 128, K_TILE = NC * K_CHUNK, V_TILE = D * 128;
+    static constexpr int  TILES = Q_BYTES + 2 * (K_TILE + V_TILE), REC = kv4_record(D);
+    static constexpr int  PIECE = KP_ROWS * (D + 2);                                 // floats
+    static constexpr size_t FIXED = (size_t) TILES + RAW * REC + KP_BARS * 8 + 128 + 1024;
+};
+
+// A in tensor memory, B in shared memory; called by a converged warp
+__device__ __forceinline__ void kp_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void kp_st16(uint32_t taddr, const uint32_t * v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+                   "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+// fp16 x fp16, fp32 accumulators, both K-major, M x N outputs
+__host__ __device__ constexpr uint32_t kp_idesc(int M, int N) { return (1u << 4) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ ka_args A) {
+    using C = kp_cfg<T, D>;
+    extern __shared__ __align__(1024) uint8_t kp_dsm[];
+    uint8_t *  sQ   = kp_dsm + ((1024u - (dt_smem(kp_dsm) & 1023u)) & 1023u);
+    uint8_t *  sK   = sQ + C::Q_BYTES, * sV = sK + 2 * C::K_TILE, * raw = sV + 2 * C::V_TILE;
+    uint64_t * bar  = reinterpret_cast<uint64_t *>(raw + C::RAW * C::REC);
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + KP_BARS);
+    volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int * raw_in = reinterpret_cast<volatile int *>(tmem_slot + 2);         // [RAW] whether the record's page is one of the cache's
+    volatile unsigned long long * v_none = reinterpret_cast<volatile unsigned long long *>(tmem_slot + 12);      // [2][W] places of a page whose values are none, of each group
+    int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 128);       // [seqs + 1]
+    __shared__ int64_t part[KP_THREADS / 32];
+    // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there / read, weights written, product done
+    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_r = b0 + 160,
+                   bar_p = b0 + 176, bar_o = b0 + 192;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::RAW; i++) { dt_mbar_init(bar_rf + 8 * i, 1); dt_mbar_init(bar_re + 8 * i, 4); }
+        for (int i = 0; i < 2; i++) {
+            dt_mbar_init(bar_kf + 8 * i, 4); dt_mbar_init(bar_vf + 8 * i, 4);
+            for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_o }) dt_mbar_init(b + 8 * i, 1);
+            dt_mbar_init(bar_q + 8 * i, 4); dt_mbar_init(bar_r + 8 * i, 4); dt_mbar_init(bar_p + 8 * i, 4);
+        }
+        *abort_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dt_smem(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pib_pdl_wait();
+    pib_pdl_trigger();
+    dt_fence_before();
+    const int64_t U = ka_prefix<KP_ROWS, KP_THREADS>(A, prefix, part, [](int, ka_seq) {});
+    dt_fence_after();
+    const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
+    ka_leave_plan<KP_THREADS>(A, prefix, runs);
+    const uint32_t tmem = *tmem_slot, tm_p = tmem + 128, tm_o = tmem + 256;          // columns: scores 0..63 and 64..127, weights 128..191 and 192..255 (32 of each part), outputs 256..383 and 384..511
+    auto seq_of = [&](int s) { return ka_load_seq(A, s); };
+    // rows of tiles without pages
+    for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
+        const ka_seq  q = seq_of(s);
+        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
+        for (int r = 0; r < ka_tiles<KP_ROWS>(A, q); r++) {
+            int first;
+            if (ka_pages<KP_ROWS>(A, q, r, first)) continue;
+            const int     row0 = r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
+            for (int64_t i = threadIdx.x; i < (int64_t) rows * A.kvh * D; i += KP_THREADS) {
+                const int c = (int) (i % D), h = (int) (i / D % A.kvh), rc = row0 + (int) (i / D / A.kvh);
+                ((T *) A.out)[(tok0 + rc / A.rep) * A.ldo + (int64_t) (h * A.rep + rc % A.rep) * D + c] = (T) 0.f;
+            }
+        }
+    }
+    const int64_t u0 = me < runs ? U * me / runs : 0, u1 = me < runs ? U * (me + 1) / runs : 0;
+    // every role walks the same items of the run: f(tokens and keys, place, rows, pages of it) until it says no
+    auto items = [&](auto f) {
+        if (u0 >= u1) return;
+        ka_place at = ka_find<KP_ROWS>(A, prefix, seq_of, u0);
+        for (int64_t u = u0; u < u1;) {
+            const ka_seq q = seq_of(at.s);
+            const int    rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - (int64_t) at.r * KP_ROWS), pages = (int) min((int64_t) (at.np - at.p), u1 - u);
+            if (!f(q, at, rows, pages)) return;
+            u += pages;
+            at.p += pages - 1;
+            if (u < u1) ka_next<KP_ROWS>(A, prefix, seq_of, at);
+        }
+    };
+    // whether some row of the item does not see all of a page
+    auto edge_of = [&](ka_seq q, const ka_place & at, int rows, int key0) {
+        const int hi = q.len - q.n + at.r * KP_ROWS / A.rep, lo = A.window > 0 ? q.len - q.n + (at.r * KP_ROWS + rows - 1) / A.rep - A.window + 1 : 0;
+        return key0 < lo || key0 + KV4_P - 1 > hi;
+    };
+
+    if (warp == 0) {
+        int st = 0;
+        uint32_t ph = 1;                                         // the first round finds its places free
+        items([&](ka_seq, const ka_place & at, int, int pages) {
+            int ids = 0;
+            for (int i = 0; i < pages; i++) {
+                const int pg = at.first + at.p + i;
+                if ((i & 31) == 0) ids = pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1;
+                const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
+                const bool in = id >= 0 && id < A.pages;
+                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_re + 8 * st, ph, abort_s))) return false;
+                if (lane == 0) {
+                    raw_in[st] = in;
+                    if (in) {
+                        dt_mbar_expect_tx(bar_rf + 8 * st, C::REC);
+                        ka_bulk(dt_smem(raw + st * C::REC), A.base + ((int64_t) id * A.kvh + at.h) * C::REC, C::REC, bar_rf + 8 * st);
+                    } else dt_arrive(bar_rf + 8 * st);
+                }
+                if (++st == C::RAW) { st = 0; ph ^= 1; }
+            }
+            return true;
+        });
+    } else if (warp == 1) {
+        constexpr uint32_t id_s = kp_idesc(128, 64), id_o = kp_idesc(128, D);
+        const uint64_t dq = dt_desc(dt_smem(sQ)), dk = dt_desc(dt_smem(sK)), dv = dt_desc(dt_smem(sV));
+        int      j = 0, n_q[2] = { 0, 0 }, n_s[2] = { 0, 0 }, n_p[2] = { 0, 0 };
+        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
+        auto scores = [&](int jj, int groups) {
+            if (!wait(bar_kf + 8 * (jj & 1), jj >> 1)) return false;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                if (w >= groups) break;
+                if (!wait(bar_r + 8 * w, n_s[w] + 1)) return false;          // the scores before have been read
+                n_s[w]++;
+                dt_fence_after();
+                bool acc = false;
+#pragma unroll
+                for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
+#pragma unroll
+                    for (int c = 0; c < C::NC; c++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            dt_mma(tmem + 64 * w, dq + (uint64_t) ((part_ * C::Q_PART + (w * C::NC + c) * C::Q_CHUNK) >> 4) + 2 * k, dk + (uint64_t) (((jj & 1) * C::K_TILE + c * C::K_CHUNK) >> 4) + 2 * k, id_s, acc);
+                            acc = true;
+                        }
+                dt_commit(bar_s + 8 * w);
+            }
+            dt_commit(bar_ke + 8 * (jj & 1));
+            return true;
+        };
+        items([&](ka_seq, const ka_place &, int rows, int pages) {
+            const int groups = rows > 128 ? 2 : 1;
+            for (int w = 0; w < groups; w++) if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
+            if (!scores(j, groups)) return false;
+            for (int i = 0; i < pages; i++, j++) {
+                if (i + 1 < pages && !scores(j + 1, groups)) return false;
+                if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    if (w >= groups) break;
+                    if (!wait(bar_p + 8 * w, n_p[w])) return false;
+                    n_p[w]++;
+                    dt_fence_after();
+#pragma unroll
+                    for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tm_p + 64 * w + 32 * part_ + 8 * k, dv + (uint64_t) ((j & 1) * C::V_TILE >> 4) + 2 * k, id_o, (i > 0) | ((part_ | k) != 0));
+                    dt_commit(bar_o + 8 * w);
+                }
+                dt_commit(bar_ve + 8 * (j & 1));
+            }
+            return true;
+        });
+    } else if (warp < 6) {
+        // ---- a page's tiles, by 128 threads
+        const int tid = threadIdx.x - 64;
+        int       j = 0, st = 0;
+        uint32_t  ph = 0;
+        items([&](ka_seq q, const ka_place & at, int rows, int pages) {
+            for (int i = 0; i < pages; i++, j++) {
+                const uint8_t * rec = raw + st * C::REC, * vr = rec + kv4_half(D);
+                const bool edge = edge_of(q, at, rows, (at.first + at.p + i) * KV4_P);
+                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_rf + 8 * st, ph, abort_s) && dt_mbar_wait(bar_ke + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_s))) return false;
+                const bool in = raw_in[st] != 0;
+                {   // keys: a thread has 32 channels (two times) of one key; of a group's four words the lanes start with different ones, for the banks
+                    uint8_t * to = sK + (j & 1) * C::K_TILE;
+                    const int key = tid & 63, half = tid >> 6;
+#pragma unroll
+                    for (int x = 0; x < C::W / 2; x++) {
+                        const int     cc = D == 128 ? (2 * half + x + (key >> 1)) & 3 : half;
+                        const uint4   n = *reinterpret_cast<const uint4 *>(rec + key * (D / 2) + cc * 16);
+                        const __half2 dm = *reinterpret_cast<const __half2 *>(rec + kv4_steps(D) + (key * C::W + cc) * 4);
+                        const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
+                        const uint32_t wv[4] = { n.x, n.y, n.z, n.w };
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            uint32_t o[4];
+                            kv4_pairs(wv[w], d2, m2, o);
+                            *reinterpret_cast<uint4 *>(to + (cc >> 1) * C::K_CHUNK + key * 128 + ((((cc & 1) * 4 + w) ^ (key & 7)) << 4)) = in ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    dt_fence_async();
+                    __syncwarp();
+                    if (lane == 0) dt_arrive(bar_kf + 8 * (j & 1));
+                }
+                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ve + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_s))) return false;
+                {   // values: a thread has eight keys (an octet, a piece of 16 bytes in the turned tile) of eight (heads of 64: four) neighbouring channels
+                    uint8_t * to = sV + (j & 1) * C::V_TILE;
+                    const int oct = tid & 7, o8 = D == 128 ? ((tid >> 5) * 4 + (lane >> 3) + 2 * oct) & 15 : (tid >> 3) & 7;
+                    uint32_t n[8];
+                    __half2  dm[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int r = kv4_row(oct * 8 + k);
+                        n[k]  = *reinterpret_cast<const uint32_t *>(vr + r * (D / 2) + ((o8 * 4) ^ kv4_flip(D, r)));
+                        dm[k] = *reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (r * C::W + (o8 >> 2)) * 4);
+                    }
+                    if (edge) {
+                        // values that are none, on a page of which some row does not see all: they take part as zeros, and the rows that see one are told
+                        if (tid < C::W) {
+                            unsigned long long none = 0;
+                            for (int k = 0; k < KV4_P; k++)
+                                if (in && __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (kv4_row(k) * C::W + tid) * 4)))) none |= 1ull << k;
+                            v_none[(j & 1) * C::W + tid] = none;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; k++) if (__hisnan(__high2half(dm[k]))) dm[k] = kv4_bits(0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (D == 64 && e != tid >> 6) continue;
+                        uint32_t v[4][4];
+#pragma unroll
+                        for (int a = 0; a < 4; a++) kv4_pairs(ka_prmt(n[2 * a], n[2 * a + 1], e ? 0x7632 : 0x5410), __lows2half2(dm[2 * a], dm[2 * a + 1]), __highs2half2(dm[2 * a], dm[2 * a + 1]), v[a]);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int row = o8 * 8 + e * 4 + c;
+                            *reinterpret_cast<uint4 *>(to + row * 128 + ((oct ^ (row & 7)) << 4)) = in ? make_uint4(v[0][c], v[1][c], v[2][c], v[3][c]) : make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    dt_fence_async();
+                    __syncwarp();
+                    if (lane == 0) { dt_arrive(bar_vf + 8 * (j & 1)); dt_arrive(bar_re + 8 * st); }
+                }
+                if (++st == C::RAW) { st = 0; ph ^= 1; }
+            }
+            return true;
+        });
+    } else {
+        // ---- a row a thread
+        const int w = (warp - 6) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
+        const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s = tmem + lanes + 64 * w, tm_pw = tm_p + lanes + 64 * w, tm_w = tm_o + lanes + 128 * w;
+        int j = 0, n = 0;                                        // pages of the run, and those of which this group has scores
+        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
+        items([&](ka_seq q, const ka_place & at, int rows, int pages) {
+            const int     row0 = at.r * KP_ROWS, ri = w * 128 + rt, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, hi = q.len - q.n + tk, lo = A.window > 0 ? max(0, hi - A.window + 1) : 0;
+            const int64_t tok = min(max(A.starts[at.s], 0), A.tokens) + tk, head = at.h * A.rep + rc % A.rep;
+            const bool    on = w == 0 || rows > 128;
+            if (!on) { j += pages; return true; }
+            float qs = 1.f;
+            {
+                // the row over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them
+                const T * p = (const T *) A.q + tok * A.ldq + head * D;
+                float top = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float v[32];
+                    ka_load<T, 32>(p + c, A.wide_q, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) top = fmaxf(top, fabsf(v[i]));
+                }
+                const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+                const float down = A.scale == 0.f ? 0.f : copysignf(__uint_as_float((254u - e) << 23), A.scale);
+                qs = A.scale == 0.f ? 1.f : fminf(fmaxf(__uint_as_float(e << 23) * fabsf(A.scale * KA_LOG2E), 1.2e-38f), 3e38f);
+                uint8_t * to = sQ + w * C::NC * C::Q_CHUNK + rt * 128;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float v[32];
+                    ka_load<T, 32>(p + c, A.wide_q, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] *= down;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at16 = (c >> 6) * C::Q_CHUNK + (((((c & 63) >> 3) + i) ^ (rt & 7)) << 4);
+                        const float * x = v + 8 * i;
+                        const uint4 h = make_uint4(ka_pack(x[0], x[4]), ka_pack(x[1], x[5]), ka_pack(x[2], x[6]), ka_pack(x[3], x[7]));
+                        *reinterpret_cast<uint4 *>(to + at16) = h;
+                        if (C::SPLIT)
+                            *reinterpret_cast<uint4 *>(to + C::Q_PART + at16) = make_uint4(ka_rest(x[0], x[4], h.x), ka_rest(x[1], x[5], h.y), ka_rest(x[2], x[6], h.z), ka_rest(x[3], x[7], h.w));
+                    }
+                }
+                dt_fence_async();
+            }
+            __syncwarp();
+            if (lane == 0) dt_arrive(bar_q + 8 * w);
+            float    m = -INFINITY, l = 0.f, l2 = 0.f;
+            int      ids = 0;
+            uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
+            for (int i = 0; i < pages; i++, j++, n++) {
+                const int key0 = (at.first + at.p + i) * KV4_P;
+                if ((i & 31) == 0) ids = at.first + at.p + i + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + at.first + at.p + i + lane] : -1;
+                const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
+                const bool in = id >= 0 && id < A.pages;
+                if (!wait(bar_s + 8 * w, n)) return false;
+                dt_fence_after();
+                float t[64];
+                dt_ld32(tm_s, reinterpret_cast<uint32_t *>(t));
+                dt_ld32(tm_s + 32, reinterpret_cast<uint32_t *>(t) + 32);
+                dt_wait_ld();
+                dt_fence_before();
+                __syncwarp();
+                if (lane == 0) dt_arrive(bar_r + 8 * w);
+                if (!in) {
+#pragma unroll
+                    for (int x = 0; x < 64; x++) t[x] = -INFINITY;
+                } else if (edge_of(q, at, rows, key0)) {
+                    const int a = lo - key0, b = hi - key0;
+#pragma unroll
+                    for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = -INFINITY;
+                    if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
+                    if (b >= 0 && a < 64) {
+                        const unsigned long long seen = (b >= 63 ? ~0ull : (1ull << (b + 1)) - 1) & ~(a > 0 ? (1ull << a) - 1 : 0ull);
+#pragma unroll
+                        for (int g = 0; g < C::W; g++) if (v_none[(j & 1) * C::W + g] & seen) none |= 1u << g;
+                    }
+                }
+                float top = t[0];
+#pragma unroll
+                for (int x = 1; x < 64; x++) top = fmaxf(top, t[x]);
+                top = __fmul_rn(top, qs);
+                const bool grow = top > m + KA_LAZY;
+                const bool rescale = __any_sync(0xffffffffu, grow);
+                float f = 1.f;
+                if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; }
+                const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
+                if (i > 0) {                                     // the group's product before has read its weights and left the accumulator
+                    if (!wait(bar_o + 8 * w, n + 1)) return false;
+                    dt_fence_after();
+                    if (rescale) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t v[32];
+                            dt_ld32(tm_w + c, v);
+                            dt_wait_ld();
+#pragma unroll
+                            for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+                            dt_st32(tm_w + c, v);
+                        }
+                        dt_wait_st();
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t h[16], r[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        // (product and sum rounded one by one, as the maximum's product is)
+                        const float a = ka_exp2(__fadd_rn(__fmul_rn(t[32 * c + 2 * x], qs), base)), b = ka_exp2(__fadd_rn(__fmul_rn(t[32 * c + 2 * x + 1], qs), base));
+                        l += a; l2 += b;
+                        h[x] = ka_pack(a, b);
+                        if (C::SPLIT) r[x] = ka_rest(a, b, h[x]);
+                    }
+                    kp_st16(tm_pw + 16 * c, h);
+                    if (C::SPLIT) kp_st16(tm_pw + 32 + 16 * c, r);
+                }
+                dt_wait_st();
+                dt_fence_before();
+                __syncwarp();
+                if (lane == 0) dt_arrive(bar_p + 8 * w);
+            }
+            // ---- the row out
+            if (!wait(bar_o + 8 * w, n + 1)) return false;
+            dt_fence_after();
+            const bool    whole = at.p == 0 && pages == at.np;
+            const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
+            float *       piece = A.pieces + (2 * me + (at.p > 0 ? 0 : 1)) * (int64_t) C::PIECE;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float v[32];
+                dt_ld32(tm_w + c, reinterpret_cast<uint32_t *>(v));
+                dt_wait_ld();
+                if (ri >= rows) continue;
+                const float k = none >> (c >> 5) & 1 ? __uint_as_float(0x7fc00000u) : whole ? inv : 1.f;
+#pragma unroll
+                for (int x = 0; x < 32; x++) v[x] *= k;
+                if (whole) ka_store<T, 32>((T *) A.out + tok * A.ldo + head * D + c, A.wide_o, v);
+                else       ka_store<float, 32>(piece + ri * D + c, true, v);
+            }
+            if (!whole && ri < rows) { piece[KP_ROWS * D + ri] = m; piece[KP_ROWS * D + KP_ROWS + ri] = sum; }
+            dt_fence_before();
+            return true;
+        });
+    }
+    __syncwarp();
+    dt_fence_before();
+    __syncthreads();
+    if (*abort_s) {
+        // a wait ran out: say so, give copies and MMAs still in flight time to land (bounded), then free the tensor memory
+        if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Blocks (run, eighth of the rows): an item that begins in the run and does not end there gets its pieces' sum, a row a warp, lanes the channels.
+template <typename T, int D>
+static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __grid_constant__ ka_args A) {
+    using C = kp_cfg<T, D>;
+    pib_pdl_wait();
+    pib_pdl_trigger();
+    const int     lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t runs = A.plan->runs, wa = blockIdx.x;
+    if (wa + 1 >= runs) return;
+    const int64_t * prefix = A.plan->prefix;
+    const int64_t U = prefix[A.seqs], u0 = U * wa / runs, u1 = U * (wa + 1) / runs;
+    auto seq_of = [&](int s) { return ka_load_seq(A, s); };
+    const ka_place at = ka_find<KP_ROWS>(A, prefix, seq_of, u1 - 1);
+    const int64_t  ib = u1 - 1 - at.p, ie = ib + at.np;
+    if (ib < u0 || ie <= u1) return;
+    const ka_seq  q = seq_of(at.s);
+    const int     row0 = at.r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
+    const int64_t wb = (ie * runs + U - 1) / U - 1, tok0 = min(max(A.starts[at.s], 0), A.tokens);
+    constexpr int CH = D / 32;
+    for (int ri = blockIdx.y * 32 + warp; ri < min(rows, (int) blockIdx.y * 32 + 32); ri += 8) {
+        float m = -INFINITY, l = 0.f, o[CH];
+#pragma unroll
+        for (int c = 0; c < CH; c++) o[c] = 0.f;
+        auto piece = [&](int64_t w) { return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
+        for (int64_t w0 = wa; w0 <= wb; w0 += 32) {
+            const int n = (int) min((int64_t) 32, wb - w0 + 1);
+            float pm = -INFINITY, pl = 0.f;
+            if (lane < n) { pm = piece(w0 + lane)[KP_ROWS * D + ri]; pl = piece(w0 + lane)[KP_ROWS * D + KP_ROWS + ri]; }
+            const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
+            m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
+#pragma unroll
+            for (int c = 0; c < CH; c++) o[c] *= a;
+#pragma unroll 4
+            for (int k = 0; k < n; k++) {
+                const float * p = piece(w0 + k) + ri * D;
+                const float   fk = __shfl_sync(0xffffffffu, f, k);
+                if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
+                else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
+            }
+        }
+        const int rc = row0 + ri;
+        T * out = (T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + lane * CH;
+        const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+        for (int c = 0; c < CH; c++) out[c] = (T) (o[c] * inv);
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------------
+template <typename T, int D> static int kp_go(const ka_args & A, cudaStream_t st) {
+    using C = kp_cfg<T, D>;
+    const size_t smem = C::FIXED + (size_t) (A.seqs + 1) * 8, most = C::FIXED + (size_t) (PIB_KV4_MAX_SEQS + 1) * 8;
+    static_assert(C::FIXED + (PIB_KV4_MAX_SEQS + 1) * 8 + 256 <= 227 * 1024, "shared memory");
+    static pib_per_device attrs;
+    PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
+    PIB_CHECK(pib_launch(kv4_prompt_kernel<T, D>, dim3((unsigned) pib_num_sms()), dim3(KP_THREADS), smem, st, A));
+    PIB_CHECK(pib_launch(kv4_prompt_join_kernel<T, D>, dim3((unsigned) pib_num_sms(), KP_ROWS / 32), dim3(256), 0, st, A));
+    return PIB_OK;
+}
+int pib_kv4_prompt(ka_args A, bool f32, cudaStream_t st) {
+    if (f32) return A.dim == 64 ? kp_go<float, 64>(A, st) : kp_go<float, 128>(A, st);
+    return A.dim == 64 ? kp_go<__nv_bfloat16, 64>(A, st) : kp_go<__nv_bfloat16, 128>(A, st);
+}

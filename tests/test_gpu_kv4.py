@@ -227,6 +227,13 @@ def test_prompts(torch, pib, t, dim, portions, lens, window, kvh, rep):
 
 
 @pytest.mark.parametrize("t", [F32, BF16])
+def test_many_items_a_block(torch, pib, t):
+    """more blocks of rows than the GPU has SMs, the last one of each portion less than half full"""
+    Case(torch, pib, t, 16, 8, 128, [100, 33, 110, 100, 64], [150, 40, 300, 1000, 64]).check()
+    Case(torch, pib, t, 16, 7, 64, [100, 40, 37, 100, 19], [100, 140, 300, 500, 640], 90).check()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
 def test_long(torch, pib, t):
     Case(torch, pib, t, 2, 8, 128, [1], [70001]).check()
     Case(torch, pib, t, 1, 8, 128, [2, 1, 1], [40000, 9, 20001], 30000).check()
