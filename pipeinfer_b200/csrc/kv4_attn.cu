@@ -49,14 +49,14 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
     pib_pdl_wait();
     pib_pdl_trigger();
 
-    const int64_t U = ka_prefix<C::RT, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
+    const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
     const int64_t warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
     ka_leave_plan<C::WARPS * 32>(A, prefix, warps);
     auto seq_of = [&](int s) { return seq[s]; };
     bool ok = true;
     if (me < warps) {
         const int64_t u0 = U * me / warps, u1 = U * (me + 1) / warps;
-        ka_place at = ka_find<C::RT>(A, prefix, seq_of, u0);
+        ka_place at = ka_find<C::RT, 0>(A, prefix, seq_of, u0);
         // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
         ka_place is = at;
         int64_t  iu = u0;
@@ -81,7 +81,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
             }
             there = in ? there | 1u << ist : there & ~(1u << ist);
             if (++ist == NST) ist = 0;
-            if (ihalf) { iu++; if (iu < u1) ka_next<C::RT>(A, prefix, seq_of, is); }
+            if (ihalf) { iu++; if (iu < u1) ka_next<C::RT, 0>(A, prefix, seq_of, is); }
             ihalf ^= 1;
         };
         for (int i = 0; i < NST; i++) issue();
@@ -341,7 +341,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                 }
             u += pages;
             at.p += pages - 1;
-            if (u < u1) ka_next<C::RT>(A, prefix, seq_of, at);
+            if (u < u1) ka_next<C::RT, 0>(A, prefix, seq_of, at);
         }
     }
     __syncthreads();

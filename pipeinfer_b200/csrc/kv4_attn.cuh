@@ -78,34 +78,36 @@ template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_
 // what both kernels know of the work: behind the pieces in the scratch
 struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // runs of units; units in front of each sequence
 
-// A place among the units: page p of np from `first` on, of head h, of tile r, of sequence s.  prefix: units in front of each sequence; seq(s): its tokens and keys
+// A place among the units: unit p of np, page first + p - LEAD, of head h, of tile r, of sequence s.  prefix: units in front of each sequence; seq(s): its tokens and keys.  An item has LEAD units in front
+// of its pages: what its start and end cost, in pages
 struct ka_place { int s, r, h, p, np, first; };
-template <int RT, typename Seq> __device__ __forceinline__ void ka_enter(const ka_args & A, const Seq & seq, ka_place & c) { c.np = ka_pages<RT>(A, seq(c.s), c.r, c.first); }
+template <int RT, int LEAD> __device__ __forceinline__ int ka_units(const ka_args & A, ka_seq q, int r, int & first) { const int n = ka_pages<RT>(A, q, r, first); return n ? n + LEAD : 0; }
+template <int RT, int LEAD, typename Seq> __device__ __forceinline__ void ka_enter(const ka_args & A, const Seq & seq, ka_place & c) { c.np = ka_units<RT, LEAD>(A, seq(c.s), c.r, c.first); }
 // only called where there is a next unit
-template <int RT, typename Seq> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, const Seq & seq, ka_place & c) {
+template <int RT, int LEAD, typename Seq> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, const Seq & seq, ka_place & c) {
     if (++c.p < c.np) return;
     c.p = 0;
     if (++c.h < A.kvh) return;
     c.h = 0;
     do {
         if (++c.r >= ka_tiles<RT>(A, seq(c.s))) { c.r = 0; do c.s++; while (prefix[c.s + 1] == prefix[c.s]); }
-        ka_enter<RT>(A, seq, c);
+        ka_enter<RT, LEAD>(A, seq, c);
     } while (c.np == 0);
 }
 // unit u < prefix[seqs]
-template <int RT, typename Seq> __device__ __forceinline__ ka_place ka_find(const ka_args & A, const int64_t * prefix, const Seq & seq, int64_t u) {
+template <int RT, int LEAD, typename Seq> __device__ __forceinline__ ka_place ka_find(const ka_args & A, const int64_t * prefix, const Seq & seq, int64_t u) {
     int lo = 0, hi = A.seqs;                                     // the last sequence with prefix <= u: it has units
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= u) lo = mid; else hi = mid; }
     int64_t  rest = u - prefix[lo];
     ka_place c;
     c.s = lo; c.r = 0;
-    for (ka_enter<RT>(A, seq, c); rest >= (int64_t) c.np * A.kvh; ka_enter<RT>(A, seq, c)) { rest -= (int64_t) c.np * A.kvh; c.r++; }
+    for (ka_enter<RT, LEAD>(A, seq, c); rest >= (int64_t) c.np * A.kvh; ka_enter<RT, LEAD>(A, seq, c)) { rest -= (int64_t) c.np * A.kvh; c.r++; }
     c.h = (int) (rest / c.np); c.p = (int) (rest % c.np);
     return c;
 }
 // Units in front of each sequence, by all THREADS threads of a block: a thread's neighbouring sequences, then warps, then the block.  part: THREADS / 32 numbers.  Ends with a barrier; the first block leaves
 // them in the plan
-template <int RT, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, const Keep & keep) {
+template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, const Keep & keep) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (A.seqs + THREADS - 1) / THREADS, s0 = threadIdx.x * per;
     int64_t sum = 0;
     for (int s = s0; s < min(s0 + per, A.seqs); s++) {
@@ -113,7 +115,7 @@ template <int RT, int THREADS, typename Keep> __device__ __forceinline__ int64_t
         keep(s, q);
         prefix[s] = sum;
         int first;
-        for (int r = 0; r < ka_tiles<RT>(A, q); r++) sum += (int64_t) ka_pages<RT>(A, q, r, first) * A.kvh;
+        for (int r = 0; r < ka_tiles<RT>(A, q); r++) sum += (int64_t) ka_units<RT, LEAD>(A, q, r, first) * A.kvh;
     }
     int64_t before = sum;
 #pragma unroll

@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #define KP_THREADS 448
+#define KP_LEAD    3           // an item's start and end, in pages
 #define KP_BARS    32
 
 template <typename T, int D> struct kp_cfg {
@@ -38,6 +39,30 @@ __device__ __forceinline__ void kp_st16(uint32_t taddr, const uint32_t * v) {
 }
 // fp16 x fp16, fp32 accumulators, both K-major, M x N outputs
 __host__ __device__ constexpr uint32_t kp_idesc(int M, int N) { return (1u << 4) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
+
+// N neighbouring values of a row in registers
+template <typename T, int N> struct kp_row {
+    uint32_t r[N * sizeof(T) / 4];
+    __device__ __forceinline__ void load(const T * p, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < (int) (N * sizeof(T) / 16); i++) { const uint4 f = reinterpret_cast<const uint4 *>(p)[i]; r[4 * i] = f.x; r[4 * i + 1] = f.y; r[4 * i + 2] = f.z; r[4 * i + 3] = f.w; }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; i++) r[i] = __float_as_uint(p[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) r[i] = (uint32_t) __bfloat16_as_ushort(p[2 * i]) | (uint32_t) __bfloat16_as_ushort(p[2 * i + 1]) << 16;
+        }
+    }
+    __device__ __forceinline__ float at(int i) const { return sizeof(T) == 4 ? __uint_as_float(r[i]) : __uint_as_float(i & 1 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16); }
+    __device__ __forceinline__ float top() const {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) m = fmaxf(m, fabsf(at(i)));
+        return m;
+    }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_constant__ ka_args A) {
@@ -73,7 +98,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     pib_pdl_wait();
     pib_pdl_trigger();
     dt_fence_before();
-    const int64_t U = ka_prefix<KP_ROWS, KP_THREADS>(A, prefix, part, [](int, ka_seq) {});
+    const int64_t U = ka_prefix<KP_ROWS, KP_LEAD, KP_THREADS>(A, prefix, part, [](int, ka_seq) {});
     dt_fence_after();
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
@@ -94,17 +119,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         }
     }
     const int64_t u0 = me < runs ? U * me / runs : 0, u1 = me < runs ? U * (me + 1) / runs : 0;
-    // every role walks the same items of the run: f(tokens and keys, place, rows, pages of it) until it says no
+    // every role walks the same items of the run: f(tokens and keys, place, rows, first of its pages, pages) until it says no
     auto items = [&](auto f) {
         if (u0 >= u1) return;
-        ka_place at = ka_find<KP_ROWS>(A, prefix, seq_of, u0);
+        ka_place at = ka_find<KP_ROWS, KP_LEAD>(A, prefix, seq_of, u0);
         for (int64_t u = u0; u < u1;) {
             const ka_seq q = seq_of(at.s);
-            const int    rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - (int64_t) at.r * KP_ROWS), pages = (int) min((int64_t) (at.np - at.p), u1 - u);
-            if (!f(q, at, rows, pages)) return;
-            u += pages;
-            at.p += pages - 1;
-            if (u < u1) ka_next<KP_ROWS>(A, prefix, seq_of, at);
+            const int    rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - (int64_t) at.r * KP_ROWS), units = (int) min((int64_t) (at.np - at.p), u1 - u);
+            const int    p0 = max(at.p - KP_LEAD, 0), pages = at.p + units - KP_LEAD - p0;
+            if (pages > 0 && !f(q, at, rows, p0, pages)) return;
+            u += units;
+            at.p += units - 1;
+            if (u < u1) ka_next<KP_ROWS, KP_LEAD>(A, prefix, seq_of, at);
         }
     };
     // whether some row of the item does not see all of a page
@@ -116,10 +142,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     if (warp == 0) {
         int st = 0;
         uint32_t ph = 1;                                         // the first round finds its places free
-        items([&](ka_seq, const ka_place & at, int, int pages) {
+        items([&](ka_seq, const ka_place & at, int, int p0, int pages) {
             int ids = 0;
             for (int i = 0; i < pages; i++) {
-                const int pg = at.first + at.p + i;
+                const int pg = at.first + p0 + i;
                 if ((i & 31) == 0) ids = pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1;
                 const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool in = id >= 0 && id < A.pages;
@@ -163,7 +189,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             dt_commit(bar_ke + 8 * (jj & 1));
             return true;
         };
-        items([&](ka_seq, const ka_place &, int rows, int pages) {
+        items([&](ka_seq, const ka_place &, int rows, int, int pages) {
             const int groups = rows > 128 ? 2 : 1;
             for (int w = 0; w < groups; w++) if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
             if (!scores(j, groups)) return false;
@@ -191,10 +217,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         const int tid = threadIdx.x - 64;
         int       j = 0, st = 0;
         uint32_t  ph = 0;
-        items([&](ka_seq q, const ka_place & at, int rows, int pages) {
+        items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
             for (int i = 0; i < pages; i++, j++) {
                 const uint8_t * rec = raw + st * C::REC, * vr = rec + kv4_half(D);
-                const bool edge = edge_of(q, at, rows, (at.first + at.p + i) * KV4_P);
+                const bool edge = edge_of(q, at, rows, (at.first + p0 + i) * KV4_P);
                 if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_rf + 8 * st, ph, abort_s) && dt_mbar_wait(bar_ke + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_s))) return false;
                 const bool in = raw_in[st] != 0;
                 {   // keys: a thread has 32 channels (two times) of one key; of a group's four words the lanes start with different ones, for the banks
@@ -267,37 +293,33 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s = tmem + lanes + 64 * w, tm_pw = tm_p + lanes + 64 * w, tm_w = tm_o + lanes + 128 * w;
         int j = 0, n = 0;                                        // pages of the run, and those of which this group has scores
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
-        items([&](ka_seq q, const ka_place & at, int rows, int pages) {
+        items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
             const int     row0 = at.r * KP_ROWS, ri = w * 128 + rt, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, hi = q.len - q.n + tk, lo = A.window > 0 ? max(0, hi - A.window + 1) : 0;
             const int64_t tok = min(max(A.starts[at.s], 0), A.tokens) + tk, head = at.h * A.rep + rc % A.rep;
             const bool    on = w == 0 || rows > 128;
             if (!on) { j += pages; return true; }
-            float qs = 1.f;
+            float qs;
             {
-                // the row over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them
+                // the row over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
                 const T * p = (const T *) A.q + tok * A.ldq + head * D;
+                constexpr int N = C::SPLIT ? 32 : D;
+                kp_row<T, N> v;
                 float top = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float v[32];
-                    ka_load<T, 32>(p + c, A.wide_q, v);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) top = fmaxf(top, fabsf(v[i]));
-                }
+                for (int c = 0; c < D; c += N) { v.load(p + c, A.wide_q); top = fmaxf(top, v.top()); }
                 const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
                 const float down = A.scale == 0.f ? 0.f : copysignf(__uint_as_float((254u - e) << 23), A.scale);
                 qs = A.scale == 0.f ? 1.f : fminf(fmaxf(__uint_as_float(e << 23) * fabsf(A.scale * KA_LOG2E), 1.2e-38f), 3e38f);
                 uint8_t * to = sQ + w * C::NC * C::Q_CHUNK + rt * 128;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float v[32];
-                    ka_load<T, 32>(p + c, A.wide_q, v);
+                for (int c = 0; c < D; c += N) {
+                    if (N < D) v.load(p + c, A.wide_q);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] *= down;
+                    for (int i = 0; i < N / 8; i++) {
+                        const int at16 = (N < D ? c >> 6 : i >> 3) * C::Q_CHUNK + (((N < D ? ((c & 63) >> 3) + i : i & 7) ^ (rt & 7)) << 4);
+                        float x[8];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int at16 = (c >> 6) * C::Q_CHUNK + (((((c & 63) >> 3) + i) ^ (rt & 7)) << 4);
-                        const float * x = v + 8 * i;
+                        for (int k = 0; k < 8; k++) x[k] = v.at(8 * i + k) * down;
                         const uint4 h = make_uint4(ka_pack(x[0], x[4]), ka_pack(x[1], x[5]), ka_pack(x[2], x[6]), ka_pack(x[3], x[7]));
                         *reinterpret_cast<uint4 *>(to + at16) = h;
                         if (C::SPLIT)
@@ -312,36 +334,43 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             int      ids = 0;
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
             for (int i = 0; i < pages; i++, j++, n++) {
-                const int key0 = (at.first + at.p + i) * KV4_P;
-                if ((i & 31) == 0) ids = at.first + at.p + i + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + at.first + at.p + i + lane] : -1;
+                const int key0 = (at.first + p0 + i) * KV4_P;
+                if ((i & 31) == 0) ids = at.first + p0 + i + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + at.first + p0 + i + lane] : -1;
                 const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool in = id >= 0 && id < A.pages;
                 if (!wait(bar_s + 8 * w, n)) return false;
                 dt_fence_after();
-                float t[64];
-                dt_ld32(tm_s, reinterpret_cast<uint32_t *>(t));
-                dt_ld32(tm_s + 32, reinterpret_cast<uint32_t *>(t) + 32);
-                dt_wait_ld();
-                dt_fence_before();
-                __syncwarp();
-                if (lane == 0) dt_arrive(bar_r + 8 * w);
-                if (!in) {
+                // (32 scores at a time, read twice: 64 in registers, and the code for them, cost more than the second reading)
+                if (!in || edge_of(q, at, rows, key0)) {
+                    const int a = in ? lo - key0 : 64, b = hi - key0;
+#pragma unroll 1
+                    for (int c = 0; c < 64; c += 32) {
+                        uint32_t t[32];
+                        dt_ld32(tm_s + c, t);
+                        dt_wait_ld();
 #pragma unroll
-                    for (int x = 0; x < 64; x++) t[x] = -INFINITY;
-                } else if (edge_of(q, at, rows, key0)) {
-                    const int a = lo - key0, b = hi - key0;
+                        for (int x = 0; x < 32; x++) if (c + x < a || c + x > b) t[x] = 0xff800000u;
+                        dt_st32(tm_s + c, t);
+                    }
+                    dt_wait_st();
+                    if (in) {
+                        if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
+                        if (b >= 0 && a < 64) {
+                            const unsigned long long seen = (b >= 63 ? ~0ull : (1ull << (b + 1)) - 1) & ~(a > 0 ? (1ull << a) - 1 : 0ull);
 #pragma unroll
-                    for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = -INFINITY;
-                    if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
-                    if (b >= 0 && a < 64) {
-                        const unsigned long long seen = (b >= 63 ? ~0ull : (1ull << (b + 1)) - 1) & ~(a > 0 ? (1ull << a) - 1 : 0ull);
-#pragma unroll
-                        for (int g = 0; g < C::W; g++) if (v_none[(j & 1) * C::W + g] & seen) none |= 1u << g;
+                            for (int g = 0; g < C::W; g++) if (v_none[(j & 1) * C::W + g] & seen) none |= 1u << g;
+                        }
                     }
                 }
-                float top = t[0];
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 32) {
+                    uint32_t t[32];
+                    dt_ld32(tm_s + c, t);
+                    dt_wait_ld();
 #pragma unroll
-                for (int x = 1; x < 64; x++) top = fmaxf(top, t[x]);
+                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(t[x]));
+                }
                 top = __fmul_rn(top, qs);
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
@@ -361,16 +390,22 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                             for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
                             dt_st32(tm_w + c, v);
                         }
-                        dt_wait_st();
                     }
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 2; c++) {
-                    uint32_t h[16], r[16];
+                    uint32_t t[32], h[16], r[16];
+                    dt_ld32(tm_s + 32 * c, t);
+                    dt_wait_ld();
+                    if (c == 1) {                                // the scores have been read
+                        dt_fence_before();
+                        __syncwarp();
+                        if (lane == 0) dt_arrive(bar_r + 8 * w);
+                    }
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
                         // (product and sum rounded one by one, as the maximum's product is)
-                        const float a = ka_exp2(__fadd_rn(__fmul_rn(t[32 * c + 2 * x], qs), base)), b = ka_exp2(__fadd_rn(__fmul_rn(t[32 * c + 2 * x + 1], qs), base));
+                        const float a = ka_exp2(__fadd_rn(__fmul_rn(__uint_as_float(t[2 * x]), qs), base)), b = ka_exp2(__fadd_rn(__fmul_rn(__uint_as_float(t[2 * x + 1]), qs), base));
                         l += a; l2 += b;
                         h[x] = ka_pack(a, b);
                         if (C::SPLIT) r[x] = ka_rest(a, b, h[x]);
@@ -386,9 +421,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             // ---- the row out
             if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
-            const bool    whole = at.p == 0 && pages == at.np;
+            const bool    whole = p0 == 0 && pages == at.np - KP_LEAD;
             const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
-            float *       piece = A.pieces + (2 * me + (at.p > 0 ? 0 : 1)) * (int64_t) C::PIECE;
+            float *       piece = A.pieces + (2 * me + (p0 > 0 ? 0 : 1)) * (int64_t) C::PIECE;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
@@ -418,7 +453,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Blocks (run, eighth of the rows): an item that begins in the run and does not end there gets its pieces' sum, a row a warp, lanes the channels.
+// Blocks (run, eighth of the rows): an item whose pages begin in the run and do not end there gets its pieces' sum, a row a warp, lanes the channels.
 template <typename T, int D>
 static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __grid_constant__ ka_args A) {
     using C = kp_cfg<T, D>;
@@ -430,9 +465,9 @@ static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __gri
     const int64_t * prefix = A.plan->prefix;
     const int64_t U = prefix[A.seqs], u0 = U * wa / runs, u1 = U * (wa + 1) / runs;
     auto seq_of = [&](int s) { return ka_load_seq(A, s); };
-    const ka_place at = ka_find<KP_ROWS>(A, prefix, seq_of, u1 - 1);
-    const int64_t  ib = u1 - 1 - at.p, ie = ib + at.np;
-    if (ib < u0 || ie <= u1) return;
+    const ka_place at = ka_find<KP_ROWS, KP_LEAD>(A, prefix, seq_of, u1 - 1);
+    const int64_t  ib = u1 - 1 - at.p + KP_LEAD, ie = ib - KP_LEAD + at.np;         // its pages' units
+    if (ib < u0 || ib >= u1 || ie <= u1) return;
     const ka_seq  q = seq_of(at.s);
     const int     row0 = at.r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
     const int64_t wb = (ie * runs + U - 1) / U - 1, tok0 = min(max(A.starts[at.s], 0), A.tokens);
