@@ -17,8 +17,8 @@ __device__ __forceinline__ void ka_mma0(float (&c)[4], uint4 a, uint32_t b0, uin
 // sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
 //   scores   mma.m16n8k16, rows as M, eight keys as N: lane (g, t) has 16 or 32 neighbouring channels of key g, one load and one step and lowest value, four of them a product's k
 //   outputs  weights straight from the scores' registers as first operand, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
-// fp32 rows enter as fp16 part and remainder: rows 0..7 of a product's sixteen the parts, 8..15 the remainders, so that a row's sum is the sum of two registers of a lane.  bfloat16 rows are exact in fp16
-// (times a power of two of the row) and take all sixteen; their weights are one fp16 number.
+// fp32 rows enter as fp16 part and remainder: rows 0..7 of a product's sixteen the parts, 8..15 the remainders, so that a row's sum is the sum of two registers of a lane.  bfloat16 rows are
+// one fp16 number, as their weights, and take all sixteen.
 // An item that lies in one warp's run is written at once, pieces of others go to scratch and kv4_join_kernel adds them up, in the order of the keys.
 template <typename T, int D, int MT> struct ka_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
@@ -113,19 +113,17 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                     float v[D / 4], top = 0.f;
                     ka_load<T, D / 4>(p, A.wide_q, v);
 #pragma unroll
-                    for (int c = 0; c < D / 4; c++) top = fmaxf(top, fabsf(v[c]));
+                    for (int c = 0; c < D / 4; c++) { v[c] *= A.scale * KA_LOG2E; top = fmaxf(top, fabsf(v[c])); }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-                    // the scale's sign goes to the queries: what scores are multiplied with is above zero, and -inf stays what it is
-                    const float down = A.scale == 0.f ? 0.f : copysignf(__uint_as_float((254u - e) << 23), A.scale);
-                    qs[mt][nr] = A.scale == 0.f ? 1.f : fminf(fmaxf(__uint_as_float(e << 23) * fabsf(A.scale * KA_LOG2E), 1.2e-38f), 3e38f);
+                    const ka_power pw = ka_power_of(top);
+                    qs[mt][nr] = pw.back;
 #pragma unroll
                     for (int k = 0; k < C::KS; k++)
 #pragma unroll
                         for (int b = 0; b < 2; b++) {            // product k of word k / 2 takes channels 2 (k % 2) + b and four further
                             const int   c = (k >> 1) * 8 + (k & 1) * 2 + b;
-                            const float x = v[c] * down, y = v[c + 4] * down;
+                            const float x = v[c] * pw.down, y = v[c + 4] * pw.down;
                             w[nr][k][b] = ka_pack(x, y);
                             if (C::SPLIT) w[1][k][b] = ka_rest(x, y, w[nr][k][b]);
                         }
@@ -251,7 +249,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
 #pragma unroll
                             for (int j = 0; j < 4; j++) top = fmaxf(top, fmaxf(S[j][mt][nr * 2], S[j][mt][nr * 2 + 1]));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = __fmul_rn(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), qs[mt][nr]);
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * qs[mt][nr];
                             if (__any_sync(0xffffffffu, top > m[mt][nr] + KA_LAZY)) {
                                 const float mn = top > m[mt][nr] + KA_LAZY ? top : m[mt][nr], a = mn == m[mt][nr] ? 1.f : ka_exp2(m[mt][nr] - mn);
                                 m[mt][nr] = mn;
@@ -265,8 +263,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                             const float base = KA_LIFT - (m[mt][nr] == -INFINITY ? 0.f : m[mt][nr]);
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                // (product and sum rounded one by one, as the maximum's product is: of scores beyond 2^24 the difference would be the product's rounding)
-                                const float x = ka_exp2(__fadd_rn(__fmul_rn(S[j][mt][nr * 2], qs[mt][nr]), base)), y = ka_exp2(__fadd_rn(__fmul_rn(S[j][mt][nr * 2 + 1], qs[mt][nr]), base));
+                                const float x = ka_exp2(fmaf(S[j][mt][nr * 2], qs[mt][nr], base)), y = ka_exp2(fmaf(S[j][mt][nr * 2 + 1], qs[mt][nr], base));
                                 l[mt][nr] += x + y;
                                 const uint32_t h = ka_pack(x, y);
                                 uint32_t & at0 = j & 1 ? P[j >> 1][mt].z : P[j >> 1][mt].x, & at1 = j & 1 ? P[j >> 1][mt].w : P[j >> 1][mt].y;

@@ -13,6 +13,13 @@ struct ka_args {
     int stages; float * pieces; struct ka_plan * plan; int * err;
 };
 
+// A row's queries enter times scale log2 e, over the power of two of the largest: what scores are multiplied with is a power of two, exact, and so is the running maximum
+struct ka_power { float down, back; };
+__device__ __forceinline__ ka_power ka_power_of(float top) {
+    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+    return { __uint_as_float((254u - e) << 23), __uint_as_float(e << 23) };
+}
+
 // n neighbouring values as floats, n a multiple of 8
 template <typename T, int N> __device__ __forceinline__ void ka_load(const T * p, bool wide, float (&v)[N]) {
     if constexpr (sizeof(T) == 4) {

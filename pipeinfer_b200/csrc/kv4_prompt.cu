@@ -6,7 +6,7 @@
 //   warps 2..5    write a page's keys [64][dim] and its values, turned, [dim][64] as fp16 into tiles of the 128-byte swizzle, two of each
 //   warp 1        issues the MMAs: scores S = Q K' of the next page, then O += P V of this one, for both groups
 //   warps 6..13   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 back into tensor memory, from where they enter the second product
-// fp32 queries and weights enter as fp16 part and remainder, two products each; bfloat16 queries are exact in fp16 (times a power of two of the row), their weights are one fp16 number.
+// fp32 queries and weights enter as fp16 part and remainder, two products each; of bfloat16 rows both are one fp16 number.
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
 
@@ -77,16 +77,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     volatile unsigned long long * v_none = reinterpret_cast<volatile unsigned long long *>(tmem_slot + 12);      // [2][W] places of a page whose values are none, of each group
     int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 128);       // [seqs + 1]
     __shared__ int64_t part[KP_THREADS / 32];
-    // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there / read, weights written, product done
-    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_r = b0 + 160,
-                   bar_p = b0 + 176, bar_o = b0 + 192;
+    // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there and weights written (of two pages: a group may be one ahead
+    // of the other), product done
+    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_p = b0 + 176, bar_o = b0 + 208;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::RAW; i++) { dt_mbar_init(bar_rf + 8 * i, 1); dt_mbar_init(bar_re + 8 * i, 4); }
         for (int i = 0; i < 2; i++) {
             dt_mbar_init(bar_kf + 8 * i, 4); dt_mbar_init(bar_vf + 8 * i, 4);
-            for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_o }) dt_mbar_init(b + 8 * i, 1);
-            dt_mbar_init(bar_q + 8 * i, 4); dt_mbar_init(bar_r + 8 * i, 4); dt_mbar_init(bar_p + 8 * i, 4);
+            for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_s + 16, bar_o }) dt_mbar_init(b + 8 * i, 1);
+            dt_mbar_init(bar_q + 8 * i, 4); dt_mbar_init(bar_p + 8 * i, 4); dt_mbar_init(bar_p + 16 + 8 * i, 4);
         }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     dt_fence_after();
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
-    const uint32_t tmem = *tmem_slot, tm_p = tmem + 128, tm_o = tmem + 256;          // columns: scores 0..63 and 64..127, weights 128..191 and 192..255 (32 of each part), outputs 256..383 and 384..511
+    const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, for each group; the weights take their scores' place; outputs 256..383 and 384..511
     auto seq_of = [&](int s) { return ka_load_seq(A, s); };
     // rows of tiles without pages
     for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
@@ -164,15 +164,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     } else if (warp == 1) {
         constexpr uint32_t id_s = kp_idesc(128, 64), id_o = kp_idesc(128, D);
         const uint64_t dq = dt_desc(dt_smem(sQ)), dk = dt_desc(dt_smem(sK)), dv = dt_desc(dt_smem(sV));
-        int      j = 0, n_q[2] = { 0, 0 }, n_s[2] = { 0, 0 }, n_p[2] = { 0, 0 };
+        int      j = 0, n_q[2] = { 0, 0 }, n_p[2] = { 0, 0 };
+        uint32_t p_ph[2] = { 0, 0 };                             // the phases of the weights' barriers
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
-        auto scores = [&](int jj, int groups) {
+        auto scores = [&](int jj, int groups, bool behind) {
             if (!wait(bar_kf + 8 * (jj & 1), jj >> 1)) return false;
+            dt_fence_after();
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 if (w >= groups) break;
-                if (!wait(bar_r + 8 * w, n_s[w] + 1)) return false;          // the scores before have been read
-                n_s[w]++;
+                // the weights of two pages ago, which lie there, have entered their product (MMAs of different accumulators may overtake each other)
+                if (behind && !wait(bar_o + 8 * w, n_p[w] + 1)) return false;
                 dt_fence_after();
                 bool acc = false;
 #pragma unroll
@@ -181,10 +183,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     for (int c = 0; c < C::NC; c++)
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            dt_mma(tmem + 64 * w, dq + (uint64_t) ((part_ * C::Q_PART + (w * C::NC + c) * C::Q_CHUNK) >> 4) + 2 * k, dk + (uint64_t) (((jj & 1) * C::K_TILE + c * C::K_CHUNK) >> 4) + 2 * k, id_s, acc);
+                            dt_mma(tmem + 128 * w + 64 * (jj & 1), dq + (uint64_t) ((part_ * C::Q_PART + (w * C::NC + c) * C::Q_CHUNK) >> 4) + 2 * k, dk + (uint64_t) (((jj & 1) * C::K_TILE + c * C::K_CHUNK) >> 4) + 2 * k, id_s, acc);
                             acc = true;
                         }
-                dt_commit(bar_s + 8 * w);
+                dt_commit(bar_s + 16 * w + 8 * (jj & 1));
             }
             dt_commit(bar_ke + 8 * (jj & 1));
             return true;
@@ -192,20 +194,21 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         items([&](ka_seq, const ka_place &, int rows, int, int pages) {
             const int groups = rows > 128 ? 2 : 1;
             for (int w = 0; w < groups; w++) if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
-            if (!scores(j, groups)) return false;
+            if (!scores(j, groups, false)) return false;
             for (int i = 0; i < pages; i++, j++) {
-                if (i + 1 < pages && !scores(j + 1, groups)) return false;
+                if (i + 1 < pages && !scores(j + 1, groups, i > 0)) return false;
                 if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                     if (w >= groups) break;
-                    if (!wait(bar_p + 8 * w, n_p[w])) return false;
+                    if (!wait(bar_p + 16 * w + 8 * (j & 1), p_ph[w] >> (j & 1))) return false;
+                    p_ph[w] ^= 1u << (j & 1);
                     n_p[w]++;
                     dt_fence_after();
 #pragma unroll
                     for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tm_p + 64 * w + 32 * part_ + 8 * k, dv + (uint64_t) ((j & 1) * C::V_TILE >> 4) + 2 * k, id_o, (i > 0) | ((part_ | k) != 0));
+                        for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * (j & 1) + (C::SPLIT ? 32 * (k >> 1) + 16 * part_ + 8 * (k & 1) : 8 * k), dv + (uint64_t) ((j & 1) * C::V_TILE >> 4) + 2 * k, id_o, (i > 0) | ((part_ | k) != 0));
                     dt_commit(bar_o + 8 * w);
                 }
                 dt_commit(bar_ve + 8 * (j & 1));
@@ -290,8 +293,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     } else {
         // ---- a row a thread
         const int w = (warp - 6) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
-        const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s = tmem + lanes + 64 * w, tm_pw = tm_p + lanes + 64 * w, tm_w = tm_o + lanes + 128 * w;
+        const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s0 = tmem + lanes + 128 * w, tm_w = tm_o + lanes + 128 * w;
         int j = 0, n = 0;                                        // pages of the run, and those of which this group has scores
+        uint32_t s_ph = 0;                                       // the phases of both scores' barriers
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
         items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
             const int     row0 = at.r * KP_ROWS, ri = w * 128 + rt, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, hi = q.len - q.n + tk, lo = A.window > 0 ? max(0, hi - A.window + 1) : 0;
@@ -300,16 +304,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             if (!on) { j += pages; return true; }
             float qs;
             {
-                // the row over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
+                // the row times scale log2 e, over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
                 const T * p = (const T *) A.q + tok * A.ldq + head * D;
                 constexpr int N = C::SPLIT ? 32 : D;
                 kp_row<T, N> v;
                 float top = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < D; c += N) { v.load(p + c, A.wide_q); top = fmaxf(top, v.top()); }
-                const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-                const float down = A.scale == 0.f ? 0.f : copysignf(__uint_as_float((254u - e) << 23), A.scale);
-                qs = A.scale == 0.f ? 1.f : fminf(fmaxf(__uint_as_float(e << 23) * fabsf(A.scale * KA_LOG2E), 1.2e-38f), 3e38f);
+                const ka_power pw = ka_power_of(top * fabsf(A.scale * KA_LOG2E));
+                qs = pw.back;
                 uint8_t * to = sQ + w * C::NC * C::Q_CHUNK + rt * 128;
 #pragma unroll 1
                 for (int c = 0; c < D; c += N) {
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         const int at16 = (N < D ? c >> 6 : i >> 3) * C::Q_CHUNK + (((N < D ? ((c & 63) >> 3) + i : i & 7) ^ (rt & 7)) << 4);
                         float x[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] = v.at(8 * i + k) * down;
+                        for (int k = 0; k < 8; k++) x[k] = v.at(8 * i + k) * (A.scale * KA_LOG2E) * pw.down;
                         const uint4 h = make_uint4(ka_pack(x[0], x[4]), ka_pack(x[1], x[5]), ka_pack(x[2], x[6]), ka_pack(x[3], x[7]));
                         *reinterpret_cast<uint4 *>(to + at16) = h;
                         if (C::SPLIT)
@@ -335,10 +338,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
             for (int i = 0; i < pages; i++, j++, n++) {
                 const int key0 = (at.first + p0 + i) * KV4_P;
+                const uint32_t tm_s = tm_s0 + 64 * (j & 1);
                 if ((i & 31) == 0) ids = at.first + p0 + i + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + at.first + p0 + i + lane] : -1;
                 const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool in = id >= 0 && id < A.pages;
-                if (!wait(bar_s + 8 * w, n)) return false;
+                if (!wait(bar_s + 16 * w + 8 * (j & 1), s_ph >> (j & 1))) return false;
+                s_ph ^= 1u << (j & 1);
                 dt_fence_after();
                 // (32 scores at a time, read twice: 64 in registers, and the code for them, cost more than the second reading)
                 if (!in || edge_of(q, at, rows, key0)) {
@@ -371,25 +376,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
 #pragma unroll
                     for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(t[x]));
                 }
-                top = __fmul_rn(top, qs);
+                top *= qs;
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
                 if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
-                if (i > 0) {                                     // the group's product before has read its weights and left the accumulator
-                    if (!wait(bar_o + 8 * w, n + 1)) return false;
+                if (i > 0 && rescale) {
+                    if (!wait(bar_o + 8 * w, n + 1)) return false;           // the product before has left the accumulator
                     dt_fence_after();
-                    if (rescale) {
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t v[32];
-                            dt_ld32(tm_w + c, v);
-                            dt_wait_ld();
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t v[32];
+                        dt_ld32(tm_w + c, v);
+                        dt_wait_ld();
 #pragma unroll
-                            for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
-                            dt_st32(tm_w + c, v);
-                        }
+                        for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+                        dt_st32(tm_w + c, v);
                     }
                 }
 #pragma unroll 1
@@ -397,29 +400,24 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     uint32_t t[32], h[16], r[16];
                     dt_ld32(tm_s + 32 * c, t);
                     dt_wait_ld();
-                    if (c == 1) {                                // the scores have been read
-                        dt_fence_before();
-                        __syncwarp();
-                        if (lane == 0) dt_arrive(bar_r + 8 * w);
-                    }
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
-                        // (product and sum rounded one by one, as the maximum's product is)
-                        const float a = ka_exp2(__fadd_rn(__fmul_rn(__uint_as_float(t[2 * x]), qs), base)), b = ka_exp2(__fadd_rn(__fmul_rn(__uint_as_float(t[2 * x + 1]), qs), base));
+                        const float a = ka_exp2(fmaf(__uint_as_float(t[2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[2 * x + 1]), qs, base));
                         l += a; l2 += b;
                         h[x] = ka_pack(a, b);
                         if (C::SPLIT) r[x] = ka_rest(a, b, h[x]);
                     }
-                    kp_st16(tm_pw + 16 * c, h);
-                    if (C::SPLIT) kp_st16(tm_pw + 32 + 16 * c, r);
+                    // in the place of scores that have been read
+                    kp_st16(tm_s + (C::SPLIT ? 32 : 16) * c, h);
+                    if (C::SPLIT) kp_st16(tm_s + 32 * c + 16, r);
                 }
                 dt_wait_st();
                 dt_fence_before();
                 __syncwarp();
-                if (lane == 0) dt_arrive(bar_p + 8 * w);
+                if (lane == 0) dt_arrive(bar_p + 16 * w + 8 * (j & 1));
             }
-            // ---- the row out
-            if (!wait(bar_o + 8 * w, n + 1)) return false;
+            // ---- the row out, behind the last product (and the one before it, which nothing has waited for: a phase two ahead would look like the one behind)
+            if ((pages > 1 && !wait(bar_o + 8 * w, n)) || !wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
             const bool    whole = p0 == 0 && pages == at.np - KP_LEAD;
             const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
