@@ -3,17 +3,17 @@
 // A block takes 256 rows (token, head of the group) of one key / value head as two groups of 128 and walks the pages they see; pages of all such items lie in one row that the blocks of the GPU (one an
 // SM) divide evenly, whatever the sequences' lengths (kv4_attn.cuh).  An item that lies in one block's run is written at once; pieces of others go to scratch and kv4_prompt_join_kernel adds them up.
 //   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
-//   warps 2..5    write a page's keys [64][dim] and its values, turned, [dim][64] as fp16 into tiles of the 128-byte swizzle, two of each
+//   warps 4..7    write a page's keys [64][dim] and its values, turned, [dim][64] as fp16 into tiles of the 128-byte swizzle, two of each
 //   warp 1        issues the MMAs: scores S = Q K' of the next page, then O += P V of this one, for both groups
-//   warps 6..13   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 back into tensor memory, from where they enter the second product
+//   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 back into tensor memory, from where they enter the second product
 // fp32 queries and weights enter as fp16 part and remainder, two products each; of bfloat16 rows both are one fp16 number.
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
 
 #include <algorithm>
 
-#define KP_THREADS 448
-#define KP_LEAD    3           // an item's start and end, in pages
+#define KP_THREADS 512
+#define KP_LEAD    8           // an item's start and end, in pages
 #define KP_BARS    32
 
 template <typename T, int D> struct kp_cfg {
@@ -103,7 +103,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
     const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, for each group; the weights take their scores' place; outputs 256..383 and 384..511
-    auto seq_of = [&](int s) { return ka_load_seq(A, s); };
+    int    last_s = -1;
+    ka_seq last = { 0, 0 };
+    auto seq_of = [&](int s) {                                   // the tables' entries of the sequence at hand stay in registers
+        if (s != last_s) { last_s = s; last = ka_load_seq(A, s); }
+        return last;
+    };
     // rows of tiles without pages
     for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
         const ka_seq  q = seq_of(s);
@@ -139,6 +144,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         return key0 < lo || key0 + KV4_P - 1 > hi;
     };
 
+    // registers go where the rows are: 512 x 128 at launch, 128 x (96 + 112 + 152 + 152) from here
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 0) {
         int st = 0;
         uint32_t ph = 1;                                         // the first round finds its places free
@@ -215,9 +223,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             }
             return true;
         });
-    } else if (warp < 6) {
+    }
+    } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         // ---- a page's tiles, by 128 threads
-        const int tid = threadIdx.x - 64;
+        const int tid = threadIdx.x - 128;
         int       j = 0, st = 0;
         uint32_t  ph = 0;
         items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
@@ -291,8 +301,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             return true;
         });
     } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         // ---- a row a thread
-        const int w = (warp - 6) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
+        const int w = (warp - 8) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
         const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s0 = tmem + lanes + 128 * w, tm_w = tm_o + lanes + 128 * w;
         int j = 0, n = 0;                                        // pages of the run, and those of which this group has scores
         uint32_t s_ph = 0;                                       // the phases of both scores' barriers
@@ -302,6 +313,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             const int64_t tok = min(max(A.starts[at.s], 0), A.tokens) + tk, head = at.h * A.rep + rc % A.rep;
             const bool    on = w == 0 || rows > 128;
             if (!on) { j += pages; return true; }
+            auto some = [&](int pg) { return pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1; };
+            int ids = some(at.first + p0);
             float qs;
             {
                 // the row times scale log2 e, over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
@@ -334,30 +347,24 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             __syncwarp();
             if (lane == 0) dt_arrive(bar_q + 8 * w);
             float    m = -INFINITY, l = 0.f, l2 = 0.f;
-            int      ids = 0;
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
             for (int i = 0; i < pages; i++, j++, n++) {
                 const int key0 = (at.first + p0 + i) * KV4_P;
                 const uint32_t tm_s = tm_s0 + 64 * (j & 1);
-                if ((i & 31) == 0) ids = at.first + p0 + i + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + at.first + p0 + i + lane] : -1;
+                if (i > 0 && (i & 31) == 0) ids = some(at.first + p0 + i);
                 const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool in = id >= 0 && id < A.pages;
                 if (!wait(bar_s + 16 * w + 8 * (j & 1), s_ph >> (j & 1))) return false;
                 s_ph ^= 1u << (j & 1);
                 dt_fence_after();
-                // (32 scores at a time, read twice: 64 in registers, and the code for them, cost more than the second reading)
+                uint32_t t[64];
+                dt_ld32(tm_s, t);
+                dt_ld32(tm_s + 32, t + 32);
+                dt_wait_ld();
                 if (!in || edge_of(q, at, rows, key0)) {
                     const int a = in ? lo - key0 : 64, b = hi - key0;
-#pragma unroll 1
-                    for (int c = 0; c < 64; c += 32) {
-                        uint32_t t[32];
-                        dt_ld32(tm_s + c, t);
-                        dt_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 32; x++) if (c + x < a || c + x > b) t[x] = 0xff800000u;
-                        dt_st32(tm_s + c, t);
-                    }
-                    dt_wait_st();
+                    for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = 0xff800000u;
                     if (in) {
                         if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
                         if (b >= 0 && a < 64) {
@@ -368,14 +375,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     }
                 }
                 float top = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 64; c += 32) {
-                    uint32_t t[32];
-                    dt_ld32(tm_s + c, t);
-                    dt_wait_ld();
 #pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(t[x]));
-                }
+                for (int x = 0; x < 64; x++) top = fmaxf(top, __uint_as_float(t[x]));
                 top *= qs;
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
@@ -395,19 +396,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         dt_st32(tm_w + c, v);
                     }
                 }
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    uint32_t t[32], h[16], r[16];
-                    dt_ld32(tm_s + 32 * c, t);
-                    dt_wait_ld();
+                    uint32_t h[16], r[16];
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
-                        const float a = ka_exp2(fmaf(__uint_as_float(t[2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[2 * x + 1]), qs, base));
+                        const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), qs, base));
                         l += a; l2 += b;
                         h[x] = ka_pack(a, b);
                         if (C::SPLIT) r[x] = ka_rest(a, b, h[x]);
                     }
-                    // in the place of scores that have been read
+                    // in the scores' place
                     kp_st16(tm_s + (C::SPLIT ? 32 : 16) * c, h);
                     if (C::SPLIT) kp_st16(tm_s + 32 * c + 16, r);
                 }
