@@ -1,54 +1,60 @@
-// kv4_attn.cu -- attention of ragged sequences over a key / value cache in 4 bits (kv4.cuh): one pass over the keys with the running maximum and sum.
+// kv4_attn.cu -- attention of ragged sequences over a key / value cache in 4 bits (kv4.cuh): one pass over the keys with the running maximum and sum.  Decode and verification batches; prompts: kv4_prompt.cu.
 #include "kv4_attn.cuh"
 
 #include <algorithm>
 
-__device__ __forceinline__ void ka_mma(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+// c += a b: 16 x 16 by 16 x 8 in fp16, fp32 sums (not volatile: the order is the compiler's)
+__device__ __forceinline__ void ka_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
 // the first product of a sum
-__device__ __forceinline__ void ka_mma0(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void ka_mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "f"(0.f));
 }
-// ---- decode and verification batches --------------------------------------------------------------------------------------------------
-// All (sequence, tile, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum and
-// sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
-//   scores   mma.m16n8k16, rows as M, eight keys as N: lane (g, t) has 16 or 32 neighbouring channels of key g, one load and one step and lowest value, four of them a product's k
-//   outputs  weights straight from the scores' registers as first operand, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
-// fp32 rows enter as fp16 part and remainder: rows 0..7 of a product's sixteen the parts, 8..15 the remainders, so that a row's sum is the sum of two registers of a lane.  bfloat16 rows are
-// one fp16 number, as their weights, and take all sixteen.
+// an 8 x 8 matrix of 16-bit numbers, two of a row a lane, turned
+__device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
+
+// All (sequence, tile of rows, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum
+// and sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
+//   scores   turned, S' = K Q': mma.m16n8k16, 16 keys as M, eight rows as N, keys straight from nibbles in registers: lane (g, t) has 16 or 32 neighbouring channels of keys g and g + 8, one load and one step
+//            and lowest value each, four of them a product's k
+//   outputs  O' = V' P': 16 channels as M, weights (turned once more by movmatrix) as N, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
+// Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  fp32 rows enter as fp16 part and remainder,
+// two products into the same sums; of bfloat16 rows queries and weights are one fp16 number.
 // An item that lies in one warp's run is written at once, pieces of others go to scratch and kv4_join_kernel adds them up, in the order of the keys.
-template <typename T, int D, int MT> struct ka_cfg {
+// warps of a block, by the registers that a warp's tile takes, and the shared memory of fp32 queries' operands
+__host__ __device__ constexpr int ka_warps(bool split, int nr) { return nr == 1 ? 16 : nr == 2 && !split ? 12 : 8; }
+template <typename T, int D, int NR> struct ka_cfg {                 // NR: tiles of eight rows
     static constexpr bool SPLIT = sizeof(T) == 4;
-    static constexpr int  RPM = SPLIT ? 8 : 16, RT = MT * RPM, NR = SPLIT ? 1 : 2, KS = D / 16, W = D / 32, NT = D / 8;
-    static constexpr int  WARPS = 8;
-    static constexpr bool QS = MT * KS >= 8;                       // the queries' operands lie in shared memory
-    static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * MT * KS * 512 : 0;
-    static constexpr int  PIECE = RT * (D + 2);                   // floats
+    static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
+    static constexpr int  WARPS = ka_warps(SPLIT, NR);
+    static constexpr int  KB = NR == 1 ? 64 : 32;                    // keys of which the scores are in registers at once
+    static constexpr bool QS = NR > 1;                               // the queries' operands lie in shared memory
+    static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
+    static constexpr int  PIECE = RT * (D + 2);                      // floats
 };
 
-template <typename T, int D, int MT>
-static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
-    using C = ka_cfg<T, D, MT>;
+template <typename T, int D, int NR>
+static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
+    using C = ka_cfg<T, D, NR>;
     extern __shared__ __align__(128) uint8_t ka_dsm[];
-    __shared__ uint64_t bars[C::WARPS * 16];
+    __shared__ uint64_t bars[C::WARPS * 8];
     __shared__ int64_t  part[C::WARPS];
     __shared__ int      abort_w;
     volatile int * abort_s = &abort_w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, NST = A.stages;
     uint8_t *  ring = ka_dsm + warp * NST * C::HALF;
-    uint4 *    qsm  = reinterpret_cast<uint4 *>(ka_dsm + C::WARPS * NST * C::HALF) + warp * MT * C::KS * 32 + lane;
+    uint2 *    qsm  = reinterpret_cast<uint2 *>(ka_dsm + C::WARPS * NST * C::HALF) + warp * NR * C::PARTS * C::KS * 32 + lane;
     int64_t *  prefix = reinterpret_cast<int64_t *>(ka_dsm + C::WARPS * NST * C::HALF + C::Q_BYTES);         // [seqs + 1]
     ka_seq *   seq  = reinterpret_cast<ka_seq *>(prefix + A.seqs + 1);
-    const uint32_t bar0 = dt_smem(bars + warp * 16), ring0 = dt_smem(ring);
+    const uint32_t bar0 = dt_smem(bars + warp * 8), ring0 = dt_smem(ring);
     if (lane == 0) for (int i = 0; i < NST; i++) dt_mbar_init(bar0 + i * 8, 1);
     if (threadIdx.x == 0) abort_w = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pib_pdl_wait();
     pib_pdl_trigger();
-
     const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
     const int64_t warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
     ka_leave_plan<C::WARPS * 32>(A, prefix, warps);
@@ -59,11 +65,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
         ka_place at = ka_find<C::RT, 0>(A, prefix, seq_of, u0);
         // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
         ka_place is = at;
-        int64_t  iu = u0;
+        int      left = (int) (u1 - u0), todo = left;            // units to ask for, units to do
         int      ihalf = 0, ist = 0, id_s = -1, id_base = 0, ids = 0, id = 0;
         uint32_t there = 0;                                      // of each stage: whether its page is one of the cache's
         auto issue = [&]() {
-            if (iu >= u1) return;
+            if (left == 0) return;
             if (!ihalf) {
                 const int pg = is.first + is.p;
                 if (is.s != id_s || pg < id_base || pg >= id_base + 32) {
@@ -81,66 +87,58 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
             }
             there = in ? there | 1u << ist : there & ~(1u << ist);
             if (++ist == NST) ist = 0;
-            if (ihalf) { iu++; if (iu < u1) ka_next<C::RT, 0>(A, prefix, seq_of, is); }
+            if (ihalf) { left--; if (left) ka_next<C::RT, 0>(A, prefix, seq_of, is); }
             ihalf ^= 1;
         };
         for (int i = 0; i < NST; i++) issue();
 
         int st = 0;
         uint32_t ph = 0;
-        int64_t u = u0;
-        while (u < u1 && ok) {
+        while (todo && ok) {
             // ---- an item, or the piece of it in this warp's run
             const ka_seq  q = seq[at.s];
-            const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = (int) min((int64_t) (at.np - at.p), u1 - u);
+            const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = min(at.np - at.p, todo);
             const bool    whole = at.p == 0 && pages == at.np;
             const int     slot = 2 * (int) me + (at.p > 0 ? 0 : 1);
             const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens);
-            const int     row0 = at.r * C::RT;
-            float qs[MT][C::NR], m[MT][C::NR], l[MT][C::NR], O[MT][C::NT][4];
-            int   lo[MT][C::NR], hi[MT][C::NR];
-            uint4 qf[C::QS ? 1 : MT][C::QS ? 1 : C::KS];
-            int   all_lo = 0, all_hi = 0x7fffffff;               // keys that all rows see
+            const int     row0 = at.r * C::RT, pos0 = q.len - q.n;
+            float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];    // of rows 2 t and 2 t + 1 of each tile
+            uint2 qf[C::QS ? 1 : C::PARTS][C::QS ? 1 : C::KS];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                uint32_t w[2][C::KS][2];                         // [row or part][product][k low, k high]
+            for (int n = 0; n < NR; n++) {
+                // as the products' second operand a lane has row g: the channels of its t
+                const int rc = row0 + min(n * 8 + g, rows - 1), tk = rc / A.rep;
+                const T * p = (const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4);
+                float v[D / 4], top = 0.f;
+                ka_load<T, D / 4>(p, A.wide_q, v);
 #pragma unroll
-                for (int nr = 0; nr < C::NR; nr++) {
-                    const int ri = mt * C::RPM + nr * 8 + g, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, pos = q.len - q.n + tk;
-                    hi[mt][nr] = pos;
-                    lo[mt][nr] = A.window > 0 ? max(0, pos - A.window + 1) : 0;
-                    const T * p = (const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4);
-                    float v[D / 4], top = 0.f;
-                    ka_load<T, D / 4>(p, A.wide_q, v);
+                for (int c = 0; c < D / 4; c++) { v[c] *= A.scale * KA_LOG2E; top = fmaxf(top, fabsf(v[c])); }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const ka_power pw = ka_power_of(top);
 #pragma unroll
-                    for (int c = 0; c < D / 4; c++) { v[c] *= A.scale * KA_LOG2E; top = fmaxf(top, fabsf(v[c])); }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const ka_power pw = ka_power_of(top);
-                    qs[mt][nr] = pw.back;
+                for (int r = 0; r < 2; r++) { qs[n][r] = __shfl_sync(0xffffffffu, pw.back, (2 * t + r) * 4); m[n][r] = -INFINITY; l[n][r] = 0.f; }
 #pragma unroll
-                    for (int k = 0; k < C::KS; k++)
-#pragma unroll
-                        for (int b = 0; b < 2; b++) {            // product k of word k / 2 takes channels 2 (k % 2) + b and four further
-                            const int   c = (k >> 1) * 8 + (k & 1) * 2 + b;
-                            const float x = v[c] * pw.down, y = v[c + 4] * pw.down;
-                            w[nr][k][b] = ka_pack(x, y);
-                            if (C::SPLIT) w[1][k][b] = ka_rest(x, y, w[nr][k][b]);
-                        }
-                    m[mt][nr] = -INFINITY; l[mt][nr] = 0.f;
+                for (int k = 0; k < C::KS; k++) {                // product k of word k / 2 takes channels 2 (k % 2), 2 (k % 2) + 1 and four further
+                    const int   c = (k >> 1) * 8 + (k & 1) * 2;
+                    const float x0 = v[c] * pw.down, x1 = v[c + 4] * pw.down, y0 = v[c + 1] * pw.down, y1 = v[c + 5] * pw.down;
+                    const uint2 hi = make_uint2(ka_pack(x0, x1), ka_pack(y0, y1));
+                    if (C::QS) qsm[(n * C::PARTS * C::KS + k) * 32] = hi; else qf[0][C::QS ? 0 : k] = hi;
+                    if (C::SPLIT) {
+                        const uint2 lo = make_uint2(ka_rest(x0, x1, hi.x), ka_rest(y0, y1, hi.y));
+                        if (C::QS) qsm[((n * C::PARTS + 1) * C::KS + k) * 32] = lo; else qf[C::QS || !C::SPLIT ? 0 : 1][C::QS ? 0 : k] = lo;
+                    }
                 }
 #pragma unroll
-                for (int k = 0; k < C::KS; k++) {
-                    const uint4 f = make_uint4(w[0][k][0], w[1][k][0], w[0][k][1], w[1][k][1]);
-                    if (C::QS) qsm[(mt * C::KS + k) * 32] = f; else qf[C::QS ? 0 : mt][C::QS ? 0 : k] = f;
-                }
+                for (int i = 0; i < C::MT; i++)
 #pragma unroll
-                for (int i = 0; i < C::NT; i++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) O[mt][i][c] = 0.f;
+                    for (int c = 0; c < 4; c++) O[n][i][c] = 0.f;
             }
-            all_hi = q.len - q.n + row0 / A.rep;                                     // the first token's last key, the last token's first one
-            all_lo = A.window > 0 ? q.len - q.n + (row0 + rows - 1) / A.rep - A.window + 1 : 0;
+            // keys that all rows see: from the last token's first one to the first token's last
+            const int all_hi = pos0 + row0 / A.rep, all_lo = A.window > 0 ? pos0 + (row0 + rows - 1) / A.rep - A.window + 1 : 0;
+            // the last key that row r of the tiles sees, and the first
+            auto high = [&](int r) { return pos0 + (row0 + min(r, rows - 1)) / A.rep; };
+            auto low  = [&](int r) { return A.window > 0 ? max(0, high(r) - A.window + 1) : 0; };
 
             for (int i = 0; i < pages && ok; i++) {
                 const int key0 = (at.first + at.p + i) * KV4_P;
@@ -150,7 +148,6 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                 const uint32_t vst = st, vph = ph;
                 if (++st == NST) { st = 0; ph ^= 1; }
                 uint8_t * kp = ring + kst * C::HALF, * vp = ring + vst * C::HALF;
-                const bool edge = key0 < all_lo || key0 + KV4_P - 1 > all_hi;
                 ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + kst * 8, kph, abort_s));
                 if (!ok) break;
                 if (!in) {                                       // no page: nothing was copied
@@ -159,76 +156,74 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                     if (ok) issue();
                     continue;
                 }
+                const bool edge = key0 < all_lo || key0 + KV4_P - 1 > all_hi;
 #pragma unroll 1
-                for (int kb = 0; kb < 2; kb++) {
-                    float S[4][MT][4];
-                    uint32_t wv[4][C::W];
-                    __half2  dm[4];
+                for (int kb = 0; kb < KV4_P; kb += C::KB) {
+                    float S[C::KB / 16][NR][4];                  // keys g and g + 8 of 16, rows 2 t and 2 t + 1
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = kb * 32 + j * 8 + g;
-                        dm[j] = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
-                        if constexpr (D == 128) { const uint4 x = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[j][0] = x.x; wv[j][1] = x.y; wv[j][2] = x.z; wv[j][3] = x.w; }
-                        else                    { const uint2 x = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[j][0] = x.x; wv[j][1] = x.y; }
-                    }
+                    for (int j = 0; j < C::KB / 16; j++) {
+                        uint32_t wv[2][C::W];
+                        __half2  dm[2];
 #pragma unroll
-                    for (int w = 0; w < C::W; w++) {
-                        uint4 f[MT][2];
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) f[mt][e] = C::QS ? qsm[(mt * C::KS + 2 * w + e) * 32] : qf[C::QS ? 0 : mt][C::QS ? 0 : 2 * w + e];
-                        uint32_t o[4][4];
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            kv4_pairs(wv[j][w], __low2half2(dm[j]), __high2half2(dm[j]), o[j]);
-#pragma unroll
-                            for (int mt = 0; mt < MT; mt++)
-                                if (w == 0) ka_mma0(S[j][mt], f[mt][0], o[j][0], o[j][1]); else ka_mma(S[j][mt], f[mt][0], o[j][0], o[j][1]);
+                        for (int x = 0; x < 2; x++) {
+                            const int r = kb + j * 16 + x * 8 + g;
+                            dm[x] = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                            if constexpr (D == 128) { const uint4 v = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[x][0] = v.x; wv[x][1] = v.y; wv[x][2] = v.z; wv[x][3] = v.w; }
+                            else                    { const uint2 v = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[x][0] = v.x; wv[x][1] = v.y; }
                         }
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
+                        for (int w = 0; w < C::W; w++) {
+                            uint32_t o[2][4];
 #pragma unroll
-                            for (int mt = 0; mt < MT; mt++) ka_mma(S[j][mt], f[mt][1], o[j][2], o[j][3]);
+                            for (int x = 0; x < 2; x++) kv4_pairs(wv[x][w], __low2half2(dm[x]), __high2half2(dm[x]), o[x]);
+#pragma unroll
+                            for (int n = 0; n < NR; n++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++)
+#pragma unroll
+                                    for (int pt = 0; pt < C::PARTS; pt++) {
+                                        const uint2 b = C::QS ? qsm[((n * C::PARTS + pt) * C::KS + 2 * w + e) * 32] : qf[C::QS ? 0 : pt][C::QS ? 0 : 2 * w + e];
+                                        if (w == 0 && e == 0 && pt == 0) ka_mma0(S[j][n], o[0][0], o[1][0], o[0][1], o[1][1], b);
+                                        else ka_mma(S[j][n], o[0][2 * e], o[1][2 * e], o[0][2 * e + 1], o[1][2 * e + 1], b);
+                                    }
+                        }
                     }
-                    if (kb == 1) {                               // the keys have been read
-                        __syncwarp();
-                        issue();
-                    } else {
+                    if (kb == 0) {
                         ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
                         if (!ok) break;
                     }
-                    if (C::SPLIT)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int mt = 0; mt < MT; mt++) { S[j][mt][0] += S[j][mt][2]; S[j][mt][1] += S[j][mt][3]; }
+                    if (kb + C::KB == KV4_P) {                   // the keys have been read
+                        __syncwarp();
+                        issue();
+                    }
                     if (edge) {
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
+                        for (int n = 0; n < NR; n++)
 #pragma unroll
-                            for (int nr = 0; nr < C::NR; nr++)
+                            for (int r = 0; r < 2; r++) {
+                                const int a = low(n * 8 + 2 * t + r) - key0 - kb - g, b = high(n * 8 + 2 * t + r) - key0 - kb - g;
 #pragma unroll
-                                for (int j = 0; j < 4; j++)
+                                for (int j = 0; j < C::KB / 16; j++)
 #pragma unroll
-                                    for (int c = 0; c < 2; c++) {
-                                        const int key = key0 + kb * 32 + j * 8 + t * 2 + c;
-                                        if (key < lo[mt][nr] || key > hi[mt][nr]) S[j][mt][nr * 2 + c] = -INFINITY;
-                                    }
+                                    for (int x = 0; x < 2; x++) if (j * 16 + x * 8 < a || j * 16 + x * 8 > b) S[j][n][2 * x + r] = -INFINITY;
+                            }
                         if (kb == 0) {
                             // values that are none, on a page of which some row does not see all: the rows that see one are none in the channels of its group, and it takes part as zeros
                             bool bad = false;
                             for (int k = lane; k < KV4_P * C::W; k += 32) bad |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + k * 4)));
                             if (__any_sync(0xffffffffu, bad)) {
-                                for (int k = 0; k < KV4_P; k++)
-                                    if (__hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (t * C::W >> 2)) * 4))))
 #pragma unroll
-                                        for (int mt = 0; mt < MT; mt++)
+                                for (int n = 0; n < NR; n++)
 #pragma unroll
-                                            for (int nr = 0; nr < C::NR; nr++)
-                                                if (key0 + k >= lo[mt][nr] && key0 + k <= hi[mt][nr])
+                                    for (int r = 0; r < 2; r++) {
+                                        const int a = low(n * 8 + 2 * t + r) - key0, b = high(n * 8 + 2 * t + r) - key0;
+                                        bool sees = false;
+                                        for (int k = max(a, 0); k <= min(b, KV4_P - 1); k++)
+                                            sees |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (g * C::W >> 3)) * 4)));
+                                        if (sees)
 #pragma unroll
-                                                    for (int n = 0; n < C::NT; n++) { O[mt][n][nr * 2] = __uint_as_float(0x7fc00000u); O[mt][n][nr * 2 + 1] = __uint_as_float(0x7fc00000u); }
+                                            for (int i3 = 0; i3 < C::MT; i3++) { O[n][i3][r] = __uint_as_float(0x7fc00000u); O[n][i3][2 + r] = __uint_as_float(0x7fc00000u); }
+                                    }
                                 __syncwarp();
                                 for (int k = lane; k < KV4_P * C::W; k += 32) {
                                     __half2 * dm = reinterpret_cast<__half2 *>(vp + kv4_steps(D) + k * 4);
@@ -240,47 +235,55 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                         }
                     }
                     // ---- weights: the rows' maxima, exponentials, sums
-                    uint4 P[2][MT];
+                    uint2 P[C::KB / 16][NR][C::PARTS];
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
+                    for (int n = 0; n < NR; n++) {
+                        float top[2];
 #pragma unroll
-                        for (int nr = 0; nr < C::NR; nr++) {
-                            float top = -INFINITY;
+                        for (int r = 0; r < 2; r++) {
+                            top[r] = fmaxf(S[0][n][r], S[0][n][2 + r]);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) top = fmaxf(top, fmaxf(S[j][mt][nr * 2], S[j][mt][nr * 2 + 1]));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * qs[mt][nr];
-                            if (__any_sync(0xffffffffu, top > m[mt][nr] + KA_LAZY)) {
-                                const float mn = top > m[mt][nr] + KA_LAZY ? top : m[mt][nr], a = mn == m[mt][nr] ? 1.f : ka_exp2(m[mt][nr] - mn);
-                                m[mt][nr] = mn;
-                                l[mt][nr] *= a;
+                            for (int j = 1; j < C::KB / 16; j++) top[r] = fmaxf(top[r], fmaxf(S[j][n][r], S[j][n][2 + r]));
+                        }
 #pragma unroll
-                                for (int n = 0; n < C::NT; n++) {
-                                    O[mt][n][nr * 2] *= a; O[mt][n][nr * 2 + 1] *= a;
-                                    if (C::SPLIT) { O[mt][n][2] *= a; O[mt][n][3] *= a; }
-                                }
+                        for (int o = 4; o < 32; o <<= 1) { top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o)); top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o)); }
+                        top[0] *= qs[n][0]; top[1] *= qs[n][1];
+                        if (__any_sync(0xffffffffu, top[0] > m[n][0] + KA_LAZY || top[1] > m[n][1] + KA_LAZY)) {
+                            float a[2];
+#pragma unroll
+                            for (int r = 0; r < 2; r++) {
+                                const float mn = top[r] > m[n][r] + KA_LAZY ? top[r] : m[n][r];
+                                a[r] = mn == m[n][r] ? 1.f : ka_exp2(m[n][r] - mn);
+                                m[n][r] = mn;
+                                l[n][r] *= a[r];
                             }
-                            const float base = KA_LIFT - (m[mt][nr] == -INFINITY ? 0.f : m[mt][nr]);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float x = ka_exp2(fmaf(S[j][mt][nr * 2], qs[mt][nr], base)), y = ka_exp2(fmaf(S[j][mt][nr * 2 + 1], qs[mt][nr], base));
-                                l[mt][nr] += x + y;
-                                const uint32_t h = ka_pack(x, y);
-                                uint32_t & at0 = j & 1 ? P[j >> 1][mt].z : P[j >> 1][mt].x, & at1 = j & 1 ? P[j >> 1][mt].w : P[j >> 1][mt].y;
-                                if (C::SPLIT) { at0 = h; at1 = ka_rest(x, y, h); }
-                                else if (nr == 0) at0 = h;
-                                else at1 = h;
+                            for (int i3 = 0; i3 < C::MT; i3++) { O[n][i3][0] *= a[0]; O[n][i3][1] *= a[1]; O[n][i3][2] *= a[0]; O[n][i3][3] *= a[1]; }
+                        }
+                        const float base0 = KA_LIFT - (m[n][0] == -INFINITY ? 0.f : m[n][0]), base1 = KA_LIFT - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+#pragma unroll
+                        for (int j = 0; j < C::KB / 16; j++) {
+                            uint32_t h[2], r[2];
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                const float a = ka_exp2(fmaf(S[j][n][2 * x], qs[n][0], base0)), b = ka_exp2(fmaf(S[j][n][2 * x + 1], qs[n][1], base1));
+                                l[n][0] += a; l[n][1] += b;
+                                h[x] = ka_pack(a, b);
+                                if (C::SPLIT) r[x] = ka_turn(ka_rest(a, b, h[x]));
+                                h[x] = ka_turn(h[x]);
                             }
+                            P[j][n][0] = make_uint2(h[0], h[1]);
+                            if (C::SPLIT) P[j][n][C::PARTS - 1] = make_uint2(r[0], r[1]);
                         }
                     }
                     // ---- outputs
 #pragma unroll
-                    for (int i2 = 0; i2 < 2; i2++) {
+                    for (int j = 0; j < C::KB / 16; j++) {
                         uint32_t a[2][C::W / 2], b[2][C::W / 2];               // this lane's channels of keys 2 t and 2 t + 1 of both groups of eight
                         __half2  d2[2], m2[2];
 #pragma unroll
                         for (int f = 0; f < 2; f++) {
-                            const int ra = kb * 32 + i2 * 16 + f * 8 + t, rb = ra + 4;         // kv4_row of the places 2 t and 2 t + 1
+                            const int ra = kb + j * 16 + f * 8 + t, rb = ra + 4;               // kv4_row of the places 2 t and 2 t + 1
                             const __half2 da = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (ra * C::W + (g * C::W >> 3)) * 4);
                             const __half2 db = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (rb * C::W + (g * C::W >> 3)) * 4);
                             d2[f] = __lows2half2(da, db); m2[f] = __highs2half2(da, db);
@@ -296,10 +299,13 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                                 uint32_t x[4], y[4];
                                 kv4_pairs(ka_prmt(a[0][w], b[0][w], e ? 0x7632 : 0x5410), d2[0], m2[0], x);
                                 kv4_pairs(ka_prmt(a[1][w], b[1][w], e ? 0x7632 : 0x5410), d2[1], m2[1], y);
+                                // rows g and g + 8 of a product are two neighbouring channels
 #pragma unroll
-                                for (int n = 0; n < 4; n++)
+                                for (int n = 0; n < NR; n++)
 #pragma unroll
-                                    for (int mt = 0; mt < MT; mt++) ka_mma(O[mt][w * 8 + e * 4 + n], P[i2][mt], x[n], y[n]);
+                                    for (int pt = 0; pt < C::PARTS; pt++)
+#pragma unroll
+                                        for (int c = 0; c < 2; c++) ka_mma(O[n][w * 4 + e * 2 + c], x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][pt]);
                             }
                     }
                 }
@@ -308,37 +314,34 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
                 issue();                                         // the values have been read
             }
             if (!ok) break;
-            // ---- rows out: lane (g, t) has D / 4 neighbouring channels of its rows
+            // ---- rows out: lane (g, t) has D / 8 neighbouring channels of rows 2 t and 2 t + 1 of each tile
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < NR; n++)
 #pragma unroll
-                for (int nr = 0; nr < C::NR; nr++) {
-                    float sum = l[mt][nr];
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    const int ri = mt * C::RPM + nr * 8 + g;
+                for (int r = 0; r < 2; r++) {
+                    float sum = l[n][r];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    const int ri = n * 8 + 2 * t + r;
                     if (ri >= rows) continue;
-                    float v[D / 4];
+                    float v[C::C8];
 #pragma unroll
-                    for (int n = 0; n < C::NT; n++) {
-                        v[n]         = C::SPLIT ? O[mt][n][0] + O[mt][n][2] : O[mt][n][nr * 2];
-                        v[n + C::NT] = C::SPLIT ? O[mt][n][1] + O[mt][n][3] : O[mt][n][nr * 2 + 1];
-                    }
+                    for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r];
                     if (whole) {
                         const float inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
 #pragma unroll
-                        for (int c = 0; c < D / 4; c++) v[c] *= inv;
+                        for (int c = 0; c < C::C8; c++) v[c] *= inv;
                         const int rc = row0 + ri;
-                        ka_store<T, D / 4>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4), A.wide_o, v);
+                        ka_store<T, C::C8>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + g * C::C8, A.wide_o, v);
                     } else {
                         float * p = A.pieces + (int64_t) slot * C::PIECE;
-                        ka_store<float, D / 4>(p + ri * D + t * (D / 4), true, v);
-                        if (t == 0) { p[C::RT * D + ri] = m[mt][nr]; p[C::RT * D + C::RT + ri] = sum; }
+                        ka_store<float, C::C8>(p + ri * D + g * C::C8, true, v);
+                        if (g == 0) { p[C::RT * D + ri] = m[n][r]; p[C::RT * D + C::RT + ri] = sum; }
                     }
                 }
-            u += pages;
+            todo -= pages;
             at.p += pages - 1;
-            if (u < u1) ka_next<C::RT, 0>(A, prefix, seq_of, at);
+            if (todo) ka_next<C::RT, 0>(A, prefix, seq_of, at);
         }
     }
     __syncthreads();
@@ -348,72 +351,89 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, MT>::WARPS * 32, 1) kv4_de
     }
 }
 
-// A block per (token, query head): rows of items that lay in several warps' runs get their pieces' sum, rows of items without pages zeros; the others are written already.
-template <typename T, int D, int MT>
-static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ ka_args A) {
-    using C = ka_cfg<T, D, MT>;
+// Rows (token, query head), WPR warps each: rows of items that lay in several warps' runs get their pieces' sum, rows of items without pages zeros; the others are written already.
+#define KJ_WARPS 8
+template <typename T, int D, int NR, int WPR>
+static __global__ void __launch_bounds__(KJ_WARPS * 32) kv4_join_kernel(const __grid_constant__ ka_args A) {
+    using C = ka_cfg<T, D, NR>;
+    constexpr int CH = D / 32;
     pib_pdl_wait();
     pib_pdl_trigger();
-    __shared__ int   found;
-    __shared__ float sm_m[8], sm_l[8], sm_o[8][D];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = A.kvh * A.rep, t = blockIdx.x / heads, hq = blockIdx.x % heads, h = hq / A.rep;
-    if (threadIdx.x == 0) found = -1;
-    __syncthreads();
-    for (int s = threadIdx.x; s < A.seqs; s += 256) if (A.starts[s] <= t && t < A.starts[s + 1]) atomicMax(&found, s);
-    __syncthreads();
-    const int s = found;
-    if (s < 0) return;
-    const ka_seq q = ka_load_seq(A, s);
-    const int tl = t - min(max(A.starts[s], 0), A.tokens), idx = tl * A.rep + hq % A.rep, r = idx / C::RT, ri = idx % C::RT;
-    if (tl >= q.n) return;
-    int     first;
-    int64_t ib = A.plan->prefix[s];
-    for (int i = 0; i < r; i++) ib += (int64_t) ka_pages<C::RT>(A, q, i, first) * A.kvh;
-    const int np = ka_pages<C::RT>(A, q, r, first);
-    ib += (int64_t) h * np;
-    T * out = (T *) A.out + (int64_t) t * A.ldo + (int64_t) hq * D;
-    if (np == 0) {
-        if (threadIdx.x < D) out[threadIdx.x] = (T) 0.f;
-        return;
+    __shared__ float sm_m[KJ_WARPS], sm_l[KJ_WARPS], sm_o[KJ_WARPS][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR, heads = A.kvh * A.rep;
+    const int64_t row = (int64_t) blockIdx.x * (KJ_WARPS / WPR) + warp / WPR;
+    int64_t wa = 0, wb = 0;
+    int     ri = 0, np = -1;
+    T *     out = nullptr;
+    if (row < (int64_t) A.tokens * heads) {
+        const int t = (int) (row / heads), hq = (int) (row % heads), h = hq / A.rep;
+        int s = -1;
+        for (int i = lane; i < A.seqs; i += 32) if (A.starts[i] <= t && t < A.starts[i + 1]) s = i;
+        s = __reduce_max_sync(0xffffffffu, s);
+        if (s >= 0) {
+            const ka_seq q = ka_load_seq(A, s);
+            const int64_t ps = A.plan->prefix[s], U = A.plan->prefix[A.seqs], W = A.plan->runs;
+            const int tl = t - min(max(A.starts[s], 0), A.tokens), idx = tl * A.rep + hq % A.rep, r = idx / C::RT;
+            ri = idx % C::RT;
+            if (tl < q.n) {
+                int     first;
+                int64_t ib = ps;
+                for (int i = 0; i < r; i++) ib += (int64_t) ka_pages<C::RT>(A, q, i, first) * A.kvh;
+                np = ka_pages<C::RT>(A, q, r, first);
+                ib += (int64_t) h * np;
+                if (np > 0) { wa = ((ib + 1) * W + U - 1) / U - 1; wb = ((ib + np) * W + U - 1) / U - 1; }
+                out = (T *) A.out + (int64_t) t * A.ldo + (int64_t) hq * D;
+            }
+        }
     }
-    const int64_t U = A.plan->prefix[A.seqs], W = A.plan->runs, wa = ((ib + 1) * W + U - 1) / U - 1, wb = ((ib + np) * W + U - 1) / U - 1;
-    if (wa == wb) return;
-    constexpr int CH = D / 32;
+    if (np == 0 && sub == 0)
+#pragma unroll
+        for (int c = 0; c < CH; c++) out[lane * CH + c] = (T) 0.f;
+    if (WPR == 1 && wa == wb) return;
     float m = -INFINITY, l = 0.f, o[CH];
 #pragma unroll
     for (int c = 0; c < CH; c++) o[c] = 0.f;
-    // a warp takes every eighth piece, 32 of them at a time: their maxima and sums, a piece a lane, then their rows, whose loads wait for nothing
-    for (int64_t w0 = wa + warp; w0 <= wb; w0 += 256) {
-        const int n = (int) min((int64_t) 32, (wb - w0) / 8 + 1);
-        auto piece = [&](int k) { const int64_t w = w0 + 8 * k; return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
-        float pm = -INFINITY, pl = 0.f;
-        if (lane < n) { pm = piece(lane)[C::RT * D + ri]; pl = piece(lane)[C::RT * D + C::RT + ri]; }
-        const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
-        m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
+    // a warp takes every WPR-th piece, 32 of them at a time: their maxima and sums, a piece a lane, then their rows, whose loads wait for nothing
+    if (wa < wb)
+        for (int64_t w0 = wa + sub; w0 <= wb; w0 += 32 * WPR) {
+            const int n = (int) min((int64_t) 32, (wb - w0) / WPR + 1);
+            auto piece = [&](int k) { const int64_t w = w0 + WPR * k; return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
+            float pm = -INFINITY, pl = 0.f;
+            if (lane < n) { pm = piece(lane)[C::RT * D + ri]; pl = piece(lane)[C::RT * D + C::RT + ri]; }
+            const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
+            m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
 #pragma unroll
-        for (int c = 0; c < CH; c++) o[c] *= a;
+            for (int c = 0; c < CH; c++) o[c] *= a;
 #pragma unroll 8
-        for (int k = 0; k < n; k++) {
-            const float * p = piece(k) + ri * D;
-            const float   fk = __shfl_sync(0xffffffffu, f, k);
-            if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
-            else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
+            for (int k = 0; k < n; k++) {
+                const float * p = piece(k) + ri * D;
+                const float   fk = __shfl_sync(0xffffffffu, f, k);
+                if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
+                else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
+            }
+        }
+    if constexpr (WPR > 1) {
+        static_assert(WPR == KJ_WARPS, "a row a block");
+        if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+#pragma unroll
+        for (int c = 0; c < CH; c++) sm_o[warp][lane * CH + c] = o[c];
+        __syncthreads();
+        if (wa == wb || warp > 0) return;
+#pragma unroll
+        for (int c = 0; c < CH; c++) o[c] = 0.f;
+        m = sm_m[0];
+        for (int i = 1; i < WPR; i++) m = fmaxf(m, sm_m[i]);
+        l = 0.f;
+        for (int i = 0; i < WPR; i++) {
+            const float a = sm_m[i] == m ? 1.f : exp2f(sm_m[i] - m);
+            l += sm_l[i] * a;
+#pragma unroll
+            for (int c = 0; c < CH; c++) o[c] = fmaf(sm_o[i][lane * CH + c], a, o[c]);
         }
     }
-    if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+    const float inv = l > 0.f ? 1.f / l : l;
 #pragma unroll
-    for (int c = 0; c < CH; c++) sm_o[warp][lane * CH + c] = o[c];
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    m = sm_m[0];
-    for (int i = 1; i < 8; i++) m = fmaxf(m, sm_m[i]);
-    float v = 0.f;
-    l = 0.f;
-    for (int i = 0; i < 8; i++) {
-        const float a = sm_m[i] == m ? 1.f : exp2f(sm_m[i] - m);
-        l += sm_l[i] * a; v += sm_o[i][threadIdx.x] * a;
-    }
-    out[threadIdx.x] = (T) (l > 0.f ? v / l : l != l ? l : 0.f);
+    for (int c = 0; c < CH; c++) out[lane * CH + c] = (T) (o[c] * inv);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
@@ -435,12 +455,14 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
-// rows (token, head of the group) of the longest portion: up to one or two products' rows by the decode kernels, more than KA_FEW on tcgen05
+// rows (token, head of the group) of the longest portion: more than KA_FEW go on tcgen05
 #define KA_FEW 64
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
-static int ka_mt(const pib_kv4 * kv, const pib_kv4_batch * b) { return ka_rows(kv, b) > (b->type == PIB_TYPE_F32 ? 8 : 16) ? 2 : 1; }
+// tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
+static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
 static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    const size_t rows = ka_rows(kv, b) > KA_FEW ? KP_ROWS : (size_t) 8 * ka_mt(kv, b) * (b->type == PIB_TYPE_F32 ? 8 : 16);
+    const int    n = ka_tiles_of(kv, b);
+    const size_t rows = ka_rows(kv, b) > KA_FEW ? KP_ROWS : (size_t) ka_warps(b->type == PIB_TYPE_F32, n) * n * 8;
     return (size_t) 2 * pib_num_sms() * rows * (kv->dim + 2) * 4;
 }
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
@@ -448,14 +470,19 @@ extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_b
     return (ka_pieces(kv, b) + sizeof(ka_plan) + 255) & ~(size_t) 255;
 }
 
-template <typename T, int D, int MT> static int ka_go(ka_args A, cudaStream_t st) {
-    using C = ka_cfg<T, D, MT>;
-    const size_t table = ((size_t) (A.seqs + 1) * 8 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127, most = 224 * 1024;
+template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st) {
+    using C = ka_cfg<T, D, NR>;
+    const size_t table = ((size_t) (A.seqs + 1) * 8 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127;
+    constexpr size_t most = 224 * 1024;
     A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
+    static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 8 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
     static pib_per_device attrs;
-    PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
-    PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, MT>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
-    PIB_CHECK(pib_launch(kv4_join_kernel<T, D, MT>, dim3((unsigned) ((int64_t) A.tokens * A.kvh * A.rep)), dim3(256), 0, st, A));
+    PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
+    PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, NR>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
+    const int64_t rows = (int64_t) A.tokens * A.kvh * A.rep;
+    // few rows have many pieces each: a block a row; many rows: a warp
+    if (rows <= 4 * pib_num_sms()) PIB_CHECK(pib_launch(kv4_join_kernel<T, D, NR, KJ_WARPS>, dim3((unsigned) rows), dim3(KJ_WARPS * 32), 0, st, A));
+    else                           PIB_CHECK(pib_launch(kv4_join_kernel<T, D, NR, 1>, dim3((unsigned) ((rows + KJ_WARPS - 1) / KJ_WARPS)), dim3(KJ_WARPS * 32), 0, st, A));
     return PIB_OK;
 }
 
@@ -483,15 +510,11 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;
     if (ka_rows(kv, b) > KA_FEW) return pib_kv4_prompt(A, size == 4, st);
-    const int form = (size == 4 ? 4 : 0) + (kv->dim == 128 ? 2 : 0) + (ka_mt(kv, b) == 2 ? 1 : 0);
-    switch (form) {
-        case 0:  return ka_go<__nv_bfloat16, 64, 1>(A, st);
-        case 1:  return ka_go<__nv_bfloat16, 64, 2>(A, st);
-        case 2:  return ka_go<__nv_bfloat16, 128, 1>(A, st);
-        case 3:  return ka_go<__nv_bfloat16, 128, 2>(A, st);
-        case 4:  return ka_go<float, 64, 1>(A, st);
-        case 5:  return ka_go<float, 64, 2>(A, st);
-        case 6:  return ka_go<float, 128, 1>(A, st);
-        default: return ka_go<float, 128, 2>(A, st);
+    const int n = ka_tiles_of(kv, b);
+    if (size == 4) {
+        if (kv->dim == 64) return n == 1 ? ka_go<float, 64, 1>(A, st) : ka_go<float, 64, 2>(A, st);
+        return n == 1 ? ka_go<float, 128, 1>(A, st) : ka_go<float, 128, 2>(A, st);
     }
+    if (kv->dim == 64) return n == 1 ? ka_go<__nv_bfloat16, 64, 1>(A, st) : n == 2 ? ka_go<__nv_bfloat16, 64, 2>(A, st) : ka_go<__nv_bfloat16, 64, 4>(A, st);
+    return n == 1 ? ka_go<__nv_bfloat16, 128, 1>(A, st) : n == 2 ? ka_go<__nv_bfloat16, 128, 2>(A, st) : ka_go<__nv_bfloat16, 128, 4>(A, st);
 }
