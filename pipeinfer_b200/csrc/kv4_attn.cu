@@ -16,16 +16,17 @@ __device__ __forceinline__ void ka_mma0(float (&c)[4], uint32_t a0, uint32_t a1,
 // an 8 x 8 matrix of 16-bit numbers, two of a row a lane, turned
 __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 
-// All (sequence, tile of rows, key / value head, page) units lie in one row, which the warps of the GPU divide evenly whatever the sequences' lengths; a warp walks its units alone, with the running maximum
-// and sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
+// All (sequence, tile of rows, key / value head, page) units lie in one row, which the blocks of the GPU divide evenly whatever the sequences' lengths, and a block's warps its run; a warp walks its units
+// alone, with the running maximum and sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
 //   scores   turned, S' = K Q': mma.m16n8k16, 16 keys as M, eight rows as N, keys straight from nibbles in registers: lane (g, t) has 16 or 32 neighbouring channels of keys g and g + 8, one load and one step
 //            and lowest value each, four of them a product's k
 //   outputs  O' = V' P': 16 channels as M, weights (turned once more by movmatrix) as N, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
 // Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  fp32 rows enter as fp16 part and remainder,
 // two products into the same sums; of bfloat16 rows queries and weights are one fp16 number.
-// An item that lies in one warp's run is written at once, pieces of others go to scratch and kv4_join_kernel adds them up, in the order of the keys.
+// An item that lies in one warp's units is written at once.  Pieces of others meet in shared memory at the end, in the order of the keys; what then is not a whole item goes to scratch, two pieces a block at
+// most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, twelve times as many, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
 // warps of a block, by the registers that a warp's tile takes, and the shared memory of fp32 queries' operands
-__host__ __device__ constexpr int ka_warps(bool split, int nr) { return nr == 1 ? 16 : nr == 2 && !split ? 12 : 8; }
+__host__ __device__ constexpr int ka_warps(bool split, int nr) { return nr == 1 || (nr == 2 && !split) ? 12 : 8; }
 template <typename T, int D, int NR> struct ka_cfg {                 // NR: tiles of eight rows
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
@@ -36,12 +37,39 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr int  PIECE = RT * (D + 2);                      // floats
 };
 
+// a warp's piece of an item: sums of the rows that there are, their maxima and denominators
+template <typename C, int NR>
+__device__ __forceinline__ void ka_leave(float * p, int rows, int g, int t, const float (&O)[NR][C::MT][4], const float (&m)[NR][2], const float (&l)[NR][2]) {
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int ri = n * 8 + 2 * t + r;
+            if (ri >= rows) continue;
+            float v[C::C8];
+#pragma unroll
+            for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r];
+            ka_store<float, C::C8>(p + ri * (C::C8 * 8) + g * C::C8, true, v);
+            if (g == 0) { p[C::RT * C::C8 * 8 + ri] = m[n][r]; p[C::RT * C::C8 * 8 + C::RT + ri] = l[n][r]; }
+        }
+}
+// row ri of an item from its sums over all keys, D / 32 channels a lane
+template <typename T, int D> __device__ __forceinline__ void ka_row_out(const ka_args & A, const ka_open & it, int ri, int lane, const float (&o)[D / 32], float l) {
+    const int   rc = it.row0 + ri;
+    const float inv = l > 0.f ? 1.f / l : l;
+    T * out = (T *) A.out + (it.tok0 + rc / A.rep) * A.ldo + (int64_t) (it.h * A.rep + rc % A.rep) * D + lane * (D / 32);
+#pragma unroll
+    for (int c = 0; c < D / 32; c++) out[c] = (T) (o[c] * inv);
+}
+
 template <typename T, int D, int NR>
 static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_decode_kernel(const __grid_constant__ ka_args A) {
     using C = ka_cfg<T, D, NR>;
     extern __shared__ __align__(128) uint8_t ka_dsm[];
     __shared__ uint64_t bars[C::WARPS * 8];
     __shared__ int64_t  part[C::WARPS];
+    __shared__ ka_open  items[C::WARPS], last_item[C::WARPS];
+    __shared__ int      flags[C::WARPS];
     __shared__ int      abort_w;
     volatile int * abort_s = &abort_w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, NST = A.stages;
@@ -56,13 +84,32 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     pib_pdl_wait();
     pib_pdl_trigger();
     const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
-    const int64_t warps = min((int64_t) gridDim.x * C::WARPS, U), me = (int64_t) warp * gridDim.x + blockIdx.x;
-    ka_leave_plan<C::WARPS * 32>(A, prefix, warps);
+    const int     runs = (int) min((int64_t) gridDim.x, U);
+    const int64_t c0 = blockIdx.x < runs ? U * blockIdx.x / runs : 0, c1 = blockIdx.x < runs ? U * (blockIdx.x + 1) / runs : 0;
     auto seq_of = [&](int s) { return seq[s]; };
+    // rows of tiles without pages
+    for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
+        const ka_seq  q = seq[s];
+        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
+        for (int r = 0; r < ka_tiles<C::RT>(A, q); r++) {
+            int first;
+            if (ka_pages<C::RT>(A, q, r, first)) continue;
+            const int row0 = r * C::RT, rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - row0);
+            for (int i = threadIdx.x; i < rows * A.kvh * D; i += C::WARPS * 32) {
+                const int c = i % D, h = i / D % A.kvh, rc = row0 + i / D / A.kvh;
+                ((T *) A.out)[(tok0 + rc / A.rep) * A.ldo + (int64_t) (h * A.rep + rc % A.rep) * D + c] = (T) 0.f;
+            }
+        }
+    }
     bool ok = true;
-    if (me < warps) {
-        const int64_t u0 = U * me / warps, u1 = U * (me + 1) / warps;
-        ka_place at = ka_find<C::RT, 0>(A, prefix, seq_of, u0);
+    // the warp's pieces of items that lie in several warps' units: one that ends here (in scratch), one that does not (in registers)
+    bool    ends = false, goes = false, begins = false;
+    int64_t item_end = 0;
+    ka_place at = { 0, 0, 0, 0, 0, 0 };
+    float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];            // of rows 2 t and 2 t + 1 of each tile
+    const int64_t u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+    if (u0 < u1) {
+        at = ka_find<C::RT, 0>(A, prefix, seq_of, u0);
         // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
         ka_place is = at;
         int      left = (int) (u1 - u0), todo = left;            // units to ask for, units to do
@@ -99,10 +146,8 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             const ka_seq  q = seq[at.s];
             const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = min(at.np - at.p, todo);
             const bool    whole = at.p == 0 && pages == at.np;
-            const int     slot = 2 * (int) me + (at.p > 0 ? 0 : 1);
             const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens);
             const int     row0 = at.r * C::RT, pos0 = q.len - q.n;
-            float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];    // of rows 2 t and 2 t + 1 of each tile
             uint2 qf[C::QS ? 1 : C::PARTS][C::QS ? 1 : C::KS];
 #pragma unroll
             for (int n = 0; n < NR; n++) {
@@ -318,32 +363,96 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
             for (int n = 0; n < NR; n++)
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    float sum = l[n][r];
+                for (int r = 0; r < 2; r++)
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    const int ri = n * 8 + 2 * t + r;
-                    if (ri >= rows) continue;
-                    float v[C::C8];
+                    for (int o = 4; o < 32; o <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], o);
+            todo -= pages;
+            if (whole) {
 #pragma unroll
-                    for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r];
-                    if (whole) {
-                        const float inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
+                for (int n = 0; n < NR; n++)
 #pragma unroll
-                        for (int c = 0; c < C::C8; c++) v[c] *= inv;
+                    for (int r = 0; r < 2; r++) {
+                        const int ri = n * 8 + 2 * t + r;
+                        if (ri >= rows) continue;
+                        const float inv = l[n][r] > 0.f ? 1.f / l[n][r] : l[n][r];     // a row that saw nothing: zeros; a sum that is none stays so
+                        float v[C::C8];
+#pragma unroll
+                        for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r] * inv;
                         const int rc = row0 + ri;
                         ka_store<T, C::C8>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + g * C::C8, A.wide_o, v);
-                    } else {
-                        float * p = A.pieces + (int64_t) slot * C::PIECE;
-                        ka_store<float, C::C8>(p + ri * D + g * C::C8, true, v);
-                        if (g == 0) { p[C::RT * D + ri] = m[n][r]; p[C::RT * D + C::RT + ri] = sum; }
                     }
-                }
-            todo -= pages;
+            } else if (at.p + pages == at.np) {
+                ends = true;
+                ka_leave<C, NR>(A.heads + (int64_t) (blockIdx.x * C::WARPS + warp) * C::PIECE, rows, g, t, O, m, l);
+                if (lane == 0) items[warp] = { 0, 0, row0, rows, at.h, tok0 };
+            } else { goes = true; begins = at.p == 0; item_end = u1 + (at.np - at.p - pages); if (lane == 0) last_item[warp] = { 0, 0, row0, rows, at.h, tok0 }; }
             at.p += pages - 1;
             if (todo) ka_next<C::RT, 0>(A, prefix, seq_of, at);
         }
     }
+    if (lane == 0) flags[warp] = (ends ? 1 : 0) | (goes ? 2 : 0) | (begins ? 4 : 0);
+    __syncthreads();                                                 // nobody reads a ring or queries any more
+    float * pieces = reinterpret_cast<float *>(ka_dsm);
+    if (goes) ka_leave<C, NR>(pieces + warp * C::PIECE, C::RT, g, t, O, m, l);
+    __syncthreads();
+    if (!*abort_s && c0 < c1) {
+        // a row a warp, lanes its channels: the warps' pieces in the order of their units
+        constexpr int CH = D / 32;
+        for (int ri = warp; ri < C::RT; ri += C::WARPS) {
+            float am = -INFINITY, al = 0.f, ao[CH];
+            bool  some = false, ours = false;                        // a chain of pieces is under way; it began in this block
+            auto add = [&](const float * p) {
+                const float pm = p[C::RT * D + ri], pl = p[C::RT * D + C::RT + ri], mn = fmaxf(am, pm), a = am == mn ? 1.f : exp2f(am - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
+                am = mn; al = al * a + pl * f;
+#pragma unroll
+                for (int c = 0; c < CH; c++) ao[c] = ao[c] * a + p[ri * D + lane * CH + c] * f;
+            };
+            auto start = [&]() {
+                am = -INFINITY; al = 0.f;
+#pragma unroll
+                for (int c = 0; c < CH; c++) ao[c] = 0.f;
+            };
+            auto leave = [&](int slot) {
+                float * p = A.pieces + (int64_t) (2 * blockIdx.x + slot) * C::PIECE;
+#pragma unroll
+                for (int c = 0; c < CH; c++) p[ri * D + lane * CH + c] = ao[c];
+                if (lane == 0) { p[C::RT * D + ri] = am; p[C::RT * D + C::RT + ri] = al; }
+            };
+            start();
+            for (int w = 0; w < C::WARPS; w++) {
+                const int f = flags[w];
+                if (f & 1) {
+                    const ka_open it = items[w];
+                    if (ri < it.rows) {
+                        add(A.heads + (int64_t) (blockIdx.x * C::WARPS + w) * C::PIECE);
+                        if (ours) ka_row_out<T, D>(A, it, ri, lane, ao, al);
+                        else      leave(0);
+                    }
+                    start();
+                    some = ours = false;
+                }
+                if (f & 2) {
+                    if (f & 4) ours = true;
+                    some = true;
+                    if (ri < last_item[w].rows) add(pieces + w * C::PIECE);
+                }
+            }
+            if (some) leave(ours ? 1 : 0);
+        }
+    }
+    // the last warp with units knows whether the run's last item goes on
+    if (blockIdx.x < runs && u1 == c1 && u0 < u1 && lane == 0) {
+        ka_open o = last_item[warp];
+        bool ours = begins;                                          // of a chain through several warps: where it began
+        for (int w = warp - 1; w >= 0 && !ours; w--) {               // (warps without units in between have no flags)
+            if (flags[w] & 4) ours = true;
+            if (flags[w] & 1) break;
+        }
+        o.runs = goes && ours;
+        o.last = goes ? (int) ((item_end * runs + U - 1) / U - 1) : 0;
+        A.open[blockIdx.x] = o;
+    }
+    if (threadIdx.x == 0 && blockIdx.x >= runs) A.open[blockIdx.x].runs = 0;
     __syncthreads();
     if (*abort_s) {                                              // a wait ran out: say so, give copies still in flight time to land (bounded)
         if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
@@ -351,89 +460,38 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     }
 }
 
-// Rows (token, query head), WPR warps each: rows of items that lay in several warps' runs get their pieces' sum, rows of items without pages zeros; the others are written already.
-#define KJ_WARPS 8
-template <typename T, int D, int NR, int WPR>
-static __global__ void __launch_bounds__(KJ_WARPS * 32) kv4_join_kernel(const __grid_constant__ ka_args A) {
+// Blocks (run, tile of eight rows): an item that begins in the run and does not end there gets its pieces' sum, a row a warp, lanes its channels.
+template <typename T, int D, int NR>
+static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ ka_args A) {
     using C = ka_cfg<T, D, NR>;
     constexpr int CH = D / 32;
     pib_pdl_wait();
     pib_pdl_trigger();
-    __shared__ float sm_m[KJ_WARPS], sm_l[KJ_WARPS], sm_o[KJ_WARPS][D];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR, heads = A.kvh * A.rep;
-    const int64_t row = (int64_t) blockIdx.x * (KJ_WARPS / WPR) + warp / WPR;
-    int64_t wa = 0, wb = 0;
-    int     ri = 0, np = -1;
-    T *     out = nullptr;
-    if (row < (int64_t) A.tokens * heads) {
-        const int t = (int) (row / heads), hq = (int) (row % heads), h = hq / A.rep;
-        int s = -1;
-        for (int i = lane; i < A.seqs; i += 32) if (A.starts[i] <= t && t < A.starts[i + 1]) s = i;
-        s = __reduce_max_sync(0xffffffffu, s);
-        if (s >= 0) {
-            const ka_seq q = ka_load_seq(A, s);
-            const int64_t ps = A.plan->prefix[s], U = A.plan->prefix[A.seqs], W = A.plan->runs;
-            const int tl = t - min(max(A.starts[s], 0), A.tokens), idx = tl * A.rep + hq % A.rep, r = idx / C::RT;
-            ri = idx % C::RT;
-            if (tl < q.n) {
-                int     first;
-                int64_t ib = ps;
-                for (int i = 0; i < r; i++) ib += (int64_t) ka_pages<C::RT>(A, q, i, first) * A.kvh;
-                np = ka_pages<C::RT>(A, q, r, first);
-                ib += (int64_t) h * np;
-                if (np > 0) { wa = ((ib + 1) * W + U - 1) / U - 1; wb = ((ib + np) * W + U - 1) / U - 1; }
-                out = (T *) A.out + (int64_t) t * A.ldo + (int64_t) hq * D;
-            }
-        }
-    }
-    if (np == 0 && sub == 0)
-#pragma unroll
-        for (int c = 0; c < CH; c++) out[lane * CH + c] = (T) 0.f;
-    if (WPR == 1 && wa == wb) return;
+    const int     lane = threadIdx.x & 31, wa = blockIdx.x, ri = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const ka_open it = A.open[wa];
+    if (!it.runs || ri >= it.rows) return;
     float m = -INFINITY, l = 0.f, o[CH];
 #pragma unroll
     for (int c = 0; c < CH; c++) o[c] = 0.f;
-    // a warp takes every WPR-th piece, 32 of them at a time: their maxima and sums, a piece a lane, then their rows, whose loads wait for nothing
-    if (wa < wb)
-        for (int64_t w0 = wa + sub; w0 <= wb; w0 += 32 * WPR) {
-            const int n = (int) min((int64_t) 32, (wb - w0) / WPR + 1);
-            auto piece = [&](int k) { const int64_t w = w0 + WPR * k; return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
-            float pm = -INFINITY, pl = 0.f;
-            if (lane < n) { pm = piece(lane)[C::RT * D + ri]; pl = piece(lane)[C::RT * D + C::RT + ri]; }
-            const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
-            m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
+    auto piece = [&](int w) { return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
+    // 32 pieces at a time: their maxima and sums, a piece a lane, then their rows, whose loads wait for nothing
+    for (int w0 = wa; w0 <= it.last; w0 += 32) {
+        const int n = min(32, it.last - w0 + 1);
+        float pm = -INFINITY, pl = 0.f;
+        if (lane < n) { pm = piece(w0 + lane)[C::RT * D + ri]; pl = piece(w0 + lane)[C::RT * D + C::RT + ri]; }
+        const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
+        m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
 #pragma unroll
-            for (int c = 0; c < CH; c++) o[c] *= a;
+        for (int c = 0; c < CH; c++) o[c] *= a;
 #pragma unroll 8
-            for (int k = 0; k < n; k++) {
-                const float * p = piece(k) + ri * D;
-                const float   fk = __shfl_sync(0xffffffffu, f, k);
-                if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
-                else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
-            }
-        }
-    if constexpr (WPR > 1) {
-        static_assert(WPR == KJ_WARPS, "a row a block");
-        if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-#pragma unroll
-        for (int c = 0; c < CH; c++) sm_o[warp][lane * CH + c] = o[c];
-        __syncthreads();
-        if (wa == wb || warp > 0) return;
-#pragma unroll
-        for (int c = 0; c < CH; c++) o[c] = 0.f;
-        m = sm_m[0];
-        for (int i = 1; i < WPR; i++) m = fmaxf(m, sm_m[i]);
-        l = 0.f;
-        for (int i = 0; i < WPR; i++) {
-            const float a = sm_m[i] == m ? 1.f : exp2f(sm_m[i] - m);
-            l += sm_l[i] * a;
-#pragma unroll
-            for (int c = 0; c < CH; c++) o[c] = fmaf(sm_o[i][lane * CH + c], a, o[c]);
+        for (int k = 0; k < n; k++) {
+            const float * p = piece(w0 + k) + ri * D;
+            const float   fk = __shfl_sync(0xffffffffu, f, k);
+            if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
+            else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
         }
     }
-    const float inv = l > 0.f ? 1.f / l : l;
-#pragma unroll
-    for (int c = 0; c < CH; c++) out[lane * CH + c] = (T) (o[c] * inv);
+    ka_row_out<T, D>(A, it, ri, lane, o, l);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
@@ -460,14 +518,23 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
 static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
-static size_t ka_pieces(const pib_kv4 * kv, const pib_kv4_batch * b) {
-    const int    n = ka_tiles_of(kv, b);
-    const size_t rows = ka_rows(kv, b) > KA_FEW ? KP_ROWS : (size_t) ka_warps(b->type == PIB_TYPE_F32, n) * n * 8;
-    return (size_t) 2 * pib_num_sms() * rows * (kv->dim + 2) * 4;
+// the scratch: two pieces a block, decode: one of each warp; then the tables
+struct ka_space { size_t heads, plan, open, total; };
+static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
+    const int    n = ka_tiles_of(kv, b), sms = pib_num_sms();
+    const bool   few = ka_rows(kv, b) <= KA_FEW;
+    const size_t piece = (size_t) (few ? n * 8 : KP_ROWS) * (kv->dim + 2) * 4;
+    auto up = [](size_t v) { return (v + 255) & ~(size_t) 255; };
+    ka_space s;
+    s.heads = up(2 * sms * piece);
+    s.plan  = s.heads + (few ? up((size_t) sms * ka_warps(b->type == PIB_TYPE_F32, n) * piece) : 0);
+    s.open  = s.plan + up(sizeof(ka_plan));
+    s.total = s.open + up(sms * sizeof(ka_open));
+    return s;
 }
 extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * b) {
     if (ka_batch_ok("pib_kv4_attn_scratch_bytes", kv, b) != PIB_OK) return 0;
-    return (ka_pieces(kv, b) + sizeof(ka_plan) + 255) & ~(size_t) 255;
+    return ka_space_of(kv, b).total;
 }
 
 template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st) {
@@ -476,13 +543,11 @@ template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st
     constexpr size_t most = 224 * 1024;
     A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
     static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 8 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
+    static_assert(C::PIECE * 4 <= 2 * C::HALF + C::Q_BYTES / C::WARPS, "pieces in the rings' and queries' place");
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
     PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, NR>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
-    const int64_t rows = (int64_t) A.tokens * A.kvh * A.rep;
-    // few rows have many pieces each: a block a row; many rows: a warp
-    if (rows <= 4 * pib_num_sms()) PIB_CHECK(pib_launch(kv4_join_kernel<T, D, NR, KJ_WARPS>, dim3((unsigned) rows), dim3(KJ_WARPS * 32), 0, st, A));
-    else                           PIB_CHECK(pib_launch(kv4_join_kernel<T, D, NR, 1>, dim3((unsigned) ((rows + KJ_WARPS - 1) / KJ_WARPS)), dim3(KJ_WARPS * 32), 0, st, A));
+    PIB_CHECK(pib_launch(kv4_join_kernel<T, D, NR>, dim3((unsigned) pib_num_sms(), NR), dim3(256), 0, st, A));
     return PIB_OK;
 }
 
@@ -505,7 +570,9 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     A.q = q; A.out = out; A.ldq = ldq; A.ldo = ldo;
     A.wide_q = ((uintptr_t) q & 15) == 0 && ldq * size % 16 == 0;
     A.wide_o = ((uintptr_t) out & 15) == 0 && ldo * size % 16 == 0;
-    A.pieces = (float *) scratch; A.plan = (ka_plan *) ((uint8_t *) scratch + ka_pieces(kv, b));
+    const ka_space sp = ka_space_of(kv, b);
+    uint8_t * sc = (uint8_t *) scratch;
+    A.pieces = (float *) sc; A.heads = (float *) (sc + sp.heads); A.plan = (ka_plan *) (sc + sp.plan); A.open = (ka_open *) (sc + sp.open);
     A.stages = 0;
     if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;

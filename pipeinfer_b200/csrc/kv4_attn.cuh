@@ -10,7 +10,7 @@ struct ka_args {
     const uint8_t * base; int64_t pages; int kvh, rep, dim;
     const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
     const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
-    int stages; float * pieces; struct ka_plan * plan; int * err;
+    int stages; float * pieces, * heads; struct ka_plan * plan; struct ka_open * open; int * err;
 };
 
 // A row's queries enter times scale log2 e, over the power of two of the largest: what scores are multiplied with is a power of two, exact, and so is the running maximum
@@ -83,7 +83,9 @@ template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_
 template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
 
 // what both kernels know of the work: behind the pieces in the scratch
-struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // runs of units; units in front of each sequence
+struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // prompts: runs of units; units in front of each sequence
+// decode: of each run whether an item begins there and does not end there; the run where it does, its rows
+struct ka_open { int runs, last, row0, rows, h; int64_t tok0; };
 
 // A place among the units: unit p of np, page first + p - LEAD, of head h, of tile r, of sequence s.  prefix: units in front of each sequence; seq(s): its tokens and keys.  An item has LEAD units in front
 // of its pages: what its start and end cost, in pages
