@@ -46,6 +46,12 @@ __device__ __forceinline__ __half2 kv4_in(uint32_t w, uint32_t mask) {
 }
 __device__ __forceinline__ __half2 kv4_low(uint32_t w)  { return __hadd2(kv4_in(w, 0x000f000fu), kv4_bits(0xe400e400u)); }
 __device__ __forceinline__ __half2 kv4_high(uint32_t w) { return __hfma2(kv4_in(w, 0x00f000f0u), kv4_bits(0x2c002c00u), kv4_bits(0xd400d400u)); }
+// a value that the compiler keeps instead of forming it again where it is used
+__device__ __forceinline__ __half2 kv4_keep(__half2 v) {
+    uint32_t r = *reinterpret_cast<const uint32_t *>(&v);
+    asm volatile("" : "+r"(r));
+    return kv4_bits(r);
+}
 __device__ __forceinline__ void kv4_pairs(uint32_t w, __half2 d, __half2 m, uint32_t (&o)[4]) {
     const __half2 a = __hfma2(kv4_low(w), d, m), b = __hfma2(kv4_high(w), d, m), c = __hfma2(kv4_low(w >> 8), d, m), e = __hfma2(kv4_high(w >> 8), d, m);
     o[0] = *reinterpret_cast<const uint32_t *>(&a); o[1] = *reinterpret_cast<const uint32_t *>(&b);

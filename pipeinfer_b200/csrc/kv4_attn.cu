@@ -107,9 +107,21 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     int64_t item_end = 0;
     ka_place at = { 0, 0, 0, 0, 0, 0 };
     float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];            // of rows 2 t and 2 t + 1 of each tile
-    const int64_t u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+    // A warp begins where an item does if that is near: items of few pages stay with one warp (a row of a chain of pieces costs 300 clocks, and the wait for what others have left in scratch)
+    if (c0 < c1) {
+        const int64_t raw = c0 + (c1 - c0) * warp / C::WARPS;
+        const int     near = max(1, (int) ((c1 - c0) / C::WARPS) / 4);
+        at = ka_find<C::RT, 0>(A, prefix, seq_of, raw);
+        int64_t u = raw;
+        if (warp > 0) {
+            if (at.p <= near && at.p <= at.np - at.p) { if (raw - at.p >= c0) { u -= at.p; at.p = 0; } }     // (not into the block before)
+            else if (at.np - at.p <= near) { u += at.np - at.p; if (u < c1) { at.p = at.np - 1; ka_next<C::RT, 0>(A, prefix, seq_of, at); } }
+        }
+        if (lane == 0) part[warp] = min(u, c1);
+    }
+    __syncthreads();
+    const int64_t u0 = c0 < c1 ? part[warp] : 0, u1 = c0 < c1 ? (warp + 1 < C::WARPS ? part[warp + 1] : c1) : 0;
     if (u0 < u1) {
-        at = ka_find<C::RT, 0>(A, prefix, seq_of, u0);
         // the stream of halves: 2 (u1 - u0) of them, the first NST ahead
         ka_place is = at;
         int      left = (int) (u1 - u0), todo = left;            // units to ask for, units to do
@@ -208,11 +220,12 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
                     for (int j = 0; j < C::KB / 16; j++) {
                         uint32_t wv[2][C::W];
-                        __half2  dm[2];
+                        __half2  d2[2], m2[2];
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
                             const int r = kb + j * 16 + x * 8 + g;
-                            dm[x] = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                            const __half2 dm = *reinterpret_cast<const __half2 *>(kp + kv4_steps(D) + (r * C::W + (t * C::W >> 2)) * 4);
+                            d2[x] = kv4_keep(__low2half2(dm)); m2[x] = kv4_keep(__high2half2(dm));
                             if constexpr (D == 128) { const uint4 v = *reinterpret_cast<const uint4 *>(kp + r * 64 + t * 16); wv[x][0] = v.x; wv[x][1] = v.y; wv[x][2] = v.z; wv[x][3] = v.w; }
                             else                    { const uint2 v = *reinterpret_cast<const uint2 *>(kp + r * 32 + t * 8); wv[x][0] = v.x; wv[x][1] = v.y; }
                         }
@@ -220,7 +233,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         for (int w = 0; w < C::W; w++) {
                             uint32_t o[2][4];
 #pragma unroll
-                            for (int x = 0; x < 2; x++) kv4_pairs(wv[x][w], __low2half2(dm[x]), __high2half2(dm[x]), o[x]);
+                            for (int x = 0; x < 2; x++) kv4_pairs(wv[x][w], d2[x], m2[x], o[x]);
 #pragma unroll
                             for (int n = 0; n < NR; n++)
 #pragma unroll
@@ -331,7 +344,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                             const int ra = kb + j * 16 + f * 8 + t, rb = ra + 4;               // kv4_row of the places 2 t and 2 t + 1
                             const __half2 da = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (ra * C::W + (g * C::W >> 3)) * 4);
                             const __half2 db = *reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (rb * C::W + (g * C::W >> 3)) * 4);
-                            d2[f] = __lows2half2(da, db); m2[f] = __highs2half2(da, db);
+                            d2[f] = kv4_keep(__lows2half2(da, db)); m2[f] = kv4_keep(__highs2half2(da, db));
                             if constexpr (D == 128) {
                                 const uint2 x = *reinterpret_cast<const uint2 *>(vp + ra * 64 + ((g * 8) ^ kv4_flip(D, ra))), y = *reinterpret_cast<const uint2 *>(vp + rb * 64 + ((g * 8) ^ kv4_flip(D, rb)));
                                 a[f][0] = x.x; a[f][1] = x.y; b[f][0] = y.x; b[f][1] = y.y;
@@ -396,48 +409,60 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     if (goes) ka_leave<C, NR>(pieces + warp * C::PIECE, C::RT, g, t, O, m, l);
     __syncthreads();
     if (!*abort_s && c0 < c1) {
-        // a row a warp, lanes its channels: the warps' pieces in the order of their units
+        // Chains of pieces: each ends with the piece of a warp whose item ends there, the last one goes on behind the block.  A row of a chain a warp, lanes its channels: maxima and sums of the pieces a lane
+        // each, then their rows; loads wait for nothing but these
         constexpr int CH = D / 32;
-        for (int ri = warp; ri < C::RT; ri += C::WARPS) {
-            float am = -INFINITY, al = 0.f, ao[CH];
-            bool  some = false, ours = false;                        // a chain of pieces is under way; it began in this block
-            auto add = [&](const float * p) {
-                const float pm = p[C::RT * D + ri], pl = p[C::RT * D + C::RT + ri], mn = fmaxf(am, pm), a = am == mn ? 1.f : exp2f(am - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
-                am = mn; al = al * a + pl * f;
+        const int fl = lane < C::WARPS ? flags[lane] : 0;
+        const uint32_t all_ends = __ballot_sync(0xffffffffu, fl & 1), all_goes = __ballot_sync(0xffffffffu, fl & 2), all_begins = __ballot_sync(0xffffffffu, fl & 4);
+        int my_end = C::WARPS;                                       // of the chain that has the lane's number; the last chain: none
+        { uint32_t b = all_ends; for (int k = 0; b; k++, b &= b - 1) if (k == lane) my_end = __ffs(b) - 1; }
+        constexpr int MANY = NR == 1 ? 1 : 4;                                      // rows of chains at a time: what they load is under way together
+        const int tasks = (__popc(all_ends) + 1) * C::RT;
+        for (int task0 = warp * MANY; task0 < tasks; task0 += C::WARPS * MANY) {
+            float lv[MANY][CH], pm[MANY], pl[MANY];
+            uint32_t mine[MANY];
+            int   end[MANY];
+            bool  ours[MANY], does[MANY];
 #pragma unroll
-                for (int c = 0; c < CH; c++) ao[c] = ao[c] * a + p[ri * D + lane * CH + c] * f;
-            };
-            auto start = [&]() {
-                am = -INFINITY; al = 0.f;
+            for (int k = 0; k < MANY; k++) {
+                const int ri = (task0 + k) % C::RT, chain = (task0 + k) / C::RT, from = __shfl_sync(0xffffffffu, my_end, max(chain - 1, 0) & 31);
+                end[k] = __shfl_sync(0xffffffffu, my_end, chain & 31);
+                // pieces in shared memory (the warp where the chain before ends may begin this one); the one of warp `end` is in scratch
+                const uint32_t span = ((1u << end[k]) - 1) & ~((1u << (chain ? from : 0)) - 1);
+                mine[k] = all_goes & span;
+                ours[k] = (all_begins & span) != 0;
+                const bool closed = end[k] < C::WARPS;
+                does[k] = task0 + k < tasks && (closed ? ri < items[end[k]].rows : mine[k] != 0);      // (rows of an open chain that are none are read by nobody)
+                const bool take = (mine[k] >> lane & 1) || (closed && lane == end[k]);
+                const float * last = A.heads + (int64_t) (blockIdx.x * C::WARPS + end[k]) * C::PIECE, * p = closed && lane == end[k] ? last : pieces + lane * C::PIECE;
 #pragma unroll
-                for (int c = 0; c < CH; c++) ao[c] = 0.f;
-            };
-            auto leave = [&](int slot) {
-                float * p = A.pieces + (int64_t) (2 * blockIdx.x + slot) * C::PIECE;
+                for (int c = 0; c < CH; c++) lv[k][c] = does[k] && closed ? last[ri * D + lane * CH + c] : 0.f;
+                pm[k] = does[k] && take ? p[C::RT * D + ri] : -INFINITY;
+                pl[k] = does[k] && take ? p[C::RT * D + C::RT + ri] : 0.f;
+            }
 #pragma unroll
-                for (int c = 0; c < CH; c++) p[ri * D + lane * CH + c] = ao[c];
-                if (lane == 0) { p[C::RT * D + ri] = am; p[C::RT * D + C::RT + ri] = al; }
-            };
-            start();
-            for (int w = 0; w < C::WARPS; w++) {
-                const int f = flags[w];
-                if (f & 1) {
-                    const ka_open it = items[w];
-                    if (ri < it.rows) {
-                        add(A.heads + (int64_t) (blockIdx.x * C::WARPS + w) * C::PIECE);
-                        if (ours) ka_row_out<T, D>(A, it, ri, lane, ao, al);
-                        else      leave(0);
-                    }
-                    start();
-                    some = ours = false;
+            for (int k = 0; k < MANY; k++) {
+                if (!does[k]) continue;
+                const int   ri = (task0 + k) % C::RT;
+                const bool  closed = end[k] < C::WARPS;
+                const float am = warp_max(pm[k]), f = pm[k] == am ? 1.f : exp2f(pm[k] - am), al = warp_sum(pl[k] * f), fe = __shfl_sync(0xffffffffu, f, end[k] & 31);
+                float ao[CH];
+#pragma unroll
+                for (int c = 0; c < CH; c++) ao[c] = closed ? lv[k][c] * fe : 0.f;
+                for (uint32_t rest = mine[k]; rest; rest &= rest - 1) {
+                    const int   w = __ffs(rest) - 1;
+                    const float fw = __shfl_sync(0xffffffffu, f, w);
+#pragma unroll
+                    for (int c = 0; c < CH; c++) ao[c] = fmaf(pieces[w * C::PIECE + ri * D + lane * CH + c], fw, ao[c]);
                 }
-                if (f & 2) {
-                    if (f & 4) ours = true;
-                    some = true;
-                    if (ri < last_item[w].rows) add(pieces + w * C::PIECE);
+                if (closed && ours[k]) ka_row_out<T, D>(A, items[end[k]], ri, lane, ao, al);
+                else {
+                    float * q = A.pieces + (int64_t) (2 * blockIdx.x + (ours[k] ? 1 : 0)) * C::PIECE;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) q[ri * D + lane * CH + c] = ao[c];
+                    if (lane == 0) { q[C::RT * D + ri] = am; q[C::RT * D + C::RT + ri] = al; }
                 }
             }
-            if (some) leave(ours ? 1 : 0);
         }
     }
     // the last warp with units knows whether the run's last item goes on
