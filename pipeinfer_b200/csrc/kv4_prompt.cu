@@ -3,9 +3,9 @@
 // A block takes 256 rows (token, head of the group) of one key / value head as two groups of 128 and walks the pages they see; pages of all such items lie in one row that the blocks of the GPU (one an
 // SM) divide evenly, whatever the sequences' lengths (kv4_attn.cuh).  An item that lies in one block's run is written at once; pieces of others go to scratch and kv4_prompt_join_kernel adds them up.
 //   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
-//   warps 4..7    write a page's keys [64][dim] and its values, turned, [dim][64] as fp16 into tiles of the 128-byte swizzle, two of each
-//   warp 1        issues the MMAs: scores S = Q K' of the next page, then O += P V of this one, for both groups
-//   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 back into tensor memory, from where they enter the second product
+//   warps 4..7    write two pages' keys [128][dim] and their values, turned, [dim][128] as fp16 into tiles of the 128-byte swizzle
+//   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; one group's products run while the other forms weights
+//   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 into the scores' place, from where they enter the second product
 // fp32 queries and weights enter as fp16 part and remainder, two products each; of bfloat16 rows both are one fp16 number.
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
@@ -18,12 +18,12 @@
 
 template <typename T, int D> struct kp_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
-    static constexpr int  RAW = SPLIT ? 2 : 3, W = D / 32, NC = D / 64;              // records under way; groups; 64-wide column chunks of a head
+    static constexpr int  W = D / 32, NC = D / 64, STG = SPLIT ? 1 : 2;               // groups; 64-wide column chunks of a head; tiles of keys and of values
     static constexpr int  Q_CHUNK = 128 * 128, Q_PART = 2 * NC * Q_CHUNK;            // both groups' rows: [group][chunk][128 rows][128 bytes]
-    static constexpr int  Q_BYTES = Q_PART * (SPLIT ? 2 : 1), K_CHUNK = 64 * 128, K_TILE = NC * K_CHUNK, V_TILE = D * 128;
-    static constexpr int  TILES = Q_BYTES + 2 * (K_TILE + V_TILE), REC = kv4_record(D);
+    static constexpr int  Q_BYTES = Q_PART * (SPLIT ? 2 : 1), K_CHUNK = 128 * 128, K_TILE = NC * K_CHUNK, V_CHUNK = D * 128, V_TILE = 2 * V_CHUNK;
+    static constexpr int  TILES = Q_BYTES + STG * (K_TILE + V_TILE), REC = kv4_record(D);
     static constexpr int  PIECE = KP_ROWS * (D + 2);                                 // floats
-    static constexpr size_t FIXED = (size_t) TILES + RAW * REC + KP_BARS * 8 + 128 + 1024;
+    static constexpr size_t FIXED = (size_t) TILES + KP_BARS * 8 + 256 + 1024;          // without records and the table
 };
 
 // A in tensor memory, B in shared memory; called by a converged warp
@@ -69,24 +69,24 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     using C = kp_cfg<T, D>;
     extern __shared__ __align__(1024) uint8_t kp_dsm[];
     uint8_t *  sQ   = kp_dsm + ((1024u - (dt_smem(kp_dsm) & 1023u)) & 1023u);
-    uint8_t *  sK   = sQ + C::Q_BYTES, * sV = sK + 2 * C::K_TILE, * raw = sV + 2 * C::V_TILE;
-    uint64_t * bar  = reinterpret_cast<uint64_t *>(raw + C::RAW * C::REC);
+    const int  RAW = A.stages;                                   // records under way: 2 or 3
+    uint8_t *  sK   = sQ + C::Q_BYTES, * sV = sK + C::STG * C::K_TILE, * raw = sV + C::STG * C::V_TILE;
+    uint64_t * bar  = reinterpret_cast<uint64_t *>(raw + RAW * C::REC);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bar + KP_BARS);
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int * raw_in = reinterpret_cast<volatile int *>(tmem_slot + 2);         // [RAW] whether the record's page is one of the cache's
-    volatile unsigned long long * v_none = reinterpret_cast<volatile unsigned long long *>(tmem_slot + 12);      // [2][W] places of a page whose values are none, of each group
-    int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 128);       // [seqs + 1]
+    volatile unsigned long long * v_none = reinterpret_cast<volatile unsigned long long *>(tmem_slot + 12);      // [STG][2][W] places of a page whose values are none, of each group
+    int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 256);       // [seqs + 1]
     __shared__ int64_t part[KP_THREADS / 32];
-    // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there and weights written (of two pages: a group may be one ahead
-    // of the other), product done
-    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_p = b0 + 176, bar_o = b0 + 208;
+    // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there, weights written, product done
+    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_p = b0 + 160, bar_o = b0 + 176;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::RAW; i++) { dt_mbar_init(bar_rf + 8 * i, 1); dt_mbar_init(bar_re + 8 * i, 4); }
+        for (int i = 0; i < RAW; i++) { dt_mbar_init(bar_rf + 8 * i, 1); dt_mbar_init(bar_re + 8 * i, 4); }
         for (int i = 0; i < 2; i++) {
             dt_mbar_init(bar_kf + 8 * i, 4); dt_mbar_init(bar_vf + 8 * i, 4);
-            for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_s + 16, bar_o }) dt_mbar_init(b + 8 * i, 1);
-            dt_mbar_init(bar_q + 8 * i, 4); dt_mbar_init(bar_p + 8 * i, 4); dt_mbar_init(bar_p + 16 + 8 * i, 4);
+            for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_o }) dt_mbar_init(b + 8 * i, 1);
+            dt_mbar_init(bar_q + 8 * i, 4); dt_mbar_init(bar_p + 8 * i, 4);
         }
         *abort_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     dt_fence_after();
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
-    const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, for each group; the weights take their scores' place; outputs 256..383 and 384..511
+    const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, of both groups; the weights take their scores' place; outputs 256..383 and 384..511
     int    last_s = -1;
     ka_seq last = { 0, 0 };
     auto seq_of = [&](int s) {                                   // the tables' entries of the sequence at hand stay in registers
@@ -165,61 +165,74 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         ka_bulk(dt_smem(raw + st * C::REC), A.base + ((int64_t) id * A.kvh + at.h) * C::REC, C::REC, bar_rf + 8 * st);
                     } else dt_arrive(bar_rf + 8 * st);
                 }
-                if (++st == C::RAW) { st = 0; ph ^= 1; }
+                if (++st == RAW) { st = 0; ph ^= 1; }
             }
             return true;
         });
     } else if (warp == 1) {
-        constexpr uint32_t id_s = kp_idesc(128, 64), id_o = kp_idesc(128, D);
+        constexpr uint32_t id_o = kp_idesc(128, D);
         const uint64_t dq = dt_desc(dt_smem(sQ)), dk = dt_desc(dt_smem(sK)), dv = dt_desc(dt_smem(sV));
-        int      j = 0, n_q[2] = { 0, 0 }, n_p[2] = { 0, 0 };
-        uint32_t p_ph[2] = { 0, 0 };                             // the phases of the weights' barriers
+        int      j = 0, n_q[2] = { 0, 0 }, n_p[2] = { 0, 0 };     // steps of two pages; queries and weights that have entered
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
-        auto scores = [&](int jj, int groups, bool behind) {
-            if (!wait(bar_kf + 8 * (jj & 1), jj >> 1)) return false;
+        auto there = [&](uint32_t b, uint32_t ph) {
+            uint32_t ok;
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(b), "r"(ph & 1) : "memory");
+            return __all_sync(0xffffffffu, ok) != 0;
+        };
+        auto scores = [&](int w, int jj, int two) {
+            const uint32_t id_s = two ? kp_idesc(128, 128) : kp_idesc(128, 64);
+            const uint64_t a0 = dq + (uint64_t) (w * C::NC * C::Q_CHUNK >> 4), k0 = dk + (uint64_t) (jj % C::STG * C::K_TILE >> 4);
             dt_fence_after();
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                if (w >= groups) break;
-                // the weights of two pages ago, which lie there, have entered their product (MMAs of different accumulators may overtake each other)
-                if (behind && !wait(bar_o + 8 * w, n_p[w] + 1)) return false;
-                dt_fence_after();
-                bool acc = false;
+            for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
+#pragma unroll
+                for (int c = 0; c < C::NC; c++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) dt_mma(tmem + 128 * w, a0 + ((part_ * C::Q_PART + c * C::Q_CHUNK) >> 4) + 2 * k, k0 + (c * C::K_CHUNK >> 4) + 2 * k, id_s, (part_ | c | k) != 0);
+            dt_commit(bar_s + 8 * w);
+        };
+        auto outputs = [&](int w, int two, bool add) {
+            const uint64_t v0 = dv + (uint64_t) (j % C::STG * C::V_TILE >> 4);
+            dt_fence_after();
+#pragma unroll 1
+            for (int h = 0; h <= two; h++)
 #pragma unroll
                 for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
 #pragma unroll
-                    for (int c = 0; c < C::NC; c++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            dt_mma(tmem + 128 * w + 64 * (jj & 1), dq + (uint64_t) ((part_ * C::Q_PART + (w * C::NC + c) * C::Q_CHUNK) >> 4) + 2 * k, dk + (uint64_t) (((jj & 1) * C::K_TILE + c * C::K_CHUNK) >> 4) + 2 * k, id_s, acc);
-                            acc = true;
-                        }
-                dt_commit(bar_s + 16 * w + 8 * (jj & 1));
-            }
-            dt_commit(bar_ke + 8 * (jj & 1));
-            return true;
+                    for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * h + 32 * part_ + 8 * k, v0 + (uint64_t) (h * C::V_CHUNK >> 4) + 2 * k, id_o, add || (h | part_ | k) != 0);
+            dt_commit(bar_o + 8 * w);
         };
         items([&](ka_seq, const ka_place &, int rows, int, int pages) {
-            const int groups = rows > 128 ? 2 : 1;
-            for (int w = 0; w < groups; w++) if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
-            if (!scores(j, groups, false)) return false;
-            for (int i = 0; i < pages; i++, j++) {
-                if (i + 1 < pages && !scores(j + 1, groups, i > 0)) return false;
-                if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
+            const int groups = rows > 128 ? 2 : 1, steps = (pages + 1) / 2;
+            if (!wait(bar_kf + 8 * (j % C::STG), j / C::STG)) return false;
+            for (int w = 0; w < groups; w++) {
+                if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
+                scores(w, j, pages > 1);
+            }
+            dt_commit(bar_ke + 8 * (j % C::STG));
+            for (int i = 0; i < steps; i++, j++) {
+                // what the groups wait for, in the order in which it comes: weights, then the end of their product
+                int  to_do = (i + 1 < steps ? 2 : 1) * groups, done[2] = { 0, 0 }, n_v = 0, n_k = 0;
+                uint32_t spins = 0;
+                while (to_do) {
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    if (w >= groups) break;
-                    if (!wait(bar_p + 16 * w + 8 * (j & 1), p_ph[w] >> (j & 1))) return false;
-                    p_ph[w] ^= 1u << (j & 1);
-                    n_p[w]++;
-                    dt_fence_after();
-#pragma unroll
-                    for (int part_ = 0; part_ < (C::SPLIT ? 2 : 1); part_++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * (j & 1) + (C::SPLIT ? 32 * (k >> 1) + 16 * part_ + 8 * (k & 1) : 8 * k), dv + (uint64_t) ((j & 1) * C::V_TILE >> 4) + 2 * k, id_o, (i > 0) | ((part_ | k) != 0));
-                    dt_commit(bar_o + 8 * w);
+                    for (int w = 0; w < 2; w++) {
+                        if (w >= groups) break;
+                        if (done[w] == 0 && there(bar_p + 8 * w, n_p[w])) {
+                            if (n_v == 0 && !wait(bar_vf + 8 * (j % C::STG), j / C::STG)) return false;
+                            outputs(w, 2 * i + 1 < pages, i > 0);
+                            n_p[w]++; done[w] = 1; to_do--; spins = 0;
+                            if (++n_v == groups) dt_commit(bar_ve + 8 * (j % C::STG));
+                        } else if (done[w] == 1 && i + 1 < steps && there(bar_o + 8 * w, n_p[w] + 1)) {
+                            if (n_k == 0 && !wait(bar_kf + 8 * ((j + 1) % C::STG), (j + 1) / C::STG)) return false;
+                            scores(w, j + 1, 2 * i + 3 < pages);
+                            done[w] = 2; to_do--; spins = 0;
+                            if (++n_k == groups) dt_commit(bar_ke + 8 * ((j + 1) % C::STG));
+                        }
+                    }
+                    if (++spins > DT_SPIN) *abort_s = 1;
+                    if ((spins & 63) == 63 && *abort_s) return false;
                 }
-                dt_commit(bar_ve + 8 * (j & 1));
             }
             return true;
         });
@@ -231,20 +244,26 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         int       j = 0, st = 0;
         uint32_t  ph = 0;
         items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
-            for (int i = 0; i < pages; i++, j++) {
-                const uint8_t * rec = raw + st * C::REC, * vr = rec + kv4_half(D);
-                const bool edge = edge_of(q, at, rows, (at.first + p0 + i) * KV4_P);
-                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_rf + 8 * st, ph, abort_s) && dt_mbar_wait(bar_ke + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_s))) return false;
-                const bool in = raw_in[st] != 0;
-                {   // keys: a thread has 32 channels (two times) of one key; of a group's four words the lanes start with different ones, for the banks
-                    uint8_t * to = sK + (j & 1) * C::K_TILE;
+            for (int i = 0; i < pages; i += 2, j++) {
+                const int two = i + 1 < pages, sg = j % C::STG;
+                const uint32_t free_ph = (j / C::STG & 1) ^ 1;
+                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ke + 8 * sg, free_ph, abort_s))) return false;
+                int      s1 = st;
+                uint32_t p1 = ph;
+#pragma unroll 1
+                for (int h = 0; h <= two; h++) {
+                    // keys: a thread has 32 channels (two times) of one key; of a group's four words the lanes start with different ones, for the banks
+                    if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_rf + 8 * s1, p1, abort_s))) return false;
+                    const bool in = raw_in[s1] != 0;
+                    const uint8_t * rec = raw + s1 * C::REC;
+                    uint8_t * to = sK + sg * C::K_TILE + h * 64 * 128;
                     const int key = tid & 63, half = tid >> 6;
 #pragma unroll
                     for (int x = 0; x < C::W / 2; x++) {
                         const int     cc = D == 128 ? (2 * half + x + (key >> 1)) & 3 : half;
                         const uint4   n = *reinterpret_cast<const uint4 *>(rec + key * (D / 2) + cc * 16);
                         const __half2 dm = *reinterpret_cast<const __half2 *>(rec + kv4_steps(D) + (key * C::W + cc) * 4);
-                        const __half2 d2 = __low2half2(dm), m2 = __high2half2(dm);
+                        const __half2 d2 = kv4_keep(__low2half2(dm)), m2 = kv4_keep(__high2half2(dm));
                         const uint32_t wv[4] = { n.x, n.y, n.z, n.w };
 #pragma unroll
                         for (int w = 0; w < 4; w++) {
@@ -253,13 +272,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                             *reinterpret_cast<uint4 *>(to + (cc >> 1) * C::K_CHUNK + key * 128 + ((((cc & 1) * 4 + w) ^ (key & 7)) << 4)) = in ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
                         }
                     }
-                    dt_fence_async();
-                    __syncwarp();
-                    if (lane == 0) dt_arrive(bar_kf + 8 * (j & 1));
+                    if (++s1 == RAW) { s1 = 0; p1 ^= 1; }
                 }
-                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ve + 8 * (j & 1), ((j >> 1) & 1) ^ 1, abort_s))) return false;
-                {   // values: a thread has eight keys (an octet, a piece of 16 bytes in the turned tile) of eight (heads of 64: four) neighbouring channels
-                    uint8_t * to = sV + (j & 1) * C::V_TILE;
+                dt_fence_async();
+                __syncwarp();
+                if (lane == 0) dt_arrive(bar_kf + 8 * sg);
+                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ve + 8 * sg, free_ph, abort_s))) return false;
+#pragma unroll 1
+                for (int h = 0; h <= two; h++) {
+                    // values: a thread has eight keys (an octet, a piece of 16 bytes in the turned tile) of eight (heads of 64: four) neighbouring channels
+                    const bool in = raw_in[st] != 0;
+                    const uint8_t * vr = raw + st * C::REC + kv4_half(D);
+                    uint8_t * to = sV + sg * C::V_TILE + h * C::V_CHUNK;
                     const int oct = tid & 7, o8 = D == 128 ? ((tid >> 5) * 4 + (lane >> 3) + 2 * oct) & 15 : (tid >> 3) & 7;
                     uint32_t n[8];
                     __half2  dm[8];
@@ -269,13 +293,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         n[k]  = *reinterpret_cast<const uint32_t *>(vr + r * (D / 2) + ((o8 * 4) ^ kv4_flip(D, r)));
                         dm[k] = *reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (r * C::W + (o8 >> 2)) * 4);
                     }
-                    if (edge) {
+                    if (edge_of(q, at, rows, (at.first + p0 + i + h) * KV4_P)) {
                         // values that are none, on a page of which some row does not see all: they take part as zeros, and the rows that see one are told
                         if (tid < C::W) {
                             unsigned long long none = 0;
                             for (int k = 0; k < KV4_P; k++)
                                 if (in && __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (kv4_row(k) * C::W + tid) * 4)))) none |= 1ull << k;
-                            v_none[(j & 1) * C::W + tid] = none;
+                            v_none[(sg * 2 + h) * C::W + tid] = none;
                         }
 #pragma unroll
                         for (int k = 0; k < 8; k++) if (__hisnan(__high2half(dm[k]))) dm[k] = kv4_bits(0);
@@ -292,11 +316,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                             *reinterpret_cast<uint4 *>(to + row * 128 + ((oct ^ (row & 7)) << 4)) = in ? make_uint4(v[0][c], v[1][c], v[2][c], v[3][c]) : make_uint4(0, 0, 0, 0);
                         }
                     }
-                    dt_fence_async();
                     __syncwarp();
-                    if (lane == 0) { dt_arrive(bar_vf + 8 * (j & 1)); dt_arrive(bar_re + 8 * st); }
+                    if (lane == 0) dt_arrive(bar_re + 8 * st);
+                    if (++st == RAW) { st = 0; ph ^= 1; }
                 }
-                if (++st == C::RAW) { st = 0; ph ^= 1; }
+                dt_fence_async();
+                __syncwarp();
+                if (lane == 0) dt_arrive(bar_vf + 8 * sg);
             }
             return true;
         });
@@ -304,15 +330,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         // ---- a row a thread
         const int w = (warp - 8) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
-        const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s0 = tmem + lanes + 128 * w, tm_w = tm_o + lanes + 128 * w;
-        int j = 0, n = 0;                                        // pages of the run, and those of which this group has scores
-        uint32_t s_ph = 0;                                       // the phases of both scores' barriers
+        const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s = tmem + lanes + 128 * w, tm_w = tm_o + lanes + 128 * w;
+        int j = 0, n = 0;                                        // steps of the run, and those of which this group has scores
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
         items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
             const int     row0 = at.r * KP_ROWS, ri = w * 128 + rt, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, hi = q.len - q.n + tk, lo = A.window > 0 ? max(0, hi - A.window + 1) : 0;
             const int64_t tok = min(max(A.starts[at.s], 0), A.tokens) + tk, head = at.h * A.rep + rc % A.rep;
             const bool    on = w == 0 || rows > 128;
-            if (!on) { j += pages; return true; }
+            if (!on) { j += (pages + 1) / 2; return true; }
             auto some = [&](int pg) { return pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1; };
             int ids = some(at.first + p0);
             float qs;
@@ -348,44 +373,50 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             if (lane == 0) dt_arrive(bar_q + 8 * w);
             float    m = -INFINITY, l = 0.f, l2 = 0.f;
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
-            for (int i = 0; i < pages; i++, j++, n++) {
-                const int key0 = (at.first + p0 + i) * KV4_P;
-                const uint32_t tm_s = tm_s0 + 64 * (j & 1);
+            for (int i = 0; i < pages; i += 2, j++, n++) {
+                const int two = i + 1 < pages;
                 if (i > 0 && (i & 31) == 0) ids = some(at.first + p0 + i);
-                const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
-                const bool in = id >= 0 && id < A.pages;
-                if (!wait(bar_s + 16 * w + 8 * (j & 1), s_ph >> (j & 1))) return false;
-                s_ph ^= 1u << (j & 1);
+                const int  id0 = __shfl_sync(0xffffffffu, ids, i & 31), id1 = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
+                if (!wait(bar_s + 8 * w, n)) return false;
                 dt_fence_after();
                 uint32_t t[64];
-                dt_ld32(tm_s, t);
-                dt_ld32(tm_s + 32, t + 32);
-                dt_wait_ld();
-                if (!in || edge_of(q, at, rows, key0)) {
-                    const int a = in ? lo - key0 : 64, b = hi - key0;
+                // a page's scores; keys that the row does not see are at -inf
+                auto load = [&](int h) {
+                    dt_ld32(tm_s + 64 * h, t);
+                    dt_ld32(tm_s + 64 * h + 32, t + 32);
+                    dt_wait_ld();
+                    const int  key0 = (at.first + p0 + i + h) * KV4_P, id = h ? id1 : id0;
+                    const bool in = id >= 0 && id < A.pages;
+                    if (!in || edge_of(q, at, rows, key0)) {
+                        const int a = in ? lo - key0 : 64, b = hi - key0;
 #pragma unroll
-                    for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = 0xff800000u;
-                    if (in) {
-                        if (!wait(bar_vf + 8 * (j & 1), j >> 1)) return false;
+                        for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = 0xff800000u;
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h <= two; h++) {
+                    load(h);
+#pragma unroll
+                    for (int x = 0; x < 64; x++) top = fmaxf(top, __uint_as_float(t[x]));
+                    const int  key0 = (at.first + p0 + i + h) * KV4_P, id = h ? id1 : id0;
+                    if (id >= 0 && id < A.pages && edge_of(q, at, rows, key0)) {
+                        const int a = lo - key0, b = hi - key0;
+                        if (!wait(bar_vf + 8 * (j % C::STG), j / C::STG)) return false;
                         if (b >= 0 && a < 64) {
                             const unsigned long long seen = (b >= 63 ? ~0ull : (1ull << (b + 1)) - 1) & ~(a > 0 ? (1ull << a) - 1 : 0ull);
 #pragma unroll
-                            for (int g = 0; g < C::W; g++) if (v_none[(j & 1) * C::W + g] & seen) none |= 1u << g;
+                            for (int g = 0; g < C::W; g++) if (v_none[((j % C::STG) * 2 + h) * C::W + g] & seen) none |= 1u << g;
                         }
                     }
                 }
-                float top = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 64; x++) top = fmaxf(top, __uint_as_float(t[x]));
                 top *= qs;
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
                 if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
-                if (i > 0 && rescale) {
-                    if (!wait(bar_o + 8 * w, n + 1)) return false;           // the product before has left the accumulator
-                    dt_fence_after();
+                if (i > 0 && rescale) {                          // (these scores came behind the end of the product before)
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t v[32];
@@ -396,27 +427,32 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         dt_st32(tm_w + c, v);
                     }
                 }
+                // the last page's scores are in registers still
+#pragma unroll 1
+                for (int h = two; h >= 0; h--) {
+                    if (h != two) load(h);
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t h[16], r[16];
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t e[16], r[16];
 #pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), qs, base));
-                        l += a; l2 += b;
-                        h[x] = ka_pack(a, b);
-                        if (C::SPLIT) r[x] = ka_rest(a, b, h[x]);
+                        for (int x = 0; x < 16; x++) {
+                            const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), qs, base));
+                            l += a; l2 += b;
+                            e[x] = ka_pack(a, b);
+                            if (C::SPLIT) r[x] = ka_rest(a, b, e[x]);
+                        }
+                        // in the page's scores' place, parts behind each other
+                        kp_st16(tm_s + 64 * h + 16 * c, e);
+                        if (C::SPLIT) kp_st16(tm_s + 64 * h + 32 + 16 * c, r);
                     }
-                    // in the scores' place
-                    kp_st16(tm_s + (C::SPLIT ? 32 : 16) * c, h);
-                    if (C::SPLIT) kp_st16(tm_s + 32 * c + 16, r);
                 }
                 dt_wait_st();
                 dt_fence_before();
                 __syncwarp();
-                if (lane == 0) dt_arrive(bar_p + 16 * w + 8 * (j & 1));
+                if (lane == 0) dt_arrive(bar_p + 8 * w);
             }
-            // ---- the row out, behind the last product (and the one before it, which nothing has waited for: a phase two ahead would look like the one behind)
-            if ((pages > 1 && !wait(bar_o + 8 * w, n)) || !wait(bar_o + 8 * w, n + 1)) return false;
+            // ---- the row out, behind the last product
+            if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
             const bool    whole = p0 == 0 && pages == at.np - KP_LEAD;
             const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
@@ -499,10 +535,14 @@ static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __gri
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
-template <typename T, int D> static int kp_go(const ka_args & A, cudaStream_t st) {
+template <typename T, int D> static int kp_go(ka_args A, cudaStream_t st) {
     using C = kp_cfg<T, D>;
-    const size_t smem = C::FIXED + (size_t) (A.seqs + 1) * 8, most = C::FIXED + (size_t) (PIB_KV4_MAX_SEQS + 1) * 8;
-    static_assert(C::FIXED + (PIB_KV4_MAX_SEQS + 1) * 8 + 256 <= 227 * 1024, "shared memory");
+    // three records under way where the sequences' table leaves room for them
+    constexpr size_t most = 226 * 1024;
+    const size_t need = C::FIXED + (size_t) (A.seqs + 1) * 8;
+    static_assert(C::FIXED + (PIB_KV4_MAX_SEQS + 1) * 8 + 2 * C::REC <= most, "shared memory");
+    A.stages = need + 3 * C::REC <= most ? 3 : 2;
+    const size_t smem = need + (size_t) A.stages * C::REC;
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
     PIB_CHECK(pib_launch(kv4_prompt_kernel<T, D>, dim3((unsigned) pib_num_sms()), dim3(KP_THREADS), smem, st, A));
