@@ -37,6 +37,10 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr int  PIECE = RT * (D + 2);                      // floats
 };
 
+// what happens once an item is a call: the loop over pages is long enough
+template <int RT> __device__ __noinline__ ka_place ka_find_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, int64_t u) { return ka_find<RT, 0>(A, prefix, seq, u); }
+template <int RT> __device__ __noinline__ ka_place ka_next_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place c) { ka_next_item<RT, 0>(A, prefix, seq, c); return c; }
+template <int RT> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place & c) { if (++c.p >= c.np) c = ka_next_call<RT>(A, prefix, seq, c); }
 // a warp's piece of an item: sums of the rows that there are, their maxima and denominators
 template <typename C, int NR>
 __device__ __forceinline__ void ka_leave(float * p, int rows, int g, int t, const float (&O)[NR][C::MT][4], const float (&m)[NR][2], const float (&l)[NR][2]) {
@@ -83,24 +87,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pib_pdl_wait();
     pib_pdl_trigger();
-    const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32>(A, prefix, part, [&](int s, ka_seq q) { seq[s] = q; });
+    const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32, ka_seq_table>(A, prefix, part, { seq });
     const int     runs = (int) min((int64_t) gridDim.x, U);
     const int64_t c0 = blockIdx.x < runs ? U * blockIdx.x / runs : 0, c1 = blockIdx.x < runs ? U * (blockIdx.x + 1) / runs : 0;
-    auto seq_of = [&](int s) { return seq[s]; };
-    // rows of tiles without pages
-    for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
-        const ka_seq  q = seq[s];
-        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
-        for (int r = 0; r < ka_tiles<C::RT>(A, q); r++) {
-            int first;
-            if (ka_pages<C::RT>(A, q, r, first)) continue;
-            const int row0 = r * C::RT, rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - row0);
-            for (int i = threadIdx.x; i < rows * A.kvh * D; i += C::WARPS * 32) {
-                const int c = i % D, h = i / D % A.kvh, rc = row0 + i / D / A.kvh;
-                ((T *) A.out)[(tok0 + rc / A.rep) * A.ldo + (int64_t) (h * A.rep + rc % A.rep) * D + c] = (T) 0.f;
-            }
-        }
-    }
+    const ka_seq_table seq_of = { seq };
+    ka_zero_rows<C::RT, C::WARPS * 32, T>(A, D);
     bool ok = true;
     // the warp's pieces of items that lie in several warps' units: one that ends here (in scratch), one that does not (in registers)
     bool    ends = false, goes = false, begins = false;
@@ -111,11 +102,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     if (c0 < c1) {
         const int64_t raw = c0 + (c1 - c0) * warp / C::WARPS;
         const int     near = max(1, (int) ((c1 - c0) / C::WARPS) / 4);
-        at = ka_find<C::RT, 0>(A, prefix, seq_of, raw);
+        at = ka_find_call<C::RT>(A, prefix, seq_of, raw);
         int64_t u = raw;
         if (warp > 0) {
             if (at.p <= near && at.p <= at.np - at.p) { if (raw - at.p >= c0) { u -= at.p; at.p = 0; } }     // (not into the block before)
-            else if (at.np - at.p <= near) { u += at.np - at.p; if (u < c1) { at.p = at.np - 1; ka_next<C::RT, 0>(A, prefix, seq_of, at); } }
+            else if (at.np - at.p <= near) { u += at.np - at.p; if (u < c1) { at.p = at.np - 1; ka_next<C::RT>(A, prefix, seq_of, at); } }
         }
         if (lane == 0) part[warp] = min(u, c1);
     }
@@ -146,13 +137,16 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             }
             there = in ? there | 1u << ist : there & ~(1u << ist);
             if (++ist == NST) ist = 0;
-            if (ihalf) { left--; if (left) ka_next<C::RT, 0>(A, prefix, seq_of, is); }
+            if (ihalf) { left--; if (left) ka_next<C::RT>(A, prefix, seq_of, is); }
             ihalf ^= 1;
         };
+#pragma unroll 1
         for (int i = 0; i < NST; i++) issue();
 
         int st = 0;
         uint32_t ph = 0;
+#pragma unroll 1
+#pragma unroll 1
         while (todo && ok) {
             // ---- an item, or the piece of it in this warp's run
             const ka_seq  q = seq[at.s];
@@ -167,7 +161,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 const int rc = row0 + min(n * 8 + g, rows - 1), tk = rc / A.rep;
                 const T * p = (const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4);
                 float v[D / 4], top = 0.f;
-                ka_load<T, D / 4>(p, A.wide_q, v);
+                ka_load<T, D / 4>(p, ka_here(A.wide_q), v);
 #pragma unroll
                 for (int c = 0; c < D / 4; c++) { v[c] *= A.scale * KA_LOG2E; top = fmaxf(top, fabsf(v[c])); }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -192,11 +186,12 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                     for (int c = 0; c < 4; c++) O[n][i][c] = 0.f;
             }
             // keys that all rows see: from the last token's first one to the first token's last
-            const int all_hi = pos0 + row0 / A.rep, all_lo = A.window > 0 ? pos0 + (row0 + rows - 1) / A.rep - A.window + 1 : 0;
+            const int all_hi = pos0 + row0 / A.rep, all_lo = max(0, pos0 + (row0 + rows - 1) / A.rep - ka_window(A) + 1);
             // the last key that row r of the tiles sees, and the first
             auto high = [&](int r) { return pos0 + (row0 + min(r, rows - 1)) / A.rep; };
-            auto low  = [&](int r) { return A.window > 0 ? max(0, high(r) - A.window + 1) : 0; };
+            auto low  = [&](int r) { return max(0, high(r) - ka_window(A) + 1); };
 
+#pragma unroll 1
             for (int i = 0; i < pages && ok; i++) {
                 const int key0 = (at.first + at.p + i) * KV4_P;
                 const bool in = there >> st & 1;
@@ -205,11 +200,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 const uint32_t vst = st, vph = ph;
                 if (++st == NST) { st = 0; ph ^= 1; }
                 uint8_t * kp = ring + kst * C::HALF, * vp = ring + vst * C::HALF;
-                ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + kst * 8, kph, abort_s));
+                ok = __all_sync(0xffffffffu, ka_wait(bar0 + kst * 8, kph, abort_s));
                 if (!ok) break;
                 if (!in) {                                       // no page: nothing was copied
                     issue();
-                    ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
+                    ok = __all_sync(0xffffffffu, ka_wait(bar0 + vst * 8, vph, abort_s));
                     if (ok) issue();
                     continue;
                 }
@@ -247,7 +242,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         }
                     }
                     if (kb == 0) {
-                        ok = __all_sync(0xffffffffu, dt_mbar_wait(bar0 + vst * 8, vph, abort_s));
+                        ok = __all_sync(0xffffffffu, ka_wait(bar0 + vst * 8, vph, abort_s));
                         if (!ok) break;
                     }
                     if (kb + C::KB == KV4_P) {                   // the keys have been read
@@ -268,6 +263,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         if (kb == 0) {
                             // values that are none, on a page of which some row does not see all: the rows that see one are none in the channels of its group, and it takes part as zeros
                             bool bad = false;
+#pragma unroll 1
                             for (int k = lane; k < KV4_P * C::W; k += 32) bad |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + k * 4)));
                             if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll
@@ -276,6 +272,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                                     for (int r = 0; r < 2; r++) {
                                         const int a = low(n * 8 + 2 * t + r) - key0, b = high(n * 8 + 2 * t + r) - key0;
                                         bool sees = false;
+#pragma unroll 1
                                         for (int k = max(a, 0); k <= min(b, KV4_P - 1); k++)
                                             sees |= __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vp + kv4_steps(D) + (kv4_row(k) * C::W + (g * C::W >> 3)) * 4)));
                                         if (sees)
@@ -283,6 +280,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                                             for (int i3 = 0; i3 < C::MT; i3++) { O[n][i3][r] = __uint_as_float(0x7fc00000u); O[n][i3][2 + r] = __uint_as_float(0x7fc00000u); }
                                     }
                                 __syncwarp();
+#pragma unroll 1
                                 for (int k = lane; k < KV4_P * C::W; k += 32) {
                                     __half2 * dm = reinterpret_cast<__half2 *>(vp + kv4_steps(D) + k * 4);
                                     if (__hisnan(__high2half(*dm))) *dm = kv4_bits(0);
@@ -392,7 +390,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
                         for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r] * inv;
                         const int rc = row0 + ri;
-                        ka_store<T, C::C8>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + g * C::C8, A.wide_o, v);
+                        ka_store<T, C::C8>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + g * C::C8, ka_here(A.wide_o), v);
                     }
             } else if (at.p + pages == at.np) {
                 ends = true;
@@ -400,7 +398,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 if (lane == 0) items[warp] = { 0, 0, row0, rows, at.h, tok0 };
             } else { goes = true; begins = at.p == 0; item_end = u1 + (at.np - at.p - pages); if (lane == 0) last_item[warp] = { 0, 0, row0, rows, at.h, tok0 }; }
             at.p += pages - 1;
-            if (todo) ka_next<C::RT, 0>(A, prefix, seq_of, at);
+            if (todo) ka_next<C::RT>(A, prefix, seq_of, at);
         }
     }
     if (lane == 0) flags[warp] = (ends ? 1 : 0) | (goes ? 2 : 0) | (begins ? 4 : 0);
@@ -415,9 +413,12 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
         const int fl = lane < C::WARPS ? flags[lane] : 0;
         const uint32_t all_ends = __ballot_sync(0xffffffffu, fl & 1), all_goes = __ballot_sync(0xffffffffu, fl & 2), all_begins = __ballot_sync(0xffffffffu, fl & 4);
         int my_end = C::WARPS;                                       // of the chain that has the lane's number; the last chain: none
-        { uint32_t b = all_ends; for (int k = 0; b; k++, b &= b - 1) if (k == lane) my_end = __ffs(b) - 1; }
+        { uint32_t b = all_ends;
+#pragma unroll 1
+            for (int k = 0; b; k++, b &= b - 1) if (k == lane) my_end = __ffs(b) - 1; }
         constexpr int MANY = NR == 1 ? 1 : 4;                                      // rows of chains at a time: what they load is under way together
         const int tasks = (__popc(all_ends) + 1) * C::RT;
+#pragma unroll 1
         for (int task0 = warp * MANY; task0 < tasks; task0 += C::WARPS * MANY) {
             float lv[MANY][CH], pm[MANY], pl[MANY];
             uint32_t mine[MANY];
@@ -449,6 +450,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 float ao[CH];
 #pragma unroll
                 for (int c = 0; c < CH; c++) ao[c] = closed ? lv[k][c] * fe : 0.f;
+#pragma unroll 1
                 for (uint32_t rest = mine[k]; rest; rest &= rest - 1) {
                     const int   w = __ffs(rest) - 1;
                     const float fw = __shfl_sync(0xffffffffu, f, w);
@@ -469,6 +471,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     if (blockIdx.x < runs && u1 == c1 && u0 < u1 && lane == 0) {
         ka_open o = last_item[warp];
         bool ours = begins;                                          // of a chain through several warps: where it began
+#pragma unroll 1
         for (int w = warp - 1; w >= 0 && !ours; w--) {               // (warps without units in between have no flags)
             if (flags[w] & 4) ours = true;
             if (flags[w] & 1) break;
@@ -481,6 +484,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     __syncthreads();
     if (*abort_s) {                                              // a wait ran out: say so, give copies still in flight time to land (bounded)
         if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
+#pragma unroll 1
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
     }
 }

@@ -13,6 +13,21 @@ struct ka_args {
     int stages; float * pieces, * heads; struct ka_plan * plan; struct ka_open * open; int * err;
 };
 
+// a condition that stays where it is written: of one that holds for a whole loop the compiler makes two loops (of three, eight: 200 KB of code, which no instruction cache holds)
+__device__ __forceinline__ int ka_here(int v) { asm volatile("" : "+r"(v)); return v; }
+// dt_mbar_wait in few instructions: there is one at every turn, and the loops' code has to stay near
+__device__ __forceinline__ bool ka_wait(uint32_t bar, uint32_t parity, volatile int * abort_s) {
+    uint32_t ok = 0;
+#pragma unroll 1
+    for (uint32_t it = 0; it < DT_SPIN; it++) {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 63) == 63 && *abort_s) return false;
+    }
+    *abort_s = 1;
+    return false;
+}
+
 // A row's queries enter times scale log2 e, over the power of two of the largest: what scores are multiplied with is a power of two, exact, and so is the running maximum
 struct ka_power { float down, back; };
 __device__ __forceinline__ ka_power ka_power_of(float top) {
@@ -66,6 +81,8 @@ template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, boo
     }
 }
 
+// the window as a distance: none is one that reaches everything
+__device__ __forceinline__ int ka_window(const ka_args & A) { return A.window > 0 ? min(A.window, 0x7fff0000) : 0x7fff0000; }
 // ---- which keys a tile of rows sees ---------------------------------------------------------------------------------------------------
 // A sequence's rows, (token, head of the group) with the heads next to each other, are taken in tiles of RT; a tile of one key / value head is an item, its pages the units of work
 struct ka_seq { int n, len; };                      // query tokens and keys; both >= 0
@@ -77,7 +94,7 @@ __device__ __forceinline__ ka_seq ka_load_seq(const ka_args & A, int s) {
 template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_seq q, int r, int & first) {
     const int t0 = r * RT / A.rep, t1 = min(q.n - 1, ((r + 1) * RT - 1) / A.rep), p0 = q.len - q.n + t0, p1 = q.len - q.n + t1;
     const int top = min(p1 < 0 ? -1 : p1 / KV4_P, A.max_pages - 1);
-    first = A.window > 0 ? max(0, p0 - A.window + 1) / KV4_P : 0;
+    first = max(0, p0 - ka_window(A) + 1) / KV4_P;
     return max(0, top - first + 1);
 }
 template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
@@ -87,43 +104,55 @@ struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // pro
 // decode: of each run whether an item begins there and does not end there; the run where it does, its rows
 struct ka_open { int runs, last, row0, rows, h; int64_t tok0; };
 
+// a sequence's tokens and keys from a table in shared memory, or from the call's
+struct ka_seq_table { ka_seq * p; __device__ __forceinline__ ka_seq operator()(int s) const { return p[s]; } __device__ __forceinline__ void operator()(int s, ka_seq q) const { p[s] = q; } };
+struct ka_seq_none  { __device__ __forceinline__ void operator()(int, ka_seq) const {} };
+struct ka_seq_call  { const ka_args * a; __device__ __forceinline__ ka_seq operator()(int s) const { return ka_load_seq(*a, s); } };
 // A place among the units: unit p of np, page first + p - LEAD, of head h, of tile r, of sequence s.  prefix: units in front of each sequence; seq(s): its tokens and keys.  An item has LEAD units in front
 // of its pages: what its start and end cost, in pages
 struct ka_place { int s, r, h, p, np, first; };
 template <int RT, int LEAD> __device__ __forceinline__ int ka_units(const ka_args & A, ka_seq q, int r, int & first) { const int n = ka_pages<RT>(A, q, r, first); return n ? n + LEAD : 0; }
 template <int RT, int LEAD, typename Seq> __device__ __forceinline__ void ka_enter(const ka_args & A, const Seq & seq, ka_place & c) { c.np = ka_units<RT, LEAD>(A, seq(c.s), c.r, c.first); }
-// only called where there is a next unit
-template <int RT, int LEAD, typename Seq> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, const Seq & seq, ka_place & c) {
-    if (++c.p < c.np) return;
+// the item behind c's; only called where there is one
+template <int RT, int LEAD, typename Seq> __device__ __forceinline__ void ka_next_item(const ka_args & A, const int64_t * prefix, const Seq & seq, ka_place & c) {
     c.p = 0;
     if (++c.h < A.kvh) return;
     c.h = 0;
+#pragma unroll 1
     do {
-        if (++c.r >= ka_tiles<RT>(A, seq(c.s))) { c.r = 0; do c.s++; while (prefix[c.s + 1] == prefix[c.s]); }
+        if (++c.r >= ka_tiles<RT>(A, seq(c.s))) {
+            c.r = 0;
+#pragma unroll 1
+            do c.s++; while (prefix[c.s + 1] == prefix[c.s]);
+        }
         ka_enter<RT, LEAD>(A, seq, c);
     } while (c.np == 0);
 }
 // unit u < prefix[seqs]
 template <int RT, int LEAD, typename Seq> __device__ __forceinline__ ka_place ka_find(const ka_args & A, const int64_t * prefix, const Seq & seq, int64_t u) {
     int lo = 0, hi = A.seqs;                                     // the last sequence with prefix <= u: it has units
+#pragma unroll 1
     while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] <= u) lo = mid; else hi = mid; }
     int64_t  rest = u - prefix[lo];
     ka_place c;
     c.s = lo; c.r = 0;
+#pragma unroll 1
     for (ka_enter<RT, LEAD>(A, seq, c); rest >= (int64_t) c.np * A.kvh; ka_enter<RT, LEAD>(A, seq, c)) { rest -= (int64_t) c.np * A.kvh; c.r++; }
     c.h = (int) (rest / c.np); c.p = (int) (rest % c.np);
     return c;
 }
 // Units in front of each sequence, by all THREADS threads of a block: a thread's neighbouring sequences, then warps, then the block.  part: THREADS / 32 numbers.  Ends with a barrier; the first block leaves
 // them in the plan
-template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, const Keep & keep) {
+template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, Keep keep) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (A.seqs + THREADS - 1) / THREADS, s0 = threadIdx.x * per;
     int64_t sum = 0;
+#pragma unroll 1
     for (int s = s0; s < min(s0 + per, A.seqs); s++) {
         const ka_seq q = ka_load_seq(A, s);
         keep(s, q);
         prefix[s] = sum;
         int first;
+#pragma unroll 1
         for (int r = 0; r < ka_tiles<RT>(A, q); r++) sum += (int64_t) ka_units<RT, LEAD>(A, q, r, first) * A.kvh;
     }
     int64_t before = sum;
@@ -133,15 +162,37 @@ template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline
     before -= sum;
     __syncthreads();
     int64_t all = 0;
+#pragma unroll 1
     for (int i = 0; i < THREADS / 32; i++) { if (i < warp) before += part[i]; all += part[i]; }
+#pragma unroll 1
     for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
     if (threadIdx.x == 0) prefix[A.seqs] = all;
     __syncthreads();
     return all;
 }
+// zeros into the rows of tiles without pages; sequences by blocks
+template <int RT, int THREADS, typename T> __device__ __forceinline__ void ka_zero_rows(const ka_args & A, int D) {
+#pragma unroll 1
+    for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
+        const ka_seq  q = ka_load_seq(A, s);
+        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
+#pragma unroll 1
+        for (int r = 0; r < ka_tiles<RT>(A, q); r++) {
+            int first;
+            if (ka_pages<RT>(A, q, r, first)) continue;
+            const int row0 = r * RT, rows = (int) min((int64_t) RT, (int64_t) q.n * A.rep - row0);
+#pragma unroll 1
+            for (int i = threadIdx.x; i < rows * A.kvh * D; i += THREADS) {          // at most 256 * 1024 * 128
+                const int c = i % D, h = i / D % A.kvh, rc = row0 + i / D / A.kvh;
+                ((T *) A.out)[(tok0 + rc / A.rep) * A.ldo + (int64_t) (h * A.rep + rc % A.rep) * D + c] = (T) 0.f;
+            }
+        }
+    }
+}
 template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_args & A, const int64_t * prefix, int64_t runs) {
     if (blockIdx.x != 0) return;
     if (threadIdx.x == 0) A.plan->runs = runs;
+#pragma unroll 1
     for (int s = threadIdx.x; s <= A.seqs; s += THREADS) A.plan->prefix[s] = prefix[s];
 }
 

@@ -2,6 +2,7 @@
 //
 // A block takes 256 rows (token, head of the group) of one key / value head as two groups of 128 and walks the pages they see; pages of all such items lie in one row that the blocks of the GPU (one an
 // SM) divide evenly, whatever the sequences' lengths (kv4_attn.cuh).  An item that lies in one block's run is written at once; pieces of others go to scratch and kv4_prompt_join_kernel adds them up.
+//   warp 2        writes down the run's items
 //   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
 //   warps 4..7    write two pages' keys [128][dim] and their values, turned, [dim][128] as fp16 into tiles of the 128-byte swizzle
 //   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; one group's products run while the other forms weights
@@ -16,6 +17,10 @@
 #define KP_LEAD    8           // an item's start and end, in pages
 #define KP_BARS    32
 
+// an item, or the piece of it in a run: its rows, pages [page, page + pages) of its sequence; keys hi and below, lo and above all its rows see; whether that is all of it, where its piece goes
+struct kp_item { int s, h, row0, rows, tok0, pos0, page, pages, hi, lo, whole, slot; };
+#define KP_ITEMS 4
+
 template <typename T, int D> struct kp_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  W = D / 32, NC = D / 64, STG = SPLIT ? 1 : 2;               // groups; 64-wide column chunks of a head; tiles of keys and of values
@@ -23,7 +28,7 @@ template <typename T, int D> struct kp_cfg {
     static constexpr int  Q_BYTES = Q_PART * (SPLIT ? 2 : 1), K_CHUNK = 128 * 128, K_TILE = NC * K_CHUNK, V_CHUNK = D * 128, V_TILE = 2 * V_CHUNK;
     static constexpr int  TILES = Q_BYTES + STG * (K_TILE + V_TILE), REC = kv4_record(D);
     static constexpr int  PIECE = KP_ROWS * (D + 2);                                 // floats
-    static constexpr size_t FIXED = (size_t) TILES + KP_BARS * 8 + 256 + 1024;          // without records and the table
+    static constexpr size_t FIXED = (size_t) TILES + KP_BARS * 8 + 512 + 1024;          // without records and the table
 };
 
 // A in tensor memory, B in shared memory; called by a converged warp
@@ -76,13 +81,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     volatile int * abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int * raw_in = reinterpret_cast<volatile int *>(tmem_slot + 2);         // [RAW] whether the record's page is one of the cache's
     volatile unsigned long long * v_none = reinterpret_cast<volatile unsigned long long *>(tmem_slot + 12);      // [STG][2][W] places of a page whose values are none, of each group
-    int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 256);       // [seqs + 1]
+    int64_t *  prefix = reinterpret_cast<int64_t *>(reinterpret_cast<uint8_t *>(bar) + KP_BARS * 8 + 512);       // [seqs + 1]
     __shared__ int64_t part[KP_THREADS / 32];
     // barriers: records there / read; key tiles written / read, value tiles written / read; of each group queries written, scores there, weights written, product done
-    const uint32_t b0 = dt_smem(bar), bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_p = b0 + 160, bar_o = b0 + 176;
+    kp_item *  list = reinterpret_cast<kp_item *>(tmem_slot + 48);                   // [KP_ITEMS]
+    const uint32_t b0 = dt_smem(bar), bar_if = b0 + 192, bar_ie = b0 + 224, bar_rf = b0, bar_re = b0 + 32, bar_kf = b0 + 64, bar_ke = b0 + 80, bar_vf = b0 + 96, bar_ve = b0 + 112, bar_q = b0 + 128, bar_s = b0 + 144, bar_p = b0 + 160, bar_o = b0 + 176;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < RAW; i++) { dt_mbar_init(bar_rf + 8 * i, 1); dt_mbar_init(bar_re + 8 * i, 4); }
+        // an item has been taken by the loader, the issuer, four warps of tiles and eight of rows
+        for (int i = 0; i < KP_ITEMS; i++) { dt_mbar_init(bar_if + 8 * i, 1); dt_mbar_init(bar_ie + 8 * i, 14); }
         for (int i = 0; i < 2; i++) {
             dt_mbar_init(bar_kf + 8 * i, 4); dt_mbar_init(bar_vf + 8 * i, 4);
             for (uint32_t b : { bar_ke, bar_ve, bar_s, bar_o }) dt_mbar_init(b + 8 * i, 1);
@@ -98,50 +106,28 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     pib_pdl_wait();
     pib_pdl_trigger();
     dt_fence_before();
-    const int64_t U = ka_prefix<KP_ROWS, KP_LEAD, KP_THREADS>(A, prefix, part, [](int, ka_seq) {});
+    const int64_t U = ka_prefix<KP_ROWS, KP_LEAD, KP_THREADS, ka_seq_none>(A, prefix, part, {});
     dt_fence_after();
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
     const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, of both groups; the weights take their scores' place; outputs 256..383 and 384..511
-    int    last_s = -1;
-    ka_seq last = { 0, 0 };
-    auto seq_of = [&](int s) {                                   // the tables' entries of the sequence at hand stay in registers
-        if (s != last_s) { last_s = s; last = ka_load_seq(A, s); }
-        return last;
-    };
-    // rows of tiles without pages
-    for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
-        const ka_seq  q = seq_of(s);
-        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
-        for (int r = 0; r < ka_tiles<KP_ROWS>(A, q); r++) {
-            int first;
-            if (ka_pages<KP_ROWS>(A, q, r, first)) continue;
-            const int     row0 = r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
-            for (int64_t i = threadIdx.x; i < (int64_t) rows * A.kvh * D; i += KP_THREADS) {
-                const int c = (int) (i % D), h = (int) (i / D % A.kvh), rc = row0 + (int) (i / D / A.kvh);
-                ((T *) A.out)[(tok0 + rc / A.rep) * A.ldo + (int64_t) (h * A.rep + rc % A.rep) * D + c] = (T) 0.f;
-            }
-        }
-    }
+    ka_zero_rows<KP_ROWS, KP_THREADS, T>(A, D);
     const int64_t u0 = me < runs ? U * me / runs : 0, u1 = me < runs ? U * (me + 1) / runs : 0;
-    // every role walks the same items of the run: f(tokens and keys, place, rows, first of its pages, pages) until it says no
-    auto items = [&](auto f) {
-        if (u0 >= u1) return;
-        ka_place at = ka_find<KP_ROWS, KP_LEAD>(A, prefix, seq_of, u0);
-        for (int64_t u = u0; u < u1;) {
-            const ka_seq q = seq_of(at.s);
-            const int    rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - (int64_t) at.r * KP_ROWS), units = (int) min((int64_t) (at.np - at.p), u1 - u);
-            const int    p0 = max(at.p - KP_LEAD, 0), pages = at.p + units - KP_LEAD - p0;
-            if (pages > 0 && !f(q, at, rows, p0, pages)) return;
-            u += units;
-            at.p += units - 1;
-            if (u < u1) ka_next<KP_ROWS, KP_LEAD>(A, prefix, seq_of, at);
-        }
-    };
     // whether some row of the item does not see all of a page
-    auto edge_of = [&](ka_seq q, const ka_place & at, int rows, int key0) {
-        const int hi = q.len - q.n + at.r * KP_ROWS / A.rep, lo = A.window > 0 ? q.len - q.n + (at.r * KP_ROWS + rows - 1) / A.rep - A.window + 1 : 0;
-        return key0 < lo || key0 + KV4_P - 1 > hi;
+    auto edge_of = [&](const kp_item & it, int key0) { return key0 < it.lo || key0 + KV4_P - 1 > it.hi; };
+    // a role takes the run's items as warp 2 writes them down, until one has no pages: f(item) says whether to go on
+    auto items = [&](auto f) {
+        int at = 0;
+        uint32_t ph = 0;
+#pragma unroll 1
+        for (;;) {
+            if (!__all_sync(0xffffffffu, ka_wait(bar_if + 8 * at, ph, abort_s))) return;
+            const kp_item it = list[at];
+            __syncwarp();
+            if (lane == 0) dt_arrive(bar_ie + 8 * at);
+            if (++at == KP_ITEMS) { at = 0; ph ^= 1; }
+            if (it.pages == 0 || !f(it)) return;
+        }
     };
 
     // registers go where the rows are: 512 x 128 at launch, 128 x (96 + 112 + 152 + 152) from here
@@ -150,30 +136,66 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     if (warp == 0) {
         int st = 0;
         uint32_t ph = 1;                                         // the first round finds its places free
-        items([&](ka_seq, const ka_place & at, int, int p0, int pages) {
+        items([&](const kp_item & it) {
             int ids = 0;
-            for (int i = 0; i < pages; i++) {
-                const int pg = at.first + p0 + i;
-                if ((i & 31) == 0) ids = pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1;
+#pragma unroll 1
+            for (int i = 0; i < it.pages; i++) {
+                const int pg = it.page + i;
+                if ((i & 31) == 0) ids = pg + lane < A.max_pages ? A.table[(int64_t) it.s * A.max_pages + pg + lane] : -1;
                 const int  id = __shfl_sync(0xffffffffu, ids, i & 31);
                 const bool in = id >= 0 && id < A.pages;
-                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_re + 8 * st, ph, abort_s))) return false;
+                if (!__all_sync(0xffffffffu, ka_wait(bar_re + 8 * st, ph, abort_s))) return false;
                 if (lane == 0) {
                     raw_in[st] = in;
                     if (in) {
                         dt_mbar_expect_tx(bar_rf + 8 * st, C::REC);
-                        ka_bulk(dt_smem(raw + st * C::REC), A.base + ((int64_t) id * A.kvh + at.h) * C::REC, C::REC, bar_rf + 8 * st);
+                        ka_bulk(dt_smem(raw + st * C::REC), A.base + ((int64_t) id * A.kvh + it.h) * C::REC, C::REC, bar_rf + 8 * st);
                     } else dt_arrive(bar_rf + 8 * st);
                 }
                 if (++st == RAW) { st = 0; ph ^= 1; }
             }
             return true;
         });
+    } else if (warp == 2) {
+        const ka_seq_call seq_of = { &A };
+        int at = 0;
+        uint32_t ph = 1;
+        auto put = [&](const kp_item & it) {
+            if (!__all_sync(0xffffffffu, ka_wait(bar_ie + 8 * at, ph, abort_s))) return false;
+            if (lane == 0) { list[at] = it; dt_arrive(bar_if + 8 * at); }
+            __syncwarp();
+            if (++at == KP_ITEMS) { at = 0; ph ^= 1; }
+            return true;
+        };
+        bool go = true;
+        if (u0 < u1) {
+            ka_place c = ka_find<KP_ROWS, KP_LEAD>(A, prefix, seq_of, u0);
+#pragma unroll 1
+            for (int64_t u = u0; u < u1 && go;) {
+                const ka_seq q = seq_of(c.s);
+                const int    units = (int) min((int64_t) (c.np - c.p), u1 - u), p0 = max(c.p - KP_LEAD, 0), pages = c.p + units - KP_LEAD - p0;
+                if (pages > 0) {
+                    kp_item it;
+                    it.s = c.s; it.h = c.h; it.row0 = c.r * KP_ROWS; it.rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - it.row0);
+                    it.tok0 = min(max(A.starts[c.s], 0), A.tokens); it.pos0 = q.len - q.n;
+                    it.page = c.first + p0; it.pages = pages;
+                    it.hi = it.pos0 + it.row0 / A.rep;
+                    it.lo = max(0, it.pos0 + (it.row0 + it.rows - 1) / A.rep - ka_window(A) + 1);
+                    it.whole = p0 == 0 && pages == c.np - KP_LEAD; it.slot = p0 > 0 ? 0 : 1;
+                    go = put(it);
+                }
+                u += units;
+                c.p += units;
+                if (u < u1 && c.p >= c.np) ka_next_item<KP_ROWS, KP_LEAD>(A, prefix, seq_of, c);
+            }
+        }
+        kp_item end = {};
+        if (go) put(end);
     } else if (warp == 1) {
         constexpr uint32_t id_o = kp_idesc(128, D);
         const uint64_t dq = dt_desc(dt_smem(sQ)), dk = dt_desc(dt_smem(sK)), dv = dt_desc(dt_smem(sV));
         int      j = 0, n_q[2] = { 0, 0 }, n_p[2] = { 0, 0 };     // steps of two pages; queries and weights that have entered
-        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
+        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, ka_wait(b, ph & 1, abort_s)) != 0; };
         auto there = [&](uint32_t b, uint32_t ph) {
             uint32_t ok;
             asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(b), "r"(ph & 1) : "memory");
@@ -202,18 +224,20 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     for (int k = 0; k < 4; k++) kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * h + 32 * part_ + 8 * k, v0 + (uint64_t) (h * C::V_CHUNK >> 4) + 2 * k, id_o, add || (h | part_ | k) != 0);
             dt_commit(bar_o + 8 * w);
         };
-        items([&](ka_seq, const ka_place &, int rows, int, int pages) {
-            const int groups = rows > 128 ? 2 : 1, steps = (pages + 1) / 2;
+        items([&](const kp_item & it) {
+            const int pages = it.pages, groups = it.rows > 128 ? 2 : 1, steps = (pages + 1) / 2;
             if (!wait(bar_kf + 8 * (j % C::STG), j / C::STG)) return false;
             for (int w = 0; w < groups; w++) {
                 if (!wait(bar_q + 8 * w, n_q[w]++)) return false;
                 scores(w, j, pages > 1);
             }
             dt_commit(bar_ke + 8 * (j % C::STG));
+#pragma unroll 1
             for (int i = 0; i < steps; i++, j++) {
                 // what the groups wait for, in the order in which it comes: weights, then the end of their product
                 int  to_do = (i + 1 < steps ? 2 : 1) * groups, done[2] = { 0, 0 }, n_v = 0, n_k = 0;
                 uint32_t spins = 0;
+#pragma unroll 1
                 while (to_do) {
 #pragma unroll
                     for (int w = 0; w < 2; w++) {
@@ -243,17 +267,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         const int tid = threadIdx.x - 128;
         int       j = 0, st = 0;
         uint32_t  ph = 0;
-        items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
+        items([&](const kp_item & it) {
+            const int pages = it.pages;
+#pragma unroll 1
             for (int i = 0; i < pages; i += 2, j++) {
                 const int two = i + 1 < pages, sg = j % C::STG;
                 const uint32_t free_ph = (j / C::STG & 1) ^ 1;
-                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ke + 8 * sg, free_ph, abort_s))) return false;
+                if (!__all_sync(0xffffffffu, ka_wait(bar_ke + 8 * sg, free_ph, abort_s))) return false;
                 int      s1 = st;
                 uint32_t p1 = ph;
 #pragma unroll 1
                 for (int h = 0; h <= two; h++) {
                     // keys: a thread has 32 channels (two times) of one key; of a group's four words the lanes start with different ones, for the banks
-                    if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_rf + 8 * s1, p1, abort_s))) return false;
+                    if (!__all_sync(0xffffffffu, ka_wait(bar_rf + 8 * s1, p1, abort_s))) return false;
                     const bool in = raw_in[s1] != 0;
                     const uint8_t * rec = raw + s1 * C::REC;
                     uint8_t * to = sK + sg * C::K_TILE + h * 64 * 128;
@@ -277,7 +303,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 dt_fence_async();
                 __syncwarp();
                 if (lane == 0) dt_arrive(bar_kf + 8 * sg);
-                if (!__all_sync(0xffffffffu, dt_mbar_wait(bar_ve + 8 * sg, free_ph, abort_s))) return false;
+                if (!__all_sync(0xffffffffu, ka_wait(bar_ve + 8 * sg, free_ph, abort_s))) return false;
 #pragma unroll 1
                 for (int h = 0; h <= two; h++) {
                     // values: a thread has eight keys (an octet, a piece of 16 bytes in the turned tile) of eight (heads of 64: four) neighbouring channels
@@ -293,10 +319,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         n[k]  = *reinterpret_cast<const uint32_t *>(vr + r * (D / 2) + ((o8 * 4) ^ kv4_flip(D, r)));
                         dm[k] = *reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (r * C::W + (o8 >> 2)) * 4);
                     }
-                    if (edge_of(q, at, rows, (at.first + p0 + i + h) * KV4_P)) {
+                    if (edge_of(it, (it.page + i + h) * KV4_P)) {
                         // values that are none, on a page of which some row does not see all: they take part as zeros, and the rows that see one are told
                         if (tid < C::W) {
                             unsigned long long none = 0;
+#pragma unroll 1
                             for (int k = 0; k < KV4_P; k++)
                                 if (in && __hisnan(__high2half(*reinterpret_cast<const __half2 *>(vr + kv4_steps(D) + (kv4_row(k) * C::W + tid) * 4)))) none |= 1ull << k;
                             v_none[(sg * 2 + h) * C::W + tid] = none;
@@ -332,14 +359,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         const int w = (warp - 8) >> 2, q4 = warp & 3, rt = q4 * 32 + lane;
         const uint32_t lanes = (uint32_t) (q4 * 32) << 16, tm_s = tmem + lanes + 128 * w, tm_w = tm_o + lanes + 128 * w;
         int j = 0, n = 0;                                        // steps of the run, and those of which this group has scores
-        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, dt_mbar_wait(b, ph & 1, abort_s)) != 0; };
-        items([&](ka_seq q, const ka_place & at, int rows, int p0, int pages) {
-            const int     row0 = at.r * KP_ROWS, ri = w * 128 + rt, rc = row0 + min(ri, rows - 1), tk = rc / A.rep, hi = q.len - q.n + tk, lo = A.window > 0 ? max(0, hi - A.window + 1) : 0;
-            const int64_t tok = min(max(A.starts[at.s], 0), A.tokens) + tk, head = at.h * A.rep + rc % A.rep;
+        auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, ka_wait(b, ph & 1, abort_s)) != 0; };
+        items([&](const kp_item & it) {
+            const int     pages = it.pages, rows = it.rows, ri = w * 128 + rt, rc = it.row0 + min(ri, rows - 1), tk = rc / A.rep, hi = it.pos0 + tk, lo = max(0, hi - ka_window(A) + 1);
+            const int64_t tok = it.tok0 + tk, head = it.h * A.rep + rc % A.rep;
             const bool    on = w == 0 || rows > 128;
             if (!on) { j += (pages + 1) / 2; return true; }
-            auto some = [&](int pg) { return pg + lane < A.max_pages ? A.table[(int64_t) at.s * A.max_pages + pg + lane] : -1; };
-            int ids = some(at.first + p0);
+            auto some = [&](int pg) { return pg + lane < A.max_pages ? A.table[(int64_t) it.s * A.max_pages + pg + lane] : -1; };
+            int ids = some(it.page);
             float qs;
             {
                 // the row times scale log2 e, over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
@@ -348,13 +375,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 kp_row<T, N> v;
                 float top = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < D; c += N) { v.load(p + c, A.wide_q); top = fmaxf(top, v.top()); }
+                for (int c = 0; c < D; c += N) { v.load(p + c, ka_here(A.wide_q)); top = fmaxf(top, v.top()); }
                 const ka_power pw = ka_power_of(top * fabsf(A.scale * KA_LOG2E));
                 qs = pw.back;
                 uint8_t * to = sQ + w * C::NC * C::Q_CHUNK + rt * 128;
 #pragma unroll 1
                 for (int c = 0; c < D; c += N) {
-                    if (N < D) v.load(p + c, A.wide_q);
+                    if (N < D) v.load(p + c, ka_here(A.wide_q));
 #pragma unroll
                     for (int i = 0; i < N / 8; i++) {
                         const int at16 = (N < D ? c >> 6 : i >> 3) * C::Q_CHUNK + (((N < D ? ((c & 63) >> 3) + i : i & 7) ^ (rt & 7)) << 4);
@@ -373,9 +400,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             if (lane == 0) dt_arrive(bar_q + 8 * w);
             float    m = -INFINITY, l = 0.f, l2 = 0.f;
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
+#pragma unroll 1
             for (int i = 0; i < pages; i += 2, j++, n++) {
                 const int two = i + 1 < pages;
-                if (i > 0 && (i & 31) == 0) ids = some(at.first + p0 + i);
+                if (i > 0 && (i & 31) == 0) ids = some(it.page + i);
                 const int  id0 = __shfl_sync(0xffffffffu, ids, i & 31), id1 = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
                 if (!wait(bar_s + 8 * w, n)) return false;
                 dt_fence_after();
@@ -385,9 +413,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     dt_ld32(tm_s + 64 * h, t);
                     dt_ld32(tm_s + 64 * h + 32, t + 32);
                     dt_wait_ld();
-                    const int  key0 = (at.first + p0 + i + h) * KV4_P, id = h ? id1 : id0;
+                    const int  key0 = (it.page + i + h) * KV4_P, id = h ? id1 : id0;
                     const bool in = id >= 0 && id < A.pages;
-                    if (!in || edge_of(q, at, rows, key0)) {
+                    if (!in || edge_of(it, key0)) {
                         const int a = in ? lo - key0 : 64, b = hi - key0;
 #pragma unroll
                         for (int x = 0; x < 64; x++) if (x < a || x > b) t[x] = 0xff800000u;
@@ -399,8 +427,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     load(h);
 #pragma unroll
                     for (int x = 0; x < 64; x++) top = fmaxf(top, __uint_as_float(t[x]));
-                    const int  key0 = (at.first + p0 + i + h) * KV4_P, id = h ? id1 : id0;
-                    if (id >= 0 && id < A.pages && edge_of(q, at, rows, key0)) {
+                    const int  key0 = (it.page + i + h) * KV4_P, id = h ? id1 : id0;
+                    if (id >= 0 && id < A.pages && edge_of(it, key0)) {
                         const int a = lo - key0, b = hi - key0;
                         if (!wait(bar_vf + 8 * (j % C::STG), j / C::STG)) return false;
                         if (b >= 0 && a < 64) {
@@ -454,9 +482,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             // ---- the row out, behind the last product
             if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
-            const bool    whole = p0 == 0 && pages == at.np - KP_LEAD;
+            const bool    whole = it.whole;
             const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
-            float *       piece = A.pieces + (2 * me + (p0 > 0 ? 0 : 1)) * (int64_t) C::PIECE;
+            float *       piece = A.pieces + (2 * me + it.slot) * (int64_t) C::PIECE;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
@@ -466,7 +494,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 const float k = none >> (c >> 5) & 1 ? __uint_as_float(0x7fc00000u) : whole ? inv : 1.f;
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] *= k;
-                if (whole) ka_store<T, 32>((T *) A.out + tok * A.ldo + head * D + c, A.wide_o, v);
+                if (whole) ka_store<T, 32>((T *) A.out + tok * A.ldo + head * D + c, ka_here(A.wide_o), v);
                 else       ka_store<float, 32>(piece + ri * D + c, true, v);
             }
             if (!whole && ri < rows) { piece[KP_ROWS * D + ri] = m; piece[KP_ROWS * D + KP_ROWS + ri] = sum; }
@@ -480,6 +508,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     if (*abort_s) {
         // a wait ran out: say so, give copies and MMAs still in flight time to land (bounded), then free the tensor memory
         if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
+#pragma unroll 1
         for (int i = 0; i < 2000; i++) __nanosleep(1000);
         __syncthreads();
     }
@@ -497,7 +526,7 @@ static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __gri
     if (wa + 1 >= runs) return;
     const int64_t * prefix = A.plan->prefix;
     const int64_t U = prefix[A.seqs], u0 = U * wa / runs, u1 = U * (wa + 1) / runs;
-    auto seq_of = [&](int s) { return ka_load_seq(A, s); };
+    const ka_seq_call seq_of = { &A };
     const ka_place at = ka_find<KP_ROWS, KP_LEAD>(A, prefix, seq_of, u1 - 1);
     const int64_t  ib = u1 - 1 - at.p + KP_LEAD, ie = ib - KP_LEAD + at.np;         // its pages' units
     if (ib < u0 || ib >= u1 || ie <= u1) return;
