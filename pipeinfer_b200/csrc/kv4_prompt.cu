@@ -5,7 +5,7 @@
 //   warp 2        writes down the run's items
 //   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
 //   warps 4..7    write two pages' keys [128][dim] and their values, turned, [dim][128] as fp16 into tiles of the 128-byte swizzle
-//   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; one group's products run while the other forms weights
+//   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; then the other group's, while the first forms weights
 //   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 into the scores' place, from where they enter the second product
 // fp32 queries and weights enter as fp16 part and remainder, two products each; of bfloat16 rows both are one fp16 number.
 // Every wait is bounded (tc_common.cuh).
@@ -196,11 +196,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
         const uint64_t dq = dt_desc(dt_smem(sQ)), dk = dt_desc(dt_smem(sK)), dv = dt_desc(dt_smem(sV));
         int      j = 0, n_q[2] = { 0, 0 }, n_p[2] = { 0, 0 };     // steps of two pages; queries and weights that have entered
         auto wait = [&](uint32_t b, uint32_t ph) { return __all_sync(0xffffffffu, ka_wait(b, ph & 1, abort_s)) != 0; };
-        auto there = [&](uint32_t b, uint32_t ph) {
-            uint32_t ok;
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(b), "r"(ph & 1) : "memory");
-            return __all_sync(0xffffffffu, ok) != 0;
-        };
         auto scores = [&](int w, int jj, int two) {
             const uint32_t id_s = two ? kp_idesc(128, 128) : kp_idesc(128, 64);
             const uint64_t a0 = dq + (uint64_t) (w * C::NC * C::Q_CHUNK >> 4), k0 = dk + (uint64_t) (jj % C::STG * C::K_TILE >> 4);
@@ -234,28 +229,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             dt_commit(bar_ke + 8 * (j % C::STG));
 #pragma unroll 1
             for (int i = 0; i < steps; i++, j++) {
-                // what the groups wait for, in the order in which it comes: weights, then the end of their product
-                int  to_do = (i + 1 < steps ? 2 : 1) * groups, done[2] = { 0, 0 }, n_v = 0, n_k = 0;
-                uint32_t spins = 0;
+                // a group at a time, its next scores right behind its outputs: the other one forms its weights meanwhile.  (Both groups' outputs, then both groups' scores: the groups fall into step and
+                // share the exponentials, then wait together)
 #pragma unroll 1
-                while (to_do) {
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        if (w >= groups) break;
-                        if (done[w] == 0 && there(bar_p + 8 * w, n_p[w])) {
-                            if (n_v == 0 && !wait(bar_vf + 8 * (j % C::STG), j / C::STG)) return false;
-                            outputs(w, 2 * i + 1 < pages, i > 0);
-                            n_p[w]++; done[w] = 1; to_do--; spins = 0;
-                            if (++n_v == groups) dt_commit(bar_ve + 8 * (j % C::STG));
-                        } else if (done[w] == 1 && i + 1 < steps && there(bar_o + 8 * w, n_p[w] + 1)) {
-                            if (n_k == 0 && !wait(bar_kf + 8 * ((j + 1) % C::STG), (j + 1) / C::STG)) return false;
-                            scores(w, j + 1, 2 * i + 3 < pages);
-                            done[w] = 2; to_do--; spins = 0;
-                            if (++n_k == groups) dt_commit(bar_ke + 8 * ((j + 1) % C::STG));
-                        }
-                    }
-                    if (++spins > DT_SPIN) *abort_s = 1;
-                    if ((spins & 63) == 63 && *abort_s) return false;
+                for (int w = 0; w < groups; w++) {
+                    if (!wait(bar_p + 8 * w, n_p[w]) || (w == 0 && !wait(bar_vf + 8 * (j % C::STG), j / C::STG))) return false;
+                    outputs(w, 2 * i + 1 < pages, i > 0);
+                    n_p[w]++;
+                    if (w == groups - 1) dt_commit(bar_ve + 8 * (j % C::STG));
+                    if (i + 1 == steps) continue;
+                    // (the weights lie where the scores go, and MMAs of different accumulators may overtake each other)
+                    if ((w == 0 && !wait(bar_kf + 8 * ((j + 1) % C::STG), (j + 1) / C::STG)) || !wait(bar_o + 8 * w, n_p[w] + 1)) return false;
+                    scores(w, j + 1, 2 * i + 3 < pages);
+                    if (w == groups - 1) dt_commit(bar_ke + 8 * ((j + 1) % C::STG));
                 }
             }
             return true;
