@@ -31,23 +31,38 @@ template <typename T> __device__ __forceinline__ void kc_load8(const T * p, bool
         for (int j = 0; j < 8; j++) v[j] = kc_float<T>(p[j]);
 }
 
-template <typename T>
-static __global__ void __launch_bounds__(KC_THREADS) kv4_write_kernel(uint8_t * __restrict__ base, int64_t pages, int heads, int dim, const T * __restrict__ k, int64_t ldk, const T * __restrict__ v,
+template <typename T, int dim>
+static __global__ void __launch_bounds__(KC_THREADS) kv4_write_kernel(uint8_t * __restrict__ base, int64_t pages, int heads, const T * __restrict__ k, int64_t ldk, const T * __restrict__ v,
                                                                       int64_t ldv, const int32_t * __restrict__ cells, int n, bool wide) {
     pib_pdl_wait();
     pib_pdl_trigger();
-    const int t = blockIdx.x, cell = cells[t], per = dim / 8;
+    constexpr int per = dim / 8;
+    const int t = blockIdx.x, all = 2 * heads * per;
+    // (whole warps enter each round: heads * dim / 4 is a multiple of 16, lanes without work repeat the last octet's reading and store nothing)
+    auto load = [&](int u0, float (&x)[8]) {
+        const int u = min(u0 + (int) threadIdx.x, all - 1), values = u >= heads * per, w = u - values * heads * per;
+        kc_load8<T>((values ? v + t * ldv : k + t * ldk) + (int64_t) (w / per) * dim + w % per * 8, wide, x);
+    };
+    // the first round's rows are on their way while the cells are looked through
+    float x[8];
+    load(0, x);
+    const int cell = cells[t];
     if (cell < 0 || cell / KV4_P >= pages) return;
     bool later = false;
-    for (int i = t + 1 + threadIdx.x; i < n; i += KC_THREADS) later |= cells[i] == cell;
+    if (((uintptr_t) cells & 15) == 0) {                             // four cells a load, the last ones one by one
+        const int whole = n & ~3;
+        for (int i = ((t + 1) & ~3) + 4 * threadIdx.x; i < whole; i += 4 * KC_THREADS) {
+            const int4 c = *reinterpret_cast<const int4 *>(cells + i);
+            later |= (c.x == cell && i > t) || (c.y == cell && i + 1 > t) || (c.z == cell && i + 2 > t) || (c.w == cell && i + 3 > t);
+        }
+        if ((int) threadIdx.x < n - whole) later |= cells[whole + threadIdx.x] == cell && whole + (int) threadIdx.x > t;
+    } else
+        for (int i = t + 1 + threadIdx.x; i < n; i += KC_THREADS) later |= cells[i] == cell;
     if (__syncthreads_or(later)) return;
     const int place = cell % KV4_P;
-    // (whole warps enter each round: heads * dim / 4 is a multiple of 16, lanes without work repeat the last octet's reading and store nothing)
-    const int all = 2 * heads * per;
     for (int u0 = 0; u0 < all; u0 += KC_THREADS) {
-        const int  u = min(u0 + (int) threadIdx.x, all - 1), values = u >= heads * per, w = u - values * heads * per, head = w / per, o = w % per;
-        float x[8];
-        kc_load8<T>((values ? v + t * ldv : k + t * ldk) + (int64_t) head * dim + o * 8, wide, x);
+        if (u0) load(u0, x);
+        const int u = min(u0 + (int) threadIdx.x, all - 1), values = u >= heads * per, w = u - values * heads * per, head = w / per, o = w % per;
         float    lo = INFINITY, hi = -INFINITY;
         uint32_t big = 0;
 #pragma unroll
@@ -67,9 +82,14 @@ static __global__ void __launch_bounds__(KC_THREADS) kv4_write_kernel(uint8_t * 
         __half   d = __float2half_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, mf), 0.f), 15.f));
         const float df = __half2float(d);
         uint32_t q = 0;
+        // The quotient by a product with 1 / d is off by less than 2^-18; only where that lies next to a half does the division itself say which side it is on.  (Eight divisions a thread were the kernel's time)
+        const float inv = __frcp_rn(df);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float r = df > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], mf), df)), 0.f), 15.f) : 0.f;
+            const float a = __fsub_rn(x[j], mf), p = a * inv;
+            float       r = rintf(p);
+            if (fabsf(p - r) > 0.49998f) r = rintf(__fdiv_rn(a, df));
+            r = df > 0.f ? fminf(fmaxf(r, 0.f), 15.f) : 0.f;
             q |= (uint32_t) (int) r << (4 * j);
         }
         if (big >= 0x7f800000u) { d = __ushort_as_half(0); m = __ushort_as_half(0x7e00); q = 0; }
@@ -81,12 +101,13 @@ static __global__ void __launch_bounds__(KC_THREADS) kv4_write_kernel(uint8_t * 
     }
 }
 
-template <typename T>
-static __global__ void __launch_bounds__(KC_THREADS) kv4_read_kernel(const uint8_t * __restrict__ base, int64_t pages, int heads, int dim, T * __restrict__ k, int64_t ldk, T * __restrict__ v, int64_t ldv,
+template <typename T, int dim>
+static __global__ void __launch_bounds__(KC_THREADS) kv4_read_kernel(const uint8_t * __restrict__ base, int64_t pages, int heads, T * __restrict__ k, int64_t ldk, T * __restrict__ v, int64_t ldv,
                                                                      const int32_t * __restrict__ cells, bool wide) {
     pib_pdl_wait();
     pib_pdl_trigger();
-    const int  t = blockIdx.x, cell = cells[t], per = dim / 8, place = cell & (KV4_P - 1);
+    constexpr int per = dim / 8;
+    const int  t = blockIdx.x, cell = cells[t], place = cell & (KV4_P - 1);
     const bool there = cell >= 0 && cell / KV4_P < pages;
     for (int u = threadIdx.x; u < 2 * heads * per; u += KC_THREADS) {
         const int values = u >= heads * per, w = u - values * heads * per, head = w / per, o = w % per;
@@ -162,8 +183,11 @@ extern "C" int pib_kv4_write(pib_kv4 * kv, int type, const void * k, int64_t ldk
     }
     if (!n) return PIB_OK;
     const bool wide = kc_wide(size, k, ldk) && kc_wide(size, v, ldv);
-    if (size == 4) PIB_CHECK(pib_launch(kv4_write_kernel<float>, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, kv->base, kv->pages, kv->heads, kv->dim, (const float *) k, ldk, (const float *) v, ldv, cells, n, wide));
-    else PIB_CHECK(pib_launch(kv4_write_kernel<__nv_bfloat16>, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, kv->base, kv->pages, kv->heads, kv->dim, (const __nv_bfloat16 *) k, ldk, (const __nv_bfloat16 *) v, ldv, cells, n, wide));
+    auto go = [&](auto kernel, auto * kp, auto * vp) { return pib_launch(kernel, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, kv->base, kv->pages, kv->heads, kp, ldk, vp, ldv, cells, n, wide); };
+    const float * kf = (const float *) k, * vf = (const float *) v;
+    const __nv_bfloat16 * kb = (const __nv_bfloat16 *) k, * vb = (const __nv_bfloat16 *) v;
+    if (kv->dim == 64) PIB_CHECK(size == 4 ? go(kv4_write_kernel<float, 64>, kf, vf) : go(kv4_write_kernel<__nv_bfloat16, 64>, kb, vb));
+    else               PIB_CHECK(size == 4 ? go(kv4_write_kernel<float, 128>, kf, vf) : go(kv4_write_kernel<__nv_bfloat16, 128>, kb, vb));
     return PIB_OK;
 }
 
@@ -177,7 +201,10 @@ extern "C" int pib_kv4_read(const pib_kv4 * kv, int type, const int32_t * cells,
     }
     if (!n || (!k && !v)) return PIB_OK;
     const bool wide = kc_wide(size, k, ldk) && kc_wide(size, v, ldv);
-    if (size == 4) PIB_CHECK(pib_launch(kv4_read_kernel<float>, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, kv->base, kv->pages, kv->heads, kv->dim, (float *) k, ldk, (float *) v, ldv, cells, wide));
-    else PIB_CHECK(pib_launch(kv4_read_kernel<__nv_bfloat16>, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, kv->base, kv->pages, kv->heads, kv->dim, (__nv_bfloat16 *) k, ldk, (__nv_bfloat16 *) v, ldv, cells, wide));
+    auto go = [&](auto kernel, auto * kp, auto * vp) { return pib_launch(kernel, dim3((unsigned) n), dim3(KC_THREADS), 0, (cudaStream_t) s, (const uint8_t *) kv->base, kv->pages, kv->heads, kp, ldk, vp, ldv, cells, wide); };
+    float * kf = (float *) k, * vf = (float *) v;
+    __nv_bfloat16 * kb = (__nv_bfloat16 *) k, * vb = (__nv_bfloat16 *) v;
+    if (kv->dim == 64) PIB_CHECK(size == 4 ? go(kv4_read_kernel<float, 64>, kf, vf) : go(kv4_read_kernel<__nv_bfloat16, 64>, kb, vb));
+    else               PIB_CHECK(size == 4 ? go(kv4_read_kernel<float, 128>, kf, vf) : go(kv4_read_kernel<__nv_bfloat16, 128>, kb, vb));
     return PIB_OK;
 }
