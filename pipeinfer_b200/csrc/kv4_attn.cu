@@ -21,8 +21,10 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 //   scores   turned, S' = K Q': mma.m16n8k16, 16 keys as M, eight rows as N, keys straight from nibbles in registers: lane (g, t) has 16 or 32 neighbouring channels of keys g and g + 8, one load and one step
 //            and lowest value each, four of them a product's k
 //   outputs  O' = V' P': 16 channels as M, weights (turned once more by movmatrix) as N, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
+// The tensor core cuts off what it adds to a sum, always towards zero: of fp32 rows the rests' scores have sums of their own, and each product of weights begins at zero and is added with rounding.  Error of
+// 20,000 keys against 64 bits 3.3e-6 -> 6.5e-7, for 48.4 -> 52.0 us of the 32 sequences below.
 // Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  fp32 rows enter as fp16 part and remainder,
-// two products into the same sums; of bfloat16 rows queries and weights are one fp16 number.
+// two products; of bfloat16 rows queries and weights are one fp16 number.
 // An item that lies in one warp's units is written at once.  Pieces of others meet in shared memory at the end, in the order of the keys; what then is not a whole item goes to scratch, two pieces a block at
 // most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, twelve times as many, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
 // warps of a block, by the registers that a warp's tile takes, and the shared memory of fp32 queries' operands
@@ -31,7 +33,7 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
     static constexpr int  WARPS = ka_warps(SPLIT, NR);
-    static constexpr int  KB = NR == 1 ? 64 : 32;                    // keys of which the scores are in registers at once
+    static constexpr int  KB = NR == 1 && !SPLIT ? 64 : 32;                    // keys of which the scores are in registers at once (fp32, one tile: 64 do not fit, 53.5 us for 52.0)
     static constexpr bool QS = NR > 1;                               // the queries' operands lie in shared memory
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
@@ -216,6 +218,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                     for (int j = 0; j < C::KB / 16; j++) {
                         uint32_t wv[2][C::W];
                         __half2  d2[2], m2[2];
+                        float    rest[C::SPLIT ? NR : 1][4];     // of fp32 rows: the tensor core cuts what it adds to a sum, so small products have one of their own
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
                             const int r = kb + j * 16 + x * 8 + g;
@@ -236,10 +239,16 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
                                     for (int pt = 0; pt < C::PARTS; pt++) {
                                         const uint2 b = C::QS ? qsm[((n * C::PARTS + pt) * C::KS + 2 * w + e) * 32] : qf[C::QS ? 0 : pt][C::QS ? 0 : 2 * w + e];
-                                        if (w == 0 && e == 0 && pt == 0) ka_mma0(S[j][n], o[0][0], o[1][0], o[0][1], o[1][1], b);
-                                        else ka_mma(S[j][n], o[0][2 * e], o[1][2 * e], o[0][2 * e + 1], o[1][2 * e + 1], b);
+                                        float (&to)[4] = pt ? rest[C::SPLIT ? n : 0] : S[j][n];
+                                        if (w == 0 && e == 0) ka_mma0(to, o[0][0], o[1][0], o[0][1], o[1][1], b);
+                                        else ka_mma(to, o[0][2 * e], o[1][2 * e], o[0][2 * e + 1], o[1][2 * e + 1], b);
                                     }
                         }
+                        if (C::SPLIT)
+#pragma unroll
+                            for (int n = 0; n < NR; n++)
+#pragma unroll
+                                for (int c = 0; c < 4; c++) S[j][n][c] += rest[C::SPLIT ? n : 0][c];
                     }
                     if (kb == 0) {
                         ok = __all_sync(0xffffffffu, ka_wait(bar0 + vst * 8, vph, abort_s));
@@ -359,9 +368,16 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
                                 for (int n = 0; n < NR; n++)
 #pragma unroll
-                                    for (int pt = 0; pt < C::PARTS; pt++)
+                                    for (int c = 0; c < 2; c++) {
+                                        float (&to)[4] = O[n][w * 4 + e * 2 + c];
+                                        if (C::SPLIT) {          // the rests' product, while the sum is small; then fp32 adds, with rounding
+                                            float own[4];
+                                            ka_mma0(own, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][C::PARTS - 1]);
+                                            ka_mma(own, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][0]);
 #pragma unroll
-                                        for (int c = 0; c < 2; c++) ka_mma(O[n][w * 4 + e * 2 + c], x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][pt]);
+                                            for (int k = 0; k < 4; k++) to[k] += own[k];
+                                        } else ka_mma(to, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][0]);
+                                    }
                             }
                     }
                 }
@@ -547,7 +563,7 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
 static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
-// the scratch: two pieces a block, decode: one of each warp; then the tables
+// the scratch: two pieces a block; decode: one of each warp, prompts of fp32: a block's sums; then the tables
 struct ka_space { size_t heads, plan, open, total; };
 static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     const int    n = ka_tiles_of(kv, b), sms = pib_num_sms();
@@ -556,7 +572,7 @@ static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     auto up = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     ka_space s;
     s.heads = up(2 * sms * piece);
-    s.plan  = s.heads + (few ? up((size_t) sms * ka_warps(b->type == PIB_TYPE_F32, n) * piece) : 0);
+    s.plan  = s.heads + (few ? up((size_t) sms * ka_warps(b->type == PIB_TYPE_F32, n) * piece) : b->type == PIB_TYPE_F32 ? (size_t) sms * KP_ROWS * kv->dim * 4 : 0);
     s.open  = s.plan + up(sizeof(ka_plan));
     s.total = s.open + up(sms * sizeof(ka_open));
     return s;

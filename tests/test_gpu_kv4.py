@@ -239,6 +239,16 @@ def test_long(torch, pib, t):
     Case(torch, pib, t, 1, 8, 128, [2, 1, 1], [40000, 9, 20001], 30000).check()
 
 
+@pytest.mark.parametrize("kvh,rep,n,lens", [(2, 4, 40, [64000]), (2, 4, 1, [64000]), (16, 8, 1, [20000] * 6)])
+def test_sums_over_many_keys_stay_whole(torch, pib, kvh, rep, n, lens):
+    """Tensor cores cut what they add: 2^-24 of a sum on average and each time, always towards zero, on the way up to the sum half of that.  Scores: 16 products in D = 128, times |s|, whose mean here is
+    scale * 1.5 * sqrt(128) * 0.8 = 1.2; outputs: 32 products until fp32 takes over.  (16 * 1.2 + 32) * 2^-25 = 1.5e-6, and
+    2^-22 each for the exponential and the rest of the parts: 2e-6.  Sums that stayed in the tensor core are off by 3.3e-6 here."""
+    c = Case(torch, pib, F32, kvh, rep, 128, [n] * len(lens), lens)
+    ref, _ = c.want()
+    assert float((c.run().double() - ref).norm() / ref.norm()) < 2e-6
+
+
 def test_many_sequences(torch, pib):
     lens = [(i * 37) % 200 for i in range(1024)]
     Case(torch, pib, BF16, 2, 4, 64, [1] * 1024, lens).check()
