@@ -43,6 +43,11 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
 template <int RT> __device__ __noinline__ ka_place ka_find_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, int64_t u) { return ka_find<RT, 0>(A, prefix, seq, u); }
 template <int RT> __device__ __noinline__ ka_place ka_next_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place c) { ka_next_item<RT, 0>(A, prefix, seq, c); return c; }
 template <int RT> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place & c) { if (++c.p >= c.np) c = ka_next_call<RT>(A, prefix, seq, c); }
+// two or four neighbouring channels
+__device__ __forceinline__ void ka_get(const float * p, float (&v)[2]) { const float2 f = *reinterpret_cast<const float2 *>(p); v[0] = f.x; v[1] = f.y; }
+__device__ __forceinline__ void ka_get(const float * p, float (&v)[4]) { const float4 f = *reinterpret_cast<const float4 *>(p); v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
+__device__ __forceinline__ void ka_put(float * p, const float (&v)[2]) { *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]); }
+__device__ __forceinline__ void ka_put(float * p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 // a warp's piece of an item: sums of the rows that there are, their maxima and denominators
 template <typename C, int NR>
 __device__ __forceinline__ void ka_leave(float * p, int rows, int g, int t, const float (&O)[NR][C::MT][4], const float (&m)[NR][2], const float (&l)[NR][2]) {
@@ -432,53 +437,59 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
         { uint32_t b = all_ends;
 #pragma unroll 1
             for (int k = 0; b; k++, b &= b - 1) if (k == lane) my_end = __ffs(b) - 1; }
-        constexpr int MANY = NR == 1 ? 1 : 4;                                      // rows of chains at a time: what they load is under way together
+        constexpr int MANY = NR == 1 ? 1 : NR == 2 ? 2 : 4;                        // neighbouring rows of a chain at a time
         const int tasks = (__popc(all_ends) + 1) * C::RT;
 #pragma unroll 1
         for (int task0 = warp * MANY; task0 < tasks; task0 += C::WARPS * MANY) {
-            float lv[MANY][CH], pm[MANY], pl[MANY];
-            uint32_t mine[MANY];
-            int   end[MANY];
-            bool  ours[MANY], does[MANY];
+            const int r0 = task0 % C::RT, chain = task0 / C::RT, from = __shfl_sync(0xffffffffu, my_end, max(chain - 1, 0) & 31), end = __shfl_sync(0xffffffffu, my_end, chain & 31);
+            // pieces in shared memory (the warp where the chain before ends may begin this one); the one of warp `end` is in scratch
+            const uint32_t span = ((1u << end) - 1) & ~((1u << (chain ? from : 0)) - 1), mine = all_goes & span;
+            const bool ours = (all_begins & span) != 0, closed = end < C::WARPS, take = (mine >> lane & 1) || (closed && lane == end);
+            const int  n = min(MANY, closed ? items[end].rows - r0 : mine ? MANY : 0);       // (rows of an open chain that are none are read by nobody)
+            if (n <= 0) continue;
+            const float * last = A.heads + (int64_t) (blockIdx.x * C::WARPS + (closed ? end : 0)) * C::PIECE, * p = closed && lane == end ? last : pieces + lane * C::PIECE;
+            float ao[MANY][CH], f[MANY], am[MANY], al[MANY];
 #pragma unroll
             for (int k = 0; k < MANY; k++) {
-                const int ri = (task0 + k) % C::RT, chain = (task0 + k) / C::RT, from = __shfl_sync(0xffffffffu, my_end, max(chain - 1, 0) & 31);
-                end[k] = __shfl_sync(0xffffffffu, my_end, chain & 31);
-                // pieces in shared memory (the warp where the chain before ends may begin this one); the one of warp `end` is in scratch
-                const uint32_t span = ((1u << end[k]) - 1) & ~((1u << (chain ? from : 0)) - 1);
-                mine[k] = all_goes & span;
-                ours[k] = (all_begins & span) != 0;
-                const bool closed = end[k] < C::WARPS;
-                does[k] = task0 + k < tasks && (closed ? ri < items[end[k]].rows : mine[k] != 0);      // (rows of an open chain that are none are read by nobody)
-                const bool take = (mine[k] >> lane & 1) || (closed && lane == end[k]);
-                const float * last = A.heads + (int64_t) (blockIdx.x * C::WARPS + end[k]) * C::PIECE, * p = closed && lane == end[k] ? last : pieces + lane * C::PIECE;
+                const int ri = r0 + min(k, n - 1);
+                if (closed) ka_get(last + ri * D + lane * CH, ao[k]);
+                else
 #pragma unroll
-                for (int c = 0; c < CH; c++) lv[k][c] = does[k] && closed ? last[ri * D + lane * CH + c] : 0.f;
-                pm[k] = does[k] && take ? p[C::RT * D + ri] : -INFINITY;
-                pl[k] = does[k] && take ? p[C::RT * D + C::RT + ri] : 0.f;
+                    for (int c = 0; c < CH; c++) ao[k][c] = 0.f;
+                am[k] = take ? p[C::RT * D + ri] : -INFINITY;
+                al[k] = take ? p[C::RT * D + C::RT + ri] : 0.f;
             }
 #pragma unroll
             for (int k = 0; k < MANY; k++) {
-                if (!does[k]) continue;
-                const int   ri = (task0 + k) % C::RT;
-                const bool  closed = end[k] < C::WARPS;
-                const float am = warp_max(pm[k]), f = pm[k] == am ? 1.f : exp2f(pm[k] - am), al = warp_sum(pl[k] * f), fe = __shfl_sync(0xffffffffu, f, end[k] & 31);
-                float ao[CH];
+                const float pm = am[k];
+                am[k] = warp_max(pm);
+                f[k]  = pm == am[k] ? 1.f : exp2f(pm - am[k]);
+                al[k] = warp_sum(al[k] * f[k]);
+                const float fe = __shfl_sync(0xffffffffu, f[k], end & 31);
 #pragma unroll
-                for (int c = 0; c < CH; c++) ao[c] = closed ? lv[k][c] * fe : 0.f;
+                for (int c = 0; c < CH; c++) ao[k][c] *= closed ? fe : 0.f;
+            }
 #pragma unroll 1
-                for (uint32_t rest = mine[k]; rest; rest &= rest - 1) {
-                    const int   w = __ffs(rest) - 1;
-                    const float fw = __shfl_sync(0xffffffffu, f, w);
+            for (uint32_t rest = mine; rest; rest &= rest - 1) {
+                const int w = __ffs(rest) - 1;
 #pragma unroll
-                    for (int c = 0; c < CH; c++) ao[c] = fmaf(pieces[w * C::PIECE + ri * D + lane * CH + c], fw, ao[c]);
+                for (int k = 0; k < MANY; k++) {
+                    const float fw = __shfl_sync(0xffffffffu, f[k], w);
+                    float v[CH];
+                    ka_get(pieces + w * C::PIECE + (r0 + min(k, n - 1)) * D + lane * CH, v);
+#pragma unroll
+                    for (int c = 0; c < CH; c++) ao[k][c] = fmaf(v[c], fw, ao[k][c]);
                 }
-                if (closed && ours[k]) ka_row_out<T, D>(A, items[end[k]], ri, lane, ao, al);
-                else {
-                    float * q = A.pieces + (int64_t) (2 * blockIdx.x + (ours[k] ? 1 : 0)) * C::PIECE;
+            }
+            float * q = A.pieces + (int64_t) (2 * blockIdx.x + (ours ? 1 : 0)) * C::PIECE;
 #pragma unroll
-                    for (int c = 0; c < CH; c++) q[ri * D + lane * CH + c] = ao[c];
-                    if (lane == 0) { q[C::RT * D + ri] = am; q[C::RT * D + C::RT + ri] = al; }
+            for (int k = 0; k < MANY; k++) {
+                if (k >= n) break;
+                const int ri = r0 + k;
+                if (closed && ours) ka_row_out<T, D>(A, items[end], ri, lane, ao[k], al[k]);
+                else {
+                    ka_put(q + ri * D + lane * CH, ao[k]);
+                    if (lane == 0) { q[C::RT * D + ri] = am[k]; q[C::RT * D + C::RT + ri] = al[k]; }
                 }
             }
         }
@@ -532,8 +543,10 @@ static __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_const
         for (int k = 0; k < n; k++) {
             const float * p = piece(w0 + k) + ri * D;
             const float   fk = __shfl_sync(0xffffffffu, f, k);
-            if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
-            else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
+            float v[CH];
+            ka_get(p + lane * CH, v);
+#pragma unroll
+            for (int c = 0; c < CH; c++) o[c] = fmaf(v[c], fk, o[c]);
         }
     }
     ka_row_out<T, D>(A, it, ri, lane, o, l);
