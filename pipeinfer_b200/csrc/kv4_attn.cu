@@ -66,9 +66,9 @@ __device__ __forceinline__ void ka_leave(float * p, int rows, int g, int t, cons
 }
 // row ri of an item from its sums over all keys, D / 32 channels a lane
 template <typename T, int D> __device__ __forceinline__ void ka_row_out(const ka_args & A, const ka_open & it, int ri, int lane, const float (&o)[D / 32], float l) {
-    const int   rc = it.row0 + ri;
+    const int   rc = it.row0 + ri, tk = ka_over(A, rc);
     const float inv = l > 0.f ? 1.f / l : l;
-    T * out = (T *) A.out + (it.tok0 + rc / A.rep) * A.ldo + (int64_t) (it.h * A.rep + rc % A.rep) * D + lane * (D / 32);
+    T * out = (T *) A.out + (it.tok0 + tk) * A.ldo + (int64_t) (it.h * A.rep + rc - tk * A.rep) * D + lane * (D / 32);
 #pragma unroll
     for (int c = 0; c < D / 32; c++) out[c] = (T) (o[c] * inv);
 }
@@ -81,6 +81,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     __shared__ int64_t  part[C::WARPS];
     __shared__ ka_open  items[C::WARPS], last_item[C::WARPS];
     __shared__ int      flags[C::WARPS];
+    __shared__ float    backs[C::WARPS][C::RT];
     __shared__ int      abort_w;
     volatile int * abort_s = &abort_w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, NST = A.stages;
@@ -88,6 +89,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     uint2 *    qsm  = reinterpret_cast<uint2 *>(ka_dsm + C::WARPS * NST * C::HALF) + warp * NR * C::PARTS * C::KS * 32 + lane;
     int64_t *  prefix = reinterpret_cast<int64_t *>(ka_dsm + C::WARPS * NST * C::HALF + C::Q_BYTES);         // [seqs + 1]
     ka_seq *   seq  = reinterpret_cast<ka_seq *>(prefix + A.seqs + 1);
+    float *    back = backs[warp];
     const uint32_t bar0 = dt_smem(bars + warp * 8), ring0 = dt_smem(ring);
     if (lane == 0) for (int i = 0; i < NST; i++) dt_mbar_init(bar0 + i * 8, 1);
     if (threadIdx.x == 0) abort_w = 0;
@@ -159,23 +161,29 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             const ka_seq  q = seq[at.s];
             const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = min(at.np - at.p, todo);
             const bool    whole = at.p == 0 && pages == at.np;
-            const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens);
-            const int     row0 = at.r * C::RT, pos0 = q.len - q.n;
+            const int     t0 = at.r * C::RT / A.rep, row0 = at.r * C::RT - t0 * A.rep, pos0 = q.len - q.n + t0;      // rows counted from the first token that has some
+            const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens) + t0;
             uint2 qf[C::QS ? 1 : C::PARTS][C::QS ? 1 : C::KS];
-#pragma unroll
+            // as the products' second operand a lane has row g: the channels of its t.  The next tile's are on their way meanwhile
+            uint32_t raw[D / 4 * sizeof(T) / 4];
+            auto fetch = [&](int n) {
+                const int rc = row0 + min(n * 8 + g, rows - 1), tk = ka_over(A, rc);
+                ka_fetch<T, D / 4>((const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc - tk * A.rep) * D + t * (D / 4), ka_here(A.wide_q), raw);
+            };
+            fetch(0);
+#pragma unroll 1
             for (int n = 0; n < NR; n++) {
-                // as the products' second operand a lane has row g: the channels of its t
-                const int rc = row0 + min(n * 8 + g, rows - 1), tk = rc / A.rep;
-                const T * p = (const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc % A.rep) * D + t * (D / 4);
                 float v[D / 4], top = 0.f;
-                ka_load<T, D / 4>(p, ka_here(A.wide_q), v);
 #pragma unroll
-                for (int c = 0; c < D / 4; c++) { v[c] *= A.scale * KA_LOG2E; top = fmaxf(top, fabsf(v[c])); }
+                for (int c = 0; c < D / 4; c++) { v[c] = ka_value<T>(raw, c) * (A.scale * KA_LOG2E); top = fmaxf(top, fabsf(v[c])); }
+                if (n + 1 < NR) fetch(n + 1);
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const ka_power pw = ka_power_of(top);
+                if (C::QS) { if (t == 0) back[n * 8 + g] = pw.back; }
+                else
 #pragma unroll
-                for (int r = 0; r < 2; r++) { qs[n][r] = __shfl_sync(0xffffffffu, pw.back, (2 * t + r) * 4); m[n][r] = -INFINITY; l[n][r] = 0.f; }
+                    for (int r = 0; r < 2; r++) qs[0][r] = __shfl_sync(0xffffffffu, pw.back, (2 * t + r) * 4);
 #pragma unroll
                 for (int k = 0; k < C::KS; k++) {                // product k of word k / 2 takes channels 2 (k % 2), 2 (k % 2) + 1 and four further
                     const int   c = (k >> 1) * 8 + (k & 1) * 2;
@@ -187,15 +195,22 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         if (C::QS) qsm[((n * C::PARTS + 1) * C::KS + k) * 32] = lo; else qf[C::QS || !C::SPLIT ? 0 : 1][C::QS ? 0 : k] = lo;
                     }
                 }
+            }
+            if (C::QS) __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+#pragma unroll
+                for (int r = 0; r < 2; r++) { if (C::QS) qs[n][r] = back[n * 8 + 2 * t + r]; m[n][r] = -INFINITY; l[n][r] = 0.f; }
 #pragma unroll
                 for (int i = 0; i < C::MT; i++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) O[n][i][c] = 0.f;
             }
+            if (C::QS) __syncwarp();                             // (the next item's may come)
             // keys that all rows see: from the last token's first one to the first token's last
-            const int all_hi = pos0 + row0 / A.rep, all_lo = max(0, pos0 + (row0 + rows - 1) / A.rep - ka_window(A) + 1);
+            const int all_hi = pos0, all_lo = max(0, pos0 + ka_over(A, row0 + rows - 1) - ka_window(A) + 1);
             // the last key that row r of the tiles sees, and the first
-            auto high = [&](int r) { return pos0 + (row0 + min(r, rows - 1)) / A.rep; };
+            auto high = [&](int r) { return pos0 + ka_over(A, row0 + min(r, rows - 1)); };
             auto low  = [&](int r) { return max(0, high(r) - ka_window(A) + 1); };
 
 #pragma unroll 1
@@ -410,8 +425,8 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         float v[C::C8];
 #pragma unroll
                         for (int c = 0; c < C::C8; c++) v[c] = O[n][c >> 1][2 * (c & 1) + r] * inv;
-                        const int rc = row0 + ri;
-                        ka_store<T, C::C8>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + g * C::C8, ka_here(A.wide_o), v);
+                        const int rc = row0 + ri, tk = ka_over(A, rc);
+                        ka_store<T, C::C8>((T *) A.out + (tok0 + tk) * A.ldo + (int64_t) (at.h * A.rep + rc - tk * A.rep) * D + g * C::C8, ka_here(A.wide_o), v);
                     }
             } else if (at.p + pages == at.np) {
                 ends = true;
@@ -623,7 +638,7 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     }
     if (ka_overlap((const uint8_t *) q, ldq * size, (const uint8_t *) out, ldo * size, row * size, b->tokens)) { pib_set_error("pib_kv4_attn: out lies over q"); return PIB_ERR_ARG; }
     ka_args A;
-    A.base = kv->base; A.pages = kv->pages; A.kvh = kv->heads; A.rep = b->heads / kv->heads; A.dim = kv->dim;
+    A.base = kv->base; A.pages = kv->pages; A.kvh = kv->heads; A.rep = b->heads / kv->heads; A.dim = kv->dim; A.part = (1u << 21) / A.rep + 1;
     A.starts = starts; A.lens = lens; A.table = pages; A.tokens = b->tokens; A.seqs = b->seqs; A.max_pages = b->max_pages; A.window = b->window; A.scale = b->scale;
     A.q = q; A.out = out; A.ldq = ldq; A.ldo = ldo;
     A.wide_q = ((uintptr_t) q & 15) == 0 && ldq * size % 16 == 0;

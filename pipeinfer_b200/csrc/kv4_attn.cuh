@@ -7,12 +7,14 @@
 #define KA_LOG2E 1.4426950408889634f
 
 struct ka_args {
-    const uint8_t * base; int64_t pages; int kvh, rep, dim;
+    const uint8_t * base; int64_t pages; int kvh, rep, dim; uint32_t part;                  // part: ka_over
     const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
     const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
     int stages; float * pieces, * heads; struct ka_plan * plan; struct ka_open * open; int * err;
 };
 
+// x / rep, x up to rep + 31 and rep up to 1024: a product, where a division in each row's place were a tenth of the decode kernel's code
+__device__ __forceinline__ int ka_over(const ka_args & A, int x) { return (int) ((uint32_t) x * A.part >> 21); }
 // a condition that stays where it is written: of one that holds for a whole loop the compiler makes two loops (of three, eight: 200 KB of code, which no instruction cache holds)
 __device__ __forceinline__ int ka_here(int v) { asm volatile("" : "+r"(v)); return v; }
 // dt_mbar_wait in few instructions: there is one at every turn, and the loops' code has to stay near
@@ -36,27 +38,20 @@ __device__ __forceinline__ ka_power ka_power_of(float top) {
 }
 
 // n neighbouring values as floats, n a multiple of 8
-template <typename T, int N> __device__ __forceinline__ void ka_load(const T * p, bool wide, float (&v)[N]) {
-    if constexpr (sizeof(T) == 4) {
-        if (wide) {
+template <typename T, int N> __device__ __forceinline__ void ka_fetch(const T * p, bool wide, uint32_t (&r)[N * sizeof(T) / 4]) {
+    if (wide) {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) { const float4 f = *reinterpret_cast<const float4 *>(p + i); v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w; }
-        } else
+        for (int i = 0; i < N * (int) sizeof(T) / 4; i += 4) { const uint4 f = reinterpret_cast<const uint4 *>(p)[i / 4]; r[i] = f.x; r[i + 1] = f.y; r[i + 2] = f.z; r[i + 3] = f.w; }
+    } else
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = p[i];
-    } else {
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < N; i += 8) {
-                const uint4 f = *reinterpret_cast<const uint4 *>(p + i);
-                const uint32_t w[4] = { f.x, f.y, f.z, f.w };
-#pragma unroll
-                for (int j = 0; j < 4; j++) { v[i + 2 * j] = __uint_as_float(w[j] << 16); v[i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
-            }
-        } else
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = __bfloat162float(p[i]);
-    }
+        for (int i = 0; i < N * (int) sizeof(T) / 4; i++) {
+            if constexpr (sizeof(T) == 4) r[i] = __float_as_uint(p[i]);
+            else                          r[i] = __bfloat16_as_ushort(p[2 * i]) | (uint32_t) __bfloat16_as_ushort(p[2 * i + 1]) << 16;
+        }
+}
+template <typename T> __device__ __forceinline__ float ka_value(const uint32_t * r, int c) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r[c]);
+    else                          return __uint_as_float(c & 1 ? r[c >> 1] & 0xffff0000u : r[c >> 1] << 16);
 }
 template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, bool wide, const float (&v)[N]) {
     if constexpr (sizeof(T) == 4) {
@@ -101,7 +96,7 @@ template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_
 
 // what both kernels know of the work: behind the pieces in the scratch
 struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // prompts: runs of units; units in front of each sequence
-// decode: of each run whether an item begins there and does not end there; the run where it does, its rows
+// decode: of each run whether an item begins there and does not end there; the run where it does, its first row counted from the first token in it (tok0), its rows
 struct ka_open { int runs, last, row0, rows, h; int64_t tok0; };
 
 // a sequence's tokens and keys from a table in shared memory, or from the call's
