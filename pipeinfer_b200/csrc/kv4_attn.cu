@@ -586,8 +586,9 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
-// rows (token, head of the group) of the longest portion: more than KA_FEW go on tcgen05
-#define KA_FEW 64
+// Rows (token, head of the group) of the longest portion: more than these go on tcgen05, which takes 256 rows in the time of one.  16 sequences of 3,000 keys, bfloat16: 59.5 us for 32 rows here (one walk over
+// the keys) and 83 there, 95 and 83.5 for 48 (two walks); fp32, 16 rows a walk: 111.5 and 126 for 48, 146 and 127 for 64.  60,000 keys of one sequence: 66 and 103, 108 and 103.5; 122 and 150, 155 and 152
+static int ka_few(int type) { return type == PIB_TYPE_F32 ? 48 : 32; }
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
 static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
@@ -595,7 +596,7 @@ static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int6
 struct ka_space { size_t heads, plan, open, total; };
 static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     const int    n = ka_tiles_of(kv, b), sms = pib_num_sms();
-    const bool   few = ka_rows(kv, b) <= KA_FEW;
+    const bool   few = ka_rows(kv, b) <= ka_few(b->type);
     const size_t piece = (size_t) (few ? n * 8 : KP_ROWS) * (kv->dim + 2) * 4;
     auto up = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     ka_space s;
@@ -649,7 +650,7 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     A.stages = 0;
     if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;
-    if (ka_rows(kv, b) > KA_FEW) return pib_kv4_prompt(A, size == 4, st);
+    if (ka_rows(kv, b) > ka_few(b->type)) return pib_kv4_prompt(A, size == 4, st);
     const int n = ka_tiles_of(kv, b);
     if (size == 4) {
         if (kv->dim == 64) return n == 1 ? ka_go<float, 64, 1>(A, st) : ka_go<float, 64, 2>(A, st);
