@@ -100,7 +100,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     const int     runs = (int) min((int64_t) gridDim.x, U);
     const int64_t c0 = blockIdx.x < runs ? U * blockIdx.x / runs : 0, c1 = blockIdx.x < runs ? U * (blockIdx.x + 1) / runs : 0;
     const ka_seq_table seq_of = { seq };
-    ka_zero_rows<C::RT, C::WARPS * 32, T>(A, D);
+    ka_zero_rows<C::RT, C::WARPS * 32, T>(A, seq_of, D);
     bool ok = true;
     // the warp's pieces of items that lie in several warps' units: one that ends here (in scratch), one that does not (in registers)
     bool    ends = false, goes = false, begins = false;
@@ -149,12 +149,9 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             if (ihalf) { left--; if (left) ka_next<C::RT>(A, prefix, seq_of, is); }
             ihalf ^= 1;
         };
-#pragma unroll 1
-        for (int i = 0; i < NST; i++) issue();
-
         int st = 0;
         uint32_t ph = 0;
-#pragma unroll 1
+        bool begun = false;
 #pragma unroll 1
         while (todo && ok) {
             // ---- an item, or the piece of it in this warp's run
@@ -162,7 +159,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             const int     rows = (int) min((int64_t) C::RT, (int64_t) q.n * A.rep - (int64_t) at.r * C::RT), pages = min(at.np - at.p, todo);
             const bool    whole = at.p == 0 && pages == at.np;
             const int     t0 = at.r * C::RT / A.rep, row0 = at.r * C::RT - t0 * A.rep, pos0 = q.len - q.n + t0;      // rows counted from the first token that has some
-            const int64_t tok0 = min(max(A.starts[at.s], 0), A.tokens) + t0;
+            const int64_t tok0 = q.start + t0;
             uint2 qf[C::QS ? 1 : C::PARTS][C::QS ? 1 : C::KS];
             // as the products' second operand a lane has row g: the channels of its t.  The next tile's are on their way meanwhile
             uint32_t raw[D / 4 * sizeof(T) / 4];
@@ -171,6 +168,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 ka_fetch<T, D / 4>((const T *) A.q + (tok0 + tk) * A.ldq + (int64_t) (at.h * A.rep + rc - tk * A.rep) * D + t * (D / 4), ka_here(A.wide_q), raw);
             };
             fetch(0);
+            if (!begun) {                                        // (behind the first queries' loads: both are on their way together)
+                begun = true;
+#pragma unroll 1
+                for (int i = 0; i < NST; i++) issue();
+            }
 #pragma unroll 1
             for (int n = 0; n < NR; n++) {
                 float v[D / 4], top = 0.f;

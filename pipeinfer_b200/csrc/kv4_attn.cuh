@@ -80,10 +80,10 @@ template <typename T, int N> __device__ __forceinline__ void ka_store(T * p, boo
 __device__ __forceinline__ int ka_window(const ka_args & A) { return A.window > 0 ? min(A.window, 0x7fff0000) : 0x7fff0000; }
 // ---- which keys a tile of rows sees ---------------------------------------------------------------------------------------------------
 // A sequence's rows, (token, head of the group) with the heads next to each other, are taken in tiles of RT; a tile of one key / value head is an item, its pages the units of work
-struct ka_seq { int n, len; };                      // query tokens and keys; both >= 0
+struct ka_seq { int n, len, start; };               // query tokens and keys, both >= 0; the first token's row
 __device__ __forceinline__ ka_seq ka_load_seq(const ka_args & A, int s) {
     const int a = min(max(A.starts[s], 0), A.tokens), b = min(max(A.starts[s + 1], 0), A.tokens);
-    return { max(b - a, 0), max(A.lens[s], 0) };
+    return { max(b - a, 0), max(A.lens[s], 0), a };
 }
 // pages [first, first + count) of tile r; keys behind the table's row are not there
 template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_seq q, int r, int & first) {
@@ -158,7 +158,7 @@ template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline
     __syncthreads();
     int64_t all = 0;
 #pragma unroll 1
-    for (int i = 0; i < THREADS / 32; i++) { if (i < warp) before += part[i]; all += part[i]; }
+    for (int i = 0; i * 32 * per < A.seqs; i++) { if (i < warp) before += part[i]; all += part[i]; }           // (warps without sequences add nothing)
 #pragma unroll 1
     for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
     if (threadIdx.x == 0) prefix[A.seqs] = all;
@@ -166,11 +166,11 @@ template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline
     return all;
 }
 // zeros into the rows of tiles without pages; sequences by blocks
-template <int RT, int THREADS, typename T> __device__ __forceinline__ void ka_zero_rows(const ka_args & A, int D) {
+template <int RT, int THREADS, typename T, typename Seq> __device__ __forceinline__ void ka_zero_rows(const ka_args & A, const Seq & seq, int D) {
 #pragma unroll 1
     for (int s = blockIdx.x; s < A.seqs; s += gridDim.x) {
-        const ka_seq  q = ka_load_seq(A, s);
-        const int64_t tok0 = min(max(A.starts[s], 0), A.tokens);
+        const ka_seq  q = seq(s);
+        const int64_t tok0 = q.start;
 #pragma unroll 1
         for (int r = 0; r < ka_tiles<RT>(A, q); r++) {
             int first;

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
     const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, of both groups; the weights take their scores' place; outputs 256..383 and 384..511
-    ka_zero_rows<KP_ROWS, KP_THREADS, T>(A, D);
+    ka_zero_rows<KP_ROWS, KP_THREADS, T>(A, ka_seq_call{ &A }, D);
     const int64_t u0 = me < runs ? U * me / runs : 0, u1 = me < runs ? U * (me + 1) / runs : 0;
     // whether some row of the item does not see all of a page
     auto edge_of = [&](const kp_item & it, int key0) { return key0 < it.lo || key0 + KV4_P - 1 > it.hi; };
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 if (pages > 0) {
                     kp_item it;
                     it.s = c.s; it.h = c.h; it.row0 = c.r * KP_ROWS; it.rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - it.row0);
-                    it.tok0 = min(max(A.starts[c.s], 0), A.tokens); it.pos0 = q.len - q.n;
+                    it.tok0 = q.start; it.pos0 = q.len - q.n;
                     it.page = c.first + p0; it.pages = pages;
                     it.hi = it.pos0 + it.row0 / A.rep;
                     it.lo = max(0, it.pos0 + (it.row0 + it.rows - 1) / A.rep - ka_window(A) + 1);
@@ -554,7 +554,7 @@ static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __gri
     if (ib < u0 || ib >= u1 || ie <= u1) return;
     const ka_seq  q = seq_of(at.s);
     const int     row0 = at.r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
-    const int64_t wb = (ie * runs + U - 1) / U - 1, tok0 = min(max(A.starts[at.s], 0), A.tokens);
+    const int64_t wb = (ie * runs + U - 1) / U - 1, tok0 = q.start;
     constexpr int CH = D / 32;
     for (int ri = blockIdx.y * 32 + warp; ri < min(rows, (int) blockIdx.y * 32 + 32); ri += 8) {
         float m = -INFINITY, l = 0.f, o[CH];
