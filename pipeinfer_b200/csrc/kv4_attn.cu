@@ -26,14 +26,15 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 // Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  fp32 rows enter as fp16 part and remainder,
 // two products; of bfloat16 rows queries and weights are one fp16 number.
 // An item that lies in one warp's units is written at once.  Pieces of others meet in shared memory at the end, in the order of the keys; what then is not a whole item goes to scratch, two pieces a block at
-// most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, twelve times as many, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
-// warps of a block, by the registers that a warp's tile takes, and the shared memory of fp32 queries' operands
-__host__ __device__ constexpr int ka_warps(bool split, int nr) { return nr == 1 || (nr == 2 && !split) ? 12 : 8; }
+// most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, as many times more, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
+// Warps of a block.  Twelve, where registers allow: bfloat16, 8 rows 57.5 us for 58.6 behind 131,071 keys, but 16.6 for 15.1 behind 2 x 600; 16 rows of 16 x 3,000 keys 41.9 for 37.5; fp32, 8 rows 50.6
+// for 48.1 of the 32 sequences
+#define KA_WARPS 8
 template <typename T, int D, int NR> struct ka_cfg {                 // NR: tiles of eight rows
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
-    static constexpr int  WARPS = ka_warps(SPLIT, NR);
-    static constexpr int  KB = NR == 1 && !SPLIT ? 64 : 32;                    // keys of which the scores are in registers at once (fp32, one tile: 64 do not fit, 53.5 us for 52.0)
+    static constexpr int  WARPS = KA_WARPS;
+    static constexpr int  KB = NR <= 2 && !SPLIT ? 64 : 32;          // keys of which the scores are in registers at once (fp32, 8 rows: with 64 the 32 sequences take 51.2 us for 48.1, 60,000 keys 40.3 for 42.5)
     static constexpr bool QS = NR > 1;                               // the queries' operands lie in shared memory
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
@@ -603,7 +604,7 @@ static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     auto up = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     ka_space s;
     s.heads = up(2 * sms * piece);
-    s.plan  = s.heads + (few ? up((size_t) sms * ka_warps(b->type == PIB_TYPE_F32, n) * piece) : b->type == PIB_TYPE_F32 ? (size_t) sms * KP_ROWS * kv->dim * 4 : 0);
+    s.plan  = s.heads + (few ? up((size_t) sms * KA_WARPS * piece) : b->type == PIB_TYPE_F32 ? (size_t) sms * KP_ROWS * kv->dim * 4 : 0);
     s.open  = s.plan + up(sizeof(ka_plan));
     s.total = s.open + up(sms * sizeof(ka_open));
     return s;
