@@ -7,8 +7,10 @@
 //   warp 0       streams blocks of both operands by TMA (a row's 128 bytes are a line of the 128-byte swizzle) through a ring; the first stages' weights start ahead of the launch wait
 //   warp 1       issues the MMAs; a commit hands the operands back, a tile's last one says that the accumulator is there
 //   warps 2..9   two groups of four, half of the columns each: a thread owns a weight row (lane)
-// The CTAs walk runs of 32 neighbouring rows, as many each as can be, in tiles of up to four (IT_GRAIN).  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks
+// The CTAs walk runs of 32 neighbouring rows, as many each as can be, in tiles of up to four.  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks
 // each and add their sums up through distributed shared memory: whole numbers, any order.
+// What bounds it: the weights' way from memory, at what one ring an SM asks for, and its start and end: 28672 x 8192 with 64 tokens 39 us (6.1 TB/s), 21999 x 5700 with 40, rounding launch included, 29.9
+// (4.2 TB/s: 688 runs on 148 SMs are 4 or 5).  One accumulator over the whole of K is what whole numbers allow: there is nothing to add up between blocks.
 // Every wait is bounded (tc_common.cuh).
 #include "i8_block.cuh"
 #include "tc_common.cuh"
@@ -241,6 +243,7 @@ int pib_i8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     const pib_i8_act L = pib_i8_act_of(w->K, b);
     int * err = pib_tc_error_word(st);
     if (!err) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
+    // pairs of SMs or this kernel, us at 96 and 128 tokens: 2560 x 2048 11.5 and 11.9 / 8.2 and 9.3, 4096 x 14336 39.5 and 40.1 / 16.6 and 18.0, 28672 x 8192 51.2 and 52.1 / 44.0 and 47.3
     if (b > 128) return pib_i8_gemm_pair(w, act, b, y, err, st);
     const int NB = b <= 16 ? 16 : b <= 32 ? 32 : b <= 48 ? 48 : b <= 64 ? 64 : b <= 96 ? 96 : 128;
     it_args A;
@@ -249,6 +252,7 @@ int pib_i8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     A.runs = (int) ((w->N + 31) / 32);
     const int tiles = (A.runs + 3) / 4;
     A.shares = 1;
+    // one / several shares, us at 16 tokens: 1024 x 2048 4.9 / 4.7, 2560 x 2048 5.5 / 4.8, 4096 x 14336 21.4 / 12.6
     while (A.shares < 8 && tiles * A.shares * 2 <= pib_num_sms() && A.KB >= A.shares * 4) A.shares *= 2;
     const pib_f8_runs & wmaps = ((const pib_f8_maps *) w->map)->runs;
     CUtensorMap xmap;

@@ -3,7 +3,8 @@
 //   m = fp16(min x), d = fp16((max x - m) / 15), n = rint((x - m) / d) in 0 .. 15; a channel stands for fp16(m + d n)
 //
 // A block per token: first its threads look whether a later token of the call has the same cell (the later one stays), then each takes eight neighbouring channels of a head's keys or values, four
-// threads a group of 32.  What bounds it: the launch for the tokens of a decode step; for prompts the way of the rows from memory.
+// threads a group of 32.  What bounds it: the launch for the tokens of a decode step (4 us each way); for prompts the blocks' short lives, a way to memory, the look at the
+// later cells, a barrier and a way out: 4,000 tokens of 8 heads of 128 in bfloat16 15 us, their values back 5.7.
 #include "kv4.cuh"
 
 #include <algorithm>
