@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     dt_fence_before();
     const int64_t U = ka_prefix<KP_ROWS, KP_LEAD, KP_THREADS, ka_seq_none>(A, prefix, part, {});
     dt_fence_after();
-    const int64_t runs = min((int64_t) gridDim.x, U), me = blockIdx.x;
+    // (runs of less than an item's start and end are not worth their pieces: 32 tokens behind 128, 512 and 4,096 keys 28 -> 20, 35 -> 28 and 49 -> 44 us)
+    const int64_t runs = min((int64_t) gridDim.x, (U + KP_LEAD - 1) / KP_LEAD), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
     const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, of both groups; the weights take their scores' place; outputs 256..383 and 384..511
     ka_zero_rows<KP_ROWS, KP_THREADS, T>(A, ka_seq_call{ &A }, D);
@@ -512,14 +513,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         v[x] = fmaf(o.x, f, v[x]); v[x + 1] = fmaf(o.y, f, v[x + 1]); v[x + 2] = fmaf(o.z, f, v[x + 2]); v[x + 3] = fmaf(o.w, f, v[x + 3]);
                     }
                 }
-                if (ri >= rows) continue;
                 const float k = none >> (c >> 5) & 1 ? __uint_as_float(0x7fc00000u) : whole ? inv : 1.f;
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] *= k;
-                if (whole) ka_store<T, 32>((T *) A.out + tok * A.ldo + head * D + c, ka_here(A.wide_o), v);
-                else       ka_store<float, 32>(piece + ri * D + c, true, v);
+                if (!whole)                                      // [D / 4][rows] of four channels each: a warp's stores are neighbours
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) reinterpret_cast<float4 *>(piece)[(c + x) / 4 * KP_ROWS + ri] = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                else if (ri < rows) ka_store<T, 32>((T *) A.out + tok * A.ldo + head * D + c, ka_here(A.wide_o), v);
+                __syncwarp();                                    // (the next columns are loaded by the warp as one)
             }
-            if (!whole && ri < rows) { piece[KP_ROWS * D + ri] = m; piece[KP_ROWS * D + KP_ROWS + ri] = sum; }
+            if (!whole) { piece[KP_ROWS * D + ri] = m; piece[KP_ROWS * D + KP_ROWS + ri] = sum; }
             dt_fence_before();
             return true;
         });
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Blocks (run, eighth of the rows): an item whose pages begin in the run and do not end there gets its pieces' sum, a row a warp, lanes the channels.
+// Blocks (run, eighth of the rows): an item whose pages begin in the run and do not end there gets its pieces' sum, a lane a row, a warp an eighth of the channels.
 template <typename T, int D>
 static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __grid_constant__ ka_args A) {
     using C = kp_cfg<T, D>;
@@ -555,34 +558,31 @@ static __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const __gri
     const ka_seq  q = seq_of(at.s);
     const int     row0 = at.r * KP_ROWS, rows = (int) min((int64_t) KP_ROWS, (int64_t) q.n * A.rep - row0);
     const int64_t wb = (ie * runs + U - 1) / U - 1, tok0 = q.start;
-    constexpr int CH = D / 32;
-    for (int ri = blockIdx.y * 32 + warp; ri < min(rows, (int) blockIdx.y * 32 + 32); ri += 8) {
-        float m = -INFINITY, l = 0.f, o[CH];
+    constexpr int CH = D / 8;
+    const int ri = blockIdx.y * 32 + lane;
+    if (ri >= rows) return;
+    auto piece = [&](int64_t w) { return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
+    float m = -INFINITY, l = 0.f, o[CH];
 #pragma unroll
-        for (int c = 0; c < CH; c++) o[c] = 0.f;
-        auto piece = [&](int64_t w) { return A.pieces + (2 * w + (w == wa ? 1 : 0)) * (int64_t) C::PIECE; };
-        for (int64_t w0 = wa; w0 <= wb; w0 += 32) {
-            const int n = (int) min((int64_t) 32, wb - w0 + 1);
-            float pm = -INFINITY, pl = 0.f;
-            if (lane < n) { pm = piece(w0 + lane)[KP_ROWS * D + ri]; pl = piece(w0 + lane)[KP_ROWS * D + KP_ROWS + ri]; }
-            const float mn = fmaxf(m, warp_max(pm)), a = m == mn ? 1.f : exp2f(m - mn), f = pm == mn ? 1.f : exp2f(pm - mn);
-            m = mn; l = l * a + warp_sum(lane < n ? pl * f : 0.f);
-#pragma unroll
-            for (int c = 0; c < CH; c++) o[c] *= a;
+    for (int c = 0; c < CH; c++) o[c] = 0.f;
 #pragma unroll 4
-            for (int k = 0; k < n; k++) {
-                const float * p = piece(w0 + k) + ri * D;
-                const float   fk = __shfl_sync(0xffffffffu, f, k);
-                if constexpr (CH == 4) { const float4 v = *reinterpret_cast<const float4 *>(p + lane * 4); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); o[2] = fmaf(v.z, fk, o[2]); o[3] = fmaf(v.w, fk, o[3]); }
-                else                   { const float2 v = *reinterpret_cast<const float2 *>(p + lane * 2); o[0] = fmaf(v.x, fk, o[0]); o[1] = fmaf(v.y, fk, o[1]); }
-            }
-        }
-        const int rc = row0 + ri;
-        T * out = (T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + lane * CH;
-        const float inv = l > 0.f ? 1.f / l : l;
+    for (int64_t w = wa; w <= wb; w++) m = fmaxf(m, piece(w)[KP_ROWS * D + ri]);
+#pragma unroll 2
+    for (int64_t w = wa; w <= wb; w++) {
+        const float * p = piece(w);
+        const float   pm = p[KP_ROWS * D + ri], f = pm == m ? 1.f : exp2f(pm - m);
+        l = fmaf(p[KP_ROWS * D + KP_ROWS + ri], f, l);
 #pragma unroll
-        for (int c = 0; c < CH; c++) out[c] = (T) (o[c] * inv);
+        for (int c = 0; c < CH; c += 4) {
+            const float4 v = reinterpret_cast<const float4 *>(p)[(warp * CH + c) / 4 * KP_ROWS + ri];
+            o[c] = fmaf(v.x, f, o[c]); o[c + 1] = fmaf(v.y, f, o[c + 1]); o[c + 2] = fmaf(v.z, f, o[c + 2]); o[c + 3] = fmaf(v.w, f, o[c + 3]);
+        }
     }
+    const int rc = row0 + ri;
+    const float inv = l > 0.f ? 1.f / l : l;
+#pragma unroll
+    for (int c = 0; c < CH; c++) o[c] *= inv;
+    ka_store<T, CH>((T *) A.out + (tok0 + rc / A.rep) * A.ldo + (int64_t) (at.h * A.rep + rc % A.rep) * D + warp * CH, A.wide_o, o);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------------
