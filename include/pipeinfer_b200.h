@@ -254,7 +254,7 @@ typedef struct pib_kv4_batch {
     int32_t window;               /* 0: all keys */
     float   scale;
 } pib_kv4_batch;
-/* scratch for such a call (a function of the batch and the device, not of the tables' contents); 0 where the batch is refused */
+/* scratch for such a call (a function of the batch and the device, not of the tables' contents; one for more tokens, or none or a higher max_tokens, serves fewer); 0 where the batch is refused */
 size_t    pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_batch * batch);
 /* q_dev and out_dev rows of heads * head_dim values, ldq and ldo elements apart; out does not overlap q.  starts_dev int32 [seqs + 1], not falling, from 0 to at most `tokens`; lens_dev int32 [seqs];
  * pages_dev int32 [seqs][max_pages].  The tables are read on the device, in the order of the stream: a captured call follows them from replay to replay.  scratch_dev: 256-byte aligned, any

@@ -589,8 +589,8 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
-// Rows (token, head of the group) of the longest portion: more than these go on tcgen05, which takes 256 rows in the time of one.  16 sequences of 3,000 keys, bfloat16: 59.5 us for 32 rows here (one walk over
-// the keys) and 83 there, 95 and 83.5 for 48 (two walks); fp32, 16 rows a walk: 111.5 and 126 for 48, 146 and 127 for 64.  60,000 keys of one sequence: 66 and 103, 108 and 103.5; 122 and 150, 155 and 152
+// Rows (token, head of the group) of the longest portion: more than these go on tcgen05, which takes 256 rows in the time of one.  16 sequences of 3,000 keys, bfloat16: 59 us for 32 rows here (one walk over the
+// keys) and 77 there, 94 and 77 for 48 (two walks); fp32, 16 rows a walk: 109 and 124 for 48, 143 and 125 for 64.  60,000 keys of one sequence: 67 and 93, 107 and 93; 120 and 140, 153 and 140
 static int ka_few(int type) { return type == PIB_TYPE_F32 ? 48 : 32; }
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large

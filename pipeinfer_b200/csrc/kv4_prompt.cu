@@ -17,7 +17,7 @@
 #include <algorithm>
 
 #define KP_THREADS 512
-#define KP_LEAD    8           // an item's start and end, in pages (portions of 1,999 tokens behind up to 4,100 keys: 568 us with 3, 495 with 8, 509 with 12, 519 with 16)
+#define KP_LEAD    8           // an item's start and end, in pages (portions of 1,999 tokens behind up to 4,100 keys: 500 us with 4, 477 with 8, 488 with 12)
 #define KP_BARS    32
 #define KP_FOLD    2           // fp32 rows: steps after which the outputs' sums leave tensor memory
 

@@ -430,6 +430,17 @@ def test_offsets_past_32_bits(torch, pib):
         assert float((out.double() - ref).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scratch_of_a_larger_batch_serves_a_smaller(torch, pib, t, dim):
+    kv = pib.Kv4(pib.load(), 4, 2, dim)
+    for rep in (1, 7, 16):
+        sizes = [kv.scratch_bytes(pib.Kv4Batch(t, 2 * rep, n, 3, 0, 5, 0, 1.0)) for n in (1, 2, 4, 5, 9, 17, 33, 64, 300, 65536)]
+        assert sizes == sorted(sizes) and sizes[0] > 0
+        hints = [kv.scratch_bytes(pib.Kv4Batch(t, 2 * rep, 300, 3, n, 5, 0, 1.0)) for n in (1, 2, 4, 9, 33, 64, 300, 0)]
+        assert hints == sorted(hints)
+
+
 def test_refusals_of_a_cache_that_is_there(torch, pib):
     lib = pib.load()
     kv = pib.Kv4(lib, 2, 2, 64)
