@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             dt_commit(bar_ke + 8 * (j % C::STG));
 #pragma unroll 1
             for (int i = 0; i < steps; i++, j++) {
-                // a group at a time, its next scores right behind its outputs: the other one forms its weights meanwhile.  (Both groups' outputs, then both groups' scores: the groups fall into step and
+                // a group at a time, its next scores right behind its outputs: the other one forms its weights meanwhile.  (Both groups' outputs, then both groups' scores, or a warp for each group's products, 529 us for 477: the groups fall into step and
                 // share the exponentials, then wait together)
 #pragma unroll 1
                 for (int w = 0; w < groups; w++) {
