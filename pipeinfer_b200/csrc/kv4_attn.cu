@@ -16,7 +16,7 @@ __device__ __forceinline__ void ka_mma0(float (&c)[4], uint32_t a0, uint32_t a1,
 // an 8 x 8 matrix of 16-bit numbers, two of a row a lane, turned
 __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 
-// All (sequence, tile of rows, key / value head, page) units lie in one row, which the blocks of the GPU divide evenly whatever the sequences' lengths, and a block's warps its run; a warp walks its units
+// All (sequence, tile of rows, key / value head, page) units lie in one row, which the blocks of the GPU divide evenly whatever the sequences' lengths (with an item's start and end counted as pages), and a block's warps its run; a warp walks its units
 // alone, with the running maximum and sum of each row in registers.  Lane 0 streams the pages' records (keys' half, values' half) by bulk copies through the warp's ring of STAGES halves.
 //   scores   turned, S' = K Q': mma.m16n8k16, 16 keys as M, eight rows as N, keys straight from nibbles in registers: lane (g, t) has 16 or 32 neighbouring channels of keys g and g + 8, one load and one step
 //            and lowest value each, four of them a product's k
@@ -36,12 +36,16 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr int  WARPS = KA_WARPS;
     static constexpr int  KB = NR <= 2 && !SPLIT ? 64 : 32;          // keys of which the scores are in registers at once (fp32, 8 rows: with 64 the 32 sequences take 51.2 us for 48.1, 60,000 keys 40.3 for 42.5)
     static constexpr bool QS = NR > 1;                               // the queries' operands lie in shared memory
+    // an item's start and end (queries, sums out, its piece's place), in pages' time: a block with one item of 16 x 4 tokens took 25.6 us, with five 36; of 32 single ones 35, and 0.8 for each more.  Without it,
+    // with 1 / 1 / 2 and with these: the former 44.6, 40.8, 39.8 us, the latter 47.9, 47.3, 45.7
+    static constexpr int  EXTRA = NR == 4 ? 3 : NR == 2 && SPLIT ? 1 : 2;
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
 };
 
 // what happens once an item is a call: the loop over pages is long enough
 template <int RT> __device__ __noinline__ ka_place ka_find_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, int64_t u) { return ka_find<RT, 0>(A, prefix, seq, u); }
+template <int RT, int EXTRA> __device__ __noinline__ int64_t ka_cut_call(const ka_args & A, const int64_t * prefix, const int * items, ka_seq_table seq, int64_t w) { return ka_cut<RT, EXTRA>(A, prefix, items, seq, w); }
 template <int RT> __device__ __noinline__ ka_place ka_next_call(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place c) { ka_next_item<RT, 0>(A, prefix, seq, c); return c; }
 template <int RT> __device__ __forceinline__ void ka_next(const ka_args & A, const int64_t * prefix, ka_seq_table seq, ka_place & c) { if (++c.p >= c.np) c = ka_next_call<RT>(A, prefix, seq, c); }
 // two or four neighbouring channels
@@ -79,7 +83,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     using C = ka_cfg<T, D, NR>;
     extern __shared__ __align__(128) uint8_t ka_dsm[];
     __shared__ uint64_t bars[C::WARPS * 8];
-    __shared__ int64_t  part[C::WARPS];
+    __shared__ int64_t  part[2 * C::WARPS];
     __shared__ ka_open  items[C::WARPS], last_item[C::WARPS];
     __shared__ int      flags[C::WARPS];
     __shared__ float    backs[C::WARPS][C::RT];
@@ -97,21 +101,25 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     pib_pdl_wait();
     pib_pdl_trigger();
-    const int64_t U = ka_prefix<C::RT, 0, C::WARPS * 32, ka_seq_table>(A, prefix, part, { seq });
+    int *         count = reinterpret_cast<int *>(seq + A.seqs);     // [seqs + 1]
+    const int64_t units = ka_prefix<C::RT, 0, C::WARPS * 32, ka_seq_table>(A, prefix, part, { seq }, count), U = units + (int64_t) C::EXTRA * count[A.seqs];
     const int     runs = (int) min((int64_t) gridDim.x, U);
-    const int64_t c0 = blockIdx.x < runs ? U * blockIdx.x / runs : 0, c1 = blockIdx.x < runs ? U * (blockIdx.x + 1) / runs : 0;
     const ka_seq_table seq_of = { seq };
+    const int64_t w0 = blockIdx.x < runs ? U * blockIdx.x / runs : 0, w1 = blockIdx.x < runs ? U * (blockIdx.x + 1) / runs : 0;
+    // (both ends at once, a lane each)
+    const int64_t cut = w0 < w1 ? ka_cut_call<C::RT, C::EXTRA>(A, prefix, count, seq_of, lane & 1 ? min(w1, U - 1) : w0) : 0;
+    const int64_t c0 = __shfl_sync(0xffffffffu, cut, 0), to = __shfl_sync(0xffffffffu, cut, 1), c1 = w0 < w1 && w1 == U ? units : to;
     ka_zero_rows<C::RT, C::WARPS * 32, T>(A, seq_of, D);
     bool ok = true;
     // the warp's pieces of items that lie in several warps' units: one that ends here (in scratch), one that does not (in registers)
     bool    ends = false, goes = false, begins = false;
-    int64_t item_end = 0;
     ka_place at = { 0, 0, 0, 0, 0, 0 };
     float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];            // of rows 2 t and 2 t + 1 of each tile
-    // A warp begins where an item does if that is near: items of few pages stay with one warp (a row of a chain of pieces costs 300 clocks, and the wait for what others have left in scratch)
+    // A warp begins where an item does if that is a page away: items of few pages stay with one warp.  (A row of a chain of pieces costs 300 clocks.  With a quarter of the warp's pages for "near" 131,071 keys took
+    // 61.2 us for 58.8, 64 fp32 sequences of up to 4,000 80.5 for 73.8: the longest warp is the block's time)
     if (c0 < c1) {
         const int64_t raw = c0 + (c1 - c0) * warp / C::WARPS;
-        const int     near = max(1, (int) ((c1 - c0) / C::WARPS) / 4);
+        const int     near = 1;
         at = ka_find_call<C::RT>(A, prefix, seq_of, raw);
         int64_t u = raw;
         if (warp > 0) {
@@ -435,7 +443,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 ends = true;
                 ka_leave<C, NR>(A.heads + (int64_t) (blockIdx.x * C::WARPS + warp) * C::PIECE, rows, g, t, O, m, l);
                 if (lane == 0) items[warp] = { 0, 0, row0, rows, at.h, tok0 };
-            } else { goes = true; begins = at.p == 0; item_end = u1 + (at.np - at.p - pages); if (lane == 0) last_item[warp] = { 0, 0, row0, rows, at.h, tok0 }; }
+            } else { goes = true; begins = at.p == 0; if (lane == 0) last_item[warp] = { 0, 0, row0, rows, at.h, tok0 }; }
             at.p += pages - 1;
             if (todo) ka_next<C::RT>(A, prefix, seq_of, at);
         }
@@ -522,10 +530,10 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             if (flags[w] & 1) break;
         }
         o.runs = goes && ours;
-        o.last = goes ? (int) ((item_end * runs + U - 1) / U - 1) : 0;
+        o.last = goes ? (int) ((ka_work<C::RT, C::EXTRA>(A, prefix, count, seq_of, at) * runs + U - 1) / U - 1) : 0;
         A.open[blockIdx.x] = o;
     }
-    if (threadIdx.x == 0 && blockIdx.x >= runs) A.open[blockIdx.x].runs = 0;
+    if (threadIdx.x == 0 && c0 >= c1) A.open[blockIdx.x].runs = 0;
     __syncthreads();
     if (*abort_s) {                                              // a wait ran out: say so, give copies still in flight time to land (bounded)
         if (threadIdx.x == 0) atomicExch(A.err, 1 + (int) blockIdx.x);
@@ -616,10 +624,10 @@ extern "C" size_t pib_kv4_attn_scratch_bytes(const pib_kv4 * kv, const pib_kv4_b
 
 template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st) {
     using C = ka_cfg<T, D, NR>;
-    const size_t table = ((size_t) (A.seqs + 1) * 8 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127;
+    const size_t table = ((size_t) (A.seqs + 1) * 12 + (size_t) A.seqs * sizeof(ka_seq) + 127) & ~(size_t) 127;
     constexpr size_t most = 224 * 1024;
     A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
-    static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 8 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
+    static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 12 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
     static_assert(C::PIECE * 4 <= 2 * C::HALF + C::Q_BYTES / C::WARPS, "pieces in the rings' and queries' place");
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));

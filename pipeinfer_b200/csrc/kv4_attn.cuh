@@ -136,34 +136,65 @@ template <int RT, int LEAD, typename Seq> __device__ __forceinline__ ka_place ka
     c.h = (int) (rest / c.np); c.p = (int) (rest % c.np);
     return c;
 }
-// Units in front of each sequence, by all THREADS threads of a block: a thread's neighbouring sequences, then warps, then the block.  part: THREADS / 32 numbers.  Ends with a barrier; the first block leaves
+// Units in front of each sequence (and items, if asked for), by all THREADS threads of a block: a thread's neighbouring sequences, then warps, then the block.  part: THREADS / 32 numbers (twice that).  Ends with a barrier; the first block leaves
 // them in the plan
-template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, Keep keep) {
+template <int RT, int LEAD, int THREADS, typename Keep> __device__ __forceinline__ int64_t ka_prefix(const ka_args & A, int64_t * prefix, int64_t * part, Keep keep, int * items = nullptr) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (A.seqs + THREADS - 1) / THREADS, s0 = threadIdx.x * per;
     int64_t sum = 0;
+    int     count = 0;
 #pragma unroll 1
     for (int s = s0; s < min(s0 + per, A.seqs); s++) {
         const ka_seq q = ka_load_seq(A, s);
         keep(s, q);
         prefix[s] = sum;
+        if (items) items[s] = count;
         int first;
 #pragma unroll 1
-        for (int r = 0; r < ka_tiles<RT>(A, q); r++) sum += (int64_t) ka_units<RT, LEAD>(A, q, r, first) * A.kvh;
+        for (int r = 0; r < ka_tiles<RT>(A, q); r++) { const int n = ka_units<RT, LEAD>(A, q, r, first); sum += (int64_t) n * A.kvh; count += n ? A.kvh : 0; }
     }
     int64_t before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int64_t v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
-    if (lane == 31) part[warp] = before;
+    int items_before = count;
+    if (items)
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, items_before, o); if (lane >= o) items_before += v; }
+    if (lane == 31) { part[warp] = before; if (items) part[THREADS / 32 + warp] = items_before; }
     before -= sum;
+    items_before -= count;
     __syncthreads();
     int64_t all = 0;
+    int     all_items = 0;
 #pragma unroll 1
-    for (int i = 0; i * 32 * per < A.seqs; i++) { if (i < warp) before += part[i]; all += part[i]; }           // (warps without sequences add nothing)
+    for (int i = 0; i * 32 * per < A.seqs; i++) {
+        if (i < warp) before += part[i];
+        all += part[i];
+        if (items) { const int v = (int) part[THREADS / 32 + i]; if (i < warp) items_before += v; all_items += v; }
+    }           // (warps without sequences add nothing)
 #pragma unroll 1
-    for (int s = s0; s < min(s0 + per, A.seqs); s++) prefix[s] += before;
-    if (threadIdx.x == 0) prefix[A.seqs] = all;
+    for (int s = s0; s < min(s0 + per, A.seqs); s++) { prefix[s] += before; if (items) items[s] += items_before; }
+    if (threadIdx.x == 0) { prefix[A.seqs] = all; if (items) items[A.seqs] = all_items; }
     __syncthreads();
     return all;
+}
+// Decode: runs are shares of work, of which an item's start and end are EXTRA pages' worth.  The first unit (page) behind share w of prefix[seqs] + EXTRA * items[seqs]
+template <int RT, int EXTRA, typename Seq> __device__ __forceinline__ int64_t ka_cut(const ka_args & A, const int64_t * prefix, const int * items, const Seq & seq, int64_t w) {
+    int lo = 0, hi = A.seqs;
+#pragma unroll 1
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (prefix[mid] + (int64_t) EXTRA * items[mid] <= w) lo = mid; else hi = mid; }
+    int64_t rest = w - prefix[lo] - (int64_t) EXTRA * items[lo], u = prefix[lo];
+    int n, first;
+#pragma unroll 1
+    for (int r = 0; (n = ka_pages<RT>(A, seq(lo), r, first)) == 0 || rest >= (int64_t) (n + EXTRA) * A.kvh; r++) if (n) { rest -= (int64_t) (n + EXTRA) * A.kvh; u += (int64_t) n * A.kvh; }
+    return u + rest / (n + EXTRA) * n + max((int) (rest % (n + EXTRA)) - EXTRA, 0);
+}
+// the work up to an item's end
+template <int RT, int EXTRA, typename Seq> __device__ __forceinline__ int64_t ka_work(const ka_args & A, const int64_t * prefix, const int * items, const Seq & seq, const ka_place & c) {
+    int64_t w = prefix[c.s] + (int64_t) EXTRA * items[c.s] + (int64_t) (c.h + 1) * (c.np + EXTRA);
+    int first;
+#pragma unroll 1
+    for (int r = 0; r < c.r; r++) { const int n = ka_pages<RT>(A, seq(c.s), r, first); if (n) w += (int64_t) (n + EXTRA) * A.kvh; }
+    return w;
 }
 // zeros into the rows of tiles without pages; sequences by blocks
 template <int RT, int THREADS, typename T, typename Seq> __device__ __forceinline__ void ka_zero_rows(const ka_args & A, const Seq & seq, int D) {
