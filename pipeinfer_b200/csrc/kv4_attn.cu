@@ -186,11 +186,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             for (int n = 0; n < NR; n++) {
                 float v[D / 4], top = 0.f;
 #pragma unroll
-                for (int c = 0; c < D / 4; c++) { v[c] = ka_value<T>(raw, c) * (A.scale * KA_LOG2E); top = fmaxf(top, fabsf(v[c])); }
+                for (int c = 0; c < D / 4; c++) { v[c] = C::SPLIT ? ka_value<T>(raw, c) * (A.scale * KA_LOG2E) : ka_value<T>(raw, c); top = fmaxf(top, fabsf(v[c])); }
                 if (n + 1 < NR) fetch(n + 1);
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const ka_power pw = ka_power_of(top);
+                const ka_power pw = ka_power_of<C::SPLIT>(top, A.scale);
                 if (C::QS) { if (t == 0) back[n * 8 + g] = pw.back; }
                 else
 #pragma unroll
@@ -218,6 +218,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                     for (int c = 0; c < 4; c++) O[n][i][c] = 0.f;
             }
             if (C::QS) __syncwarp();                             // (the next item's may come)
+            int huge = 0;                                        // bfloat16, of each tile: whether a row's maximum is beyond KA_HUGE
             // keys that all rows see: from the last token's first one to the first token's last
             const int all_hi = pos0, all_lo = max(0, pos0 + ka_over(A, row0 + rows - 1) - ka_window(A) + 1);
             // the last key that row r of the tiles sees, and the first
@@ -355,6 +356,13 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                             }
 #pragma unroll
                             for (int i3 = 0; i3 < C::MT; i3++) { O[n][i3][0] *= a[0]; O[n][i3][1] *= a[1]; O[n][i3][2] *= a[0]; O[n][i3][3] *= a[1]; }
+                            if (!C::SPLIT) huge = (huge & ~(1 << n)) | (__any_sync(0xffffffffu, fmaxf(fabsf(m[n][0]), fabsf(m[n][1])) > KA_HUGE) ? 1 << n : 0);
+                        }
+                        float q0 = qs[n][0], q1 = qs[n][1];
+                        if (!C::SPLIT && (huge >> n & 1)) {
+#pragma unroll
+                            for (int j = 0; j < C::KB / 16; j++) { S[j][n][0] *= q0; S[j][n][1] *= q1; S[j][n][2] *= q0; S[j][n][3] *= q1; }
+                            q0 = q1 = 1.f;
                         }
                         const float base0 = KA_LIFT - (m[n][0] == -INFINITY ? 0.f : m[n][0]), base1 = KA_LIFT - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
 #pragma unroll
@@ -362,7 +370,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                             uint32_t h[2], r[2];
 #pragma unroll
                             for (int x = 0; x < 2; x++) {
-                                const float a = ka_exp2(fmaf(S[j][n][2 * x], qs[n][0], base0)), b = ka_exp2(fmaf(S[j][n][2 * x + 1], qs[n][1], base1));
+                                const float a = ka_exp2(fmaf(S[j][n][2 * x], q0, base0)), b = ka_exp2(fmaf(S[j][n][2 * x + 1], q1, base1));
                                 l[n][0] += a; l[n][1] += b;
                                 h[x] = ka_pack(a, b);
                                 if (C::SPLIT) r[x] = ka_turn(ka_rest(a, b, h[x]));

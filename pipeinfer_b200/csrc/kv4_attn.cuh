@@ -30,11 +30,17 @@ __device__ __forceinline__ bool ka_wait(uint32_t bar, uint32_t parity, volatile 
     return false;
 }
 
-// A row's queries enter times scale log2 e, over the power of two of the largest: what scores are multiplied with is a power of two, exact, and so is the running maximum
+// A row's queries enter over the power of two that brings the largest to 2^14 .. 2^15.  fp32 rows, times scale log2 e before: two fp16 numbers hold 22 bits of a channel down to 2^-17 of the row's largest and
+// 2^-39 of the largest below; what scores are multiplied with is the power of two, exact, and so is the running maximum.  bfloat16 rows: one fp16 number holds every channel as it is down to 2^-30 of the
+// largest, so |scale| log2 e is left to the factor that scores are multiplied with (never 0: what is not seen stands at -inf); a maximum beyond KA_HUGE is rounded too far for one fused operation, and its
+// row's scores are then multiplied, and rounded, first
+#define KA_HUGE 1048576.f
 struct ka_power { float down, back; };
-__device__ __forceinline__ ka_power ka_power_of(float top) {
-    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-    return { __uint_as_float((254u - e) << 23), __uint_as_float(e << 23) };
+template <bool SPLIT> __device__ __forceinline__ ka_power ka_power_of(float top, float scale) {
+    const uint32_t e = min(max((int) (__float_as_uint(top) >> 23) - 14, 1), 240);
+    const float    down = __uint_as_float((254u - e) << 23), back = __uint_as_float(e << 23);
+    if (SPLIT) return { down, back };
+    return { copysignf(down, scale), fminf(fmaxf(back * fabsf(scale) * KA_LOG2E, 1.17549435e-38f), 3.4e38f) };
 }
 
 // n neighbouring values as floats, n a multiple of 8

@@ -362,14 +362,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             int ids = some(it.page);
             float qs;
             {
-                // the row times scale log2 e, over a power of two of its largest value, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
+                // the row as ka_power says, [0, 4, 1, 5, 2, 6, 3, 7] of eight channels as the keys have them.  Heads' rows of bfloat16 stay in registers between the passes
                 const T * p = (const T *) A.q + tok * A.ldq + head * D;
                 constexpr int N = C::SPLIT ? 32 : D;
                 kp_row<T, N> v;
                 float top = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < D; c += N) { v.load(p + c, ka_here(A.wide_q)); top = fmaxf(top, v.top()); }
-                const ka_power pw = ka_power_of(top * fabsf(A.scale * KA_LOG2E));
+                const ka_power pw = ka_power_of<C::SPLIT>(C::SPLIT ? top * fabsf(A.scale * KA_LOG2E) : top, A.scale);
                 qs = pw.back;
                 uint8_t * to = sQ + w * C::NC * C::Q_CHUNK + rt * 128;
 #pragma unroll 1
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         const int at16 = (N < D ? c >> 6 : i >> 3) * C::Q_CHUNK + (((N < D ? ((c & 63) >> 3) + i : i & 7) ^ (rt & 7)) << 4);
                         float x[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) x[k] = v.at(8 * i + k) * (A.scale * KA_LOG2E) * pw.down;
+                        for (int k = 0; k < 8; k++) x[k] = (C::SPLIT ? v.at(8 * i + k) * (A.scale * KA_LOG2E) : v.at(8 * i + k)) * pw.down;
                         const uint4 h = make_uint4(ka_pack(x[0], x[4]), ka_pack(x[1], x[5]), ka_pack(x[2], x[6]), ka_pack(x[3], x[7]));
                         *reinterpret_cast<uint4 *>(to + at16) = h;
                         if (C::SPLIT)
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             __syncwarp();
             if (lane == 0) dt_arrive(bar_q + 8 * w);
             float    m = -INFINITY, l = 0.f, l2 = 0.f, m_acc = -INFINITY;
-            bool     folded = false;
+            bool     folded = false, huge = false;
             float4 * acc = reinterpret_cast<float4 *>(A.heads) + me * (KP_ROWS * D / 4) + ri;         // [D / 4][rows]: what has left tensor memory, relative to m_acc
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
 #pragma unroll 1
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
-                if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; }
+                if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
                 if (i > 0 && rescale && !fold) {
 #pragma unroll 1
@@ -474,12 +474,19 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
 #pragma unroll 1
                 for (int h = two; h >= 0; h--) {
                     if (h != two) load(h);
+                    float q = qs;
+                    if (!C::SPLIT && __any_sync(0xffffffffu, huge)) {
+                        const float k = huge ? qs : 1.f;
+#pragma unroll
+                        for (int x = 0; x < 64; x++) t[x] = __float_as_uint(__uint_as_float(t[x]) * k);
+                        if (huge) q = 1.f;
+                    }
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         uint32_t e[16], r[16];
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
-                            const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), qs, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), qs, base));
+                            const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), q, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), q, base));
                             l += a; l2 += b;
                             e[x] = ka_pack(a, b);
                             if (C::SPLIT) r[x] = ka_rest(a, b, e[x]);
