@@ -23,8 +23,9 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 //   outputs  O' = V' P': 16 channels as M, weights (turned once more by movmatrix) as N, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
 // The tensor core cuts off what it adds to a sum, always towards zero: of fp32 rows the rests' scores have sums of their own, and each product of weights begins at zero and is added with rounding.  Error of
 // 20,000 keys against 64 bits 3.3e-6 -> 6.5e-7, for 48.4 -> 52.0 us of the 32 sequences below.
-// Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  fp32 rows enter as fp16 part and remainder,
-// two products; of bfloat16 rows queries and weights are one fp16 number.
+// Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  Queries of fp32 rows enter as fp16 part and
+// remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven bfloat16 outputs to its neighbour (now one of 2,000), for 60.2
+// instead of 63.7 us behind 131,071 keys and 40.4 instead of 41.8 for 16 x 4 tokens.
 // An item that lies in one warp's units is written at once.  Pieces of others meet in shared memory at the end, in the order of the keys; what then is not a whole item goes to scratch, two pieces a block at
 // most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, as many times more, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
 // Warps of a block.  Twelve, where registers allow: bfloat16, 8 rows 57.5 us for 58.6 behind 131,071 keys, but 16.6 for 15.1 behind 2 x 600; 16 rows of 16 x 3,000 keys 41.9 for 37.5; fp32, 8 rows 50.6
@@ -332,7 +333,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                         }
                     }
                     // ---- weights: the rows' maxima, exponentials, sums
-                    uint2 P[C::KB / 16][NR][C::PARTS];
+                    uint2 P[C::KB / 16][NR][2];              // and what fp16 took away of them
 #pragma unroll
                     for (int n = 0; n < NR; n++) {
                         float top[2];
@@ -373,11 +374,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                                 const float a = ka_exp2(fmaf(S[j][n][2 * x], q0, base0)), b = ka_exp2(fmaf(S[j][n][2 * x + 1], q1, base1));
                                 l[n][0] += a; l[n][1] += b;
                                 h[x] = ka_pack(a, b);
-                                if (C::SPLIT) r[x] = ka_turn(ka_rest(a, b, h[x]));
+                                r[x] = ka_turn(ka_rest(a, b, h[x]));
                                 h[x] = ka_turn(h[x]);
                             }
                             P[j][n][0] = make_uint2(h[0], h[1]);
-                            if (C::SPLIT) P[j][n][C::PARTS - 1] = make_uint2(r[0], r[1]);
+                            P[j][n][1] = make_uint2(r[0], r[1]);
                         }
                     }
                     // ---- outputs
@@ -411,11 +412,14 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                                         float (&to)[4] = O[n][w * 4 + e * 2 + c];
                                         if (C::SPLIT) {          // the rests' product, while the sum is small; then fp32 adds, with rounding
                                             float own[4];
-                                            ka_mma0(own, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][C::PARTS - 1]);
+                                            ka_mma0(own, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][1]);
                                             ka_mma(own, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][0]);
 #pragma unroll
                                             for (int k = 0; k < 4; k++) to[k] += own[k];
-                                        } else ka_mma(to, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][0]);
+                                        } else {
+                                            ka_mma(to, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][1]);
+                                            ka_mma(to, x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1], P[j][n][0]);
+                                        }
                                     }
                             }
                     }

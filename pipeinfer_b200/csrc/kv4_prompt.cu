@@ -10,7 +10,8 @@
 // The tensor core cuts off what it adds to a sum instead of rounding it, always towards zero: of fp32 rows the rests' products come first, while the sum is small, and the outputs' sums go to scratch
 // every KP_FOLD steps, are added there with rounding, and begin anew.  Error of 64,000 keys against 64 bits: 3.3e-6 of the outputs without either, 9.5e-7 with both at 2 steps (7.3e-7 at 1);
 // 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
-// fp32 queries and weights enter as fp16 part and remainder, two products each; of bfloat16 rows both are one fp16 number.
+// Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven
+// bfloat16 outputs to its neighbour, for 478 instead of 540 us (1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
 
@@ -218,12 +219,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             const uint64_t v0 = dv + (uint64_t) (j % C::STG * C::V_TILE >> 4);
             dt_fence_after();
 #pragma unroll 1
-            for (int r = 0; r < (C::SPLIT ? 2 : 1); r++)
+            for (int r = 0; r < 2; r++)
 #pragma unroll 1
                 for (int h = 0; h <= two; h++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * h + (C::SPLIT ? 32 - 32 * r : 0) + 8 * k, v0 + (uint64_t) (h * C::V_CHUNK >> 4) + 2 * k, id_o, add || (r | h | k) != 0);
+                        kp_mma_ts(tm_o + 128 * w, tmem + 128 * w + 64 * h + 32 - 32 * r + 8 * k, v0 + (uint64_t) (h * C::V_CHUNK >> 4) + 2 * k, id_o, add || (r | h | k) != 0);
             dt_commit(bar_o + 8 * w);
         };
         items([&](const kp_item & it) {
@@ -391,7 +392,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) dt_arrive(bar_q + 8 * w);
-            float    m = -INFINITY, l = 0.f, l2 = 0.f, m_acc = -INFINITY;
+            uint64_t ll = 0;
+            float    m = -INFINITY, m_acc = -INFINITY;
             bool     folded = false, huge = false;
             float4 * acc = reinterpret_cast<float4 *>(A.heads) + me * (KP_ROWS * D / 4) + ri;         // [D / 4][rows]: what has left tensor memory, relative to m_acc
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
-                if (grow) { f = ka_exp2(m - top); m = top; l *= f; l2 *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
+                if (grow) { f = ka_exp2(m - top); m = top; ll = ka_fma2(ll, ka_two(f, f), 0); huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
                 if (i > 0 && rescale && !fold) {
 #pragma unroll 1
@@ -486,14 +488,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                         uint32_t e[16], r[16];
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
-                            const float a = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x]), q, base)), b = ka_exp2(fmaf(__uint_as_float(t[32 * c + 2 * x + 1]), q, base));
-                            l += a; l2 += b;
-                            e[x] = ka_pack(a, b);
-                            if (C::SPLIT) r[x] = ka_rest(a, b, e[x]);
+                            const float2 z = ka_each(ka_fma2(ka_two(__uint_as_float(t[32 * c + 2 * x]), __uint_as_float(t[32 * c + 2 * x + 1])), ka_two(q, q), ka_two(base, base)));
+                            const uint64_t w2 = ka_two(ka_exp2(z.x), ka_exp2(z.y));
+                            ll = ka_add2(ll, w2);
+                            const float2 wf = ka_each(w2);
+                            e[x] = ka_pack(wf.x, wf.y);
+                            const float2 hf = ka_float2(e[x]);
+                            const float2 rf = ka_each(ka_sub2(w2, ka_two(hf.x, hf.y)));
+                            r[x] = ka_pack(rf.x, rf.y);
                         }
                         // in the page's scores' place, parts behind each other
                         kp_st16(tm_s + 64 * h + 16 * c, e);
-                        if (C::SPLIT) kp_st16(tm_s + 64 * h + 32 + 16 * c, r);
+                        kp_st16(tm_s + 64 * h + 32 + 16 * c, r);
                     }
                 }
                 dt_wait_st();
@@ -505,7 +511,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
             const bool    whole = it.whole;
-            const float   sum = l + l2, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
+            const float2  lf = ka_each(ll);
+            const float   sum = lf.x + lf.y, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
             float *       piece = A.pieces + (2 * me + it.slot) * (int64_t) C::PIECE;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {

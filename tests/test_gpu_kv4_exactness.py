@@ -46,3 +46,17 @@ def test_scores_of_the_queries_as_they_are(torch, pib, dim, n, rep, t, spread, s
     got = c.run()
     c.q *= scale                                          # what `want` takes times |scale|
     c.check(got)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rep,portions,lens", [(8, [1] * 40, [3 + 5 * i for i in range(40)]), (4, [4] * 30, [5 + 7 * i for i in range(30)]), (8, [150, 40], [150, 600]), (1, [300], [300])])
+def test_bfloat16_outputs_are_rounded_once(torch, pib, dim, rep, portions, lens):
+    """Weights beside bfloat16 rows have the bits that they have beside fp32 ones: outputs lie half a step of bfloat16 from the exact ones, and the bound of fp32 rows.  (Queries a tenth as large: scores of
+    about 1, so that this bound is a few 10^-6; weights of 11 bits are 2^-12 off.)"""
+    c = Case(torch, pib, BF16, 2, rep, dim, portions, lens)
+    c.q *= 0.1
+    got = c.run()[:c.rows].double()
+    c.t = F32
+    ref, lim = c.want()
+    half = torch.ldexp(torch.ones_like(ref), torch.frexp(ref.abs() + lim)[1] - 9)          # |o| in [2^(e - 1), 2^e): steps of 2^(e - 8)
+    assert ((got - ref).abs() <= half + lim).all(), float((((got - ref).abs() - half) / lim).max())
