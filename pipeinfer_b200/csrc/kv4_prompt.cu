@@ -12,6 +12,7 @@
 // 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
 // Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven
 // bfloat16 outputs to its neighbour, for 478 instead of 540 us (1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
+// A row's denominator is added up step by step with what the additions round away beside it: as one chain it was off by up to 5e-6 behind 64,000 keys.
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
 
@@ -392,8 +393,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) dt_arrive(bar_q + 8 * w);
-            uint64_t ll = 0;
-            float    m = -INFINITY, m_acc = -INFINITY;
+            float    m = -INFINITY, l = 0.f, l_low = 0.f, m_acc = -INFINITY;        // l_low: what additions to l rounded away
             bool     folded = false, huge = false;
             float4 * acc = reinterpret_cast<float4 *>(A.heads) + me * (KP_ROWS * D / 4) + ri;         // [D / 4][rows]: what has left tensor memory, relative to m_acc
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 const bool grow = top > m + KA_LAZY;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
-                if (grow) { f = ka_exp2(m - top); m = top; ll = ka_fma2(ll, ka_two(f, f), 0); huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
+                if (grow) { f = ka_exp2(m - top); m = top; l *= f; l_low *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
                 if (i > 0 && rescale && !fold) {
 #pragma unroll 1
@@ -473,6 +473,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     }
                 }
                 // the last page's scores are in registers still
+                uint64_t ll = 0;
 #pragma unroll 1
                 for (int h = two; h >= 0; h--) {
                     if (h != two) load(h);
@@ -506,13 +507,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 dt_fence_before();
                 __syncwarp();
                 if (lane == 0) dt_arrive(bar_p + 8 * w);
+                const float2 l2 = ka_each(ll);
+                const float  ls = l2.x + l2.y, lt = l + ls, lz = lt - l;
+                l_low += (l - (lt - lz)) + (ls - lz);
+                l = lt;
             }
             // ---- the row out, behind the last product
             if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
             const bool    whole = it.whole;
-            const float2  lf = ka_each(ll);
-            const float   sum = lf.x + lf.y, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
+            const float   sum = l + l_low, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
             float *       piece = A.pieces + (2 * me + it.slot) * (int64_t) C::PIECE;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {

@@ -1,7 +1,10 @@
-"""Attention over a 4-bit cache (csrc/kv4_attn.cu, kv4_prompt.cu) where few bits inside would show: scores far from zero whose difference decides, queries far below a row's largest."""
+"""Attention over a 4-bit cache (csrc/kv4_attn.cu, kv4_prompt.cu) where few bits inside would show: scores far from zero whose difference decides, queries far below a row's largest,
+sums over many keys that one warp or block takes alone, weights far below a row's largest."""
+import math
+
 import pytest
 
-from .test_gpu_kv4 import BF16, F32, Case, dtype, write
+from .test_gpu_kv4 import BF16, F32, PAGE, Case, dtype, read, write
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +63,68 @@ def test_bfloat16_outputs_are_rounded_once(torch, pib, dim, rep, portions, lens)
     ref, lim = c.want()
     half = torch.ldexp(torch.ones_like(ref), torch.frexp(ref.abs() + lim)[1] - 9)          # |o| in [2^(e - 1), 2^e): steps of 2^(e - 8)
     assert ((got - ref).abs() <= half + lim).all(), float((((got - ref).abs() - half) / lim).max())
+
+
+class Long:
+    """`seqs` sequences of the same `l` keys on the same pages, with as many items as the GPU has warps (single rows) or SMs (portions) and more, so that most of them lie whole in one run.  All have the same
+    queries, `n` tokens of `rep` heads: one sequence's exact rows are those of all."""
+
+    def __init__(self, torch, pib, t, n, rep, l, keys, values):
+        self.torch, self.t, self.n, self.rep, self.l, self.dim, self.kvh = torch, t, n, rep, l, 128, 8
+        sms = torch.cuda.get_device_properties(0).multi_processor_count
+        self.seqs = sms * (8 if n * rep <= 32 else 1) // self.kvh * 5 // 4 + 1
+        pages = (l + PAGE - 1) // PAGE
+        self.kv = pib.Kv4(pib.load(), pages, self.kvh, self.dim)
+        for i in range(0, l, 8192):
+            m = min(8192, l - i)
+            cells = torch.arange(i, i + m, dtype=torch.int32, device="cuda")
+            write(torch, self.kv, F32, keys(i, m), values(i, m), cells)
+        self.table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(self.seqs, 1)
+        self.starts = torch.arange(self.seqs + 1, dtype=torch.int32, device="cuda") * n
+        self.lens = torch.full((self.seqs,), l, dtype=torch.int32, device="cuda")
+        self.batch = pib.Kv4Batch(t, self.kvh * rep, n * self.seqs, self.seqs, n, pages, 0, self.dim ** -0.5)
+        self.scratch = torch.empty(self.kv.scratch_bytes(self.batch), dtype=torch.uint8, device="cuda")
+
+    def run(self, q):
+        """q [n, heads, dim] -> [seqs, n, heads, dim]"""
+        torch, w = self.torch, self.kvh * self.rep * self.dim
+        q = q.to(dtype(torch, self.t)).repeat(self.seqs, 1, 1, 1)
+        out = torch.full_like(q, 3.0)
+        self.kv.attention(self.batch, q.data_ptr(), w, self.starts.data_ptr(), self.lens.data_ptr(), self.table.data_ptr(), out.data_ptr(), w, self.scratch.data_ptr())
+        self.kv.lib.gemm_check(0)
+        return out
+
+    def want(self, q, heads):
+        """float64 rows of some query heads"""
+        torch, out = self.torch, []
+        K, V = (x.double() for x in read(torch, self.kv, F32, torch.arange(self.l, dtype=torch.int32, device="cuda"), self.kvh, self.dim))
+        hidden = torch.arange(self.l, device="cuda") > torch.arange(self.l - self.n, self.l, device="cuda").unsqueeze(1)
+        for h in heads:
+            s = (q[:, h].to(dtype(torch, self.t)).double() @ K[:, h // self.rep].T * self.dim ** -0.5).masked_fill(hidden, -math.inf)
+            out.append(torch.softmax(s, 1) @ V[:, h // self.rep])
+        return torch.stack(out, 1)
+
+
+def normal(torch, seed, scale):
+    def some(i, m):
+        g = torch.Generator(device="cuda").manual_seed(seed * 1000003 + i)
+        return torch.randn(m, 8, 128, device="cuda", generator=g) * scale
+    return some
+
+
+def ones(torch):
+    return lambda i, m: torch.ones(m, 8, 128, device="cuda")
+
+
+# a portion of many rows
+@pytest.mark.parametrize("n,rep", [(8, 8)])
+@pytest.mark.parametrize("l", [64000, 262144])
+def test_weights_add_up_to_one(torch, pib, n, rep, l):
+    """fp32, all values one, scores of 1.2: outputs are the sum of the weights in the products over their sum in the denominator.
+
+    An addition to a sum of one sign is off by at most 2^-24 of it, by 2^-24 / sqrt(3) in the mean square, and a chain of N of them by 2^-24 sqrt(N) / 3; one in a million passes five times that.  Chains of
+    64: 8e-7, for numerator and denominator 1.1e-6.  Inside 256 keys tensor cores add 32 times and cut up to 2^-23 of what the sum has grown to, half of that on average, half of the way up: 1e-6.
+    Exponentials and parts, 2^-22 each, are another for each key and the same above and below.  2.4e-6 with the output's own rounding; one chain through 64,000 keys may be off by 7e-6, and is."""
+    c = Long(torch, pib, F32, n, rep, l, normal(torch, 1, 1.0), ones(torch))
+    q = torch.randn(n, 8 * rep, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 1.2
+    assert float((c.run(q) - 1).abs().max()) < 2.4e-6
