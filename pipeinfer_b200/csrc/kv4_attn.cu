@@ -615,8 +615,8 @@ static int ka_few(int type) { return type == PIB_TYPE_F32 ? 48 : 32; }
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
 static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
-// the scratch: two pieces a block; decode: one of each warp, prompts of fp32: a block's sums; then the tables
-struct ka_space { size_t heads, plan, open, total; };
+// the scratch: two pieces a block; decode: one of each warp, prompts: a block's sums; then the tables
+struct ka_space { size_t heads, sums, plan, open, total; };
 static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     const int    n = ka_tiles_of(kv, b), sms = pib_num_sms();
     const bool   few = ka_rows(kv, b) <= ka_few(b->type);
@@ -624,7 +624,8 @@ static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     auto up = [](size_t v) { return (v + 255) & ~(size_t) 255; };
     ka_space s;
     s.heads = up(2 * sms * piece);
-    s.plan  = s.heads + (few ? up((size_t) sms * KA_WARPS * piece) : b->type == PIB_TYPE_F32 ? (size_t) sms * KP_ROWS * kv->dim * 4 : 0);
+    s.sums  = s.heads + (few ? up((size_t) sms * KA_WARPS * piece) : 0);
+    s.plan  = s.sums + (few ? 0 : up((size_t) sms * kp_sums(b->type == PIB_TYPE_F32, kv->dim) * 4));
     s.open  = s.plan + up(sizeof(ka_plan));
     s.total = s.open + up(sms * sizeof(ka_open));
     return s;
@@ -669,7 +670,7 @@ extern "C" int pib_kv4_attn(const pib_kv4 * kv, const pib_kv4_batch * b, const v
     A.wide_o = ((uintptr_t) out & 15) == 0 && ldo * size % 16 == 0;
     const ka_space sp = ka_space_of(kv, b);
     uint8_t * sc = (uint8_t *) scratch;
-    A.pieces = (float *) sc; A.heads = (float *) (sc + sp.heads); A.plan = (ka_plan *) (sc + sp.plan); A.open = (ka_open *) (sc + sp.open);
+    A.pieces = (float *) sc; A.heads = (float *) (sc + sp.heads); A.sums = (float *) (sc + sp.sums); A.plan = (ka_plan *) (sc + sp.plan); A.open = (ka_open *) (sc + sp.open);
     A.stages = 0;
     if (!(A.err = pib_tc_error_word((cudaStream_t) s))) { pib_set_error("pib_kv4_attn: no memory for the error word"); return PIB_ERR_NOMEM; }
     const cudaStream_t st = (cudaStream_t) s;

@@ -10,7 +10,7 @@ struct ka_args {
     const uint8_t * base; int64_t pages; int kvh, rep, dim; uint32_t part;                  // part: ka_over
     const int32_t * starts, * lens, * table; int tokens, seqs, max_pages, window; float scale;
     const void * q; void * out; int64_t ldq, ldo; bool wide_q, wide_o;       // rows that 16-byte loads and stores may take
-    int stages; float * pieces, * heads; struct ka_plan * plan; struct ka_open * open; int * err;
+    int stages; float * pieces, * heads, * sums; struct ka_plan * plan; struct ka_open * open; int * err;
 };
 
 // x / rep, x up to rep + 31 and rep up to 1024: a product, where a division in each row's place were a tenth of the decode kernel's code
@@ -247,6 +247,7 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// kv4_prompt.cu: launches; pieces in floats
+// kv4_prompt.cu: launches; rows of a block; floats of a block's sums that have left tensor memory
 #define KP_ROWS 256
+__host__ __device__ constexpr size_t kp_sums(bool f32, int dim) { return (size_t) (f32 ? 2 : 1) * KP_ROWS * (dim + 1); }
 int    pib_kv4_prompt(ka_args A, bool f32, cudaStream_t st);

@@ -7,9 +7,10 @@
 //   warps 4..7    write two pages' keys [128][dim] and their values, turned, [dim][128] as fp16 into tiles of the 128-byte swizzle
 //   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; then the other group's, while the first forms weights
 //   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 into the scores' place, from where they enter the second product
-// The tensor core cuts off what it adds to a sum instead of rounding it, always towards zero: of fp32 rows the rests' products come first, while the sum is small, and the outputs' sums go to scratch
-// every KP_FOLD steps, are added there with rounding, and begin anew.  Error of 64,000 keys against 64 bits: 3.3e-6 of the outputs without either, 9.5e-7 with both at 2 steps (7.3e-7 at 1);
-// 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
+// The tensor core cuts off what it adds to a sum instead of rounding it, always towards zero, some 2^-24 of it each time: of fp32 rows the rests' products come first, while the sum is small, and the outputs'
+// sums go to scratch every FOLD steps (fp32: 256 keys, bfloat16: 4,096), are added there with rounding, and begin anew; of fp32 rows those go on to a second sum every KP_FOLDS times.  Outputs of long items
+// that a block takes whole, all values one: fp32 within 4.8e-7 behind 64,000 and 7.2e-7 behind a million keys, bfloat16 low by 3e-5 beside their rounding at any length (without: 0.9e-3 behind 131,072 keys,
+// 0.005 behind a million).  fp32, 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
 // Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven
 // bfloat16 outputs to its neighbour, for 478 instead of 540 us (1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
 // A row's denominator is added up step by step with what the additions round away beside it: as one chain it was off by up to 5e-6 behind 64,000 keys.
@@ -21,7 +22,7 @@
 #define KP_THREADS 512
 #define KP_LEAD    8           // an item's start and end, in pages (portions of 1,999 tokens behind up to 4,100 keys: 500 us with 4, 477 with 8, 488 with 12)
 #define KP_BARS    32
-#define KP_FOLD    2           // fp32 rows: steps after which the outputs' sums leave tensor memory
+#define KP_FOLDS   64          // fp32 rows: times after which the sums in scratch go on to a second one
 
 // an item, or the piece of it in a run: its rows, pages [page, page + pages) of its sequence; keys hi and below, lo and above all its rows see; whether that is all of it, where its piece goes
 struct kp_item { int s, h, row0, rows, tok0, pos0, page, pages, hi, lo, whole, slot; };
@@ -30,6 +31,7 @@ struct kp_item { int s, h, row0, rows, tok0, pos0, page, pages, hi, lo, whole, s
 template <typename T, int D> struct kp_cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  W = D / 32, NC = D / 64, STG = SPLIT ? 1 : 2;               // groups; 64-wide column chunks of a head; tiles of keys and of values
+    static constexpr int  FOLD = SPLIT ? 2 : 32;                                     // steps after which the outputs' sums leave tensor memory
     static constexpr int  Q_CHUNK = 128 * 128, Q_PART = 2 * NC * Q_CHUNK;            // both groups' rows: [group][chunk][128 rows][128 bytes]
     static constexpr int  Q_BYTES = Q_PART * (SPLIT ? 2 : 1), K_CHUNK = 128 * 128, K_TILE = NC * K_CHUNK, V_CHUNK = D * 128, V_TILE = 2 * V_CHUNK;
     static constexpr int  TILES = Q_BYTES + STG * (K_TILE + V_TILE), REC = kv4_record(D);
@@ -48,6 +50,7 @@ __device__ __forceinline__ void kp_st16(uint32_t taddr, const uint32_t * v) {
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
                    "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
+__device__ __forceinline__ void kp_add(float4 & o, float4 a, float f) { o.x = fmaf(a.x, f, o.x); o.y = fmaf(a.y, f, o.y); o.z = fmaf(a.z, f, o.z); o.w = fmaf(a.w, f, o.w); }
 // fp16 x fp16, fp32 accumulators, both K-major, M x N outputs
 __host__ __device__ constexpr uint32_t kp_idesc(int M, int N) { return (1u << 4) | ((uint32_t) (N >> 3) << 17) | ((uint32_t) (M >> 4) << 24); }
 
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
 #pragma unroll 1
                 for (int w = 0; w < groups; w++) {
                     if (!wait(bar_p + 8 * w, n_p[w]) || (w == 0 && !wait(bar_vf + 8 * (j % C::STG), j / C::STG))) return false;
-                    outputs(w, 2 * i + 1 < pages, i > 0 && !(C::SPLIT && i % KP_FOLD == 0));
+                    outputs(w, 2 * i + 1 < pages, i % C::FOLD != 0);
                     n_p[w]++;
                     if (w == groups - 1) dt_commit(bar_ve + 8 * (j % C::STG));
                     if (i + 1 == steps) continue;
@@ -393,20 +396,21 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) dt_arrive(bar_q + 8 * w);
-            float    m = -INFINITY, l = 0.f, l_low = 0.f, m_acc = -INFINITY;        // l_low: what additions to l rounded away
-            bool     folded = false, huge = false;
-            float4 * acc = reinterpret_cast<float4 *>(A.heads) + me * (KP_ROWS * D / 4) + ri;         // [D / 4][rows]: what has left tensor memory, relative to m_acc
+            float    m = -INFINITY, l = 0.f, l_low = 0.f;        // l_low: what additions to l rounded away
+            bool     huge = false;
+            // what has left tensor memory, [D / 4][rows] of four channels each, and the maxima to which it is relative; of fp32 rows twice
+            auto sums = [&]() { return reinterpret_cast<float4 *>(A.sums + me * kp_sums(C::SPLIT, D)) + ka_here(ri); };
+            auto sums_m = [&](int level) -> float & { return (A.sums + me * kp_sums(C::SPLIT, D))[(C::SPLIT ? 2 : 1) * KP_ROWS * D + level * KP_ROWS + ka_here(ri)]; };
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
 #pragma unroll 1
-            for (int i = 0; i < pages; i += 2, j++, n++) {
-                const int two = i + 1 < pages;
-                if (i > 0 && (i & 31) == 0) ids = some(it.page + i);
-                const int  id0 = __shfl_sync(0xffffffffu, ids, i & 31), id1 = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
-                if (!wait(bar_s + 8 * w, n)) return false;
-                dt_fence_after();
-                const bool fold = C::SPLIT && i > 0 && i / 2 % KP_FOLD == 0;
-                if (fold) {                                      // (these scores came behind the end of the product before)
-                    const float f = m_acc == m ? 1.f : ka_exp2(m_acc - m);
+            for (int i0 = 0; i0 < pages; i0 += 2 * C::FOLD) {
+                if (i0 > 0) {                                    // (the next scores come behind the end of the product before)
+                    if (!wait(bar_s + 8 * w, n)) return false;
+                    dt_fence_after();
+                    const int   k = i0 / 2 / C::FOLD;            // the k-th time
+                    float4 *    acc = sums();
+                    const bool  have = C::SPLIT ? (k - 1) % KP_FOLDS != 0 : k > 1;
+                    const float ma = have ? sums_m(0) : m, f = ma == m ? 1.f : ka_exp2(ma - m);
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t v[32];
@@ -415,15 +419,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
 #pragma unroll
                         for (int x = 0; x < 32; x += 4) {
                             float4 * a = acc + (c + x) / 4 * KP_ROWS;
-                            float4   o = folded ? *a : make_float4(0.f, 0.f, 0.f, 0.f);
-                            o.x = fmaf(o.x, f, __uint_as_float(v[x])); o.y = fmaf(o.y, f, __uint_as_float(v[x + 1]));
-                            o.z = fmaf(o.z, f, __uint_as_float(v[x + 2])); o.w = fmaf(o.w, f, __uint_as_float(v[x + 3]));
+                            float4   o = make_float4(__uint_as_float(v[x]), __uint_as_float(v[x + 1]), __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
+                            if (have) kp_add(o, *a, f);
                             *a = o;
                         }
                     }
-                    folded = true;
-                    m_acc = m;
+                    sums_m(0) = m;
+                    if (C::SPLIT && k % KP_FOLDS == 0) {         // on to the second sum
+                        const float mb = k > KP_FOLDS ? sums_m(1) : m, fb = mb == m ? 1.f : ka_exp2(mb - m);
+#pragma unroll 1
+                        for (int c = 0; c < D / 4; c++) {
+                            float4 o = acc[c * KP_ROWS];
+                            if (k > KP_FOLDS) kp_add(o, acc[(c + D / 4) * KP_ROWS], fb);
+                            acc[(c + D / 4) * KP_ROWS] = o;
+                        }
+                        sums_m(1) = m;
+                    }
                 }
+#pragma unroll 1
+            for (int i = i0; i < min(i0 + 2 * C::FOLD, pages); i += 2, j++, n++) {
+                const int two = i + 1 < pages;
+                if (i > 0 && (i & 31) == 0) ids = some(it.page + i);
+                const int  id0 = __shfl_sync(0xffffffffu, ids, i & 31), id1 = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
+                if (!wait(bar_s + 8 * w, n)) return false;
+                dt_fence_after();
                 uint32_t t[64];
                 // a page's scores; keys that the row does not see are at -inf
                 auto load = [&](int h) {
@@ -461,7 +480,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 float f = 1.f;
                 if (grow) { f = ka_exp2(m - top); m = top; l *= f; l_low *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
                 const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
-                if (i > 0 && rescale && !fold) {
+                if (i > i0 && rescale) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t v[32];
@@ -512,25 +531,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 l_low += (l - (lt - lz)) + (ls - lz);
                 l = lt;
             }
+            }
             // ---- the row out, behind the last product
             if (!wait(bar_o + 8 * w, n + 1)) return false;
             dt_fence_after();
             const bool    whole = it.whole;
             const float   sum = l + l_low, inv = sum > 0.f ? 1.f / sum : sum;           // a row that saw nothing: zeros; a sum that is none stays so
             float *       piece = A.pieces + (2 * me + it.slot) * (int64_t) C::PIECE;
+            const int     folds = (pages - 1) / 2 / C::FOLD;     // how often sums have left
+            const float4 * acc = sums();
+            const bool    have = !C::SPLIT ? folds > 0 : folds % KP_FOLDS != 0, more = C::SPLIT && folds >= KP_FOLDS;
+            const float   ma = have ? sums_m(0) : m, f = ma == m ? 1.f : ka_exp2(ma - m), mb = more ? sums_m(1) : m, fb = mb == m ? 1.f : ka_exp2(mb - m);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
                 dt_ld32(tm_w + c, reinterpret_cast<uint32_t *>(v));
                 dt_wait_ld();
-                if (C::SPLIT && folded) {
-                    const float f = m_acc == m ? 1.f : ka_exp2(m_acc - m);
+                if (folds)
 #pragma unroll
                     for (int x = 0; x < 32; x += 4) {
-                        const float4 o = acc[(c + x) / 4 * KP_ROWS];
-                        v[x] = fmaf(o.x, f, v[x]); v[x + 1] = fmaf(o.y, f, v[x + 1]); v[x + 2] = fmaf(o.z, f, v[x + 2]); v[x + 3] = fmaf(o.w, f, v[x + 3]);
+                        float4 o = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                        if (have) kp_add(o, acc[(c + x) / 4 * KP_ROWS], f);
+                        if (more) kp_add(o, acc[(c + x) / 4 * KP_ROWS + KP_ROWS * D / 4], fb);
+                        v[x] = o.x; v[x + 1] = o.y; v[x + 2] = o.z; v[x + 3] = o.w;
                     }
-                }
                 const float k = none >> (c >> 5) & 1 ? __uint_as_float(0x7fc00000u) : whole ? inv : 1.f;
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] *= k;

@@ -118,7 +118,7 @@ def ones(torch):
 
 # a portion of many rows
 @pytest.mark.parametrize("n,rep", [(8, 8)])
-@pytest.mark.parametrize("l", [64000, 262144])
+@pytest.mark.parametrize("l", [64000, 262144, 1 << 20])
 def test_weights_add_up_to_one(torch, pib, n, rep, l):
     """fp32, all values one, scores of 1.2: outputs are the sum of the weights in the products over their sum in the denominator.
 
@@ -128,3 +128,20 @@ def test_weights_add_up_to_one(torch, pib, n, rep, l):
     c = Long(torch, pib, F32, n, rep, l, normal(torch, 1, 1.0), ones(torch))
     q = torch.randn(n, 8 * rep, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 1.2
     assert float((c.run(q) - 1).abs().max()) < 2.4e-6
+
+
+@pytest.mark.parametrize("n,rep", [(8, 8)])
+def test_bfloat16_sums_over_many_keys(torch, pib, n, rep):
+    """Values of one sign, 131,072 keys an item, outputs next to the middle between two numbers of bfloat16: sums that are low by a part in a thousand end on the wrong side.  Between two additions in fp32
+    lie 4,096 keys, 512 products; each cuts less than 2^-23 of what the sum has grown to, and the sum is halfway up on average: 512 * 2^-24 = 3.05e-5 of the output beside its rounding, and 1e-6 for what fp32
+    adds (chains of 32)."""
+    l = 131072
+
+    def values(i, m):
+        step = (torch.arange(i, i + m, device="cuda") * 7919 % 128).view(-1, 1) < torch.arange(128, device="cuda")
+        return (1 + 2.0 ** -8 + 2.0 ** -10 * step).unsqueeze(1).repeat(1, 8, 1)
+    c = Long(torch, pib, BF16, n, rep, l, normal(torch, 1, 1.0), values)
+    q = torch.randn(n, 8 * rep, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 1.2
+    got, heads = c.run(q), [0, rep, 7 * rep, 8 * rep - 1]
+    ref = c.want(q, heads)
+    assert float(((got[:, :, heads].double() - ref).abs()).max()) <= 2.0 ** -8 + 3.2e-5
