@@ -31,6 +31,9 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 // Warps of a block.  Twelve, where registers allow: bfloat16, 8 rows 57.5 us for 58.6 behind 131,071 keys, but 16.6 for 15.1 behind 2 x 600; 16 rows of 16 x 3,000 keys 41.9 for 37.5; fp32, 8 rows 50.6
 // for 48.1 of the 32 sequences
 #define KA_WARPS 8
+// Pages after which a warp's sums leave its registers.  They are added to those of the same item before, and begin anew: an item's chains of additions are of 64 pages' products (fp32), or of the products
+// that a tensor core adds and cuts (bfloat16), and of one number for each 4,096 keys.  (Without, items of 64,000 keys whose values are one were off by 3e-6, bfloat16 ones of a million by all of 0.008)
+#define KA_FOLD 64
 template <typename T, int D, int NR> struct ka_cfg {                 // NR: tiles of eight rows
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
@@ -42,6 +45,7 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr int  EXTRA = NR == 4 ? 3 : NR == 2 && SPLIT ? 1 : 2;
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
+    static constexpr int  SUMS = NR * (MT + 1) * 32;                 // a warp's sums that have left its registers, in four floats: of each tile outputs, and {maxima, denominators}
 };
 
 // what happens once an item is a call: the loop over pages is long enough
@@ -227,7 +231,9 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
             auto low  = [&](int r) { return max(0, high(r) - ka_window(A) + 1); };
 
 #pragma unroll 1
-            for (int i = 0; i < pages && ok; i++) {
+            for (int p0 = 0; p0 < pages; p0 += KA_FOLD) {
+#pragma unroll 1
+            for (int i = p0; i < min(p0 + KA_FOLD, pages) && ok; i++) {
                 const int key0 = (at.first + at.p + i) * KV4_P;
                 const bool in = there >> st & 1;
                 const uint32_t kst = st, kph = ph;
@@ -429,6 +435,34 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 issue();                                         // the values have been read
             }
             if (!ok) break;
+            float4 * sums = reinterpret_cast<float4 *>(A.sums) + (int64_t) (blockIdx.x * C::WARPS + warp) * C::SUMS + lane;
+            if (p0 > 0) {                                        // what has left the registers comes on top, relative to the present maxima (which never fall)
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    const float4 ml = sums[(NR * C::MT + n) * 32];
+                    const float  f0 = ml.x == m[n][0] ? 1.f : ka_exp2(ml.x - m[n][0]), f1 = ml.y == m[n][1] ? 1.f : ka_exp2(ml.y - m[n][1]);
+                    l[n][0] = fmaf(ml.z, f0, l[n][0]); l[n][1] = fmaf(ml.w, f1, l[n][1]);
+#pragma unroll
+                    for (int k = 0; k < C::MT; k++) {
+                        const float4 o = sums[(n * C::MT + k) * 32];
+                        O[n][k][0] = fmaf(o.x, f0, O[n][k][0]); O[n][k][1] = fmaf(o.y, f1, O[n][k][1]); O[n][k][2] = fmaf(o.z, f0, O[n][k][2]); O[n][k][3] = fmaf(o.w, f1, O[n][k][3]);
+                    }
+                }
+            }
+            if (p0 + KA_FOLD < pages)
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    sums[(NR * C::MT + n) * 32] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
+                    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < C::MT; k++) {
+                        sums[(n * C::MT + k) * 32] = make_float4(O[n][k][0], O[n][k][1], O[n][k][2], O[n][k][3]);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) O[n][k][c] = 0.f;
+                    }
+                }
+            }
+            if (!ok) break;
             // ---- rows out: lane (g, t) has D / 8 neighbouring channels of rows 2 t and 2 t + 1 of each tile
 #pragma unroll
             for (int n = 0; n < NR; n++)
@@ -615,7 +649,7 @@ static int ka_few(int type) { return type == PIB_TYPE_F32 ? 48 : 32; }
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large
 static int ka_tiles_of(const pib_kv4 * kv, const pib_kv4_batch * b) { const int64_t r = ka_rows(kv, b); return r <= 8 ? 1 : r <= 16 || b->type == PIB_TYPE_F32 ? 2 : 4; }
-// the scratch: two pieces a block; decode: one of each warp, prompts: a block's sums; then the tables
+// the scratch: two pieces a block; decode: one of each warp and the sums that have left its registers, prompts: a block's sums; then the tables
 struct ka_space { size_t heads, sums, plan, open, total; };
 static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     const int    n = ka_tiles_of(kv, b), sms = pib_num_sms();
@@ -625,7 +659,7 @@ static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     ka_space s;
     s.heads = up(2 * sms * piece);
     s.sums  = s.heads + (few ? up((size_t) sms * KA_WARPS * piece) : 0);
-    s.plan  = s.sums + (few ? 0 : up((size_t) sms * kp_sums(b->type == PIB_TYPE_F32, kv->dim) * 4));
+    s.plan  = s.sums + up((size_t) sms * (few ? (size_t) KA_WARPS * n * (kv->dim / 16 + 1) * 512 : kp_sums(b->type == PIB_TYPE_F32, kv->dim) * 4));
     s.open  = s.plan + up(sizeof(ka_plan));
     s.total = s.open + up(sms * sizeof(ka_open));
     return s;
@@ -642,6 +676,7 @@ template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st
     A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
     static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 12 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
     static_assert(C::PIECE * 4 <= 2 * C::HALF + C::Q_BYTES / C::WARPS, "pieces in the rings' and queries' place");
+    static_assert(C::SUMS * 16 == NR * (D / 16 + 1) * 512, "sums in the scratch");
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
     PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, NR>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));
