@@ -31,8 +31,9 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 // Warps of a block.  Twelve, where registers allow: bfloat16, 8 rows 57.5 us for 58.6 behind 131,071 keys, but 16.6 for 15.1 behind 2 x 600; 16 rows of 16 x 3,000 keys 41.9 for 37.5; fp32, 8 rows 50.6
 // for 48.1 of the 32 sequences
 #define KA_WARPS 8
-// Pages after which a warp's sums leave its registers.  They are added to those of the same item before, and begin anew: an item's chains of additions are of 64 pages' products (fp32), or of the products
-// that a tensor core adds and cuts (bfloat16), and of one number for each 4,096 keys.  (Without, items of 64,000 keys whose values are one were off by 3e-6, bfloat16 ones of a million by all of 0.008)
+// Pages after which a warp's sums leave its registers.  They are added to those of the same item before, fp32 rows' with compensation, and begin anew: additions with rounding (fp32 rows, one for each 16 keys)
+// and those of a tensor core that cuts (bfloat16 rows) are chains of 256 whatever the item's length.  (Without, fp32 outputs behind 64,000 keys whose values are one were off by 3e-6, bfloat16 ones behind
+// 131,072 keys low by 0.9e-3)
 #define KA_FOLD 64
 template <typename T, int D, int NR> struct ka_cfg {                 // NR: tiles of eight rows
     static constexpr bool SPLIT = sizeof(T) == 4;
@@ -45,7 +46,8 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr int  EXTRA = NR == 4 ? 3 : NR == 2 && SPLIT ? 1 : 2;
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
-    static constexpr int  SUMS = NR * (MT + 1) * 32;                 // a warp's sums that have left its registers, in four floats: of each tile outputs, and {maxima, denominators}
+    // a warp's sums that have left its registers, in four floats: of each tile outputs, and {maxima, denominators}; of fp32 rows behind them what additions to those rounded away
+    static constexpr int  REST = NR * (MT + 1) * 32, SUMS = SPLIT ? 2 * REST : REST;
 };
 
 // what happens once an item is a call: the loop over pages is long enough
@@ -352,11 +354,11 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) { top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o)); top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o)); }
                         top[0] *= qs[n][0]; top[1] *= qs[n][1];
-                        if (__any_sync(0xffffffffu, top[0] > m[n][0] + KA_LAZY || top[1] > m[n][1] + KA_LAZY)) {
+                        if (__any_sync(0xffffffffu, top[0] > m[n][0] + ka_lazy<C::SPLIT> || top[1] > m[n][1] + ka_lazy<C::SPLIT>)) {
                             float a[2];
 #pragma unroll
                             for (int r = 0; r < 2; r++) {
-                                const float mn = top[r] > m[n][r] + KA_LAZY ? top[r] : m[n][r];
+                                const float mn = top[r] > m[n][r] + ka_lazy<C::SPLIT> ? top[r] : m[n][r];
                                 a[r] = mn == m[n][r] ? 1.f : ka_exp2(m[n][r] - mn);
                                 m[n][r] = mn;
                                 l[n][r] *= a[r];
@@ -371,7 +373,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                             for (int j = 0; j < C::KB / 16; j++) { S[j][n][0] *= q0; S[j][n][1] *= q1; S[j][n][2] *= q0; S[j][n][3] *= q1; }
                             q0 = q1 = 1.f;
                         }
-                        const float base0 = KA_LIFT - (m[n][0] == -INFINITY ? 0.f : m[n][0]), base1 = KA_LIFT - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+                        const float base0 = ka_lift<C::SPLIT> - (m[n][0] == -INFINITY ? 0.f : m[n][0]), base1 = ka_lift<C::SPLIT> - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
 #pragma unroll
                         for (int j = 0; j < C::KB / 16; j++) {
                             uint32_t h[2], r[2];
@@ -435,32 +437,31 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                 issue();                                         // the values have been read
             }
             if (!ok) break;
-            float4 * sums = reinterpret_cast<float4 *>(A.sums) + (int64_t) (blockIdx.x * C::WARPS + warp) * C::SUMS + lane;
-            if (p0 > 0) {                                        // what has left the registers comes on top, relative to the present maxima (which never fall)
+            const bool last = p0 + KA_FOLD >= pages;
+            if (p0 > 0 || !last) {                               // what has left the registers, relative to the maxima of then (they never fall), and this portion's
+                float4 * sums = reinterpret_cast<float4 *>(A.sums) + (int64_t) (blockIdx.x * C::WARPS + warp) * C::SUMS + lane;
 #pragma unroll
                 for (int n = 0; n < NR; n++) {
-                    const float4 ml = sums[(NR * C::MT + n) * 32];
-                    const float  f0 = ml.x == m[n][0] ? 1.f : ka_exp2(ml.x - m[n][0]), f1 = ml.y == m[n][1] ? 1.f : ka_exp2(ml.y - m[n][1]);
-                    l[n][0] = fmaf(ml.z, f0, l[n][0]); l[n][1] = fmaf(ml.w, f1, l[n][1]);
+                    float4 * ml = sums + (NR * C::MT + n) * 32;
+                    float4   before = make_float4(m[n][0], m[n][1], 0.f, 0.f), e = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p0 > 0) { before = *ml; if (C::SPLIT) e = ml[C::REST]; }
+                    const float f0 = before.x == m[n][0] ? 1.f : ka_exp2(before.x - m[n][0]), f1 = before.y == m[n][1] ? 1.f : ka_exp2(before.y - m[n][1]);
+                    e.x *= f0; e.y *= f1;
+                    l[n][0] = ka_sum(before.z * f0, l[n][0], e.x); l[n][1] = ka_sum(before.w * f1, l[n][1], e.y);
+                    if (last) { if (C::SPLIT) { l[n][0] += e.x; l[n][1] += e.y; } }
+                    else { *ml = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]); if (C::SPLIT) ml[C::REST] = e; l[n][0] = l[n][1] = 0.f; }
 #pragma unroll
                     for (int k = 0; k < C::MT; k++) {
-                        const float4 o = sums[(n * C::MT + k) * 32];
-                        O[n][k][0] = fmaf(o.x, f0, O[n][k][0]); O[n][k][1] = fmaf(o.y, f1, O[n][k][1]); O[n][k][2] = fmaf(o.z, f0, O[n][k][2]); O[n][k][3] = fmaf(o.w, f1, O[n][k][3]);
+                        float4 * at = sums + (n * C::MT + k) * 32;
+                        float4   o = make_float4(O[n][k][0], O[n][k][1], O[n][k][2], O[n][k][3]);
+                        e = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (p0 > 0) { if (C::SPLIT) e = ka_times(at[C::REST], f0, f1); o = ka_sum(ka_times(*at, f0, f1), o, e); }
+                        if (!last) { *at = o; if (C::SPLIT) at[C::REST] = e; o = e = make_float4(0.f, 0.f, 0.f, 0.f); }
+                        O[n][k][0] = o.x; O[n][k][1] = o.y; O[n][k][2] = o.z; O[n][k][3] = o.w;
+                        if (C::SPLIT) { O[n][k][0] += e.x; O[n][k][1] += e.y; O[n][k][2] += e.z; O[n][k][3] += e.w; }
                     }
                 }
             }
-            if (p0 + KA_FOLD < pages)
-#pragma unroll
-                for (int n = 0; n < NR; n++) {
-                    sums[(NR * C::MT + n) * 32] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
-                    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-                    for (int k = 0; k < C::MT; k++) {
-                        sums[(n * C::MT + k) * 32] = make_float4(O[n][k][0], O[n][k][1], O[n][k][2], O[n][k][3]);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) O[n][k][c] = 0.f;
-                    }
-                }
             }
             if (!ok) break;
             // ---- rows out: lane (g, t) has D / 8 neighbouring channels of rows 2 t and 2 t + 1 of each tile
@@ -659,7 +660,7 @@ static ka_space ka_space_of(const pib_kv4 * kv, const pib_kv4_batch * b) {
     ka_space s;
     s.heads = up(2 * sms * piece);
     s.sums  = s.heads + (few ? up((size_t) sms * KA_WARPS * piece) : 0);
-    s.plan  = s.sums + up((size_t) sms * (few ? (size_t) KA_WARPS * n * (kv->dim / 16 + 1) * 512 : kp_sums(b->type == PIB_TYPE_F32, kv->dim) * 4));
+    s.plan  = s.sums + up((size_t) sms * (few ? (size_t) KA_WARPS * n * (kv->dim / 16 + 1) * (b->type == PIB_TYPE_F32 ? 1024 : 512) : kp_sums(b->type == PIB_TYPE_F32, kv->dim) * 4));
     s.open  = s.plan + up(sizeof(ka_plan));
     s.total = s.open + up(sms * sizeof(ka_open));
     return s;
@@ -676,7 +677,7 @@ template <typename T, int D, int NR> static int ka_go(ka_args A, cudaStream_t st
     A.stages = (int) std::min<size_t>(8, (most - C::Q_BYTES - table) / (C::WARPS * C::HALF));
     static_assert((most - C::Q_BYTES - (PIB_KV4_MAX_SEQS + 1) * 12 - PIB_KV4_MAX_SEQS * sizeof(ka_seq) - 128) / (C::WARPS * C::HALF) >= 2, "keys and values of a page");
     static_assert(C::PIECE * 4 <= 2 * C::HALF + C::Q_BYTES / C::WARPS, "pieces in the rings' and queries' place");
-    static_assert(C::SUMS * 16 == NR * (D / 16 + 1) * 512, "sums in the scratch");
+    static_assert(C::SUMS * 16 == NR * (D / 16 + 1) * (C::SPLIT ? 1024 : 512), "sums in the scratch");
     static pib_per_device attrs;
     PIB_CHECK(attrs.once([&] { return cudaFuncSetAttribute(kv4_decode_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) most); }));
     PIB_CHECK(pib_launch(kv4_decode_kernel<T, D, NR>, dim3((unsigned) pib_num_sms()), dim3(C::WARPS * 32), (size_t) C::WARPS * A.stages * C::HALF + C::Q_BYTES + table, st, A));

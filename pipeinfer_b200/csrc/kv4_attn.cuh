@@ -100,6 +100,11 @@ template <int RT> __device__ __forceinline__ int ka_pages(const ka_args & A, ka_
 }
 template <int RT> __device__ __forceinline__ int ka_tiles(const ka_args & A, ka_seq q) { return (int) (((int64_t) q.n * A.rep + RT - 1) / RT); }
 
+// a + b, and what the addition rounds away comes on top of e
+__device__ __forceinline__ float ka_sum(float a, float b, float & e) { const float t = a + b, z = t - a; e += (a - (t - z)) + (b - z); return t; }
+__device__ __forceinline__ float4 ka_sum(float4 a, float4 b, float4 & e) { return make_float4(ka_sum(a.x, b.x, e.x), ka_sum(a.y, b.y, e.y), ka_sum(a.z, b.z, e.z), ka_sum(a.w, b.w, e.w)); }
+__device__ __forceinline__ float4 ka_times(float4 a, float f, float g) { return make_float4(a.x * f, a.y * g, a.z * f, a.w * g); }
+
 // what both kernels know of the work: behind the pieces in the scratch
 struct ka_plan { int64_t runs, prefix[PIB_KV4_MAX_SEQS + 1]; };           // prompts: runs of units; units in front of each sequence
 // decode: of each run whether an item begins there and does not end there; the run where it does, its first row counted from the first token in it (tok0), its rows
@@ -228,8 +233,10 @@ template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_ar
     for (int s = threadIdx.x; s <= A.seqs; s += THREADS) A.plan->prefix[s] = prefix[s];
 }
 
-#define KA_LIFT  7.0f        // weights are e^(s - m) 2^7: fp16 then holds them down to 2^-31 of e^(s - m) = 1
-#define KA_LAZY  8.0f        // m follows the running maximum once that is 2^8 ahead: a weight is 2^15 at most, and few blocks of keys rescale the sums
+// Weights are e^(s - m) 2^lift, where m follows the running maximum once that is 2^lazy ahead: 2^15 at most.  Part and remainder in fp16 hold them down to 2^-25, that is 2^-32 (fp32 rows: 2^-39) of a row's
+// largest weight: less is nothing in the products, and a million keys of which each loses 2^-40 are 2^-20.  With a lazy maximum few blocks of keys rescale the sums, and bfloat16 outputs do not see what is lost
+template <bool SPLIT> constexpr float ka_lift = SPLIT ? 14.f : 7.f;
+template <bool SPLIT> constexpr float ka_lazy = SPLIT ? 1.f : 8.f;
 
 __device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
@@ -249,5 +256,5 @@ __device__ __forceinline__ void ka_bulk(uint32_t dst, const void * src, uint32_t
 
 // kv4_prompt.cu: launches; rows of a block; floats of a block's sums that have left tensor memory
 #define KP_ROWS 256
-__host__ __device__ constexpr size_t kp_sums(bool f32, int dim) { return (size_t) (f32 ? 2 : 1) * KP_ROWS * (dim + 1); }
+__host__ __device__ constexpr size_t kp_sums(bool f32, int dim) { return (size_t) KP_ROWS * (f32 ? 3 * dim + 2 : dim + 1); }
 int    pib_kv4_prompt(ka_args A, bool f32, cudaStream_t st);

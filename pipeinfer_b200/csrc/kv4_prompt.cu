@@ -6,10 +6,10 @@
 //   warp 0        brings pages' records (keys and values in 4 bits) by bulk copies through a ring
 //   warps 4..7    write two pages' keys [128][dim] and their values, turned, [dim][128] as fp16 into tiles of the 128-byte swizzle
 //   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; then the other group's, while the first forms weights
-//   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^KA_LAZY behind), weights as fp16 into the scores' place, from where they enter the second product
+//   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^ka_lazy behind), weights as fp16 into the scores' place, from where they enter the second product
 // The tensor core cuts off what it adds to a sum instead of rounding it, always towards zero, some 2^-24 of it each time: of fp32 rows the rests' products come first, while the sum is small, and the outputs'
-// sums go to scratch every FOLD steps (fp32: 256 keys, bfloat16: 4,096), are added there with rounding, and begin anew; of fp32 rows those go on to a second sum every KP_FOLDS times.  Outputs of long items
-// that a block takes whole, all values one: fp32 within 4.8e-7 behind 64,000 and 7.2e-7 behind a million keys, bfloat16 low by 3e-5 beside their rounding at any length (without: 0.9e-3 behind 131,072 keys,
+// sums go to scratch every FOLD steps (fp32: 256 keys, bfloat16: 4,096), are added there with rounding, and begin anew; of fp32 rows those go on to a second sum, with compensation, every KP_FOLDS times.  Outputs of long items
+// that a block takes whole, all values one: fp32 within 4.2e-7 behind 64,000 keys and a million, bfloat16 low by 3e-5 beside their rounding at any length (without: 0.9e-3 behind 131,072 keys,
 // 0.005 behind a million).  fp32, 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
 // Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven
 // bfloat16 outputs to its neighbour, for 478 instead of 540 us (1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
@@ -22,7 +22,7 @@
 #define KP_THREADS 512
 #define KP_LEAD    8           // an item's start and end, in pages (portions of 1,999 tokens behind up to 4,100 keys: 500 us with 4, 477 with 8, 488 with 12)
 #define KP_BARS    32
-#define KP_FOLDS   64          // fp32 rows: times after which the sums in scratch go on to a second one
+#define KP_FOLDS   16          // fp32 rows: times after which the sums in scratch go on to a second one (an addition of less than 2^-25 of a sum is lost: behind one large weight those of up to 4,096 keys)
 
 // an item, or the piece of it in a run: its rows, pages [page, page + pages) of its sequence; keys hi and below, lo and above all its rows see; whether that is all of it, where its piece goes
 struct kp_item { int s, h, row0, rows, tok0, pos0, page, pages, hi, lo, whole, slot; };
@@ -398,9 +398,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             if (lane == 0) dt_arrive(bar_q + 8 * w);
             float    m = -INFINITY, l = 0.f, l_low = 0.f;        // l_low: what additions to l rounded away
             bool     huge = false;
-            // what has left tensor memory, [D / 4][rows] of four channels each, and the maxima to which it is relative; of fp32 rows twice
+            // what has left tensor memory, [D / 4][rows] of four channels each, of fp32 rows three times (the sum, the second sum, what additions to that rounded away); then the maxima to which they are relative
             auto sums = [&]() { return reinterpret_cast<float4 *>(A.sums + me * kp_sums(C::SPLIT, D)) + ka_here(ri); };
-            auto sums_m = [&](int level) -> float & { return (A.sums + me * kp_sums(C::SPLIT, D))[(C::SPLIT ? 2 : 1) * KP_ROWS * D + level * KP_ROWS + ka_here(ri)]; };
+            auto sums_m = [&](int level) -> float & { return (A.sums + me * kp_sums(C::SPLIT, D))[(C::SPLIT ? 3 : 1) * KP_ROWS * D + level * KP_ROWS + ka_here(ri)]; };
             uint32_t none = 0;                                   // groups of channels of which this row sees a value that is none
 #pragma unroll 1
             for (int i0 = 0; i0 < pages; i0 += 2 * C::FOLD) {
@@ -427,11 +427,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     sums_m(0) = m;
                     if (C::SPLIT && k % KP_FOLDS == 0) {         // on to the second sum
                         const float mb = k > KP_FOLDS ? sums_m(1) : m, fb = mb == m ? 1.f : ka_exp2(mb - m);
+                        float4 *    sum = acc + KP_ROWS * D / 4, * low = sum + KP_ROWS * D / 4;
 #pragma unroll 1
                         for (int c = 0; c < D / 4; c++) {
-                            float4 o = acc[c * KP_ROWS];
-                            if (k > KP_FOLDS) kp_add(o, acc[(c + D / 4) * KP_ROWS], fb);
-                            acc[(c + D / 4) * KP_ROWS] = o;
+                            float4 o = acc[c * KP_ROWS], e = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (k > KP_FOLDS) { e = ka_times(low[c * KP_ROWS], fb, fb); o = ka_sum(ka_times(sum[c * KP_ROWS], fb, fb), o, e); }
+                            sum[c * KP_ROWS] = o;
+                            low[c * KP_ROWS] = e;
                         }
                         sums_m(1) = m;
                     }
@@ -475,11 +477,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     }
                 }
                 top *= qs;
-                const bool grow = top > m + KA_LAZY;
+                const bool grow = top > m + ka_lazy<C::SPLIT>;
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
                 if (grow) { f = ka_exp2(m - top); m = top; l *= f; l_low *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
-                const float base = KA_LIFT - (m == -INFINITY ? 0.f : m);
+                const float base = ka_lift<C::SPLIT> - (m == -INFINITY ? 0.f : m);
                 if (i > i0 && rescale) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -527,9 +529,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) dt_arrive(bar_p + 8 * w);
                 const float2 l2 = ka_each(ll);
-                const float  ls = l2.x + l2.y, lt = l + ls, lz = lt - l;
-                l_low += (l - (lt - lz)) + (ls - lz);
-                l = lt;
+                l = ka_sum(l, l2.x + l2.y, l_low);
             }
             }
             // ---- the row out, behind the last product
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                     for (int x = 0; x < 32; x += 4) {
                         float4 o = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
                         if (have) kp_add(o, acc[(c + x) / 4 * KP_ROWS], f);
-                        if (more) kp_add(o, acc[(c + x) / 4 * KP_ROWS + KP_ROWS * D / 4], fb);
+                        if (more) { kp_add(o, acc[(c + x) / 4 * KP_ROWS + KP_ROWS * D / 2], fb); kp_add(o, acc[(c + x) / 4 * KP_ROWS + KP_ROWS * D / 4], fb); }
                         v[x] = o.x; v[x + 1] = o.y; v[x + 2] = o.z; v[x + 3] = o.w;
                     }
                 const float k = none >> (c >> 5) & 1 ? __uint_as_float(0x7fc00000u) : whole ? inv : 1.f;
