@@ -244,7 +244,7 @@ int       pib_kv4_read(const pib_kv4 * kv, int type, const int32_t * cells_dev, 
  * pages[s * max_pages + j / PIB_KV4_PAGE]; several sequences may share pages.  Keys behind the table's row and on pages that the cache has not are not seen; a row that sees nothing is zeros.  Query head h
  * reads key / value head h / (heads / kv_heads).  Rows of out behind starts[seqs] are left as they are.  Scores, softmax and sums are fp32.  Queries enter the products with
  * 22 bits (fp32, times scale log2 e; down to 2^-17 of a row's largest) or as they are (bfloat16; down to 2^-30 of it), smaller ones to within 2^-39 of the row's largest.  Weights enter them with 22 bits,
- * to within 2^-40 of the largest that a row has seen (bfloat16: 2^-32). */
+ * to within 2^-39 of the largest that a row has seen (bfloat16: 2^-32). */
 typedef struct pib_kv4_batch {
     int32_t type;                 /* of q and out: PIB_TYPE_F32 or PIB_TYPE_BF16 */
     int32_t heads;                /* a multiple of the cache's */

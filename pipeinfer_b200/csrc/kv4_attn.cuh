@@ -234,7 +234,7 @@ template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_ar
 }
 
 // Weights are e^(s - m) 2^lift, where m follows the running maximum once that is 2^lazy ahead: 2^15 at most.  Part and remainder in fp16 hold them down to 2^-25, that is 2^-32 (fp32 rows: 2^-39) of a row's
-// largest weight: less is nothing in the products, and a million keys of which each loses 2^-40 are 2^-20.  With a lazy maximum few blocks of keys rescale the sums, and bfloat16 outputs do not see what is lost
+// largest weight: less is nothing in the products, and a million keys of which each loses 2^-39 are 2^-19.  With a lazy maximum few blocks of keys rescale the sums, and bfloat16 outputs do not see what is lost
 template <bool SPLIT> constexpr float ka_lift = SPLIT ? 14.f : 7.f;
 template <bool SPLIT> constexpr float ka_lazy = SPLIT ? 1.f : 8.f;
 
