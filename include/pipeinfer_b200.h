@@ -250,7 +250,8 @@ typedef struct pib_kv4_batch {
     int32_t heads;                /* a multiple of the cache's */
     int32_t tokens;               /* rows of q and out */
     int32_t seqs;
-    int32_t max_tokens;           /* most query tokens of one sequence, 0: not known.  Chooses the kernels; results hold whatever it says */
+    int32_t max_tokens;           /* most query tokens of one sequence, 0: not known, which counts as `tokens`.  Chooses the kernels, for all sequences of the call: one for few rows (max_tokens times
+                                   * heads that share a key / value head up to 32, fp32 48), one that takes 256 rows in the time of one.  Results hold whatever it says */
     int32_t max_pages;            /* entries of a row of pages_dev */
     int32_t window;               /* 0: all keys */
     float   scale;

@@ -9,8 +9,8 @@
 //   warps 2..9   two groups of four, half of the columns each: a thread owns a weight row (lane)
 // The CTAs walk runs of 32 neighbouring rows, as many each as can be, in tiles of up to four.  Where the tiles leave most SMs idle, 2, 4 or 8 CTAs of a cluster take a share of the blocks
 // each and add their sums up through distributed shared memory: whole numbers, any order.
-// What bounds it: the weights' way from memory, at what one ring an SM asks for, and its start and end: 28672 x 8192 with 64 tokens 39 us (6.1 TB/s), 21999 x 5700 with 40, rounding launch included, 29.9
-// (4.2 TB/s: 688 runs on 148 SMs are 4 or 5).  One accumulator over the whole of K is what whole numbers allow: there is nothing to add up between blocks.
+// What bounds it: the weights' way from memory, at what one ring an SM asks for, and its start and end: 28672 x 8192 with 64 tokens 39 us (6.1 TB/s), 21999 x 5700 with 40 25.3
+// (5.0 TB/s: 688 runs on 148 SMs are 4 or 5, and tiles begin inside row blocks; 18944 rows, four runs each, 5.5).  One accumulator over the whole of K is what whole numbers allow: there is nothing to add up between blocks.
 // Every wait is bounded (tc_common.cuh).
 #include "i8_block.cuh"
 #include "tc_common.cuh"
@@ -243,7 +243,9 @@ int pib_i8_gemm(const pib_weight * w, const void * act, int b, float * y, cudaSt
     const pib_i8_act L = pib_i8_act_of(w->K, b);
     int * err = pib_tc_error_word(st);
     if (!err) { pib_set_error("pib_gemm: no memory for the error word"); return PIB_ERR_NOMEM; }
-    // pairs of SMs or this kernel, us at 96 and 128 tokens: 2560 x 2048 11.5 and 11.9 / 8.2 and 9.3, 4096 x 14336 39.5 and 40.1 / 16.6 and 18.0, 28672 x 8192 51.2 and 52.1 / 44.0 and 47.3
+    // pairs of SMs or this kernel, us at 96 and 128 tokens: 2560 x 2048 11.5 and 11.9 / 8.2 and 9.3, 4096 x 14336 39.5 and 40.1 / 16.6 and 18.0, 28672 x 8192 51.2 and 52.1 / 44.0 and 47.3.
+    // Beyond 128 tokens this kernel would read the weights once for each 128: that is slower where the pairs have tiles for most SMs, and faster where they have not (4096 x 14336, 129 to 256 tokens: 38 on 16 of
+    // 74 pairs, twice 15 here), of which the rule takes no notice
     if (b > 128) return pib_i8_gemm_pair(w, act, b, y, err, st);
     const int NB = b <= 16 ? 16 : b <= 32 ? 32 : b <= 48 ? 48 : b <= 64 ? 64 : b <= 96 ? 96 : 128;
     it_args A;

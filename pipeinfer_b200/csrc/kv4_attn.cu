@@ -21,15 +21,14 @@ __device__ __forceinline__ uint32_t ka_turn(uint32_t v) { uint32_t r; asm("movma
 //   scores   turned, S' = K Q': mma.m16n8k16, 16 keys as M, eight rows as N, keys straight from nibbles in registers: lane (g, t) has 16 or 32 neighbouring channels of keys g and g + 8, one load and one step
 //            and lowest value each, four of them a product's k
 //   outputs  O' = V' P': 16 channels as M, weights (turned once more by movmatrix) as N, 16 keys as k; lane (g, t) has D / 8 neighbouring channels of four keys
-// The tensor core cuts off what it adds to a sum, always towards zero: of fp32 rows the rests' scores have sums of their own, and each product of weights begins at zero and is added with rounding.  Error of
-// 20,000 keys against 64 bits 3.3e-6 -> 6.5e-7, for 48.4 -> 52.0 us of the 32 sequences below.
-// Rows as N cost what is there in steps of eight: with rows as M eight rows were a product of sixteen, 128 of them a page and as many registers for outputs.  Queries of fp32 rows enter as fp16 part and
-// remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven bfloat16 outputs to its neighbour (now one of 2,000), for 60.2
-// instead of 63.7 us behind 131,071 keys and 40.4 instead of 41.8 for 16 x 4 tokens.
+// The tensor core cuts off what it adds to a sum, always towards zero: of fp32 rows the rests' scores have sums of their own, and each product of weights begins at zero and is added with rounding.
+// Rows as N cost what is there in steps of eight (as M, eight rows are a product of sixteen).  Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.
+// Weights are two products beside either: as one fp16 number they move one of eleven bfloat16 outputs to its neighbour (now one of 2,000), for 4 % of the time.
 // An item that lies in one warp's units is written at once.  Pieces of others meet in shared memory at the end, in the order of the keys; what then is not a whole item goes to scratch, two pieces a block at
-// most, and kv4_join_kernel adds those up.  (Warps that left their pieces in scratch, as many times more, had a join of 14 us behind 131071 keys and of 13 behind 16 x 4 tokens.)
-// Warps of a block.  Twelve, where registers allow: bfloat16, 8 rows 57.5 us for 58.6 behind 131,071 keys, but 16.6 for 15.1 behind 2 x 600; 16 rows of 16 x 3,000 keys 41.9 for 37.5; fp32, 8 rows 50.6
-// for 48.1 of the 32 sequences
+// most, and kv4_join_kernel adds those up.
+// What bounds it: two warps an SM quarter, each a chain of conversions, products, the rows' maxima and exponentials; of 64 / 8 heads of 128 one bfloat16 token behind 131,071 keys takes 61 us (its records'
+// bytes 26), 32 ragged fp32 sequences 47 (13), 16 x 4 bfloat16 tokens 41 (4: two pages a warp, so the start, queries, pieces and the join are most of it, and that kernel spills 248 bytes of its registers).
+// Captured calls' times, here and below.  Warps of a block: registers (217 to 255 a thread) allow no more
 #define KA_WARPS 8
 // Pages after which a warp's sums leave its registers.  They are added to those of the same item before, fp32 rows' with compensation, and begin anew: additions with rounding (fp32 rows, one for each 16 keys)
 // and those of a tensor core that cuts (bfloat16 rows) are chains of 256 whatever the item's length.  (Without, fp32 outputs behind 64,000 keys whose values are one were off by 3e-6, bfloat16 ones behind
@@ -39,10 +38,10 @@ template <typename T, int D, int NR> struct ka_cfg {                 // NR: tile
     static constexpr bool SPLIT = sizeof(T) == 4;
     static constexpr int  RT = 8 * NR, PARTS = SPLIT ? 2 : 1, KS = D / 16, W = D / 32, MT = D / 16, C8 = D / 8;
     static constexpr int  WARPS = KA_WARPS;
-    static constexpr int  KB = NR <= 2 && !SPLIT ? 64 : 32;          // keys of which the scores are in registers at once (fp32, 8 rows: with 64 the 32 sequences take 51.2 us for 48.1, 60,000 keys 40.3 for 42.5)
+    // keys of which the scores are in registers at once.  bfloat16, 8 rows, 131,071 keys: 61.4 us with 64, 65.1 with 32; 32 ragged sequences 67.1 and 71.6; 16 rows 40.7 and 41.2.  fp32 has registers for 32
+    static constexpr int  KB = NR <= 2 && !SPLIT ? 64 : 32;
     static constexpr bool QS = NR > 1;                               // the queries' operands lie in shared memory
-    // an item's start and end (queries, sums out, its piece's place), in pages' time: a block with one item of 16 x 4 tokens took 25.6 us, with five 36; of 32 single ones 35, and 0.8 for each more.  Without it,
-    // with 1 / 1 / 2 and with these: the former 44.6, 40.8, 39.8 us, the latter 47.9, 47.3, 45.7
+    // an item's start and end (queries, sums out, its piece's place), in pages' time.  With these and without: 16 x 4 tokens behind 300 to 8,190 keys 99 and 106 us, 32 such single ones 67 and 71, fp32 79 and 83
     static constexpr int  EXTRA = NR == 4 ? 3 : NR == 2 && SPLIT ? 1 : 2;
     static constexpr int  HALF = kv4_half(D), Q_BYTES = QS ? WARPS * NR * PARTS * KS * 256 : 0;
     static constexpr int  PIECE = RT * (D + 2);                      // floats
@@ -122,8 +121,8 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
     bool    ends = false, goes = false, begins = false;
     ka_place at = { 0, 0, 0, 0, 0, 0 };
     float qs[NR][2], m[NR][2], l[NR][2], O[NR][C::MT][4];            // of rows 2 t and 2 t + 1 of each tile
-    // A warp begins where an item does if that is a page away: items of few pages stay with one warp.  (A row of a chain of pieces costs 300 clocks.  With a quarter of the warp's pages for "near" 131,071 keys took
-    // 61.2 us for 58.8, 64 fp32 sequences of up to 4,000 80.5 for 73.8: the longest warp is the block's time)
+    // A warp begins where an item does if that is a page away: items of few pages stay with one warp.  Not further: the longest warp is the block's time (a quarter of the warp's pages: 32 fp32 sequences 89 us
+    // for 79, 131,071 keys 65 for 61; never: level)
     if (c0 < c1) {
         const int64_t raw = c0 + (c1 - c0) * warp / C::WARPS;
         const int     near = 1;
@@ -644,8 +643,8 @@ static bool ka_overlap(const uint8_t * a, int64_t lda, const uint8_t * b, int64_
     return true;
 }
 
-// Rows (token, head of the group) of the longest portion: more than these go on tcgen05, which takes 256 rows in the time of one.  16 sequences of 3,000 keys, bfloat16: 59 us for 32 rows here (one walk over the
-// keys) and 77 there, 94 and 77 for 48 (two walks); fp32, 16 rows a walk: 109 and 124 for 48, 143 and 125 for 64.  60,000 keys of one sequence: 67 and 93, 107 and 93; 120 and 140, 153 and 140
+// Rows (token, head of the group) of the longest portion: more than these go on tcgen05, which takes 256 rows in the time of one.  us here (a walk over the keys for each 32 rows, fp32 16) and there:
+//   16 x 3,000 keys: bfloat16 32 rows 64 / 92, 48 rows 101 / 93; fp32 48 rows 108 / 127, 64 rows 138 / 128.  60,000 keys: bfloat16 71 / 109, 114 / 110; fp32 124 / 143, 162 / 144
 static int ka_few(int type) { return type == PIB_TYPE_F32 ? 48 : 32; }
 static int64_t ka_rows(const pib_kv4 * kv, const pib_kv4_batch * b) { return (int64_t) (b->max_tokens ? std::min(b->max_tokens, b->tokens) : b->tokens) * (b->heads / kv->heads); }
 // tiles of eight rows that a warp takes at once; four only of bfloat16, whose queries' operands are half as large

@@ -238,6 +238,7 @@ template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_ar
 template <bool SPLIT> constexpr float ka_lift = SPLIT ? 14.f : 7.f;
 template <bool SPLIT> constexpr float ka_lazy = SPLIT ? 1.f : 8.f;
 
+// within 2^-22 of 2^x
 __device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t ka_pack(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
 __device__ __forceinline__ float2 ka_float2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }

@@ -8,19 +8,20 @@
 //   warp 1        issues the MMAs: a group's O += P V when its weights are there, its scores S = Q K' of the next two pages when that product is done; then the other group's, while the first forms weights
 //   warps 8..15   a thread owns a row: scores from tensor memory, mask, running maximum (it moves once 2^ka_lazy behind), weights as fp16 into the scores' place, from where they enter the second product
 // The tensor core cuts off what it adds to a sum instead of rounding it, always towards zero, some 2^-24 of it each time: of fp32 rows the rests' products come first, while the sum is small, and the outputs'
-// sums go to scratch every FOLD steps (fp32: 256 keys, bfloat16: 4,096), are added there with rounding, and begin anew; of fp32 rows those go on to a second sum, with compensation, every KP_FOLDS times.  Outputs of long items
-// that a block takes whole, all values one: fp32 within 4.2e-7 behind 64,000 keys and a million, bfloat16 low by 3e-5 beside their rounding at any length (without: 0.9e-3 behind 131,072 keys,
-// 0.005 behind a million).  fp32, 1,999 tokens of 32 heads: 264-276 us without, 294 at 2 steps, 340 at 1.
-// Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they moved one of eleven
-// bfloat16 outputs to its neighbour, for 478 instead of 540 us (1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
-// A row's denominator is added up step by step with what the additions round away beside it: as one chain it was off by up to 5e-6 behind 64,000 keys.
+// sums go to scratch every FOLD steps (fp32: 256 keys, bfloat16: 4,096), are added there with rounding, and begin anew; of fp32 rows those go on to a second sum, with compensation, every KP_FOLDS times.
+// Outputs of long items that a block takes whole, all values one: fp32 within 4.2e-7 behind 64,000 keys and a million, bfloat16 low by 3e-5 beside their rounding at any length (without: 0.9e-3 behind 131,072
+// keys).  fp32 portions of 1,999 and 1,200 tokens of up to 4,100 keys: 700 us without, 868 at 2 steps, 1,065 at 1.  Denominators are added up step by step, with compensation.
+// Queries of fp32 rows enter as fp16 part and remainder, two products, those of bfloat16 rows as one fp16 number.  Weights are two products beside either: as one fp16 number they move one of eleven
+// bfloat16 outputs to its neighbour (now one of 400), for 478 instead of 540 us (portions of 1,999 tokens of two sequences of up to 4,100 keys, 64 / 8 heads of 128).
+// What bounds it: no unit is full; a row's scores, weights and the two products follow one another, and two groups of rows are what tensor memory holds.  The portions above 545 us, in fp32 799; their operations at
+// the measured bfloat16 rate 155, at four products for two 310.
 // Every wait is bounded (tc_common.cuh).
 #include "kv4_attn.cuh"
 
 #include <algorithm>
 
 #define KP_THREADS 512
-#define KP_LEAD    8           // an item's start and end, in pages (portions of 1,999 tokens behind up to 4,100 keys: 500 us with 4, 477 with 8, 488 with 12)
+#define KP_LEAD    8           // an item's start and end, in pages (4, 8, 12: bfloat16 portions of 1,999 and 1,200 tokens 584, 588, 597 us, fp32 878, 868, 883; 32 tokens behind 4,096 keys 36, 36, 42; 1,999 fp32 tokens alone 188, 174, 182)
 #define KP_BARS    32
 #define KP_FOLDS   16          // fp32 rows: times after which the sums in scratch go on to a second one (an addition of less than 2^-25 of a sum is lost: behind one large weight those of up to 4,096 keys)
 
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
     dt_fence_before();
     const int64_t U = ka_prefix<KP_ROWS, KP_LEAD, KP_THREADS, ka_seq_none>(A, prefix, part, {});
     dt_fence_after();
-    // (runs of less than an item's start and end are not worth their pieces: 32 tokens behind 128, 512 and 4,096 keys 28 -> 20, 35 -> 28 and 49 -> 44 us)
+    // (runs of less than an item's start and end are not worth their pieces)
     const int64_t runs = min((int64_t) gridDim.x, (U + KP_LEAD - 1) / KP_LEAD), me = blockIdx.x;
     ka_leave_plan<KP_THREADS>(A, prefix, runs);
     const uint32_t tmem = *tmem_slot, tm_o = tmem + 256;          // columns: scores of two pages, 64 each, of both groups; the weights take their scores' place; outputs 256..383 and 384..511
@@ -241,8 +242,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
             dt_commit(bar_ke + 8 * (j % C::STG));
 #pragma unroll 1
             for (int i = 0; i < steps; i++, j++) {
-                // a group at a time, its next scores right behind its outputs: the other one forms its weights meanwhile.  (Both groups' outputs, then both groups' scores, or a warp for each group's products, 529 us for 477: the groups fall into step and
-                // share the exponentials, then wait together)
+                // a group at a time, its next scores right behind its outputs: the other one forms its weights meanwhile.  (Both groups' outputs, then both groups' scores, or a warp for each group's products, take a
+                // tenth longer: the groups fall into step, share the exponentials, then wait together)
 #pragma unroll 1
                 for (int w = 0; w < groups; w++) {
                     if (!wait(bar_p + 8 * w, n_p[w]) || (w == 0 && !wait(bar_vf + 8 * (j % C::STG), j / C::STG))) return false;

@@ -127,8 +127,11 @@ def test_weights_add_up_to_one(torch, pib, n, rep, l):
     Exponentials and parts, 2^-22 each, are another for each key and the same above and below.  2.4e-6 with the output's own rounding; one chain through 64,000 keys may be off by 7e-6, and is."""
     c = Long(torch, pib, F32, n, rep, l, normal(torch, 1, 1.0), ones(torch))
     q = torch.randn(n, 8 * rep, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 1.2
-    off = float((c.run(q) - 1).abs().max())
+    got = c.run(q)
+    off = float((got - 1).abs().max())
     assert off < 2.4e-6
+    c.scratch.fill_(255)
+    assert torch.equal(c.run(q), got)                     # whatever the scratch holds
 
 
 @pytest.mark.parametrize("n,rep", [(1, 8), (1, 1), (2, 8), (4, 8), (8, 8)])
