@@ -372,7 +372,7 @@ static __global__ void __launch_bounds__(ka_cfg<T, D, NR>::WARPS * 32, 1) kv4_de
                             for (int j = 0; j < C::KB / 16; j++) { S[j][n][0] *= q0; S[j][n][1] *= q1; S[j][n][2] *= q0; S[j][n][3] *= q1; }
                             q0 = q1 = 1.f;
                         }
-                        const float base0 = ka_lift<C::SPLIT> - (m[n][0] == -INFINITY ? 0.f : m[n][0]), base1 = ka_lift<C::SPLIT> - (m[n][1] == -INFINITY ? 0.f : m[n][1]);
+                        const float base0 = ka_base<C::SPLIT>(m[n][0]), base1 = ka_base<C::SPLIT>(m[n][1]);
 #pragma unroll
                         for (int j = 0; j < C::KB / 16; j++) {
                             uint32_t h[2], r[2];

@@ -237,6 +237,8 @@ template <int THREADS> __device__ __forceinline__ void ka_leave_plan(const ka_ar
 // largest weight: less is nothing in the products, and a million keys of which each loses 2^-39 are 2^-19.  With a lazy maximum few blocks of keys rescale the sums, and bfloat16 outputs do not see what is lost
 template <bool SPLIT> constexpr float ka_lift = SPLIT ? 14.f : 7.f;
 template <bool SPLIT> constexpr float ka_lazy = SPLIT ? 1.f : 8.f;
+// what exponents get beside their score: lift - m, rounded down, since maxima from 2^25 on have no such numbers between their own, and weights of more than 2^15 are none in fp16
+template <bool SPLIT> __device__ __forceinline__ float ka_base(float m) { return __fsub_rd(ka_lift<SPLIT>, m == -INFINITY ? 0.f : m); }
 
 // within 2^-22 of 2^x
 __device__ __forceinline__ float ka_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }

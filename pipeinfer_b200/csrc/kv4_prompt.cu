@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv4_prompt_kernel(const __grid_
                 const bool rescale = __any_sync(0xffffffffu, grow);
                 float f = 1.f;
                 if (grow) { f = ka_exp2(m - top); m = top; l *= f; l_low *= f; huge = !C::SPLIT && fabsf(m) > KA_HUGE; }
-                const float base = ka_lift<C::SPLIT> - (m == -INFINITY ? 0.f : m);
+                const float base = ka_base<C::SPLIT>(m);
                 if (i > i0 && rescale) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {

@@ -166,3 +166,30 @@ def test_weights_far_below_the_largest_count(torch, pib, n, rep, l):
     c = Long(torch, pib, F32, n, rep, l, keys, ones(torch))
     off = float((c.run(torch.ones(n, 8 * rep, 128, device="cuda")) - 1).abs().max())
     assert off < 2.4e-6 + l * 2.0 ** -39
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n,rep,dim", [(1, 8, 128), (1, 1, 64), (4, 4, 64), (120, 1, 128)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_all_magnitudes(torch, pib, t, n, rep, dim, sign):
+    """Scores about 2^k for k from 0 to 60, most of them too far apart for a softmax: where the largest leads by more than 64 times what scores are known to, the output is its key's value, and elsewhere it lies
+    between the values' ends.  `sign`: all of them positive, or negative."""
+    seqs = 122 // n + 1
+    c = Case(torch, pib, t, 1, rep, dim, [n] * seqs, [n + 300] * seqs)
+    k = [torch.rand(n + 300, 1, dim, device="cuda", generator=c.g) + 0.5 for _ in range(seqs)]
+    v = [torch.randn(n + 300, 1, dim, device="cuda", generator=c.g) for _ in range(seqs)]
+    for i in range(seqs):
+        write(torch, c.kv, F32, k[i], v[i], c.cells(i, n + 300).contiguous())
+    c.q = (c.q.abs() * sign * 2.0 ** (torch.arange(c.rows, device="cuda") % 61 - 2 - dim // 64).view(-1, 1, 1)).to(dtype(torch, t))
+    got = c.run().double()
+    assert got.isfinite().all()
+    for i in range(seqs):
+        K, V = (x.double() for x in read(torch, c.kv, F32, c.cells(i, n + 300), 1, dim))
+        q, o = c.q[i * n:(i + 1) * n].double(), got[i * n:(i + 1) * n]
+        s = torch.einsum("thd,kd->thk", q, K[:, 0]) * dim ** -0.5
+        s.masked_fill_((torch.arange(n + 300, device="cuda") > torch.arange(300, n + 300, device="cuda").view(-1, 1)).unsqueeze(1), -math.inf)
+        top, at = s.topk(2, -1)
+        E = s[..., 0].abs() * 2 * ((dim / 8) * 2.0 ** -22 + 2.0 ** -21)          # as in Case.want
+        clear = top[..., 0] - top[..., 1] > 64 * E + 64
+        assert ((o - V[:, 0][at[..., 0]]).abs()[clear] <= V.abs().max() * (2.0 ** -20 if t == F32 else 2.0 ** -8)).all()
+        assert (o <= V.max() * 1.01).all() and (o >= V.min() * 1.01).all()
