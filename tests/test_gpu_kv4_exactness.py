@@ -69,8 +69,8 @@ class Long:
     """`seqs` sequences of the same `l` keys on the same pages, with as many items as the GPU has warps (single rows) or SMs (portions) and more, so that most of them lie whole in one run.  All have the same
     queries, `n` tokens of `rep` heads: one sequence's exact rows are those of all."""
 
-    def __init__(self, torch, pib, t, n, rep, l, keys, values):
-        self.torch, self.t, self.n, self.rep, self.l, self.dim, self.kvh = torch, t, n, rep, l, 128, 8
+    def __init__(self, torch, pib, t, n, rep, l, keys, values, window=0):
+        self.torch, self.t, self.n, self.rep, self.l, self.dim, self.kvh, self.window = torch, t, n, rep, l, 128, 8, window
         sms = torch.cuda.get_device_properties(0).multi_processor_count
         self.seqs = sms * (8 if n * rep <= 32 else 1) // self.kvh * 5 // 4 + 1
         pages = (l + PAGE - 1) // PAGE
@@ -82,7 +82,7 @@ class Long:
         self.table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(self.seqs, 1)
         self.starts = torch.arange(self.seqs + 1, dtype=torch.int32, device="cuda") * n
         self.lens = torch.full((self.seqs,), l, dtype=torch.int32, device="cuda")
-        self.batch = pib.Kv4Batch(t, self.kvh * rep, n * self.seqs, self.seqs, n, pages, 0, self.dim ** -0.5)
+        self.batch = pib.Kv4Batch(t, self.kvh * rep, n * self.seqs, self.seqs, n, pages, window, self.dim ** -0.5)
         self.scratch = torch.empty(self.kv.scratch_bytes(self.batch), dtype=torch.uint8, device="cuda")
 
     def run(self, q):
@@ -98,7 +98,8 @@ class Long:
         """float64 rows of some query heads"""
         torch, out = self.torch, []
         K, V = (x.double() for x in read(torch, self.kv, F32, torch.arange(self.l, dtype=torch.int32, device="cuda"), self.kvh, self.dim))
-        hidden = torch.arange(self.l, device="cuda") > torch.arange(self.l - self.n, self.l, device="cuda").unsqueeze(1)
+        gap = torch.arange(self.l - self.n, self.l, device="cuda").unsqueeze(1) - torch.arange(self.l, device="cuda")
+        hidden = (gap < 0) | (gap >= (self.window or self.l))
         for h in heads:
             s = (q[:, h].to(dtype(torch, self.t)).double() @ K[:, h // self.rep].T * self.dim ** -0.5).masked_fill(hidden, -math.inf)
             out.append(torch.softmax(s, 1) @ V[:, h // self.rep])
@@ -193,3 +194,24 @@ def test_scores_of_all_magnitudes(torch, pib, t, n, rep, dim, sign):
         clear = top[..., 0] - top[..., 1] > 64 * E + 64
         assert ((o - V[:, 0][at[..., 0]]).abs()[clear] <= V.abs().max() * (2.0 ** -20 if t == F32 else 2.0 ** -8)).all()
         assert (o <= V.max() * 1.01).all() and (o >= V.min() * 1.01).all()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n,rep", [(1, 8), (2, 8), (4, 8), (8, 8)])
+def test_long_items_with_a_window_and_values_that_are_none(torch, pib, t, n, rep):
+    """sums that have left registers and tensor memory, first pages that a window cuts, and a last key whose values are none in one group: the last token's rows are none there, and no other bit changes.
+    Scores of 1.2 as before, E of Case.want 3e-5 with S = 7: 4 E, and half a step of bfloat16"""
+    l, window = 64000, 30001
+    c = Long(torch, pib, t, n, rep, l, normal(torch, 1, 1.0), normal(torch, 2, 1.0), window)
+    q = torch.randn(n, 8 * rep, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 1.2
+    got, heads = c.run(q), [0, rep, 7 * rep, 8 * rep - 1]
+    ref = c.want(q, heads)
+    off = float((got[:, :, heads].double() - ref).abs().max())
+    assert off <= 1.2e-4 + (0 if t == F32 else float(ref.abs().max()) * 2.0 ** -8)
+    K, V = read(torch, c.kv, F32, torch.tensor([l - 1], dtype=torch.int32, device="cuda"), 8, 128)
+    V[:, 0, 32:64] = math.nan
+    write(torch, c.kv, F32, K, V, torch.tensor([l - 1], dtype=torch.int32, device="cuda"))
+    none = c.run(q)
+    assert none[:, n - 1, :rep, 32:64].isnan().all()
+    none[:, n - 1, :rep, 32:64] = got[:, n - 1, :rep, 32:64]
+    assert torch.equal(none, got)
